@@ -52,6 +52,14 @@ extern "C" {
 
 #define LF_DTYPE_F32 0
 #define LF_DTYPE_BF16 1
+#define LF_DTYPE_F16 2          /* the dense operators only */
+#define LF_DTYPE_E4M3 3         /* 8-bit floats, 448 the largest (torch.float8_e4m3fn) */
+#define LF_DTYPE_I8 4
+
+#define LF_ACT_NONE 0
+#define LF_ACT_RELU 1
+#define LF_ACT_GELU 2           /* z Phi(z), Phi by erf */
+#define LF_ACT_SILU 3           /* z / (1 + exp(-z)) */
 
 #define LF_COST_REFERENCE 0     /* format_algos.py:1035-1166 bit for bit */
 #define LF_COST_GFX950 1        /* measured cost of ELL rows, staged slots and slab bytes on MI355X; same search */
@@ -424,6 +432,55 @@ int lf_bsr_spmm_trusted(const int32_t* d_indptr, const int32_t* d_indices, const
 int lf_bsr_spmm_trusted_nnz(const int32_t* d_indptr, const int32_t* d_indices, const void* d_data,
                             int64_t num_block_rows, int64_t num_block_cols, int64_t nnz_blocks, int32_t block_size,
                             int32_t feat_size, const void* d_X, void* d_Y, lf_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Dense rows of features: what a graph layer does beside the sparse product.  No counterpart in the reference, which
+ * ends with the product (format_algos.py:388-605).  Row-major matrices; ld_* counts elements from one row to the next
+ * (at least the row's length), addresses need the alignment of an element only.  Rows of at most 2^24
+ * elements.  Results do not depend on scheduling.  Outputs may not overlap inputs, but h may be the residual itself.
+ *
+ * lf_rms_norm: h = x + residual (NULL: h = x, and d_h is NULL too), y = h / sqrt(mean(h^2) + eps) * weight (NULL: ones).  d_h receives
+ * h in the residual's type.  y_dtype LF_DTYPE_E4M3 / LF_DTYPE_I8: q = y / scale to the nearest, with d_scale[row] = max|y| / 448 (/ 127),
+ * 0 for a row of zeros, NaN for one with Inf or NaN; d_scale is NULL otherwise.
+ * lf_quantize_rows: the same 8-bit form of rows as they are (a weight).
+ * lf_rms_norm_grad: from dy and h, dx = gradient of h - x and the residual have the same one - plus d_dh (NULL: none), what comes
+ * down the residual stream; dw [dim] in the weight's type (NULL: not wanted; else lf_rms_norm_grad_work_bytes bytes of work space,
+ * 16-byte aligned).  dx and d_dh have h's type.
+ * ------------------------------------------------------------------------------------ */
+int lf_rms_norm(const void* d_x, int64_t ld_x, int32_t x_dtype, const void* d_residual, int64_t ld_residual, int32_t residual_dtype,
+                const void* d_weight, int32_t weight_dtype, int64_t rows, int64_t dim, float eps, void* d_y, int64_t ld_y, int32_t y_dtype,
+                float* d_scale, void* d_h, int64_t ld_h, lf_stream_t stream);
+int lf_quantize_rows(const void* d_x, int64_t ld_x, int32_t x_dtype, int64_t rows, int64_t dim, void* d_q, int64_t ld_q, int32_t q_dtype,
+                     float* d_scale, lf_stream_t stream);
+size_t lf_rms_norm_grad_work_bytes(int64_t rows, int64_t dim);
+int lf_rms_norm_grad(const void* d_dy, int64_t ld_dy, int32_t dy_dtype, const void* d_h, int64_t ld_h, int32_t h_dtype, const void* d_weight,
+                     int32_t weight_dtype, const void* d_dh, int64_t ld_dh, int64_t rows, int64_t dim, float eps, void* d_dx, int64_t ld_dx,
+                     void* d_dw, void* d_work, size_t work_bytes, lf_stream_t stream);
+
+/* y = act(x w^T + bias) + residual for x [m][k], w [n][k] of one type, `dtype`.  float32, bfloat16 and float16; LF_DTYPE_E4M3 and LF_DTYPE_I8 with a
+ * scale for every row of x and of w (k < 2^17 for int8).  Sums are in 32 bits (float32: as exact as a float32 product).  bias [n], residual
+ * [m][n] and z [m][n], which receives x w^T + bias, may be NULL; they and y are float32, bfloat16 or float16, each of its own.
+ * lf_linear_work_bytes bytes of device memory, 16-byte aligned, that no other call uses meanwhile (0: d_work may be NULL).
+ *
+ * lf_linear_grad: dz = dy act'(z) (activation LF_ACT_NONE: z is not read), dx = dz w, dw = dz^T x, db = column sums of dz; any of d_dx, d_dw and d_db
+ * may be NULL.  The residual's gradient is dy.  For m = 0 dw and db are cleared.  Work space as above. */
+typedef struct lf_linear_args {
+    const void* d_x; const void* d_w; const float* d_x_scale; const float* d_w_scale;
+    const void* d_bias; const void* d_residual; void* d_y; void* d_z;
+    int64_t ld_x, ld_w, ld_residual, ld_y, ld_z;
+    int64_t m, n, k;
+    int32_t dtype, bias_dtype, residual_dtype, y_dtype, z_dtype, activation;
+} lf_linear_args;
+typedef struct lf_linear_grad_args {
+    const void* d_dy; const void* d_z; const void* d_x; const void* d_w; void* d_dx; void* d_dw; void* d_db;
+    int64_t ld_dy, ld_z, ld_x, ld_w, ld_dx, ld_dw;
+    int64_t m, n, k;
+    int32_t dtype, db_dtype, activation;
+} lf_linear_grad_args;
+size_t lf_linear_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype);
+int lf_linear(const lf_linear_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream);
+size_t lf_linear_grad_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t activation, int32_t want_dx, int32_t want_dw, int32_t want_db);
+int lf_linear_grad(const lf_linear_grad_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -25,6 +25,10 @@ LF_STATS_FIELDS = 4
 LF_SPMM_INFO_FIELDS = 9
 LF_DTYPE_F32 = 0
 LF_DTYPE_BF16 = 1
+LF_DTYPE_F16 = 2
+LF_DTYPE_E4M3 = 3
+LF_DTYPE_I8 = 4
+LF_ACT_NONE, LF_ACT_RELU, LF_ACT_GELU, LF_ACT_SILU = range(4)
 LF_COST_REFERENCE = 0
 LF_COST_GFX950 = 1
 LF_CSR_CANONICAL = 1
@@ -43,6 +47,20 @@ class BucketDesc(C.Structure):
     """struct lf_bucket_desc"""
     _fields_ = [("width", C.c_int32), ("part", C.c_int32), ("num_ell_rows", C.c_int64),
                 ("d_rows", vp), ("d_cols", vp), ("d_vals", vp), ("d_meta", vp)]
+
+
+class LinearArgs(C.Structure):
+    """struct lf_linear_args"""
+    _fields_ = ([(n, vp) for n in ("x", "w", "x_scale", "w_scale", "bias", "residual", "y", "z")]
+                + [(n, C.c_int64) for n in ("ld_x", "ld_w", "ld_residual", "ld_y", "ld_z", "m", "n", "k")]
+                + [(n, C.c_int32) for n in ("dtype", "bias_dtype", "residual_dtype", "y_dtype", "z_dtype", "activation")])
+
+
+class LinearGradArgs(C.Structure):
+    """struct lf_linear_grad_args"""
+    _fields_ = ([(n, vp) for n in ("dy", "z", "x", "w", "dx", "dw", "db")]
+                + [(n, C.c_int64) for n in ("ld_dy", "ld_z", "ld_x", "ld_w", "ld_dx", "ld_dw", "m", "n", "k")]
+                + [(n, C.c_int32) for n in ("dtype", "db_dtype", "activation")])
 
 
 # name -> (restype, argtypes); one entry per function declared in the header
@@ -97,6 +115,16 @@ SIGNATURES = {
     "lf_bsr_spmm": (C.c_int, [vp, vp, vp, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, vp, vp, vp, vp]),
     "lf_bsr_spmm_trusted": (C.c_int, [vp, vp, vp, C.c_int64, C.c_int64, C.c_int32, C.c_int32, vp, vp, vp]),
     "lf_bsr_spmm_trusted_nnz": (C.c_int, [vp, vp, vp, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, vp, vp, vp]),
+    "lf_rms_norm": (C.c_int, [vp, C.c_int64, C.c_int32, vp, C.c_int64, C.c_int32, vp, C.c_int32, C.c_int64, C.c_int64, C.c_float, vp, C.c_int64,
+                              C.c_int32, vp, vp, C.c_int64, vp]),
+    "lf_quantize_rows": (C.c_int, [vp, C.c_int64, C.c_int32, C.c_int64, C.c_int64, vp, C.c_int64, C.c_int32, vp, vp]),
+    "lf_rms_norm_grad_work_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
+    "lf_rms_norm_grad": (C.c_int, [vp, C.c_int64, C.c_int32, vp, C.c_int64, C.c_int32, vp, C.c_int32, vp, C.c_int64, C.c_int64, C.c_int64, C.c_float,
+                                   vp, C.c_int64, vp, vp, C.c_size_t, vp]),
+    "lf_linear_work_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64, C.c_int32]),
+    "lf_linear": (C.c_int, [vp, vp, C.c_size_t, vp]),
+    "lf_linear_grad_work_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "lf_linear_grad": (C.c_int, [vp, vp, C.c_size_t, vp]),
 }
 
 _lock = threading.Lock()

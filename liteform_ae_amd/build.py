@@ -10,13 +10,15 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblfhip.so")
 
-SOURCES = ["lf_error.cpp", "lf_search.cpp", "lf_format.hip", "lf_spmm.hip", "lf_csr.hip", "lf_cells.hip", "lf_bsr.hip", "lf_ingest.hip"]
+SOURCES = ["lf_error.cpp", "lf_search.cpp", "lf_format.hip", "lf_spmm.hip", "lf_csr.hip", "lf_cells.hip", "lf_bsr.hip", "lf_ingest.hip",
+           "lf_norm.hip", "lf_linear.hip"]
 
 # -ffp-contract=off: the width search must add and multiply doubles exactly like CPython.
 # packed-fp32-ops is switched off for device code on purpose (scalar fp32 FMAs only).
@@ -40,15 +42,17 @@ def build(verbose: bool = True, extra_flags=(), out: str = LIB, objdir: str | No
     hipcc = hipcc_path()
     objdir = objdir or os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    objs = []
+    objs, cmds = [], []
     for src in SOURCES:
         obj = os.path.join(objdir, os.path.splitext(src)[0] + ".o")
         cmd = [hipcc, *HIPCC_FLAGS, *extra_flags, "-I", os.path.join(ROOT, "include"), "-I", CSRC]
         if src.endswith(".cpp"):
             cmd += ["-x", "hip"]
         cmd += ["-c", os.path.join(CSRC, src), "-o", obj]
-        _run(cmd, verbose)
+        cmds.append(cmd)
         objs.append(obj)
+    with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+        list(pool.map(lambda cmd: _run(cmd, verbose), cmds))
     _run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out, *objs], verbose)
     return out
 

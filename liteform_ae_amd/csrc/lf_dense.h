@@ -1,0 +1,103 @@
+// What the kernels for dense rows of features (lf_norm.hip, lf_linear.hip) share: element types, loads and
+// stores of eight elements at any alignment, activations.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <cstdint>
+
+#include "lf_internal.h"
+
+namespace lf {
+
+typedef float float8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr bool is_float_dtype(int32_t t) { return t == LF_DTYPE_F32 || t == LF_DTYPE_BF16 || t == LF_DTYPE_F16; }
+constexpr bool is_8bit_dtype(int32_t t) { return t == LF_DTYPE_E4M3 || t == LF_DTYPE_I8; }
+constexpr int dtype_bytes(int32_t t) { return t == LF_DTYPE_F32 ? 4 : is_8bit_dtype(t) ? 1 : 2; }
+
+// Eight elements at any address that is a multiple of the element's size: the hardware takes 16-byte accesses there, and a
+// row of an odd number of 2-byte elements, or a row inside a wider buffer, needs no code of its own.
+template <typename T> struct Eight {
+    typedef T vec __attribute__((ext_vector_type(8)));
+    struct __attribute__((packed, aligned(sizeof(T)))) Any { vec v; };
+};
+template <typename T> __device__ __forceinline__ float8_t load8(const T* p) {
+    return __builtin_convertvector(reinterpret_cast<const typename Eight<T>::Any*>(p)->v, float8_t);
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, float8_t f) {
+    reinterpret_cast<typename Eight<T>::Any*>(p)->v = __builtin_convertvector(f, typename Eight<T>::vec);
+}
+// The first `n` of them (any n; others read as zero).
+template <typename T> __device__ __forceinline__ float8_t load_upto8(const T* p, int n) {
+    if (n >= 8) return load8(p);
+    float8_t f = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < n) f[i] = (float)p[i];
+    return f;
+}
+template <typename T> __device__ __forceinline__ void store_upto8(T* p, float8_t f, int n) {
+    if (n >= 8) return store8(p, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < n) p[i] = (T)f[i];
+}
+// The same of a type that is known at run time (one for the whole launch).
+__device__ __forceinline__ float8_t load_upto8(const void* p, int64_t at, int32_t dtype, int n) {
+    if (dtype == LF_DTYPE_F32) return load_upto8((const float*)p + at, n);
+    if (dtype == LF_DTYPE_BF16) return load_upto8((const __bf16*)p + at, n);
+    return load_upto8((const _Float16*)p + at, n);
+}
+__device__ __forceinline__ void store_upto8(void* p, int64_t at, int32_t dtype, float8_t f, int n) {
+    if (dtype == LF_DTYPE_F32) return store_upto8((float*)p + at, f, n);
+    if (dtype == LF_DTYPE_BF16) return store_upto8((__bf16*)p + at, f, n);
+    return store_upto8((_Float16*)p + at, f, n);
+}
+
+// Eight values as e4m3 (nearest, ties to even; |v| <= 448 is the caller's, NaN stays NaN).
+__device__ __forceinline__ uint2_t to_e4m3(float8_t v) {
+    uint2_t r = {0u, 0u};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h], v[4 * h + 1], 0, false);
+        r[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2], v[4 * h + 3], w, true);
+    }
+    return r;
+}
+// ... and as int8.
+__device__ __forceinline__ uint2_t to_int8(float8_t v) {
+    uint2_t r = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i >> 2] |= ((uint32_t)(int)rintf(v[i]) & 0xffu) << (8 * (i & 3));
+    return r;
+}
+
+// act(z) and act'(z).  gelu is z Phi(z) with the normal distribution's Phi (erf).
+__device__ __forceinline__ float activate(float z, int32_t act) {
+    if (act == LF_ACT_RELU) return z < 0.f ? 0.f : z;                    // (NaN stays)
+    if (act == LF_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+    if (act == LF_ACT_SILU) return z / (1.f + __expf(-z));
+    return z;
+}
+__device__ __forceinline__ float activate_grad(float z, int32_t act) {
+    if (act == LF_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    if (act == LF_ACT_GELU) return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+    if (act == LF_ACT_SILU) {
+        const float s = 1.f / (1.f + __expf(-z));
+        return s * (1.f + z * (1.f - s));
+    }
+    return 1.f;
+}
+
+// Columns of [n][dim] partial sums, added up in order (lf_norm.hip).
+int column_sums(const float* part, int64_t n, int64_t dim, void* out, int32_t dtype, hipStream_t stream);
+
+}  // namespace lf
+
+#define LF_TRY(call)                  \
+    do {                              \
+        if (int rc_ = (call)) return rc_; \
+    } while (0)
