@@ -79,7 +79,20 @@ __device__ __forceinline__ uint2_t to_int8(float8_t v) {
 __device__ __forceinline__ float activate(float z, int32_t act) {
     if (act == LF_ACT_RELU) return z < 0.f ? 0.f : z;                    // (NaN stays)
     if (act == LF_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678f));
-    if (act == LF_ACT_SILU) return z / (1.f + __expf(-z));
+    if (act == LF_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+    return z;
+}
+__device__ __forceinline__ float8_t activate(float8_t z, int32_t act) {
+    if (act == LF_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = activate(z[i], LF_ACT_RELU);
+    } else if (act == LF_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = activate(z[i], LF_ACT_GELU);
+    } else if (act == LF_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = activate(z[i], LF_ACT_SILU);
+    }
     return z;
 }
 __device__ __forceinline__ float activate_grad(float z, int32_t act) {

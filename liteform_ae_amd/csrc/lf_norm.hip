@@ -365,22 +365,23 @@ rms_norm_grad_long_kernel(GradArgs a) {
     }
 }
 
-// Columns of [n][dim] partial sums: 32 columns to a workgroup, every 32nd row to a thread, then the threads in order.
+// Columns of [n][dim] partial sums: 16 columns to a workgroup, every 64th row to a thread, then the threads in order.
 __global__ void __launch_bounds__(1024) column_sums_kernel(const float* part, int64_t n, int32_t dim, void* out, int32_t dtype) {
-    __shared__ float s[32][33];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+    __shared__ float s[64][17];
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
+    const float* src = part + min(col, dim - 1);
     float v = 0.f;
-    if (col < dim)
-        for (int64_t r = slice; r < n; r += 32) v += part[r * dim + col];
-    s[slice][threadIdx.x & 31] = v;
+#pragma unroll 8
+    for (int64_t r = slice; r < n; r += 64) v += src[r * dim];
+    s[slice][threadIdx.x & 15] = v;
     __syncthreads();
-    if (slice == 0 && col < dim) {
-        v = 0.f;
-        for (int i = 0; i < 32; ++i) v += s[i][threadIdx.x];
-        if (dtype == LF_DTYPE_F32) ((float*)out)[col] = v;
-        else if (dtype == LF_DTYPE_BF16) ((__bf16*)out)[col] = (__bf16)v;
-        else ((_Float16*)out)[col] = (_Float16)v;
-    }
+    if (slice || col >= dim) return;
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v += s[i][threadIdx.x];
+    if (dtype == LF_DTYPE_F32) ((float*)out)[col] = v;
+    else if (dtype == LF_DTYPE_BF16) ((__bf16*)out)[col] = (__bf16)v;
+    else ((_Float16*)out)[col] = (_Float16)v;
 }
 
 // Threads that hold a row, and pieces of eight of each (more than two: the kernels for long rows).
@@ -451,7 +452,7 @@ int check_shape(int64_t rows, int64_t dim) {
 
 namespace lf {
 int column_sums(const float* part, int64_t n, int64_t dim, void* out, int32_t dtype, hipStream_t stream) {
-    column_sums_kernel<<<(unsigned)ceil_div(dim, 32), 1024, 0, stream>>>(part, n, (int32_t)dim, out, dtype);
+    column_sums_kernel<<<(unsigned)ceil_div(dim, 16), 1024, 0, stream>>>(part, n, (int32_t)dim, out, dtype);
     LF_HIP(hipGetLastError());
     return LF_OK;
 }

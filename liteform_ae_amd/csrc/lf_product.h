@@ -1,0 +1,741 @@
+// The tiled products behind lf_linear and lf_linear_grad: dense rows of features with a weight, on the matrix cores:
+//
+//     Y = act(X W^T + b) + R          X [m][k], W [n][k] of float32, bfloat16, float16, or 8 bits with a scale a row
+//     dZ = dY act'(Z);  dX = dZ W;  dW = dZ^T X;  db = column sums of dZ
+//
+// One tiled kernel makes all of them.  It computes D[m][n] = sum over k of P[m][k] Q[n][k]; either operand may be
+// stored with k along its rows (X, W of the forward product) or across them (W of dX, both of dW).
+//   * A tile of TM x TN outputs belongs to a workgroup; a step stages 128 bytes of k (float32: 32 elements) of its
+//     TM + TN rows in LDS, in two buffers, so that one step is read while the next is on its way: global loads into registers
+//     a step ahead, LDS stores after the products, one barrier a step.
+//   * In LDS both operands have k along the rows, in pieces of 16 bytes that are swapped about by a key of the row, so
+//     that the 16 rows that a matrix instruction reads at once lie in different banks.  Operands stored across k are turned in
+//     registers on their way there, four k at a time.
+//   * Q gives the rows of a matrix instruction and P its columns: a lane holds four consecutive outputs of a row.  They go through LDS into
+//     whole rows, in which the epilogue (scales, bias, activation, residual) reads and writes.
+//   * float32 has no fast matrix instruction.  A value is cut into three bfloat16 of 8 bits each (exactly: by truncation), and
+//     six of the nine products - all but those below 2^-24 of the largest - go through the bfloat16 one, which is 16 times as fast
+//     as the float32 one.  Inf and NaN do not survive the cut; outputs that are not finite are computed again from the operands.
+//   * Few tiles are cut along k as well: partial sums in 32 bits, added up in a fixed order by a second kernel with the epilogue.
+// Up to 16 rows of X are another problem - W is read once, nothing is shared - and have a kernel of their own.
+#pragma once
+#include <algorithm>
+#include <type_traits>
+
+#include "lf_dense.h"
+
+namespace lf {
+
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef int int4v __attribute__((ext_vector_type(4)));
+typedef int int8v __attribute__((ext_vector_type(8)));
+
+struct e4m3_t { uint8_t b; };
+
+// ---------------------------------------------------------------------------- the epilogue
+
+struct Epilogue {
+    void* y; const void* res; void* z; const void* bias; const float* x_scale; const float* w_scale;
+    int64_t ld_y, ld_res, ld_z;
+    int32_t y_dtype, res_dtype, z_dtype, bias_dtype, act;
+};
+
+struct Product {
+    const void* p; const void* q;
+    int64_t ld_p, ld_q;
+    int64_t m, n, k;
+    int64_t k_split;                // elements of k to a split, a multiple of a step's
+    int32_t tiles_m, tiles_n, splits;
+    void* part;                     // [splits][m][n] partial sums, or NULL: the epilogue follows at once
+    Epilogue e;
+};
+using ProductFn = void (*)(Product);
+
+// The kernel for operands of a type: px, qx: P, Q stored across k; tile: 64 or 128 (any operands), 256 (kWideTile: rows that
+// are 16-byte aligned).
+constexpr int kWideTile = 256;
+ProductFn product_f32(bool px, bool qx, int tile);
+ProductFn product_bf16(bool px, bool qx, int tile);
+ProductFn product_f16(bool px, bool qx, int tile);
+ProductFn product_e4m3(bool px, bool qx, int tile);
+ProductFn product_i8(bool px, bool qx, int tile);
+
+}  // namespace lf
+
+namespace {
+
+using namespace lf;
+
+// ---------------------------------------------------------------------------- element types
+
+template <typename T> struct Elem;
+template <> struct Elem<__bf16> { static constexpr int kPlanes = 1; using Acc = float4_t; };
+template <> struct Elem<_Float16> { static constexpr int kPlanes = 1; using Acc = float4_t; };
+template <> struct Elem<e4m3_t> { static constexpr int kPlanes = 1; using Acc = float4_t; };
+template <> struct Elem<int8_t> { static constexpr int kPlanes = 1; using Acc = int4v; };
+template <> struct Elem<float> { static constexpr int kPlanes = 3; using Acc = float4_t; };
+
+__device__ __forceinline__ float4_t mma(uint4_t a, uint4_t b, float4_t c, __bf16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float4_t mma(uint4_t a, uint4_t b, float4_t c, _Float16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ int4v mma(uint4_t a, uint4_t b, int4v c, int8_t) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4v, a), __builtin_bit_cast(int4v, b), c, 0, 0, 0);
+}
+// Two pieces of each at once: which k a byte stands for is free, as long as it is the same one on both sides.
+__device__ __forceinline__ float4_t mma_e4m3(uint4_t a0, uint4_t a1, uint4_t b0, uint4_t b1, float4_t c) {
+    const int8v a = {(int)a0[0], (int)a0[1], (int)a0[2], (int)a0[3], (int)a1[0], (int)a1[1], (int)a1[2], (int)a1[3]};
+    const int8v b = {(int)b0[0], (int)b0[1], (int)b0[2], (int)b0[3], (int)b1[0], (int)b1[1], (int)b1[2], (int)b1[3]};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+
+// 16 bytes at any address that suits the type
+template <typename T> __device__ __forceinline__ uint4_t load16(const T* p) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Any { uint4_t v; };
+    return reinterpret_cast<const Any*>(p)->v;
+}
+// the first n elements of them, zeros behind
+template <typename T> __device__ __forceinline__ uint4_t load16_upto(const T* p, int n) {
+    constexpr int E = 16 / sizeof(T);
+    if (n >= E) return load16(p);
+    uint4_t r = {0u, 0u, 0u, 0u};
+    for (int i = 0; i < E; ++i)
+        if (i < n) {
+            if constexpr (sizeof(T) == 4) r[i] = __builtin_bit_cast(uint32_t, p[i]);
+            else if constexpr (sizeof(T) == 2) r[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << (16 * (i & 1));
+            else r[i >> 2] |= (uint32_t)__builtin_bit_cast(uint8_t, p[i]) << (8 * (i & 3));
+        }
+    return r;
+}
+
+// Two floats as the halves of three words: 8 bits of each per word, which together are the floats exactly.
+__device__ __forceinline__ void cut(float a, float b, uint32_t (&w)[3]) {
+    const uint32_t top = 0xffff0000u;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+        w[p] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+        a -= __uint_as_float(ua & top);
+        b -= __uint_as_float(ub & top);
+    }
+}
+
+// ---------------------------------------------------------------------------- the epilogue
+
+// `count` outputs (at most eight) of row m from column n on
+__device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int64_t n, int count, float8_t v) {
+    if (e.x_scale) v = v * e.x_scale[m] * load_upto8(e.w_scale + n, count);
+    if (e.bias) v += load_upto8(e.bias, n, e.bias_dtype, count);
+    if (e.z) store_upto8(e.z, m * e.ld_z + n, e.z_dtype, v, count);
+    if (e.act != LF_ACT_NONE)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = activate(v[i], e.act);
+    if (e.res) v += load_upto8(e.res, m * e.ld_res + n, e.res_dtype, count);
+    store_upto8(e.y, m * e.ld_y + n, e.y_dtype, v, count);
+}
+
+// Eight elements as they lie in memory, so that many loads can be under way before the first is converted.
+template <typename T> __device__ __forceinline__ typename Eight<T>::vec raw_upto8(const T* p, int n) {
+    typename Eight<T>::vec v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (n >= 8) {
+        v = reinterpret_cast<const typename Eight<T>::Any*>(p)->v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) v[i] = p[i];
+    }
+    return v;
+}
+template <typename F> __device__ __forceinline__ void with_type(int32_t dtype, F f) {
+    if (dtype == LF_DTYPE_F32) f(0.f);
+    else if (dtype == LF_DTYPE_BF16) f((__bf16)0.f);
+    else f((_Float16)0.f);
+}
+
+// ---------------------------------------------------------------------------- the tiled product
+
+// Where 16-byte piece c of a row stands among the row's pieces: matrix instructions read 16 consecutive rows at one c, operands across k are
+// stored at rows 8 apart.
+template <int PIECES> __device__ __forceinline__ int slot(int row, int c) {
+    return PIECES == 8 ? row * 8 + (c ^ ((row ^ row >> 3) & 7)) : row * 4 + (c ^ ((row >> 1 ^ row >> 3) & 3));
+}
+
+// One operand's tile of ROWS x (a step of k): global memory -> registers -> LDS.
+template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
+    static constexpr int kPlanes = Elem<T>::kPlanes;
+    static constexpr int kStep = sizeof(T) == 4 ? 32 : 128 / sizeof(T);   // elements of k
+    static constexpr int kPieces = sizeof(T) == 4 ? 4 : 8;                // pieces of a row in LDS (of each plane)
+    static constexpr int kElems = kStep / kPieces;                        // elements of a piece
+    static constexpr int kSlots = ROWS * kPieces;                         // 16-byte slots of a plane
+    // along k: a unit is a piece (float32: 32 bytes).  Across: 4 k of 16 bytes of neighbouring rows.
+    static constexpr int kWide = 16 / sizeof(T);                          // rows of a unit across
+    static constexpr int kUnits = ACROSS ? (ROWS / kWide) * (kStep / 4) : ROWS * kPieces;
+    static constexpr int kMine = (kUnits + THREADS - 1) / THREADS;
+    static constexpr int kRegs = ACROSS ? 4 : kPlanes == 3 ? 2 : 1;       // 16-byte registers of a unit
+    uint4_t r[kMine][kRegs];
+
+    // `left`: elements of k from this step on (more than a step: the fast way)
+    __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t left, int tid) {
+        const bool whole = left >= kStep;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int u = tid + i * THREADS;
+            if (kUnits % THREADS && u >= kUnits) continue;
+            if constexpr (!ACROSS) {
+                const int64_t row = min(row0 + u / kPieces, rows - 1);    // (rows past the end are read for the last one and not used)
+                const int at = (u % kPieces) * kElems;
+                const T* src = base + row * ld + k0 + at;
+#pragma unroll
+                for (int h = 0; h < kRegs; ++h) {
+                    if (whole) r[i][h] = load16(src + h * kWide);
+                    else r[i][h] = load16_upto(src + h * kWide, (int)left - at - h * kWide);
+                }
+            } else {
+                const Across a(u);
+                const int64_t row = row0 + a.row;
+                const int n = (int)min((int64_t)kWide, rows - row);
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const T* src = base + (k0 + a.k + h) * ld + row;
+                    const bool in = whole || a.k + h < left;
+                    if (in && n == kWide) r[i][h] = load16(src);
+                    else r[i][h] = load16_upto(src, in ? n : 0);
+                }
+            }
+        }
+    }
+    struct Across {
+        int row, k;                                                       // of the unit in the tile
+        __device__ __forceinline__ explicit Across(int u) {
+            // eight neighbouring units along k, then along the rows: 128 bytes of a row of the operand to a load instruction
+            constexpr int KU = kStep / 4, RU = ROWS / kWide;
+            static_assert(KU % 8 == 0 && RU % 8 == 0, "");
+            const int kl = u & 7, rl = u >> 3 & 7, rest = u >> 6;
+            row = (rl + 8 * (rest % (RU / 8))) * kWide;
+            k = (kl + 8 * (rest / (RU / 8))) * 4;
+        }
+    };
+    __device__ __forceinline__ void store(uint4_t* lds, int tid) const {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int u = tid + i * THREADS;
+            if (kUnits % THREADS && u >= kUnits) continue;
+            if constexpr (!ACROSS && kPlanes == 1) {
+                lds[slot<kPieces>(u / kPieces, u % kPieces)] = r[i][0];
+            } else if constexpr (!ACROSS) {
+                uint4_t out[3];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t w[3];
+                    cut(__uint_as_float(r[i][j >> 1][2 * (j & 1)]), __uint_as_float(r[i][j >> 1][2 * (j & 1) + 1]), w);
+                    out[0][j] = w[0]; out[1][j] = w[1]; out[2][j] = w[2];
+                }
+#pragma unroll
+                for (int p = 0; p < 3; ++p) lds[p * kSlots + slot<kPieces>(u / kPieces, u % kPieces)] = out[p];
+            } else {
+                const Across a(u);
+                uint2_t* half = reinterpret_cast<uint2_t*>(lds);
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) {
+                    const int at = 2 * slot<kPieces>(a.row + j, a.k / kElems) + (a.k / 4 & 1);
+                    if constexpr (kPlanes == 1) {
+                        const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+                        half[at] = uint2_t{__builtin_amdgcn_perm(r[i][1][j >> 1], r[i][0][j >> 1], sel), __builtin_amdgcn_perm(r[i][3][j >> 1], r[i][2][j >> 1], sel)};
+                    } else {
+                        uint32_t lo[3], hi[3];
+                        cut(__uint_as_float(r[i][0][j]), __uint_as_float(r[i][1][j]), lo);
+                        cut(__uint_as_float(r[i][2][j]), __uint_as_float(r[i][3][j]), hi);
+#pragma unroll
+                        for (int p = 0; p < 3; ++p) half[2 * p * kSlots + at] = uint2_t{lo[p], hi[p]};
+                    }
+                }
+            }
+        }
+    }
+};
+
+// One output of a float32 product from the operands themselves, whose elements are so far apart.
+__device__ __forceinline__ float dot_f32(const float* p, int64_t p_step, const float* q, int64_t q_step, int64_t k) {
+    float s = 0.f;
+    for (; k > 0; --k, p += p_step, q += q_step) s = fmaf(*p, *q, s);
+    return s;
+}
+
+// What a wavefront does with its WC columns of sums from (m, n) on: partial ones go to the work space, others through the epilogue.
+// They pass through its part of LDS (`lds`, room for PR rows), from the matrix instructions' order into rows, so that the
+// residual is read and the output written in whole lines, by a loop that is compiled once and has the loads of four
+// rows under way.  float32: `again(row, column)` computes an output from the operands.
+struct None {};
+template <int FM, int FN, int PR, typename Acc, typename Again>
+__device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN], uint4_t* lds, int64_t m, int64_t n, Again again) {
+    using S = std::conditional_t<std::is_same_v<Acc, int4v>, int32_t, float>;
+    constexpr int WC = 16 * FN, LANES = WC / 8, AT_ONCE = 64 / LANES, U = PR / AT_ONCE < 4 ? PR / AT_ONCE : 4;
+    static_assert(FM * 16 % PR == 0 && PR % AT_ONCE == 0, "");
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    const int mine = lane / LANES, piece = lane % LANES;
+    n += piece * 8;
+    const int count = (int)max((int64_t)0, min((int64_t)8, g.n - n));
+    const Epilogue& e = g.e;
+    float8_t bias = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, ws = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+    if (!g.part && count) {
+        if (e.bias) bias = load_upto8(e.bias, n, e.bias_dtype, count);
+        if (e.w_scale) ws = load_upto8(e.w_scale + n, count);
+    }
+#pragma unroll
+    for (int first = 0; first < FM * 16; first += PR) {
+#pragma unroll
+        for (int i = 0; i < PR / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int row = 16 * i + li, c = 4 * j + lg;
+                lds[row * (WC / 4) + (c ^ (row & 7))] = __builtin_bit_cast(uint4_t, acc[first / 16 + i][j]);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if constexpr (!std::is_same_v<Again, None>) {
+#pragma unroll 1
+            for (int row = mine; row < PR && m + first + row < g.m; row += AT_ONCE) {
+                bool fine = true;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) fine = fine && fabsf(__uint_as_float(lds[row * (WC / 4) + ((2 * piece + h) ^ (row & 7))][i])) < __builtin_inff();
+                if (!fine)
+#pragma unroll 1
+                    for (int i = 0; i < count; ++i) {
+                        float* s = (float*)(lds + row * (WC / 4) + ((2 * piece + (i >> 2)) ^ (row & 7))) + (i & 3);
+                        if (!(fabsf(*s) < __builtin_inff())) *s = again(m + first + row, n + i);
+                    }
+            }
+        }
+#pragma unroll 1
+        for (int r0 = mine; r0 < PR; r0 += U * AT_ONCE) {
+            const int64_t top = m + first + r0;
+            float8_t v[U], res[U];
+            float xs[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int row = r0 + u * AT_ONCE;
+                S s[8];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint4_t w = lds[row * (WC / 4) + ((2 * piece + h) ^ (row & 7))];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t word = w[i];             // (bit_cast of an element takes the first one)
+                        s[4 * h + i] = __builtin_bit_cast(S, word);
+                    }
+                }
+                if (std::is_same_v<S, int32_t> && g.part) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[u][i] = __builtin_bit_cast(float, s[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[u][i] = (float)s[i];
+                }
+            }
+            if (g.part) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (top + u * AT_ONCE < g.m && count) store_upto8((float*)g.part + ((int64_t)blockIdx.y * g.m + top + u * AT_ONCE) * g.n + n, v[u], count);
+                continue;
+            }
+            if (e.res)
+                with_type(e.res_dtype, [&](auto t) {
+                    using R = decltype(t);
+                    typename Eight<R>::vec raw[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) raw[u] = raw_upto8((const R*)e.res + min(top + u * AT_ONCE, g.m - 1) * e.ld_res + n, count);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) res[u] = __builtin_convertvector(raw[u], float8_t);
+                });
+            if (e.x_scale) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) xs[u] = e.x_scale[min(top + u * AT_ONCE, g.m - 1)];
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] = v[u] * xs[u] * ws;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] += bias;
+            if (e.z) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (top + u * AT_ONCE < g.m && count) store_upto8(e.z, (top + u * AT_ONCE) * e.ld_z + n, e.z_dtype, v[u], count);
+            }
+            if (e.act != LF_ACT_NONE) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] = activate(v[u], e.act);
+            }
+            if (e.res) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] += res[u];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (top + u * AT_ONCE < g.m && count) store_upto8(e.y, (top + u * AT_ONCE) * e.ld_y + n, e.y_dtype, v[u], count);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The tile of a workgroup.  Workgroups go to the eight XCDs in turn: each XCD gets a run of neighbouring tiles, eight rows of
+// tiles deep, so that what its L2 holds of both operands is used by its 32 CUs at once.
+__device__ __forceinline__ void tile_of(const Product& g, unsigned id, int& tm, int& tn) {
+    const unsigned n = (unsigned)g.tiles_m * g.tiles_n, xcd = id % 8, each = n / 8, more = n % 8;
+    unsigned t = xcd * each + min(xcd, more) + id / 8;
+    constexpr unsigned kDeep = 8;
+    const unsigned band = t / (kDeep * g.tiles_n), first = band * kDeep, deep = min(kDeep, (unsigned)g.tiles_m - first);
+    t -= band * kDeep * g.tiles_n;
+    tm = (int)(first + t % deep);
+    tn = (int)(t / deep);
+}
+
+template <typename T, bool PX, bool QX, int TM, int TN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN)
+product_kernel(Product g) {
+    constexpr int THREADS = 64 * WM * WN, FM = TM / WM / 16, FN = TN / WN / 16;
+    using Acc = typename Elem<T>::Acc;
+    using StageP = Stage<T, PX, TM, THREADS>;
+    using StageQ = Stage<T, QX, TN, THREADS>;
+    constexpr int PL = StageP::kPlanes, PC = StageP::kPieces, KS = StageP::kStep;
+    // float32 takes three planes: one buffer, so that a CU holds two workgroups, one of which multiplies while the other stores
+    constexpr int NB = PL == 3 ? 1 : 2;
+    constexpr int SP = PL * StageP::kSlots, SQ = PL * StageQ::kSlots;
+    __shared__ uint4_t s_all[NB * (SP + SQ)];
+    uint4_t *const s_p = s_all, *const s_q = s_all + NB * SP;
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
+    int tm, tn;
+    tile_of(g, blockIdx.x, tm, tn);
+    const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * TN;
+    const int64_t k_first = (int64_t)blockIdx.y * g.k_split, k_last = min(g.k, k_first + g.k_split);
+
+    Acc acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = Acc{0, 0, 0, 0};
+
+    // rows of the matrix instructions' operands in the tile
+    const int row_p = wm * (TM / WM) + li, row_q = wn * (TN / WN) + li;
+    auto multiply = [&](const uint4_t* sp, const uint4_t* sq) {
+        if constexpr (PL == 3) {
+            // a step is one 32-deep instruction, for six pairs of planes
+            uint4_t a[3][FN];
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) a[p][j] = sq[p * StageQ::kSlots + slot<PC>(row_q + j * 16, lg)];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                uint4_t b[3];
+#pragma unroll
+                for (int p = 0; p < 3; ++p) b[p] = sp[p * StageP::kSlots + slot<PC>(row_p + i * 16, lg)];
+#pragma unroll
+                for (int p = 2; p >= 0; --p)                              // the smallest products first
+#pragma unroll
+                    for (int q = 2 - p; q >= 0; --q)
+#pragma unroll
+                        for (int j = 0; j < FN; ++j) acc[i][j] = mma(a[q][j], b[p], acc[i][j], (__bf16)0.f);
+            }
+        } else if constexpr (sizeof(T) == 1 && !std::is_same_v<T, int8_t>) {
+            uint4_t a[FN][2];
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) a[j][h] = sq[slot<PC>(row_q + j * 16, 4 * h + lg)];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                uint4_t b[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) b[h] = sp[slot<PC>(row_p + i * 16, 4 * h + lg)];
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mma_e4m3(a[j][0], a[j][1], b[0], b[1], acc[i][j]);
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint4_t a[FN];
+#pragma unroll
+                for (int j = 0; j < FN; ++j) a[j] = sq[slot<PC>(row_q + j * 16, 4 * h + lg)];
+#pragma unroll
+                for (int i = 0; i < FM; ++i) {
+                    const uint4_t b = sp[slot<PC>(row_p + i * 16, 4 * h + lg)];
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = mma(a[j], b, acc[i][j], T{});
+                }
+            }
+        }
+    };
+
+    const int64_t steps = k_last > k_first ? (k_last - k_first + KS - 1) / KS : 0;
+    if (steps > 0) {
+        StageP p;
+        StageQ q;
+        auto load = [&](int64_t s) {
+            const int64_t k = k_first + s * KS;
+            p.load((const T*)g.p, g.ld_p, m0, g.m, k, k_last - k, tid);
+            q.load((const T*)g.q, g.ld_q, n0, g.n, k, k_last - k, tid);
+        };
+        load(0);
+        if constexpr (NB == 1) {
+            for (int64_t s = 0; s < steps; ++s) {
+                p.store(s_p, tid);
+                q.store(s_q, tid);
+                __syncthreads();
+                if (s + 1 < steps) load(s + 1);
+                multiply(s_p, s_q);
+                __syncthreads();
+            }
+        } else {
+        p.store(s_p, tid);
+        q.store(s_q, tid);
+        if (steps > 1) load(1);
+        __syncthreads();
+        for (int64_t s = 0; s < steps; ++s) {
+            const int now = (int)(s & 1);
+            multiply(s_p + now * SP, s_q + now * SQ);
+            if (s + 1 < steps) {
+                p.store(s_p + (now ^ 1) * SP, tid);
+                q.store(s_q + (now ^ 1) * SQ, tid);
+                if (s + 2 < steps) load(s + 2);
+            }
+            __syncthreads();
+        }
+        }
+    }
+
+    // (the last step is behind a barrier: LDS is free)
+    constexpr int SLOTS = NB * PL * (StageP::kSlots + StageQ::kSlots) / (WM * WN), WHOLE = FM * 16, FIT = SLOTS / (FN * 4);
+    constexpr int PR = FIT >= WHOLE ? WHOLE : FIT >= WHOLE / 2 ? WHOLE / 2 : WHOLE / 4;
+    static_assert(PR <= FIT && PR % 16 == 0, "");
+    uint4_t* mine = s_all + wave * SLOTS;
+    const int64_t m = m0 + wm * (TM / WM), n = n0 + wn * (TN / WN);
+    if constexpr (PL == 3)
+        leave<FM, FN, PR>(g, acc, mine, m, n, [&](int64_t row, int64_t col) {
+            return dot_f32((const float*)g.p + (PX ? k_first * g.ld_p + row : row * g.ld_p + k_first), PX ? g.ld_p : 1,
+                           (const float*)g.q + (QX ? k_first * g.ld_q + col : col * g.ld_q + k_first), QX ? g.ld_q : 1, k_last - k_first);
+        });
+    else
+        leave<FM, FN, PR>(g, acc, mine, m, n, None{});
+}
+
+// ---------------------------------------------------------------------------- the tiled product, large tiles
+
+// A tile of 256 x 256 for operands whose rows are 16-byte aligned: four wavefronts of 128 x 128 outputs, which read 32 KB of LDS for
+// 4 x 2 MB of products a step, half of what eight of 128 x 64 read.  Operands go from memory into LDS without registers in between (64 lanes
+// x 16 bytes to consecutive addresses; the order of the pieces there follows from the addresses they are read from).  Operands across k
+// lie in LDS as they do in memory and are turned by the transposing LDS load.
+// A step: the second half of the rows of P is read during the products of the first one, then - behind the only barrier, when the next
+// buffer has arrived and this one is read - the next step's Q and first half during the products of the second.
+// A last step of less than 128 bytes of k goes through registers, with zeros behind the end.
+
+template <typename T> struct Frag { uint4_t c[2]; };                      // 64 bytes of k of a row: two pieces of a lane
+
+// The sums fill the 256 accumulation registers of a lane to the last one.  The compiler's own matrix instructions write to other
+// registers than they add to and would need spare ones: with none left it moves 400 registers about a step (half the
+// speed).  These add in place.  What the compiler knows about its own it does not know about them, so two idle cycles keep
+// a move into an operand away from its use, and settle() the last instruction from the reading of its sums.
+template <typename T> __device__ __forceinline__ void add_product(typename Elem<T>::Acc& c, const Frag<T>& a, const Frag<T>& b, int half) {
+    if constexpr (std::is_same_v<T, e4m3_t>) {
+        const int8v x = __builtin_shufflevector(__builtin_bit_cast(int4v, a.c[0]), __builtin_bit_cast(int4v, a.c[1]), 0, 1, 2, 3, 4, 5, 6, 7);
+        const int8v y = __builtin_shufflevector(__builtin_bit_cast(int4v, b.c[0]), __builtin_bit_cast(int4v, b.c[1]), 0, 1, 2, 3, 4, 5, 6, 7);
+        asm("s_nop 1\n\tv_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, %0" : "+a"(c) : "v"(x), "v"(y));
+    } else if constexpr (std::is_same_v<T, int8_t>) {
+        asm("s_nop 1\n\tv_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a.c[half]), "v"(b.c[half]));
+    } else if constexpr (std::is_same_v<T, __bf16>) {
+        asm("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a.c[half]), "v"(b.c[half]));
+    } else {
+        asm("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a.c[half]), "v"(b.c[half]));
+    }
+}
+template <typename Acc> __device__ __forceinline__ void settle(Acc (&c)[8]) {
+    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7]));
+}
+
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4_t lds_short4;
+typedef __attribute__((address_space(3))) uint32_t lds_word;
+typedef const __attribute__((address_space(1))) uint32_t global_word;
+
+// One operand's tile of 256 x (a step of k) on its way from memory to the matrix instructions.
+template <typename T, bool ACROSS> struct Wide {
+    static constexpr int kStep = 128 / sizeof(T), kElems = 16 / sizeof(T);
+    // LDS slots from a wavefront's load instruction to the next: across, 64 bytes more than two k, so that four k lie in different banks
+    static constexpr int kLoad = ACROSS ? 68 : 64, kSlots = 32 * kLoad;
+    const char* base;                  // of what a wavefront's first load instruction reads next
+    int64_t step_bytes, load_bytes;    // from step to step, from a load instruction to the next
+    uint32_t off;                      // from there to what this lane reads
+    int at;                            // element of k (along), k (across) of that
+    int wave, lane, li, lg;
+
+    // A load instruction reads eight rows (along) or two k (across); the wavefronts take them in turn.  Along, piece c of row r stands at
+    // place c ^ (r & 7) of the row; across, piece c of k stands at place 2 c + (k & 1) of the pair.
+    __device__ __forceinline__ Wide(const void* p, int64_t ld, int64_t row0, int64_t k0) {
+        lane = threadIdx.x & 63;
+        li = lane & 15;
+        lg = lane >> 4;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int64_t ld_bytes = ld * sizeof(T);
+        if constexpr (!ACROSS) {
+            base = (const char*)p + (row0 + 8 * wave) * ld_bytes + k0 * sizeof(T);
+            step_bytes = 128;
+            load_bytes = 32 * ld_bytes;
+            const int c = (lane & 7) ^ (lane >> 3);
+            off = (lane >> 3) * (uint32_t)ld_bytes + c * 16;
+            at = c * kElems;
+        } else {
+            base = (const char*)p + (k0 + 2 * wave) * ld_bytes + row0 * sizeof(T);
+            step_bytes = kStep * ld_bytes;
+            load_bytes = 8 * ld_bytes;
+            at = 2 * wave + (lane & 1);
+            off = (lane & 1) * (uint32_t)ld_bytes + (lane >> 1) * 16;
+        }
+    }
+    __device__ __forceinline__ void load(uint4_t* lds) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            __builtin_amdgcn_global_load_lds((global_word*)(base + i * load_bytes + off), (lds_word*)(lds + (wave + 4 * i) * kLoad), 16, 0, 0);
+        base += step_bytes;
+    }
+    __device__ __forceinline__ void load_last(uint4_t* lds, int left) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            lds[(wave + 4 * i) * kLoad + lane] = load16_upto((const T*)(base + i * load_bytes + off), ACROSS ? (at + 8 * i < left ? kElems : 0) : left - at);
+    }
+    // rows `row` .. + 15 of the tile as an operand of the matrix instructions
+    __device__ __forceinline__ Frag<T> read(const uint4_t* lds, int row) const {
+        Frag<T> f;
+        if constexpr (!ACROSS) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) f.c[h] = lds[(row + li) * 8 + ((4 * h + lg) ^ (li & 7))];
+        } else {
+            // 16 lanes read 16 rows of four k, lane 4 r + s rows 4 s .. of the r-th, and receive four k of a row each
+            const char* src = (const char*)lds + (4 * lg + (li >> 3)) * (kLoad * 16) + (li & 2) * 16 + (li >> 2 & 1) * 16 + (li & 1) * 8;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const uint2_t v = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(src + (16 * h + 2 * t) * (kLoad * 16) + row * 4)));
+                    f.c[h][2 * t] = v[0];
+                    f.c[h][2 * t + 1] = v[1];
+                }
+        }
+        return f;
+    }
+};
+
+template <typename T, bool PX, bool QX>
+__global__ void __launch_bounds__(256)
+wide_kernel(Product g) {
+    using Acc = typename Elem<T>::Acc;
+    using F = Frag<T>;
+    constexpr int KS = 128 / sizeof(T);
+    // (arrays of their own: what is read from one must not wait for what is on its way into another)
+    __shared__ uint4_t s_p0[Wide<T, PX>::kSlots], s_q0[Wide<T, QX>::kSlots], s_p1[Wide<T, PX>::kSlots], s_q1[Wide<T, QX>::kSlots];
+    int tm, tn;
+    tile_of(g, blockIdx.x, tm, tn);
+    // (the last tiles reach back to be whole ones: outputs of two tiles are computed twice, alike)
+    const int64_t m0 = min((int64_t)tm * 256, g.m - 256), n0 = min((int64_t)tn * 256, g.n - 256);
+    const int64_t k_first = (int64_t)blockIdx.y * g.k_split, k_last = min(g.k, k_first + g.k_split);
+    Wide<T, PX> P(g.p, g.ld_p, m0, k_first);
+    Wide<T, QX> Q(g.q, g.ld_q, n0, k_first);
+    const int wm = P.wave & 1, wn = P.wave >> 1, row_p = wm * 128, row_q = wn * 128;
+
+    Acc acc[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = Acc{0, 0, 0, 0};
+
+    auto read_q = [&](const uint4_t* s, F (&q)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = Q.read(s, row_q + j * 16);
+    };
+    auto read_p = [&](const uint4_t* s, F (&p)[4], int half) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = P.read(s, row_p + half * 64 + i * 16);
+    };
+    auto multiply = [&](const F (&p)[4], const F (&q)[8], int half) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < (std::is_same_v<T, e4m3_t> ? 1 : 2); ++h)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) add_product<T>(acc[4 * half + i][j], q[j], p[i], h);
+    };
+    auto arrived = [] {
+        __builtin_amdgcn_s_waitcnt(0x70);             // loads and LDS: none under way
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    const int64_t length = k_last > k_first ? k_last - k_first : 0, steps = length / KS;
+    const int left = (int)(length - steps * KS);
+    F q0[8], q1[8], p0[4], p1[4];
+    if (steps > 0) {
+        P.load(s_p0);
+        Q.load(s_q0);
+        arrived();
+        if (steps > 1) {
+            P.load(s_p1);
+            Q.load(s_q1);
+        }
+        read_q(s_q0, q0);
+        read_p(s_p0, p0, 0);
+        auto step = [&](uint4_t* sp, uint4_t* sq, const uint4_t* next_p, const uint4_t* next_q, F (&q)[8], F (&next)[8], bool more, bool further) {
+            read_p(sp, p1, 1);
+            multiply(p0, q, 0);
+            arrived();
+            if (further) {
+                P.load(sp);
+                Q.load(sq);
+            }
+            if (more) {
+                read_q(next_q, next);
+                read_p(next_p, p0, 0);
+            }
+            multiply(p1, q, 1);
+        };
+        int64_t s = 0;
+        for (; s + 3 < steps; s += 2) {
+            step(s_p0, s_q0, s_p1, s_q1, q0, q1, true, true);
+            step(s_p1, s_q1, s_p0, s_q0, q1, q0, true, true);
+        }
+        for (; s < steps; s += 2) {
+            step(s_p0, s_q0, s_p1, s_q1, q0, q1, s + 1 < steps, s + 2 < steps);
+            if (s + 1 < steps) step(s_p1, s_q1, s_p0, s_q0, q1, q0, s + 2 < steps, s + 3 < steps);
+        }
+    }
+    if (left > 0) {
+        __syncthreads();
+        P.load_last(s_p0, left);
+        Q.load_last(s_q0, left);
+        __syncthreads();
+        read_q(s_q0, q0);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            read_p(s_p0, p0, half);
+            multiply(p0, q0, half);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) settle(acc[i]);
+    __syncthreads();
+    uint4_t* mine = P.wave == 0 ? s_p0 : P.wave == 1 ? s_q0 : P.wave == 2 ? s_p1 : s_q1;
+    leave<8, 8, 64>(g, acc, mine, m0 + row_p, n0 + row_q, None{});
+}
+
+template <typename T, bool PX, bool QX> ProductFn kernel_of(int tile) {
+    if constexpr (!std::is_same_v<T, float>)
+        if (tile == kWideTile) return wide_kernel<T, PX, QX>;
+    return tile == 128 ? product_kernel<T, PX, QX, 128, 128, 2, 2> : product_kernel<T, PX, QX, 64, 64, 2, 2>;
+}
+template <typename T> ProductFn kernel_of(bool px, bool qx, int tile) {
+    return px ? kernel_of<T, true, true>(tile) : qx ? kernel_of<T, false, true>(tile) : kernel_of<T, false, false>(tile);
+}
+
+}  // namespace

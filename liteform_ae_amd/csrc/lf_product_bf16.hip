@@ -1,0 +1,5 @@
+#include "lf_product.h"
+
+namespace lf {
+ProductFn product_bf16(bool px, bool qx, int tile) { return kernel_of<__bf16>(px, qx, tile); }
+}  // namespace lf
