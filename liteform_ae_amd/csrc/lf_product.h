@@ -529,8 +529,10 @@ product_kernel(Product g) {
 // 4 x 2 MB of products a step, half of what eight of 128 x 64 read.  Operands go from memory into LDS without registers in between (64 lanes
 // x 16 bytes to consecutive addresses; the order of the pieces there follows from the addresses they are read from).  Operands across k
 // lie in LDS as they do in memory and are turned by the transposing LDS load.
-// A step: the second half of the rows of P is read during the products of the first one, then - behind the only barrier, when the next
-// buffer has arrived and this one is read - the next step's Q and first half during the products of the second.
+// A step: three quarters of P are read during the products of the first quarter; then - behind the only barrier, when the next buffer has
+// arrived and this one is read - the next step's Q and first quarter are read, and the step after it is loaded, during the products of the
+// others.  The order of the instructions is the one written here: one of these beside every product or two.  (Left to the compiler's scheduler, reads stood
+// together and products waited for them: bf16 8192^3 999 us.)
 // A last step of less than 128 bytes of k goes through registers, with zeros behind the end.
 
 template <typename T> struct Frag { uint4_t c[2]; };                      // 64 bytes of k of a row: two pieces of a lane
@@ -595,36 +597,31 @@ template <typename T, bool ACROSS> struct Wide {
             off = (lane & 1) * (uint32_t)ld_bytes + (lane >> 1) * 16;
         }
     }
-    __device__ __forceinline__ void load(uint4_t* lds) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            __builtin_amdgcn_global_load_lds((global_word*)(base + i * load_bytes + off), (lds_word*)(lds + (wave + 4 * i) * kLoad), 16, 0, 0);
-        base += step_bytes;
+    // Load instruction i of a step.  (In assembly, since the compiler would have every transposing read wait for all loads.  It has no
+    // output in registers; arrived() waits for it.)
+    __device__ __forceinline__ void load(uint4_t* lds, int i) const {
+        const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_word*)(lds + (wave + 4 * i) * kLoad));
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base + i * load_bytes), "s"(to) : "memory");
     }
-    __device__ __forceinline__ void load_last(uint4_t* lds, int left) {
+    __device__ __forceinline__ void load_last(uint4_t* lds, int left) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             lds[(wave + 4 * i) * kLoad + lane] = load16_upto((const T*)(base + i * load_bytes + off), ACROSS ? (at + 8 * i < left ? kElems : 0) : left - at);
     }
-    // rows `row` .. + 15 of the tile as an operand of the matrix instructions
-    __device__ __forceinline__ Frag<T> read(const uint4_t* lds, int row) const {
-        Frag<T> f;
+    // half h of rows `row` .. + 15 of the tile as an operand of the matrix instructions
+    __device__ __forceinline__ void read(Frag<T>& f, const uint4_t* lds, int row, int h) const {
         if constexpr (!ACROSS) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) f.c[h] = lds[(row + li) * 8 + ((4 * h + lg) ^ (li & 7))];
+            f.c[h] = lds[(row + li) * 8 + ((4 * h + lg) ^ (li & 7))];
         } else {
             // 16 lanes read 16 rows of four k, lane 4 r + s rows 4 s .. of the r-th, and receive four k of a row each
             const char* src = (const char*)lds + (4 * lg + (li >> 3)) * (kLoad * 16) + (li & 2) * 16 + (li >> 2 & 1) * 16 + (li & 1) * 8;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const uint2_t v = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(src + (16 * h + 2 * t) * (kLoad * 16) + row * 4)));
-                    f.c[h][2 * t] = v[0];
-                    f.c[h][2 * t + 1] = v[1];
-                }
+            for (int t = 0; t < 2; ++t) {
+                const uint2_t v = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(src + (16 * h + 2 * t) * (kLoad * 16) + row * 4)));
+                f.c[h][2 * t] = v[0];
+                f.c[h][2 * t + 1] = v[1];
+            }
         }
-        return f;
     }
 };
 
@@ -651,23 +648,19 @@ wide_kernel(Product g) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[i][j] = Acc{0, 0, 0, 0};
 
-    auto read_q = [&](const uint4_t* s, F (&q)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = Q.read(s, row_q + j * 16);
+    constexpr int ROW = std::is_same_v<T, e4m3_t> ? 8 : 16;              // products of a row of instructions: eight, or twice eight
+    F p[8], q0[8], q1[8];
+    auto product = [&](int n, const F (&q)[8]) {                          // the n-th of a step
+        const int i = n / ROW, h = n % ROW / 8, j = n % 8;
+        add_product<T>(acc[i][j], q[j], p[i], h);
     };
-    auto read_p = [&](const uint4_t* s, F (&p)[4], int half) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = P.read(s, row_p + half * 64 + i * 16);
-    };
-    auto multiply = [&](const F (&p)[4], const F (&q)[8], int half) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int h = 0; h < (std::is_same_v<T, e4m3_t> ? 1 : 2); ++h)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) add_product<T>(acc[4 * half + i][j], q[j], p[i], h);
+    auto read_p = [&](const uint4_t* s, int n) { P.read(p[n / 2], s, row_p + n / 2 * 16, n % 2); };
+    auto read_q = [&](const uint4_t* s, F (&q)[8], int n) { Q.read(q[n / 2], s, row_q + n / 2 * 16, n % 2); };
+    auto load = [&](uint4_t* sp, uint4_t* sq, int n) {
+        if (n < 8) P.load(sp, n); else Q.load(sq, n - 8);
     };
     auto arrived = [] {
+        asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0x70);             // loads and LDS: none under way
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -675,52 +668,70 @@ wide_kernel(Product g) {
 
     const int64_t length = k_last > k_first ? k_last - k_first : 0, steps = length / KS;
     const int left = (int)(length - steps * KS);
-    F q0[8], q1[8], p0[4], p1[4];
+    const char *const p_first = P.base, *const q_first = Q.base;
+    auto go_to = [&](int64_t s) {
+        P.base = p_first + s * P.step_bytes;
+        Q.base = q_first + s * Q.step_bytes;
+    };
     if (steps > 0) {
-        P.load(s_p0);
-        Q.load(s_q0);
+        // (a load past the last step loads that one again, where nobody reads it)
+        auto both = [&](uint4_t* sp, uint4_t* sq) {
+#pragma unroll
+            for (int n = 0; n < 16; ++n) load(sp, sq, n);
+        };
+        both(s_p0, s_q0);
         arrived();
-        if (steps > 1) {
-            P.load(s_p1);
-            Q.load(s_q1);
-        }
-        read_q(s_q0, q0);
-        read_p(s_p0, p0, 0);
-        auto step = [&](uint4_t* sp, uint4_t* sq, const uint4_t* next_p, const uint4_t* next_q, F (&q)[8], F (&next)[8], bool more, bool further) {
-            read_p(sp, p1, 1);
-            multiply(p0, q, 0);
+        go_to(min((int64_t)1, steps - 1));
+        both(s_p1, s_q1);
+        go_to(min((int64_t)2, steps - 1));
+#pragma unroll
+        for (int n = 0; n < 16; ++n) read_q(s_q0, q0, n);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) read_p(s_p0, n);
+        auto step = [&](int64_t s, uint4_t* sp, uint4_t* sq, const uint4_t* next_p, const uint4_t* next_q, const F (&q)[8], F (&next)[8]) {
+#pragma unroll
+            for (int n = 0; n < 2 * ROW; ++n) {
+                product(n, q);
+                if (n % (ROW / 8) == 0 && n / (ROW / 8) < 12) read_p(sp, 4 + n / (ROW / 8));
+                __builtin_amdgcn_sched_barrier(0);
+            }
             arrived();
-            if (further) {
-                P.load(sp);
-                Q.load(sq);
+#pragma unroll
+            for (int n = 0; n < 6 * ROW; ++n) {
+                product(2 * ROW + n, q);
+                if (n % (ROW / 8) == 0 && n / (ROW / 8) < 16) load(sp, sq, n / (ROW / 8));
+                if (n % (ROW / 4) == 1) {
+                    const int r = n / (ROW / 4);
+                    if (r < 16) read_q(next_q, next, r);
+                    else if (r < 20) read_p(next_p, r - 16);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (more) {
-                read_q(next_q, next);
-                read_p(next_p, p0, 0);
+            if (s + 3 < steps) {
+                P.base += P.step_bytes;
+                Q.base += Q.step_bytes;
             }
-            multiply(p1, q, 1);
         };
         int64_t s = 0;
-        for (; s + 3 < steps; s += 2) {
-            step(s_p0, s_q0, s_p1, s_q1, q0, q1, true, true);
-            step(s_p1, s_q1, s_p0, s_q0, q1, q0, true, true);
+        for (; s + 1 < steps; s += 2) {
+            step(s, s_p0, s_q0, s_p1, s_q1, q0, q1);
+            step(s + 1, s_p1, s_q1, s_p0, s_q0, q1, q0);
         }
-        for (; s < steps; s += 2) {
-            step(s_p0, s_q0, s_p1, s_q1, q0, q1, s + 1 < steps, s + 2 < steps);
-            if (s + 1 < steps) step(s_p1, s_q1, s_p0, s_q0, q1, q0, s + 2 < steps, s + 3 < steps);
-        }
+        if (s < steps) step(s, s_p0, s_q0, s_p1, s_q1, q0, q1);
+        arrived();
     }
     if (left > 0) {
-        __syncthreads();
+        go_to(steps);
         P.load_last(s_p0, left);
         Q.load_last(s_q0, left);
         __syncthreads();
-        read_q(s_q0, q0);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            read_p(s_p0, p0, half);
-            multiply(p0, q0, half);
+        for (int n = 0; n < 16; ++n) {
+            read_q(s_q0, q0, n);
+            read_p(s_p0, n);
         }
+#pragma unroll
+        for (int n = 0; n < 8 * ROW; ++n) product(n, q0);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) settle(acc[i]);
