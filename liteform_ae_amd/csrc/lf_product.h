@@ -265,120 +265,134 @@ __device__ __forceinline__ float dot_f32(const float* p, int64_t p_step, const f
 
 // What a wavefront does with its WC columns of sums from (m, n) on: partial ones go to the work space, others through the epilogue.
 // They pass through its part of LDS (`lds`, room for PR rows), from the matrix instructions' order into rows, so that the
-// residual is read and the output written in whole lines, by a loop that is compiled once and has the loads of four
-// rows under way.  float32: `again(row, column)` computes an output from the operands.
+// residual is read and the output written in whole lines.  The residual of PR rows is under way while their sums are turned and activated: one
+// after the other, its pieces would wait for memory each (bf16 8192^3, four rows at a time: 889 us).  Wavefronts at the last
+// columns, with pieces of less than eight, take them one by one.
+// float32: `again(row, column)` computes an output from the operands.
 struct None {};
 template <int FM, int FN, int PR, typename Acc, typename Again>
 __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN], uint4_t* lds, int64_t m, int64_t n, Again again) {
-    using S = std::conditional_t<std::is_same_v<Acc, int4v>, int32_t, float>;
-    constexpr int WC = 16 * FN, LANES = WC / 8, AT_ONCE = 64 / LANES, U = PR / AT_ONCE < 4 ? PR / AT_ONCE : 4;
-    static_assert(FM * 16 % PR == 0 && PR % AT_ONCE == 0, "");
+    constexpr int WC = 16 * FN, LANES = WC / 8, AT_ONCE = 64 / LANES, U = PR / AT_ONCE, PHASES = FM * 16 / PR;
+    constexpr bool INT = std::is_same_v<Acc, int4v>;
+    static_assert(FM * 16 % PR == 0 && PR % AT_ONCE == 0 && PHASES <= 4, "");
     const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
     const int mine = lane / LANES, piece = lane % LANES;
     n += piece * 8;
     const int count = (int)max((int64_t)0, min((int64_t)8, g.n - n));
     const Epilogue& e = g.e;
+    const bool whole = __all(count == 0 || count == 8) && !g.part;
     float8_t bias = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, ws = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
     if (!g.part && count) {
         if (e.bias) bias = load_upto8(e.bias, n, e.bias_dtype, count);
         if (e.w_scale) ws = load_upto8(e.w_scale + n, count);
     }
+    auto place = [&](int row, int h) { return lds + row * (WC / 4) + ((2 * piece + h) ^ (row & 7)); };
+    auto sums = [&](int row) {
+        const uint4_t a = *place(row, 0), b = *place(row, 1);
+        const uint32_t w[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        float8_t v;
 #pragma unroll
-    for (int first = 0; first < FM * 16; first += PR) {
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+        return v;
+    };
+    auto phase = [&](auto number) {
+        constexpr int FIRST = decltype(number)::value * PR;
+        const int64_t top = m + FIRST + mine;                                     // the lane's first row
+        uint4_t raw[U][2];
+        if (whole && e.res && count) {
+            const int size = e.res_dtype == LF_DTYPE_F32 ? 4 : 2;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const char* src = (const char*)e.res + (min(top + u * AT_ONCE, g.m - 1) * e.ld_res + n) * size;
+                raw[u][0] = load16((const uint16_t*)src);
+                if (size == 4) raw[u][1] = load16((const uint16_t*)src + 8);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < PR / 16; ++i)
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
                 const int row = 16 * i + li, c = 4 * j + lg;
-                lds[row * (WC / 4) + (c ^ (row & 7))] = __builtin_bit_cast(uint4_t, acc[first / 16 + i][j]);
+                lds[row * (WC / 4) + (c ^ (row & 7))] = __builtin_bit_cast(uint4_t, acc[FIRST / 16 + i][j]);
             }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if constexpr (!std::is_same_v<Again, None>) {
 #pragma unroll 1
-            for (int row = mine; row < PR && m + first + row < g.m; row += AT_ONCE) {
+            for (int row = mine; row < PR && m + FIRST + row < g.m; row += AT_ONCE) {
+                const float8_t v = sums(row);
                 bool fine = true;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) fine = fine && fabsf(__uint_as_float(lds[row * (WC / 4) + ((2 * piece + h) ^ (row & 7))][i])) < __builtin_inff();
+                for (int i = 0; i < 8; ++i) fine = fine && fabsf(v[i]) < __builtin_inff();
                 if (!fine)
 #pragma unroll 1
                     for (int i = 0; i < count; ++i) {
-                        float* s = (float*)(lds + row * (WC / 4) + ((2 * piece + (i >> 2)) ^ (row & 7))) + (i & 3);
-                        if (!(fabsf(*s) < __builtin_inff())) *s = again(m + first + row, n + i);
+                        float* s = (float*)place(row, i >> 2) + (i & 3);
+                        if (!(fabsf(*s) < __builtin_inff())) *s = again(m + FIRST + row, n + i);
                     }
             }
         }
-#pragma unroll 1
-        for (int r0 = mine; r0 < PR; r0 += U * AT_ONCE) {
-            const int64_t top = m + first + r0;
-            float8_t v[U], res[U];
-            float xs[U];
+        if (g.part) {
+#pragma unroll 2
+            for (int row = mine; row < PR; row += AT_ONCE)
+                if (m + FIRST + row < g.m && count) store_upto8((float*)g.part + ((int64_t)blockIdx.y * g.m + m + FIRST + row) * g.n + n, sums(row), count);
+        } else if (whole) {
+            // a lane's own places of LDS: sums -> outputs without the residual
+            if (INT || e.x_scale || e.bias || e.z || e.act != LF_ACT_NONE)
+#pragma unroll 2
+                for (int row = mine; row < PR; row += AT_ONCE) {
+                    const int64_t at = min(m + FIRST + row, g.m - 1);
+                    float8_t v = sums(row);
+                    if constexpr (INT)
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int row = r0 + u * AT_ONCE;
-                S s[8];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint4_t w = lds[row * (WC / 4) + ((2 * piece + h) ^ (row & 7))];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t word = w[i];             // (bit_cast of an element takes the first one)
-                        s[4 * h + i] = __builtin_bit_cast(S, word);
-                    }
+                        for (int i = 0; i < 8; ++i) v[i] = (float)__float_as_int(v[i]);
+                    if (e.x_scale) v = v * e.x_scale[at] * ws;
+                    v += bias;
+                    if (e.z && m + FIRST + row < g.m && count) store_upto8(e.z, at * e.ld_z + n, e.z_dtype, v, 8);
+                    if (e.act != LF_ACT_NONE) v = activate(v, e.act);
+                    *place(row, 0) = __builtin_bit_cast(uint4_t, float4_t{v[0], v[1], v[2], v[3]});
+                    *place(row, 1) = __builtin_bit_cast(uint4_t, float4_t{v[4], v[5], v[6], v[7]});
                 }
-                if (std::is_same_v<S, int32_t> && g.part) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[u][i] = __builtin_bit_cast(float, s[i]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[u][i] = (float)s[i];
-                }
-            }
-            if (g.part) {
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (top + u * AT_ONCE < g.m && count) store_upto8((float*)g.part + ((int64_t)blockIdx.y * g.m + top + u * AT_ONCE) * g.n + n, v[u], count);
-                continue;
-            }
+            float8_t v[U];
             if (e.res)
                 with_type(e.res_dtype, [&](auto t) {
                     using R = decltype(t);
-                    typename Eight<R>::vec raw[U];
 #pragma unroll
-                    for (int u = 0; u < U; ++u) raw[u] = raw_upto8((const R*)e.res + min(top + u * AT_ONCE, g.m - 1) * e.ld_res + n, count);
-#pragma unroll
-                    for (int u = 0; u < U; ++u) res[u] = __builtin_convertvector(raw[u], float8_t);
+                    for (int u = 0; u < U; ++u) {
+                        if constexpr (sizeof(R) == 4) {
+                            const float4_t a = __builtin_bit_cast(float4_t, raw[u][0]), b = __builtin_bit_cast(float4_t, raw[u][1]);
+                            v[u] = float8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                        } else {
+                            v[u] = __builtin_convertvector(__builtin_bit_cast(typename Eight<R>::vec, raw[u][0]), float8_t);
+                        }
+                    }
                 });
-            if (e.x_scale) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) xs[u] = e.x_scale[min(top + u * AT_ONCE, g.m - 1)];
+            for (int u = 0; u < U; ++u) v[u] = e.res ? sums(mine + u * AT_ONCE) + v[u] : sums(mine + u * AT_ONCE);
+            if (count)
+                with_type(e.y_dtype, [&](auto t) {
+                    using Y = decltype(t);
 #pragma unroll
-                for (int u = 0; u < U; ++u) v[u] = v[u] * xs[u] * ws;
+                    for (int u = 0; u < U; ++u)
+                        if (top + u * AT_ONCE < g.m) store8((Y*)e.y + (top + u * AT_ONCE) * e.ld_y + n, v[u]);
+                });
+        } else {
+#pragma unroll 1
+            for (int row = mine; row < PR; row += AT_ONCE) {
+                float8_t v = sums(row);
+                if constexpr (INT)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = (float)__float_as_int(v[i]);
+                if (m + FIRST + row < g.m && count) finish(e, m + FIRST + row, n, count, v);
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) v[u] += bias;
-            if (e.z) {
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (top + u * AT_ONCE < g.m && count) store_upto8(e.z, (top + u * AT_ONCE) * e.ld_z + n, e.z_dtype, v[u], count);
-            }
-            if (e.act != LF_ACT_NONE) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) v[u] = activate(v[u], e.act);
-            }
-            if (e.res) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) v[u] += res[u];
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (top + u * AT_ONCE < g.m && count) store_upto8(e.y, (top + u * AT_ONCE) * e.ld_y + n, e.y_dtype, v[u], count);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-    }
+    };
+    phase(std::integral_constant<int, 0>{});
+    if constexpr (PHASES > 1) phase(std::integral_constant<int, 1>{});
+    if constexpr (PHASES > 2) phase(std::integral_constant<int, 2>{});
+    if constexpr (PHASES > 3) phase(std::integral_constant<int, 3>{});
 }
 
 // The tile of a workgroup.  Workgroups go to the eight XCDs in turn: each XCD gets a run of neighbouring tiles, eight rows of
