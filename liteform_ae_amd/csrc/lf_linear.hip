@@ -201,10 +201,10 @@ template <int WAVES> ProductFn few_rows_of(int32_t dtype) {
 
 constexpr int64_t kFewRows = 16;
 
-// Whether the kernel for large tiles may read the operands: a whole tile, 16-byte pieces that are aligned (across k whole ones, too), a
-// load instruction's eight rows within 32-bit offsets.
+// Whether the kernel for large tiles may read the operands: a whole tile, 16-byte pieces that are aligned (across k whole ones, too), the
+// rows of a tile within 32-bit offsets.
 bool wide_operand(const void* p, int64_t ld, int64_t rows, bool across, int bytes) {
-    return rows >= 256 && (uintptr_t)p % 16 == 0 && ld * bytes % 16 == 0 && 8 * ld * bytes < (1ll << 31) && (!across || rows % 8 == 0);
+    return rows >= 256 && (uintptr_t)p % 16 == 0 && ld * bytes % 16 == 0 && (across ? 64 : 256) * ld * bytes < (1ll << 31) && (!across || rows % 8 == 0);
 }
 bool wide_operands(const Product& g, int32_t dtype, bool px, bool qx) {
     return wide_operand(g.p, g.ld_p, g.m, px, dtype_bytes(dtype)) && wide_operand(g.q, g.ld_q, g.n, qx, dtype_bytes(dtype));

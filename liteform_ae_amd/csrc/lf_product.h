@@ -575,17 +575,17 @@ template <typename Acc> __device__ __forceinline__ void settle(Acc (&c)[8]) {
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4_t lds_short4;
 typedef __attribute__((address_space(3))) uint32_t lds_word;
-typedef const __attribute__((address_space(1))) uint32_t global_word;
+template <int N> __device__ __forceinline__ uint32_t lds_address(uint4_t (&s)[N]) { return (uint32_t)(uintptr_t)(lds_word*)&s[0]; }
 
 // One operand's tile of 256 x (a step of k) on its way from memory to the matrix instructions.
 template <typename T, bool ACROSS> struct Wide {
     static constexpr int kStep = 128 / sizeof(T), kElems = 16 / sizeof(T);
     // LDS slots from a wavefront's load instruction to the next: across, 64 bytes more than two k, so that four k lie in different banks
     static constexpr int kLoad = ACROSS ? 68 : 64, kSlots = 32 * kLoad;
-    const char* base;                  // of what a wavefront's first load instruction reads next
-    int64_t step_bytes, load_bytes;    // from step to step, from a load instruction to the next
-    uint32_t off;                      // from there to what this lane reads
-    int at;                            // element of k (along), k (across) of that
+    const char* base;                  // of the tile at the step that is loaded next
+    int64_t step_bytes;                // from step to step
+    uint32_t off[8];                   // bytes from there to what this lane reads by the eight load instructions of its wavefront
+    int at;                            // element of k (along), k (across) of the first one
     int wave, lane, li, lg;
 
     // A load instruction reads eight rows (along) or two k (across); the wavefronts take them in turn.  Along, piece c of row r stands at
@@ -595,32 +595,33 @@ template <typename T, bool ACROSS> struct Wide {
         li = lane & 15;
         lg = lane >> 4;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const int64_t ld_bytes = ld * sizeof(T);
+        const uint32_t ld_bytes = (uint32_t)(ld * sizeof(T));
+        uint32_t first;
         if constexpr (!ACROSS) {
-            base = (const char*)p + (row0 + 8 * wave) * ld_bytes + k0 * sizeof(T);
+            base = (const char*)p + (row0 * ld + k0) * sizeof(T);
             step_bytes = 128;
-            load_bytes = 32 * ld_bytes;
             const int c = (lane & 7) ^ (lane >> 3);
-            off = (lane >> 3) * (uint32_t)ld_bytes + c * 16;
+            first = (8 * wave + (lane >> 3)) * ld_bytes + c * 16;
             at = c * kElems;
         } else {
-            base = (const char*)p + (k0 + 2 * wave) * ld_bytes + row0 * sizeof(T);
-            step_bytes = kStep * ld_bytes;
-            load_bytes = 8 * ld_bytes;
+            base = (const char*)p + (k0 * ld + row0) * sizeof(T);
+            step_bytes = kStep * ld * sizeof(T);
             at = 2 * wave + (lane & 1);
-            off = (lane & 1) * (uint32_t)ld_bytes + (lane >> 1) * 16;
+            first = at * ld_bytes + (lane >> 1) * 16;
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) off[i] = first + i * (ACROSS ? 8 : 32) * ld_bytes;
     }
-    // Load instruction i of a step.  (In assembly, since the compiler would have every transposing read wait for all loads.  It has no
-    // output in registers; arrived() waits for it.)
-    __device__ __forceinline__ void load(uint4_t* lds, int i) const {
-        const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_word*)(lds + (wave + 4 * i) * kLoad));
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base + i * load_bytes), "s"(to) : "memory");
+    // Load instruction i of a step, into the array of LDS that begins at `lds`.  (In assembly, since the compiler would have every transposing
+    // read wait for all loads.  It has no output in registers; arrived() waits for it.)
+    __device__ __forceinline__ void load(uint32_t lds, int i) const {
+        asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[i]), "s"(base), "s"(wave * (kLoad * 16)), "s"(lds + i * (4 * kLoad * 16))
+                     : "memory", "scc");
     }
     __device__ __forceinline__ void load_last(uint4_t* lds, int left) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            lds[(wave + 4 * i) * kLoad + lane] = load16_upto((const T*)(base + i * load_bytes + off), ACROSS ? (at + 8 * i < left ? kElems : 0) : left - at);
+            lds[(wave + 4 * i) * kLoad + lane] = load16_upto((const T*)(base + off[i]), ACROSS ? (at + 8 * i < left ? kElems : 0) : left - at);
     }
     // half h of rows `row` .. + 15 of the tile as an operand of the matrix instructions
     __device__ __forceinline__ void read(Frag<T>& f, const uint4_t* lds, int row, int h) const {
@@ -670,9 +671,10 @@ wide_kernel(Product g) {
     };
     auto read_p = [&](const uint4_t* s, int n) { P.read(p[n / 2], s, row_p + n / 2 * 16, n % 2); };
     auto read_q = [&](const uint4_t* s, F (&q)[8], int n) { Q.read(q[n / 2], s, row_q + n / 2 * 16, n % 2); };
-    auto load = [&](uint4_t* sp, uint4_t* sq, int n) {
+    auto load = [&](uint32_t sp, uint32_t sq, int n) {
         if (n < 8) P.load(sp, n); else Q.load(sq, n - 8);
     };
+    const uint32_t at_p0 = lds_address(s_p0), at_q0 = lds_address(s_q0), at_p1 = lds_address(s_p1), at_q1 = lds_address(s_q1);
     auto arrived = [] {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0x70);             // loads and LDS: none under way
@@ -689,20 +691,20 @@ wide_kernel(Product g) {
     };
     if (steps > 0) {
         // (a load past the last step loads that one again, where nobody reads it)
-        auto both = [&](uint4_t* sp, uint4_t* sq) {
+        auto both = [&](uint32_t sp, uint32_t sq) {
 #pragma unroll
             for (int n = 0; n < 16; ++n) load(sp, sq, n);
         };
-        both(s_p0, s_q0);
+        both(at_p0, at_q0);
         arrived();
         go_to(min((int64_t)1, steps - 1));
-        both(s_p1, s_q1);
+        both(at_p1, at_q1);
         go_to(min((int64_t)2, steps - 1));
 #pragma unroll
         for (int n = 0; n < 16; ++n) read_q(s_q0, q0, n);
 #pragma unroll
         for (int n = 0; n < 4; ++n) read_p(s_p0, n);
-        auto step = [&](int64_t s, uint4_t* sp, uint4_t* sq, const uint4_t* next_p, const uint4_t* next_q, const F (&q)[8], F (&next)[8]) {
+        auto step = [&](int64_t s, const uint4_t* sp, uint32_t at_p, uint32_t at_q, const uint4_t* next_p, const uint4_t* next_q, const F (&q)[8], F (&next)[8]) {
 #pragma unroll
             for (int n = 0; n < 2 * ROW; ++n) {
                 product(n, q);
@@ -713,7 +715,7 @@ wide_kernel(Product g) {
 #pragma unroll
             for (int n = 0; n < 6 * ROW; ++n) {
                 product(2 * ROW + n, q);
-                if (n % (ROW / 8) == 0 && n / (ROW / 8) < 16) load(sp, sq, n / (ROW / 8));
+                if (n % (ROW / 8) == 0 && n / (ROW / 8) < 16) load(at_p, at_q, n / (ROW / 8));
                 if (n % (ROW / 4) == 1) {
                     const int r = n / (ROW / 4);
                     if (r < 16) read_q(next_q, next, r);
@@ -728,10 +730,10 @@ wide_kernel(Product g) {
         };
         int64_t s = 0;
         for (; s + 1 < steps; s += 2) {
-            step(s, s_p0, s_q0, s_p1, s_q1, q0, q1);
-            step(s + 1, s_p1, s_q1, s_p0, s_q0, q1, q0);
+            step(s, s_p0, at_p0, at_q0, s_p1, s_q1, q0, q1);
+            step(s + 1, s_p1, at_p1, at_q1, s_p0, s_q0, q1, q0);
         }
-        if (s < steps) step(s, s_p0, s_q0, s_p1, s_q1, q0, q1);
+        if (s < steps) step(s, s_p0, at_p0, at_q0, s_p1, s_q1, q0, q1);
         arrived();
     }
     if (left > 0) {
