@@ -265,10 +265,22 @@ __device__ __forceinline__ float dot_f32(const float* p, int64_t p_step, const f
 
 // What a wavefront does with its WC columns of sums from (m, n) on: partial ones go to the work space, others through the epilogue.
 // They pass through its part of LDS (`lds`, room for PR rows), from the matrix instructions' order into rows, so that the
-// residual is read and the output written in whole lines.  The residual of PR rows is under way while their sums are turned and activated: one
-// after the other, its pieces would wait for memory each (bf16 8192^3, four rows at a time: 889 us).  Wavefronts at the last
+// residual is read and the output written in whole lines.  The residual of PR rows is under way while their sums are turned: one after the
+// other, its pieces would wait for memory each (bf16 8192^3, four rows at a time: 889 us).  Wavefronts at the last
 // columns, with pieces of less than eight, take them one by one.
 // float32: `again(row, column)` computes an output from the operands.
+template <int N> __device__ __forceinline__ void activate_all(float8_t (&v)[N], int32_t act) {
+    if (act == LF_ACT_RELU) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[u] = activate(v[u], LF_ACT_RELU);
+    } else if (act == LF_ACT_GELU) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[u] = activate(v[u], LF_ACT_GELU);
+    } else if (act == LF_ACT_SILU) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[u] = activate(v[u], LF_ACT_SILU);
+    }
+}
 struct None {};
 template <int FM, int FN, int PR, typename Acc, typename Again>
 __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN], uint4_t* lds, int64_t m, int64_t n, Again again) {
@@ -299,6 +311,7 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
         constexpr int FIRST = decltype(number)::value * PR;
         const int64_t top = m + FIRST + mine;                                     // the lane's first row
         uint4_t raw[U][2];
+        const float xs = e.x_scale && whole ? e.x_scale[min(m + FIRST + lane, g.m - 1)] : 1.f;      // (of row `lane`)
         if (whole && e.res && count) {
             const int size = e.res_dtype == LF_DTYPE_F32 ? 4 : 2;
 #pragma unroll
@@ -337,45 +350,61 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
             for (int row = mine; row < PR; row += AT_ONCE)
                 if (m + FIRST + row < g.m && count) store_upto8((float*)g.part + ((int64_t)blockIdx.y * g.m + m + FIRST + row) * g.n + n, sums(row), count);
         } else if (whole) {
-            // a lane's own places of LDS: sums -> outputs without the residual
-            if (INT || e.x_scale || e.bias || e.z || e.act != LF_ACT_NONE)
-#pragma unroll 2
-                for (int row = mine; row < PR; row += AT_ONCE) {
-                    const int64_t at = min(m + FIRST + row, g.m - 1);
-                    float8_t v = sums(row);
-                    if constexpr (INT)
+            // What follows the sums and comes before the residual, in a lane's own places of LDS: a loop, since its code is long and would be read
+            // from memory for every tile if it stood there sixteen times (gelu: 44 us of the 285 of an e4m3 product of 16k x 4k x 4k, 25 as a loop)
+            constexpr int H = U < 4 ? U : 4;
+            const bool first_pass = INT || e.x_scale || e.z || e.act != LF_ACT_NONE;
+            if (first_pass)
+#pragma unroll 1
+                for (int r0 = mine; r0 < PR; r0 += H * AT_ONCE) {
+                    float8_t v[H];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = (float)__float_as_int(v[i]);
-                    if (e.x_scale) v = v * e.x_scale[at] * ws;
-                    v += bias;
-                    if (e.z && m + FIRST + row < g.m && count) store_upto8(e.z, at * e.ld_z + n, e.z_dtype, v, 8);
-                    if (e.act != LF_ACT_NONE) v = activate(v, e.act);
-                    *place(row, 0) = __builtin_bit_cast(uint4_t, float4_t{v[0], v[1], v[2], v[3]});
-                    *place(row, 1) = __builtin_bit_cast(uint4_t, float4_t{v[4], v[5], v[6], v[7]});
-                }
-            float8_t v[U];
-            if (e.res)
-                with_type(e.res_dtype, [&](auto t) {
-                    using R = decltype(t);
+                    for (int u = 0; u < H; ++u) {
+                        v[u] = sums(r0 + u * AT_ONCE);
+                        if constexpr (INT)
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        if constexpr (sizeof(R) == 4) {
-                            const float4_t a = __builtin_bit_cast(float4_t, raw[u][0]), b = __builtin_bit_cast(float4_t, raw[u][1]);
-                            v[u] = float8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-                        } else {
-                            v[u] = __builtin_convertvector(__builtin_bit_cast(typename Eight<R>::vec, raw[u][0]), float8_t);
-                        }
+                            for (int i = 0; i < 8; ++i) v[u][i] = (float)__float_as_int(v[u][i]);
+                        if (e.x_scale) v[u] = v[u] * __shfl(xs, r0 + u * AT_ONCE) * ws;
+                        v[u] += bias;
+                        const int64_t row = m + FIRST + r0 + u * AT_ONCE;
+                        if (e.z && row < g.m && count) store_upto8(e.z, row * e.ld_z + n, e.z_dtype, v[u], 8);
                     }
-                });
+                    activate_all(v, e.act);
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = e.res ? sums(mine + u * AT_ONCE) + v[u] : sums(mine + u * AT_ONCE);
-            if (count)
-                with_type(e.y_dtype, [&](auto t) {
-                    using Y = decltype(t);
+                    for (int u = 0; u < H; ++u) {
+                        *place(r0 + u * AT_ONCE, 0) = __builtin_bit_cast(uint4_t, float4_t{v[u][0], v[u][1], v[u][2], v[u][3]});
+                        *place(r0 + u * AT_ONCE, 1) = __builtin_bit_cast(uint4_t, float4_t{v[u][4], v[u][5], v[u][6], v[u][7]});
+                    }
+                }
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (top + u * AT_ONCE < g.m) store8((Y*)e.y + (top + u * AT_ONCE) * e.ld_y + n, v[u]);
-                });
+            for (int u0 = 0; u0 < U; u0 += H) {
+                float8_t v[H];
+#pragma unroll
+                for (int u = 0; u < H; ++u) {
+                    v[u] = sums(mine + (u0 + u) * AT_ONCE);
+                    if (!first_pass) v[u] += bias;
+                }
+                if (e.res)
+                    with_type(e.res_dtype, [&](auto t) {
+                        using R = decltype(t);
+#pragma unroll
+                        for (int u = 0; u < H; ++u) {
+                            if constexpr (sizeof(R) == 4) {
+                                const float4_t a = __builtin_bit_cast(float4_t, raw[u0 + u][0]), b = __builtin_bit_cast(float4_t, raw[u0 + u][1]);
+                                v[u] += float8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                            } else {
+                                v[u] += __builtin_convertvector(__builtin_bit_cast(typename Eight<R>::vec, raw[u0 + u][0]), float8_t);
+                            }
+                        }
+                    });
+                if (count)
+                    with_type(e.y_dtype, [&](auto t) {
+                        using Y = decltype(t);
+#pragma unroll
+                        for (int u = 0; u < H; ++u)
+                            if (top + (u0 + u) * AT_ONCE < g.m) store8((Y*)e.y + (top + (u0 + u) * AT_ONCE) * e.ld_y + n, v[u]);
+                    });
+            }
         } else {
 #pragma unroll 1
             for (int row = mine; row < PR; row += AT_ONCE) {
@@ -524,8 +553,8 @@ product_kernel(Product g) {
 
     // (the last step is behind a barrier: LDS is free)
     constexpr int SLOTS = NB * PL * (StageP::kSlots + StageQ::kSlots) / (WM * WN), WHOLE = FM * 16, FIT = SLOTS / (FN * 4);
-    constexpr int PR = FIT >= WHOLE ? WHOLE : FIT >= WHOLE / 2 ? WHOLE / 2 : WHOLE / 4;
-    static_assert(PR <= FIT && PR % 16 == 0, "");
+    constexpr int PR = 32;                       // (64 would take the registers of the CU's second workgroup)
+    static_assert(PR <= FIT && WHOLE % PR == 0, "");
     uint4_t* mine = s_all + wave * SLOTS;
     const int64_t m = m0 + wm * (TM / WM), n = n0 + wn * (TN / WN);
     if constexpr (PL == 3)
