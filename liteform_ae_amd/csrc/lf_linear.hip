@@ -46,10 +46,10 @@ __global__ void __launch_bounds__(256) join_kernel(const A* part, int64_t m, int
     finish(e, row, col, count, v);
 }
 template <typename A> int launch_join(const Product& g, hipStream_t st) {
-    const int slices = g.splits <= 4 ? 1 : g.splits <= 32 ? 8 : 32;
+    const int slices = g.splits <= 4 ? 1 : g.splits <= 32 ? 8 : g.splits <= 128 ? 32 : 64;
     const int64_t groups = ceil_div(g.m * ceil_div(g.n, 8), 256 / slices);
     LF_REQUIRE(groups < (1ll << 31), LF_ERR_UNSUPPORTED, "too many outputs");
-    auto kernel = slices == 1 ? join_kernel<A, 1> : slices == 8 ? join_kernel<A, 8> : join_kernel<A, 32>;
+    auto kernel = slices == 1 ? join_kernel<A, 1> : slices == 8 ? join_kernel<A, 8> : slices == 32 ? join_kernel<A, 32> : join_kernel<A, 64>;
     kernel<<<(unsigned)groups, 256, 0, st>>>((const A*)g.part, g.m, g.n, g.splits, g.e);
     LF_HIP(hipGetLastError());
     return LF_OK;
@@ -129,19 +129,22 @@ few_rows_kernel(Product g) {
 
 // ---------------------------------------------------------------------------- gradient of the activation
 
-// dz = dy act'(z), in rows of `ld_dz` elements, and the column sums of a slab of rows (before rounding).
-template <typename T>
+// dz = dy act'(z), in rows of `ld_dz` elements, and the column sums of a slab of rows (before rounding): ACROSS threads of eight columns
+// each, the others take further rows.
+template <typename T, int ACROSS>
 __global__ void __launch_bounds__(256)
 activation_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* dz, int64_t ld_dz, float* part, int64_t m, int64_t n, int32_t act,
                        int64_t slab) {
-    __shared__ float s[8][32][9];
-    const int lx = threadIdx.x & 31, ly = threadIdx.x >> 5;
-    const int64_t col = ((int64_t)blockIdx.x * 32 + lx) * 8;
+    constexpr int DOWN = 256 / ACROSS;
+    __shared__ float s[DOWN][ACROSS][9];
+    const int lx = threadIdx.x % ACROSS, ly = threadIdx.x / ACROSS;
+    const int64_t col = ((int64_t)blockIdx.x * ACROSS + lx) * 8;
     const int count = (int)min((int64_t)8, n - col);
     const int64_t r1 = min(m, ((int64_t)blockIdx.y + 1) * slab);
     float8_t sum = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (count > 0)
-        for (int64_t r = (int64_t)blockIdx.y * slab + ly; r < r1; r += 8) {
+#pragma unroll 2
+        for (int64_t r = (int64_t)blockIdx.y * slab + ly; r < r1; r += DOWN) {
             float8_t d = load_upto8(dy + r * ld_dy + col, count);
             if (act != LF_ACT_NONE) {
                 const float8_t v = load_upto8(z + r * ld_z + col, count);
@@ -155,11 +158,11 @@ activation_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* 
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[ly][lx][i] = sum[i];
     __syncthreads();
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= n) return;
+    const int64_t c = (int64_t)blockIdx.x * ACROSS * 8 + threadIdx.x;
+    if (threadIdx.x >= ACROSS * 8 || c >= n) return;
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t += s[i][threadIdx.x >> 3][threadIdx.x & 7];
+    for (int i = 0; i < DOWN; ++i) t += s[i][threadIdx.x >> 3][threadIdx.x & 7];
     part[(int64_t)blockIdx.y * n + c] = t;
 }
 
@@ -171,22 +174,23 @@ struct Cut { int tile; int splits; int64_t k_split; size_t bytes; };
 Cut cut_product(int32_t dtype, int64_t m, int64_t n, int64_t k) {
     const int step = dtype == LF_DTYPE_F32 ? 32 : 128 / dtype_bytes(dtype);
     auto tiles = [&](int t) { return ceil_div(m, t) * ceil_div(n, t); };
-    const int tile = dtype != LF_DTYPE_F32 && tiles(kWideTile) >= 200 ? kWideTile : tiles(128) >= 200 || (m > 64 && n > 64) ? 128 : 64;
+    const int tile = dtype != LF_DTYPE_F32 && tiles(kWideTile) >= 200 ? kWideTile : tiles(128) >= 200 || (m > 64 && n > 64) ? (getenv("LF_T64") ? 64 : 128) : 64;
     const int64_t t = tiles(tile), steps = ceil_div(k, step);
     int64_t splits = 1;
-    if (t < 200 && steps >= 16) splits = std::min<int64_t>(ceil_div(512, t), steps / 8);
+    const int W_ = getenv("LF_W") ? atoi(getenv("LF_W")) : 512, S_ = getenv("LF_S") ? atoi(getenv("LF_S")) : 8;
+    if (t < 200 && steps >= 16) splits = std::min<int64_t>(ceil_div(W_, t), steps / S_);
     const int64_t each = std::max<int64_t>(1, ceil_div(steps, splits));
     splits = std::max<int64_t>(1, ceil_div(steps, each));
     return {tile, (int)splits, each * step, splits > 1 ? (size_t)splits * (size_t)m * (size_t)n * 4 : 0};
 }
 
-ProductFn product_of(int32_t dtype, bool px, bool qx, int tile) {
+ProductFn product_of(int32_t dtype, bool px, bool qx, int tile, bool aligned) {
     switch (dtype) {
-        case LF_DTYPE_F32: return product_f32(px, qx, tile);
-        case LF_DTYPE_BF16: return product_bf16(px, qx, tile);
-        case LF_DTYPE_F16: return product_f16(px, qx, tile);
-        case LF_DTYPE_E4M3: return product_e4m3(px, qx, tile);
-        default: return product_i8(px, qx, tile);
+        case LF_DTYPE_F32: return product_f32(px, qx, tile, aligned);
+        case LF_DTYPE_BF16: return product_bf16(px, qx, tile, aligned);
+        case LF_DTYPE_F16: return product_f16(px, qx, tile, aligned);
+        case LF_DTYPE_E4M3: return product_e4m3(px, qx, tile, aligned);
+        default: return product_i8(px, qx, tile, aligned);
     }
 }
 template <int WAVES> ProductFn few_rows_of(int32_t dtype) {
@@ -201,13 +205,13 @@ template <int WAVES> ProductFn few_rows_of(int32_t dtype) {
 
 constexpr int64_t kFewRows = 16;
 
-// Whether the kernel for large tiles may read the operands: a whole tile, 16-byte pieces that are aligned (across k whole ones, too), the
-// rows of a tile within 32-bit offsets.
-bool wide_operand(const void* p, int64_t ld, int64_t rows, bool across, int bytes) {
-    return rows >= 256 && (uintptr_t)p % 16 == 0 && ld * bytes % 16 == 0 && (across ? 64 : 256) * ld * bytes < (1ll << 31) && (!across || rows % 8 == 0);
+// Whether an operand can go straight into LDS: pieces of 16 bytes that are aligned (across k whole ones, too), and the rows of a tile within
+// 32-bit offsets.
+bool aligned_operand(const void* p, int64_t ld, int64_t rows, bool across, int bytes) {
+    return (uintptr_t)p % 16 == 0 && ld * bytes % 16 == 0 && (across ? 64 : 256) * ld * bytes < (1ll << 31) && (!across || rows % 8 == 0);
 }
-bool wide_operands(const Product& g, int32_t dtype, bool px, bool qx) {
-    return wide_operand(g.p, g.ld_p, g.m, px, dtype_bytes(dtype)) && wide_operand(g.q, g.ld_q, g.n, qx, dtype_bytes(dtype));
+bool aligned_operands(const Product& g, int32_t dtype, bool px, bool qx) {
+    return aligned_operand(g.p, g.ld_p, g.m, px, dtype_bytes(dtype)) && aligned_operand(g.q, g.ld_q, g.n, qx, dtype_bytes(dtype));
 }
 
 int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipStream_t st) {
@@ -222,7 +226,8 @@ int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipSt
         return LF_OK;
     }
     Cut c = cut_product(dtype, g.m, g.n, g.k);
-    if (c.tile == kWideTile && !wide_operands(g, dtype, px, qx)) c.tile = 128;
+    const bool aligned = dtype != LF_DTYPE_F32 && aligned_operands(g, dtype, px, qx);
+    if (c.tile == kWideTile && !aligned) c.tile = 128;
     const int64_t tm = ceil_div(g.m, c.tile), tn = ceil_div(g.n, c.tile);
     LF_REQUIRE(tm < (1ll << 27) && tn < (1ll << 27) && tm * tn < (1ll << 31), LF_ERR_UNSUPPORTED, "too many tiles");
     g.tiles_m = (int32_t)tm;
@@ -230,7 +235,7 @@ int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipSt
     g.splits = c.splits;
     g.k_split = c.k_split;
     g.part = c.splits > 1 ? work : nullptr;
-    product_of(dtype, px, qx, c.tile)<<<dim3((unsigned)(tm * tn), (unsigned)c.splits), 256, 0, st>>>(g);
+    product_of(dtype, px, qx, c.tile, aligned)<<<dim3((unsigned)(tm * tn), (unsigned)c.splits), 256, 0, st>>>(g);
     LF_HIP(hipGetLastError());
     if (c.splits > 1) {
         LF_TRY(dtype == LF_DTYPE_I8 ? launch_join<int32_t>(g, st) : launch_join<float>(g, st));
@@ -259,8 +264,11 @@ int check_sizes(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act) {
 // Rows of dz are padded to a multiple of 16 bytes.
 int64_t ld_dz(int64_t n) { return ceil_div(n, 8) * 8; }
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
-// Slabs of rows whose column sums are kept apart: enough workgroups to fill the GPU.
-int64_t slabs_of(int64_t m, int64_t n) { return std::max<int64_t>(1, std::min(ceil_div(m, 64), ceil_div(2048, ceil_div(n, 256)))); }
+// Threads across a row (of eight columns each), and slabs of rows whose column sums are kept apart: enough workgroups to fill the GPU.
+int threads_across(int64_t n) { return n <= 64 ? 8 : n <= 128 ? 16 : 32; }
+int64_t slabs_of(int64_t m, int64_t n) {
+    return std::max<int64_t>(1, std::min(ceil_div(m, 64), ceil_div(512, std::min<int64_t>(4, ceil_div(n, 256)))));
+}
 
 struct GradWork { size_t dz, sums, parts, total; };
 GradWork grad_work(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act, bool dx, bool dw, bool db) {
@@ -339,10 +347,12 @@ int lf_linear_grad(const lf_linear_grad_args* h_args, void* d_work, size_t work_
     void* parts = at + w.dz + w.sums;
     const int64_t slabs = slabs_of(a.m, a.n), slab = ceil_div(std::max<int64_t>(a.m, 1), slabs);
     if ((dz || sums) && a.n > 0) {
-        const dim3 grid((unsigned)ceil_div(a.n, 256), (unsigned)slabs);
+        const int across = threads_across(a.n);
+        const dim3 grid((unsigned)ceil_div(a.n, 8 * across), (unsigned)slabs);
         auto go = [&](auto t) {
             using T = decltype(t);
-            activation_grad_kernel<T><<<grid, 256, 0, st>>>((const T*)a.d_dy, a.ld_dy, (const T*)a.d_z, a.ld_z, (T*)dz, ld_dz(a.n), sums, a.m, a.n, a.activation, slab);
+            auto kernel = across == 8 ? activation_grad_kernel<T, 8> : across == 16 ? activation_grad_kernel<T, 16> : activation_grad_kernel<T, 32>;
+            kernel<<<grid, 256, 0, st>>>((const T*)a.d_dy, a.ld_dy, (const T*)a.d_z, a.ld_z, (T*)dz, ld_dz(a.n), sums, a.m, a.n, a.activation, slab);
         };
         if (a.dtype == LF_DTYPE_F32) go(0.f); else if (a.dtype == LF_DTYPE_BF16) go((__bf16)0.f); else go((_Float16)0.f);
         LF_HIP(hipGetLastError());

@@ -51,14 +51,14 @@ struct Product {
 };
 using ProductFn = void (*)(Product);
 
-// The kernel for operands of a type: px, qx: P, Q stored across k; tile: 64 or 128 (any operands), 256 (kWideTile: rows that
-// are 16-byte aligned).
+// The kernel for operands of a type: px, qx: P, Q stored across k; tile: 64, 128 or, aligned and not float32, 256 (kWideTile); aligned: pieces of
+// 16 bytes of the operands are, and across k they are whole.
 constexpr int kWideTile = 256;
-ProductFn product_f32(bool px, bool qx, int tile);
-ProductFn product_bf16(bool px, bool qx, int tile);
-ProductFn product_f16(bool px, bool qx, int tile);
-ProductFn product_e4m3(bool px, bool qx, int tile);
-ProductFn product_i8(bool px, bool qx, int tile);
+ProductFn product_f32(bool px, bool qx, int tile, bool aligned);
+ProductFn product_bf16(bool px, bool qx, int tile, bool aligned);
+ProductFn product_f16(bool px, bool qx, int tile, bool aligned);
+ProductFn product_e4m3(bool px, bool qx, int tile, bool aligned);
+ProductFn product_i8(bool px, bool qx, int tile, bool aligned);
 
 }  // namespace lf
 
@@ -568,7 +568,7 @@ product_kernel(Product g) {
 
 // ---------------------------------------------------------------------------- the tiled product, large tiles
 
-// A tile of 256 x 256 for operands whose rows are 16-byte aligned: four wavefronts of 128 x 128 outputs, which read 32 KB of LDS for
+// A tile of 256 x 256 for operands whose pieces of 16 bytes are aligned: four wavefronts of 128 x 128 outputs, which read 32 KB of LDS for
 // 4 x 2 MB of products a step, half of what eight of 128 x 64 read.  Operands go from memory into LDS without registers in between (64 lanes
 // x 16 bytes to consecutive addresses; the order of the pieces there follows from the addresses they are read from).  Operands across k
 // lie in LDS as they do in memory and are turned by the transposing LDS load.
@@ -606,40 +606,43 @@ typedef __attribute__((address_space(3))) short4_t lds_short4;
 typedef __attribute__((address_space(3))) uint32_t lds_word;
 template <int N> __device__ __forceinline__ uint32_t lds_address(uint4_t (&s)[N]) { return (uint32_t)(uintptr_t)(lds_word*)&s[0]; }
 
-// One operand's tile of 256 x (a step of k) on its way from memory to the matrix instructions.
-template <typename T, bool ACROSS> struct Wide {
+// One operand's tile of ROWS x (a step of k: 128 bytes) on its way from memory to the matrix instructions, for four wavefronts.
+template <typename T, bool ACROSS, int ROWS> struct Direct {
     static constexpr int kStep = 128 / sizeof(T), kElems = 16 / sizeof(T);
-    // LDS slots from a wavefront's load instruction to the next: across, 64 bytes more than two k, so that four k lie in different banks
-    static constexpr int kLoad = ACROSS ? 68 : 64, kSlots = 32 * kLoad;
+    static constexpr int kLoads = ROWS / 32;                              // instructions of a wavefront for a step
+    // LDS slots from a load instruction to the next.  Across k, 64 bytes more than what it loads: four k read at once lie in different banks
+    static constexpr int kLoad = ACROSS ? 68 : 64, kSlots = 4 * kLoads * kLoad;
+    static constexpr int kPair = ROWS / 4, kPairs = 64 / kPair;           // across: slots of two k, pairs of a load instruction
     const char* base;                  // of the tile at the step that is loaded next
     int64_t step_bytes;                // from step to step
-    uint32_t off[8];                   // bytes from there to what this lane reads by the eight load instructions of its wavefront
+    uint32_t off[kLoads];              // bytes from there to what this lane reads by the load instructions of its wavefront
     int at;                            // element of k (along), k (across) of the first one
     int wave, lane, li, lg;
 
-    // A load instruction reads eight rows (along) or two k (across); the wavefronts take them in turn.  Along, piece c of row r stands at
-    // place c ^ (r & 7) of the row; across, piece c of k stands at place 2 c + (k & 1) of the pair.
-    __device__ __forceinline__ Wide(const void* p, int64_t ld, int64_t row0, int64_t k0) {
+    // A load instruction reads eight rows (along) or some pairs of k (across); the wavefronts take them in turn.  Along, piece c of row r stands
+    // at place c ^ (r & 7) of the row; across, piece c of k stands at place 2 c + (k & 1) of the pair.  Rows past the end are read for
+    // the last ones, and not used.
+    __device__ __forceinline__ Direct(const void* p, int64_t ld, int64_t row0, int64_t rows, int64_t k0) {
         lane = threadIdx.x & 63;
         li = lane & 15;
         lg = lane >> 4;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t ld_bytes = (uint32_t)(ld * sizeof(T));
-        uint32_t first;
         if constexpr (!ACROSS) {
             base = (const char*)p + (row0 * ld + k0) * sizeof(T);
             step_bytes = 128;
             const int c = (lane & 7) ^ (lane >> 3);
-            first = (8 * wave + (lane >> 3)) * ld_bytes + c * 16;
             at = c * kElems;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) off[i] = (uint32_t)min((int64_t)(8 * (wave + 4 * i) + (lane >> 3)), rows - 1 - row0) * ld_bytes + c * 16;
         } else {
             base = (const char*)p + (k0 * ld + row0) * sizeof(T);
             step_bytes = kStep * ld * sizeof(T);
-            at = 2 * wave + (lane & 1);
-            first = at * ld_bytes + (lane >> 1) * 16;
-        }
+            at = 2 * (kPairs * wave + lane / kPair) + (lane & 1);
+            const uint32_t c = (uint32_t)min((int64_t)(lane % kPair / 2 * 8), rows - 8 - row0) * (int)sizeof(T);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) off[i] = first + i * (ACROSS ? 8 : 32) * ld_bytes;
+            for (int i = 0; i < kLoads; ++i) off[i] = (at + 8 * kPairs * i) * ld_bytes + c;
+        }
     }
     // Load instruction i of a step, into the array of LDS that begins at `lds`.  (In assembly, since the compiler would have every transposing
     // read wait for all loads.  It has no output in registers; arrived() waits for it.)
@@ -649,8 +652,8 @@ template <typename T, bool ACROSS> struct Wide {
     }
     __device__ __forceinline__ void load_last(uint4_t* lds, int left) const {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            lds[(wave + 4 * i) * kLoad + lane] = load16_upto((const T*)(base + off[i]), ACROSS ? (at + 8 * i < left ? kElems : 0) : left - at);
+        for (int i = 0; i < kLoads; ++i)
+            lds[(wave + 4 * i) * kLoad + lane] = load16_upto((const T*)(base + off[i]), ACROSS ? (at + 8 * kPairs * i < left ? kElems : 0) : left - at);
     }
     // half h of rows `row` .. + 15 of the tile as an operand of the matrix instructions
     __device__ __forceinline__ void read(Frag<T>& f, const uint4_t* lds, int row, int h) const {
@@ -658,16 +661,24 @@ template <typename T, bool ACROSS> struct Wide {
             f.c[h] = lds[(row + li) * 8 + ((4 * h + lg) ^ (li & 7))];
         } else {
             // 16 lanes read 16 rows of four k, lane 4 r + s rows 4 s .. of the r-th, and receive four k of a row each
-            const char* src = (const char*)lds + (4 * lg + (li >> 3)) * (kLoad * 16) + (li & 2) * 16 + (li >> 2 & 1) * 16 + (li & 1) * 8;
+            auto pair = [&](int n) { return (n / kPairs * kLoad + n % kPairs * kPair) * 16; };
+            const char* src = (const char*)lds + pair(4 * lg) + (li & 2) * 16 + (li >> 2 & 1) * 16 + (li & 1) * 8 + (kPairs > 1 ? (li >> 3) * (kPair * 16) : (li >> 3) * (kLoad * 16));
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const uint2_t v = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(src + (16 * h + 2 * t) * (kLoad * 16) + row * 4)));
+                const uint2_t v = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(src + pair(16 * h + 2 * t) + row * 4)));
                 f.c[h][2 * t] = v[0];
                 f.c[h][2 * t + 1] = v[1];
             }
         }
     }
 };
+// No load and no access to LDS of this wavefront is under way, and none of the others'.
+__device__ __forceinline__ void arrived() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x70);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
 template <typename T, bool PX, bool QX>
 __global__ void __launch_bounds__(256)
@@ -676,14 +687,15 @@ wide_kernel(Product g) {
     using F = Frag<T>;
     constexpr int KS = 128 / sizeof(T);
     // (arrays of their own: what is read from one must not wait for what is on its way into another)
-    __shared__ uint4_t s_p0[Wide<T, PX>::kSlots], s_q0[Wide<T, QX>::kSlots], s_p1[Wide<T, PX>::kSlots], s_q1[Wide<T, QX>::kSlots];
+    __shared__ uint4_t s_p0[Direct<T, PX, 256>::kSlots], s_q0[Direct<T, QX, 256>::kSlots], s_p1[Direct<T, PX, 256>::kSlots], s_q1[Direct<T, QX, 256>::kSlots];
     int tm, tn;
     tile_of(g, blockIdx.x, tm, tn);
-    // (the last tiles reach back to be whole ones: outputs of two tiles are computed twice, alike)
-    const int64_t m0 = min((int64_t)tm * 256, g.m - 256), n0 = min((int64_t)tn * 256, g.n - 256);
+    const int64_t m0 = (int64_t)tm * 256, n0 = (int64_t)tn * 256;
     const int64_t k_first = (int64_t)blockIdx.y * g.k_split, k_last = min(g.k, k_first + g.k_split);
-    Wide<T, PX> P(g.p, g.ld_p, m0, k_first);
-    Wide<T, QX> Q(g.q, g.ld_q, n0, k_first);
+    using DP = Direct<T, PX, 256>;
+    using DQ = Direct<T, QX, 256>;
+    DP P(g.p, g.ld_p, m0, g.m, k_first);
+    DQ Q(g.q, g.ld_q, n0, g.n, k_first);
     const int wm = P.wave & 1, wn = P.wave >> 1, row_p = wm * 128, row_q = wn * 128;
 
     Acc acc[8][8];
@@ -704,12 +716,6 @@ wide_kernel(Product g) {
         if (n < 8) P.load(sp, n); else Q.load(sq, n - 8);
     };
     const uint32_t at_p0 = lds_address(s_p0), at_q0 = lds_address(s_q0), at_p1 = lds_address(s_p1), at_q1 = lds_address(s_q1);
-    auto arrived = [] {
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x70);             // loads and LDS: none under way
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
 
     const int64_t length = k_last > k_first ? k_last - k_first : 0, steps = length / KS;
     const int left = (int)(length - steps * KS);
@@ -744,7 +750,8 @@ wide_kernel(Product g) {
 #pragma unroll
             for (int n = 0; n < 6 * ROW; ++n) {
                 product(2 * ROW + n, q);
-                if (n % (ROW / 8) == 0 && n / (ROW / 8) < 16) load(at_p, at_q, n / (ROW / 8));
+                // 16 loads in two thirds of the time: closer, they queue up and products wait (791 -> 761 us, 8192^3 without residual), later they arrive late
+                if (n < 4 * ROW && n % (ROW / 4) == 0) load(at_p, at_q, n / (ROW / 4));
                 if (n % (ROW / 4) == 1) {
                     const int r = n / (ROW / 4);
                     if (r < 16) read_q(next_q, next, r);
@@ -785,13 +792,88 @@ wide_kernel(Product g) {
     leave<8, 8, 64>(g, acc, mine, m0 + row_p, n0 + row_q, None{});
 }
 
-template <typename T, bool PX, bool QX> ProductFn kernel_of(int tile) {
+// ---------------------------------------------------------------------------- the tiled product, aligned operands, small tiles
+
+// The same way into LDS for tiles of 128 x 128 (two workgroups to a CU) and 64 x 64 (five), whose wavefronts cover one another's waits:
+// two buffers, a barrier a step, the order of the instructions left to the compiler.
+template <typename T, bool PX, bool QX, int TILE>
+__global__ void __launch_bounds__(256)
+direct_kernel(Product g) {
+    using Acc = typename Elem<T>::Acc;
+    using DP = Direct<T, PX, TILE>;
+    using DQ = Direct<T, QX, TILE>;
+    constexpr int KS = 128 / sizeof(T), FR = TILE / 32, SB = DP::kSlots + DQ::kSlots;
+    __shared__ uint4_t s[2 * SB];
+    int tm, tn;
+    tile_of(g, blockIdx.x, tm, tn);
+    const int64_t m0 = (int64_t)tm * TILE, n0 = (int64_t)tn * TILE;
+    const int64_t k_first = (int64_t)blockIdx.y * g.k_split, k_last = min(g.k, k_first + g.k_split);
+    DP P(g.p, g.ld_p, m0, g.m, k_first);
+    DQ Q(g.q, g.ld_q, n0, g.n, k_first);
+    const int row_p = (P.wave & 1) * (TILE / 2), row_q = (P.wave >> 1) * (TILE / 2);
+    Acc acc[FR][FR];
+#pragma unroll
+    for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int j = 0; j < FR; ++j) acc[i][j] = Acc{0, 0, 0, 0};
+    auto multiply = [&](const uint4_t* tile) {
+        Frag<T> p[FR], q[FR];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < FR; ++i) {
+                Q.read(q[i], tile + DP::kSlots, row_q + i * 16, h);
+                P.read(p[i], tile, row_p + i * 16, h);
+            }
+#pragma unroll
+        for (int h = 0; h < (std::is_same_v<T, e4m3_t> ? 1 : 2); ++h)
+#pragma unroll
+            for (int i = 0; i < FR; ++i)
+#pragma unroll
+                for (int j = 0; j < FR; ++j) {
+                    if constexpr (std::is_same_v<T, e4m3_t>) acc[i][j] = mma_e4m3(q[j].c[0], q[j].c[1], p[i].c[0], p[i].c[1], acc[i][j]);
+                    else acc[i][j] = mma(q[j].c[h], p[i].c[h], acc[i][j], T{});
+                }
+    };
+    const uint32_t at = lds_address(s);
+    auto load = [&](uint32_t buffer) {
+#pragma unroll
+        for (int i = 0; i < DP::kLoads; ++i) P.load(at + buffer, i);
+#pragma unroll
+        for (int i = 0; i < DQ::kLoads; ++i) Q.load(at + buffer + DP::kSlots * 16, i);
+        P.base += P.step_bytes;
+        Q.base += Q.step_bytes;
+    };
+    const int64_t length = k_last > k_first ? k_last - k_first : 0, steps = length / KS;
+    const int left = (int)(length - steps * KS);
+    if (steps > 0) load(0);
+    uint32_t now = 0;                                                     // bytes to the buffer of this step
+    for (int64_t t = 0; t < steps; ++t) {
+        arrived();
+        if (t + 1 < steps) load(SB * 16 - now);
+        multiply(s + now / 16);
+        now = SB * 16 - now;
+    }
+    if (left > 0) {
+        // (the other buffer than the last step's: nobody reads it any more)
+        P.load_last(s + now / 16, left);
+        Q.load_last(s + now / 16 + DP::kSlots, left);
+        arrived();
+        multiply(s + now / 16);
+    }
+    __syncthreads();
+    leave<FR, FR, TILE / 2 < 32 ? TILE / 2 : 32>(g, acc, s + P.wave * (SB / 2), m0 + row_p, n0 + row_q, None{});
+}
+
+template <typename T, bool PX, bool QX> ProductFn kernel_of(int tile, bool aligned) {
     if constexpr (!std::is_same_v<T, float>)
         if (tile == kWideTile) return wide_kernel<T, PX, QX>;
+    if constexpr (!std::is_same_v<T, float>)
+        if (aligned) return tile == 128 ? direct_kernel<T, PX, QX, 128> : direct_kernel<T, PX, QX, 64>;
     return tile == 128 ? product_kernel<T, PX, QX, 128, 128, 2, 2> : product_kernel<T, PX, QX, 64, 64, 2, 2>;
 }
-template <typename T> ProductFn kernel_of(bool px, bool qx, int tile) {
-    return px ? kernel_of<T, true, true>(tile) : qx ? kernel_of<T, false, true>(tile) : kernel_of<T, false, false>(tile);
+template <typename T> ProductFn kernel_of(bool px, bool qx, int tile, bool aligned) {
+    return px ? kernel_of<T, true, true>(tile, aligned) : qx ? kernel_of<T, false, true>(tile, aligned) : kernel_of<T, false, false>(tile, aligned);
 }
 
 }  // namespace
