@@ -184,13 +184,13 @@ Cut cut_product(int32_t dtype, int64_t m, int64_t n, int64_t k) {
     return {tile, (int)splits, each * step, splits > 1 ? (size_t)splits * (size_t)m * (size_t)n * 4 : 0};
 }
 
-ProductFn product_of(int32_t dtype, bool px, bool qx, int tile, bool aligned) {
+ProductFn product_of(int32_t dtype, bool px, bool qx, int tile, bool aligned, bool deep) {
     switch (dtype) {
-        case LF_DTYPE_F32: return product_f32(px, qx, tile, aligned);
-        case LF_DTYPE_BF16: return product_bf16(px, qx, tile, aligned);
-        case LF_DTYPE_F16: return product_f16(px, qx, tile, aligned);
-        case LF_DTYPE_E4M3: return product_e4m3(px, qx, tile, aligned);
-        default: return product_i8(px, qx, tile, aligned);
+        case LF_DTYPE_F32: return product_f32(px, qx, tile, aligned, deep);
+        case LF_DTYPE_BF16: return product_bf16(px, qx, tile, aligned, deep);
+        case LF_DTYPE_F16: return product_f16(px, qx, tile, aligned, deep);
+        case LF_DTYPE_E4M3: return product_e4m3(px, qx, tile, aligned, deep);
+        default: return product_i8(px, qx, tile, aligned, deep);
     }
 }
 template <int WAVES> ProductFn few_rows_of(int32_t dtype) {
@@ -235,7 +235,7 @@ int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipSt
     g.splits = c.splits;
     g.k_split = c.k_split;
     g.part = c.splits > 1 ? work : nullptr;
-    product_of(dtype, px, qx, c.tile, aligned)<<<dim3((unsigned)(tm * tn), (unsigned)c.splits), 256, 0, st>>>(g);
+    product_of(dtype, px, qx, c.tile, aligned, getenv("LF_DEEP") ? atoi(getenv("LF_DEEP")) : tm * tn * c.splits <= (c.tile == 128 ? 256 : 512))<<<dim3((unsigned)(tm * tn), (unsigned)c.splits), 256, 0, st>>>(g);
     LF_HIP(hipGetLastError());
     if (c.splits > 1) {
         LF_TRY(dtype == LF_DTYPE_I8 ? launch_join<int32_t>(g, st) : launch_join<float>(g, st));

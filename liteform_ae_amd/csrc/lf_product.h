@@ -52,13 +52,13 @@ struct Product {
 using ProductFn = void (*)(Product);
 
 // The kernel for operands of a type: px, qx: P, Q stored across k; tile: 64, 128 or, aligned and not float32, 256 (kWideTile); aligned: pieces of
-// 16 bytes of the operands are, and across k they are whole.
+// 16 bytes of the operands are, and across k they are whole; deep: few workgroups.
 constexpr int kWideTile = 256;
-ProductFn product_f32(bool px, bool qx, int tile, bool aligned);
-ProductFn product_bf16(bool px, bool qx, int tile, bool aligned);
-ProductFn product_f16(bool px, bool qx, int tile, bool aligned);
-ProductFn product_e4m3(bool px, bool qx, int tile, bool aligned);
-ProductFn product_i8(bool px, bool qx, int tile, bool aligned);
+ProductFn product_f32(bool px, bool qx, int tile, bool aligned, bool deep);
+ProductFn product_bf16(bool px, bool qx, int tile, bool aligned, bool deep);
+ProductFn product_f16(bool px, bool qx, int tile, bool aligned, bool deep);
+ProductFn product_e4m3(bool px, bool qx, int tile, bool aligned, bool deep);
+ProductFn product_i8(bool px, bool qx, int tile, bool aligned, bool deep);
 
 }  // namespace lf
 
@@ -794,16 +794,17 @@ wide_kernel(Product g) {
 
 // ---------------------------------------------------------------------------- the tiled product, aligned operands, small tiles
 
-// The same way into LDS for tiles of 128 x 128 (two workgroups to a CU) and 64 x 64 (five), whose wavefronts cover one another's waits:
-// two buffers, a barrier a step, the order of the instructions left to the compiler.
-template <typename T, bool PX, bool QX, int TILE>
+// The same way into LDS for tiles of 128 x 128 and 64 x 64: a barrier a step, the order of the instructions left to the compiler.  With two buffers a
+// CU holds two (four) workgroups, whose wavefronts cover one another's waits; where there are too few workgroups for that, four
+// buffers have three steps on their way instead of one.
+template <typename T, bool PX, bool QX, int TILE, int BUFFERS>
 __global__ void __launch_bounds__(256)
 direct_kernel(Product g) {
     using Acc = typename Elem<T>::Acc;
     using DP = Direct<T, PX, TILE>;
     using DQ = Direct<T, QX, TILE>;
     constexpr int KS = 128 / sizeof(T), FR = TILE / 32, SB = DP::kSlots + DQ::kSlots;
-    __shared__ uint4_t s[2 * SB];
+    __shared__ uint4_t s[BUFFERS * SB];
     int tm, tn;
     tile_of(g, blockIdx.x, tm, tn);
     const int64_t m0 = (int64_t)tm * TILE, n0 = (int64_t)tn * TILE;
@@ -841,39 +842,61 @@ direct_kernel(Product g) {
         for (int i = 0; i < DP::kLoads; ++i) P.load(at + buffer, i);
 #pragma unroll
         for (int i = 0; i < DQ::kLoads; ++i) Q.load(at + buffer + DP::kSlots * 16, i);
-        P.base += P.step_bytes;
-        Q.base += Q.step_bytes;
     };
     const int64_t length = k_last > k_first ? k_last - k_first : 0, steps = length / KS;
     const int left = (int)(length - steps * KS);
-    if (steps > 0) load(0);
-    uint32_t now = 0;                                                     // bytes to the buffer of this step
-    for (int64_t t = 0; t < steps; ++t) {
-        arrived();
-        if (t + 1 < steps) load(SB * 16 - now);
-        multiply(s + now / 16);
-        now = SB * 16 - now;
+    constexpr int ON_THE_WAY = (BUFFERS - 2) * (DP::kLoads + DQ::kLoads), SIZE = SB * 16;
+    static_assert(ON_THE_WAY < 64, "");
+    const char *const p_first = P.base, *const q_first = Q.base;
+    if (steps > 0) {
+        // (a load past the last step loads that one again, where nobody reads it: the number under way is always the same)
+        auto advance = [&](int64_t next) {
+            if (next < steps) {
+                P.base += P.step_bytes;
+                Q.base += Q.step_bytes;
+            }
+        };
+#pragma unroll
+        for (int b = 0; b < BUFFERS - 1; ++b) {
+            load(b * SIZE);
+            advance(b + 1);
+        }
+        uint32_t now = 0, then = (BUFFERS - 1) * SIZE;                    // bytes to the buffer of this step, of the one that is loaded
+        for (int64_t t = 0; t < steps; ++t) {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt((ON_THE_WAY & 15) | (ON_THE_WAY >> 4) << 14 | 0x70);
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            load(then);
+            advance(t + BUFFERS);
+            multiply(s + now / 16);
+            then = now;
+            now = now == (BUFFERS - 1) * SIZE ? 0 : now + SIZE;
+        }
     }
     if (left > 0) {
-        // (the other buffer than the last step's: nobody reads it any more)
-        P.load_last(s + now / 16, left);
-        Q.load_last(s + now / 16 + DP::kSlots, left);
+        P.base = p_first + steps * P.step_bytes;
+        Q.base = q_first + steps * Q.step_bytes;
         arrived();
-        multiply(s + now / 16);
+        P.load_last(s, left);
+        Q.load_last(s + DP::kSlots, left);
+        arrived();
+        multiply(s);
     }
-    __syncthreads();
+    arrived();
     leave<FR, FR, TILE / 2 < 32 ? TILE / 2 : 32>(g, acc, s + P.wave * (SB / 2), m0 + row_p, n0 + row_q, None{});
 }
 
-template <typename T, bool PX, bool QX> ProductFn kernel_of(int tile, bool aligned) {
+template <typename T, bool PX, bool QX> ProductFn kernel_of(int tile, bool aligned, bool deep) {
     if constexpr (!std::is_same_v<T, float>)
         if (tile == kWideTile) return wide_kernel<T, PX, QX>;
     if constexpr (!std::is_same_v<T, float>)
-        if (aligned) return tile == 128 ? direct_kernel<T, PX, QX, 128> : direct_kernel<T, PX, QX, 64>;
+        if (aligned) return tile == 128 ? (deep ? direct_kernel<T, PX, QX, 128, 4> : direct_kernel<T, PX, QX, 128, 2>)
+                               : deep ? direct_kernel<T, PX, QX, 64, 4> : direct_kernel<T, PX, QX, 64, 2>;
     return tile == 128 ? product_kernel<T, PX, QX, 128, 128, 2, 2> : product_kernel<T, PX, QX, 64, 64, 2, 2>;
 }
-template <typename T> ProductFn kernel_of(bool px, bool qx, int tile, bool aligned) {
-    return px ? kernel_of<T, true, true>(tile, aligned) : qx ? kernel_of<T, false, true>(tile, aligned) : kernel_of<T, false, false>(tile, aligned);
+template <typename T> ProductFn kernel_of(bool px, bool qx, int tile, bool aligned, bool deep) {
+    return px ? kernel_of<T, true, true>(tile, aligned, deep) : qx ? kernel_of<T, false, true>(tile, aligned, deep) : kernel_of<T, false, false>(tile, aligned, deep);
 }
 
 }  // namespace
