@@ -171,17 +171,40 @@ activation_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* 
 // How a product is cut up: tile, splits of k, bytes of partial sums.
 struct Cut { int tile; int splits; int64_t k_split; size_t bytes; };
 
+// Microseconds of a step (128 bytes of k; float32 32 elements) of all workgroups that are on the GPU at once, `each` of them to a CU, as
+// measured with products of 64 .. 4096 rows and columns on 256 CUs.  Large tiles do the most to an operand's byte, small ones are more: bf16
+// 1024 x 2048 x 2048 in tiles of 128 / 64 takes 25 / 14 us, 4096 x 2048 x 1024 21 / 28, 3000^3 in tiles of 256 / 128 82 / 102.
+double step_us(bool f32, int tile, int64_t each) {
+    static const double k16[2][4] = {{0.23, 0.30, 0.52, 0.80}, {0.65, 1.15, 0, 0}}, k32[2][4] = {{0.70, 1.08, 1.40, 1.74}, {1.80, 2.60, 0, 0}};
+    return tile == kWideTile ? 1.5 : (f32 ? k32 : k16)[tile == 128][each - 1];
+}
+// Of a launch, of an epilogue of a large tile, and of the second kernel where k is split, which reads what the first one wrote at 4 TB/s.
+constexpr double kLaunchUs = 4.0, kWideUs = 8.0, kJoinUs = 5.0, kJoinBytesPerUs = 4e6;
+constexpr int kCus = 256;
+
 Cut cut_product(int32_t dtype, int64_t m, int64_t n, int64_t k) {
-    const int step = dtype == LF_DTYPE_F32 ? 32 : 128 / dtype_bytes(dtype);
-    auto tiles = [&](int t) { return ceil_div(m, t) * ceil_div(n, t); };
-    const int tile = dtype != LF_DTYPE_F32 && tiles(kWideTile) >= 200 ? kWideTile : tiles(128) >= 200 || (m > 64 && n > 64) ? (getenv("LF_T64") ? 64 : 128) : 64;
-    const int64_t t = tiles(tile), steps = ceil_div(k, step);
-    int64_t splits = 1;
-    const int W_ = getenv("LF_W") ? atoi(getenv("LF_W")) : 512, S_ = getenv("LF_S") ? atoi(getenv("LF_S")) : 8;
-    if (t < 200 && steps >= 16) splits = std::min<int64_t>(ceil_div(W_, t), steps / S_);
-    const int64_t each = std::max<int64_t>(1, ceil_div(steps, splits));
-    splits = std::max<int64_t>(1, ceil_div(steps, each));
-    return {tile, (int)splits, each * step, splits > 1 ? (size_t)splits * (size_t)m * (size_t)n * 4 : 0};
+    const bool f32 = dtype == LF_DTYPE_F32;
+    const int step = f32 ? 32 : 128 / dtype_bytes(dtype);
+    const int64_t steps = std::max<int64_t>(1, ceil_div(k, step));
+    Cut best{64, 1, steps * step, 0};
+    double best_us = 1e300;
+    for (const int tile : {64, 128, kWideTile}) {
+        if (tile == kWideTile && f32) continue;
+        const int64_t tiles = ceil_div(m, tile) * ceil_div(n, tile), most = (tile == 64 ? 4 : tile == 128 ? 2 : 1) * kCus;
+        for (int64_t want = 1; want <= 512 && want * 2 <= steps + 1; want += std::max<int64_t>(1, want / 2)) {
+            const int64_t each = ceil_div(steps, want), splits = ceil_div(steps, each);
+            const int64_t groups = tiles * splits, rest = groups % most;
+            if (splits > 1 && groups > 2 * most) break;
+            const double bytes = splits > 1 ? 4.0 * (double)splits * (double)m * (double)n : 0.0;
+            const double us = (double)each * ((double)(groups / most) * step_us(f32, tile, most / kCus) + (rest ? step_us(f32, tile, ceil_div(rest, kCus)) : 0.0)) + kLaunchUs +
+                              (tile == kWideTile ? kWideUs * (double)ceil_div(groups, most) : 0.0) + (splits > 1 ? kJoinUs + 2 * bytes / kJoinBytesPerUs : 0.0);
+            if (us < best_us) {
+                best_us = us;
+                best = {tile, (int)splits, each * step, (size_t)bytes};
+            }
+        }
+    }
+    return best;
 }
 
 ProductFn product_of(int32_t dtype, bool px, bool qx, int tile, bool aligned, bool deep) {
@@ -235,7 +258,7 @@ int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipSt
     g.splits = c.splits;
     g.k_split = c.k_split;
     g.part = c.splits > 1 ? work : nullptr;
-    product_of(dtype, px, qx, c.tile, aligned, getenv("LF_DEEP") ? atoi(getenv("LF_DEEP")) : tm * tn * c.splits <= (c.tile == 128 ? 256 : 512))<<<dim3((unsigned)(tm * tn), (unsigned)c.splits), 256, 0, st>>>(g);
+    product_of(dtype, px, qx, c.tile, aligned, tm * tn * c.splits <= kCus)<<<dim3((unsigned)(tm * tn), (unsigned)c.splits), 256, 0, st>>>(g);
     LF_HIP(hipGetLastError());
     if (c.splits > 1) {
         LF_TRY(dtype == LF_DTYPE_I8 ? launch_join<int32_t>(g, st) : launch_join<float>(g, st));

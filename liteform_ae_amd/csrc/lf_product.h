@@ -794,11 +794,11 @@ wide_kernel(Product g) {
 
 // ---------------------------------------------------------------------------- the tiled product, aligned operands, small tiles
 
-// The same way into LDS for tiles of 128 x 128 and 64 x 64: a barrier a step, the order of the instructions left to the compiler.  With two buffers a
-// CU holds two (four) workgroups, whose wavefronts cover one another's waits; where there are too few workgroups for that, four
-// buffers have three steps on their way instead of one.
+// The same way into LDS for tiles of 128 x 128 and 64 x 64: a barrier a step, the operands of the next one read during the products
+// of this one, the order of the instructions left to the compiler.  With two buffers a CU holds two (four) workgroups, whose wavefronts
+// cover one another's waits; where there are too few workgroups for that, four buffers have more steps on their way.
 template <typename T, bool PX, bool QX, int TILE, int BUFFERS>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, BUFFERS == 4 ? 1 : TILE == 128 ? 2 : 4)
 direct_kernel(Product g) {
     using Acc = typename Elem<T>::Acc;
     using DP = Direct<T, PX, TILE>;
@@ -817,23 +817,25 @@ direct_kernel(Product g) {
     for (int i = 0; i < FR; ++i)
 #pragma unroll
         for (int j = 0; j < FR; ++j) acc[i][j] = Acc{0, 0, 0, 0};
-    auto multiply = [&](const uint4_t* tile) {
-        Frag<T> p[FR], q[FR];
+    struct Operands { Frag<T> p[FR], q[FR]; };
+    auto read = [&](Operands& o, const uint4_t* tile) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < FR; ++i) {
-                Q.read(q[i], tile + DP::kSlots, row_q + i * 16, h);
-                P.read(p[i], tile, row_p + i * 16, h);
+                Q.read(o.q[i], tile + DP::kSlots, row_q + i * 16, h);
+                P.read(o.p[i], tile, row_p + i * 16, h);
             }
+    };
+    auto multiply = [&](const Operands& o) {
 #pragma unroll
         for (int h = 0; h < (std::is_same_v<T, e4m3_t> ? 1 : 2); ++h)
 #pragma unroll
             for (int i = 0; i < FR; ++i)
 #pragma unroll
                 for (int j = 0; j < FR; ++j) {
-                    if constexpr (std::is_same_v<T, e4m3_t>) acc[i][j] = mma_e4m3(q[j].c[0], q[j].c[1], p[i].c[0], p[i].c[1], acc[i][j]);
-                    else acc[i][j] = mma(q[j].c[h], p[i].c[h], acc[i][j], T{});
+                    if constexpr (std::is_same_v<T, e4m3_t>) acc[i][j] = mma_e4m3(o.q[j].c[0], o.q[j].c[1], o.p[i].c[0], o.p[i].c[1], acc[i][j]);
+                    else acc[i][j] = mma(o.q[j].c[h], o.p[i].c[h], acc[i][j], T{});
                 }
     };
     const uint32_t at = lds_address(s);
@@ -856,23 +858,38 @@ direct_kernel(Product g) {
                 Q.base += Q.step_bytes;
             }
         };
+        auto wait = [] {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt((ON_THE_WAY & 15) | (ON_THE_WAY >> 4) << 14 | 0x70);
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
 #pragma unroll
         for (int b = 0; b < BUFFERS - 1; ++b) {
             load(b * SIZE);
             advance(b + 1);
         }
-        uint32_t now = 0, then = (BUFFERS - 1) * SIZE;                    // bytes to the buffer of this step, of the one that is loaded
-        for (int64_t t = 0; t < steps; ++t) {
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_s_waitcnt((ON_THE_WAY & 15) | (ON_THE_WAY >> 4) << 14 | 0x70);
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            load(then);
-            advance(t + BUFFERS);
-            multiply(s + now / 16);
-            then = now;
-            now = now == (BUFFERS - 1) * SIZE ? 0 : now + SIZE;
+        wait();
+        load((BUFFERS - 1) * SIZE);
+        advance(BUFFERS);
+        Operands even, odd;
+        read(even, s);
+        uint32_t now = 0;                                                 // bytes to the buffer of the step whose operands are in registers
+        auto step = [&](int64_t t, const Operands& o, Operands& next) {
+            const uint32_t then = now == (BUFFERS - 1) * SIZE ? 0 : now + SIZE;
+            wait();                                                       // the next step's buffer has arrived, this one's has been read
+            load(now);
+            advance(t + BUFFERS + 1);
+            read(next, s + then / 16);
+            multiply(o);
+            now = then;
+        };
+        int64_t t = 0;
+        for (; t + 1 < steps; t += 2) {
+            step(t, even, odd);
+            step(t + 1, odd, even);
         }
+        if (t < steps) multiply(even);
     }
     if (left > 0) {
         P.base = p_first + steps * P.step_bytes;
@@ -881,7 +898,9 @@ direct_kernel(Product g) {
         P.load_last(s, left);
         Q.load_last(s + DP::kSlots, left);
         arrived();
-        multiply(s);
+        Operands o;
+        read(o, s);
+        multiply(o);
     }
     arrived();
     leave<FR, FR, TILE / 2 < 32 ? TILE / 2 : 32>(g, acc, s + P.wave * (SB / 2), m0 + row_p, n0 + row_q, None{});
