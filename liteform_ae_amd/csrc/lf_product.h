@@ -616,12 +616,17 @@ template <typename T, bool ACROSS, int ROWS> struct Direct {
     const char* base;                  // of the tile at the step that is loaded next
     int64_t step_bytes;                // from step to step
     uint32_t off[kLoads];              // bytes from there to what this lane reads by the load instructions of its wavefront
-    int at;                            // element of k (along), k (across) of the first one
     int wave, lane, li, lg;
 
     // A load instruction reads eight rows (along) or some pairs of k (across); the wavefronts take them in turn.  Along, piece c of row r stands
-    // at place c ^ (r & 7) of the row; across, piece c of k stands at place 2 c + (k & 1) of the pair.  Rows past the end are read for
-    // the last ones, and not used.
+    // at place c ^ (r & 7) of the row; across, piece c of k stands at place 2 c + (k & 1) of the pair, and pairs that are read at once
+    // (see read) are neighbours.  Rows past the end are read for the last ones, and not used.
+    // Element of k (along), k (across) that this lane reads by load instruction i.
+    __device__ __forceinline__ int at(int i) const {
+        if constexpr (!ACROSS) return ((lane & 7) ^ (lane >> 3)) * kElems;
+        const int n = kPairs * (wave + 4 * i) + lane / kPair;
+        return 2 * ((n & 16) | (n >> 1 & 3) * 4 | (n >> 3 & 1) * 2 | (n & 1)) + (lane & 1);
+    }
     __device__ __forceinline__ Direct(const void* p, int64_t ld, int64_t row0, int64_t rows, int64_t k0) {
         lane = threadIdx.x & 63;
         li = lane & 15;
@@ -631,17 +636,14 @@ template <typename T, bool ACROSS, int ROWS> struct Direct {
         if constexpr (!ACROSS) {
             base = (const char*)p + (row0 * ld + k0) * sizeof(T);
             step_bytes = 128;
-            const int c = (lane & 7) ^ (lane >> 3);
-            at = c * kElems;
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) off[i] = (uint32_t)min((int64_t)(8 * (wave + 4 * i) + (lane >> 3)), rows - 1 - row0) * ld_bytes + c * 16;
+            for (int i = 0; i < kLoads; ++i) off[i] = (uint32_t)min((int64_t)(8 * (wave + 4 * i) + (lane >> 3)), rows - 1 - row0) * ld_bytes + at(i) * (int)sizeof(T);
         } else {
             base = (const char*)p + (k0 * ld + row0) * sizeof(T);
             step_bytes = kStep * ld * sizeof(T);
-            at = 2 * (kPairs * wave + lane / kPair) + (lane & 1);
             const uint32_t c = (uint32_t)min((int64_t)(lane % kPair / 2 * 8), rows - 8 - row0) * (int)sizeof(T);
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) off[i] = (at + 8 * kPairs * i) * ld_bytes + c;
+            for (int i = 0; i < kLoads; ++i) off[i] = at(i) * ld_bytes + c;
         }
     }
     // Load instruction i of a step, into the array of LDS that begins at `lds`.  (In assembly, since the compiler would have every transposing
@@ -653,19 +655,20 @@ template <typename T, bool ACROSS, int ROWS> struct Direct {
     __device__ __forceinline__ void load_last(uint4_t* lds, int left) const {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i)
-            lds[(wave + 4 * i) * kLoad + lane] = load16_upto((const T*)(base + off[i]), ACROSS ? (at + 8 * kPairs * i < left ? kElems : 0) : left - at);
+            lds[(wave + 4 * i) * kLoad + lane] = load16_upto((const T*)(base + off[i]), ACROSS ? (at(i) < left ? kElems : 0) : left - at(i));
     }
     // half h of rows `row` .. + 15 of the tile as an operand of the matrix instructions
     __device__ __forceinline__ void read(Frag<T>& f, const uint4_t* lds, int row, int h) const {
         if constexpr (!ACROSS) {
             f.c[h] = lds[(row + li) * 8 + ((4 * h + lg) ^ (li & 7))];
         } else {
-            // 16 lanes read 16 rows of four k, lane 4 r + s rows 4 s .. of the r-th, and receive four k of a row each
+            // 16 lanes read 16 rows of four k, lane 4 r + s rows 4 s .. of the r-th, and receive four k of a row each.  The k of a lane are the eight
+            // from 8 lg on, as along; the two pairs that a group of lanes reads at once lie beside those of the next group, in other banks.
             auto pair = [&](int n) { return (n / kPairs * kLoad + n % kPairs * kPair) * 16; };
-            const char* src = (const char*)lds + pair(4 * lg) + (li & 2) * 16 + (li >> 2 & 1) * 16 + (li & 1) * 8 + (kPairs > 1 ? (li >> 3) * (kPair * 16) : (li >> 3) * (kLoad * 16));
+            const char* src = (const char*)lds + pair(2 * lg) + (li & 2) * 16 + (li >> 2 & 1) * 16 + (li & 1) * 8 + (kPairs > 1 ? (li >> 3) * (kPair * 16) : (li >> 3) * (kLoad * 16));
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const uint2_t v = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(src + pair(16 * h + 2 * t) + row * 4)));
+                const uint2_t v = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(src + pair(16 * h + 8 * t) + row * 4)));
                 f.c[h][2 * t] = v[0];
                 f.c[h][2 * t + 1] = v[1];
             }
