@@ -33,11 +33,22 @@ __global__ void __launch_bounds__(256) join_kernel(const A* part, int64_t m, int
 #pragma unroll
         for (int i = 0; i < 8; ++i) s_sum[slice][threadIdx.x % UNITS][i] = sum[i];
         __syncthreads();
+        // all threads add up some slices of an output, then the first ones their sums
+        constexpr int OUT = UNITS * 8, PARTS = 256 / OUT, EACH = SLICES / PARTS;
+        const int o = threadIdx.x % OUT, first = threadIdx.x / OUT * EACH;
+        A t = s_sum[first][o / 8][o % 8];
+#pragma unroll
+        for (int i = 1; i < EACH; ++i) t += s_sum[first + i][o / 8][o % 8];
+        __syncthreads();
+        s_sum[first][o / 8][o % 8] = t;
+        __syncthreads();
         if (slice) return;
 #pragma unroll
-        for (int t = 1; t < SLICES; ++t)
+        for (int i = 0; i < 8; ++i) sum[i] = s_sum[0][threadIdx.x][i];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += s_sum[t][threadIdx.x][i];
+        for (int p = 1; p < PARTS; ++p)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += s_sum[p * EACH][threadIdx.x][i];
     }
     if (count == 0) return;
     float8_t v;
@@ -106,8 +117,8 @@ few_rows_kernel(Product g) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int left = (int)min((int64_t)E, g.k - s * KS - lg * MINE - h * E);
-            a[h] = load16_upto(w + s * KS + h * E, left);
-            b[h] = load16_upto(x + s * KS + h * E, on ? left : 0);
+            a[h] = load16_each(w + s * KS + h * E, left);
+            b[h] = load16_each(x + s * KS + h * E, on ? left : 0);
         }
         multiply(a, b);
     }

@@ -96,8 +96,8 @@ template <typename T> __device__ __forceinline__ uint4_t load16(const T* p) {
     struct __attribute__((packed, aligned(sizeof(T)))) Any { uint4_t v; };
     return reinterpret_cast<const Any*>(p)->v;
 }
-// the first n elements of them, zeros behind
-template <typename T> __device__ __forceinline__ uint4_t load16_upto(const T* p, int n) {
+// The first n elements of them, zeros behind, one by one: loads that nothing waits for.
+template <typename T> __device__ __forceinline__ uint4_t load16_each(const T* p, int n) {
     constexpr int E = 16 / sizeof(T);
     if (n >= E) return load16(p);
     uint4_t r = {0u, 0u, 0u, 0u};
@@ -108,6 +108,38 @@ template <typename T> __device__ __forceinline__ uint4_t load16_upto(const T* p,
             else r[i >> 2] |= (uint32_t)__builtin_bit_cast(uint8_t, p[i]) << (8 * (i & 3));
         }
     return r;
+}
+// The same as eight, four, two bytes and one, where their number has that bit.  In two steps, so that several
+// such loads can be under way: part16 leaves what it loads beside each other, join16 puts it together.
+template <typename T> __device__ __forceinline__ uint4_t part16(const T* p, int n) {
+    constexpr int S = sizeof(T);
+    uint4_t r = {0u, 0u, 0u, 0u};
+    if (n >= 16 / S) {
+        r = load16(p);
+    } else if (n > 0) {
+        const char* src = (const char*)p;
+        const int bytes = n * S;
+        struct __attribute__((packed, aligned(S))) Any8 { uint2_t v; };
+        struct __attribute__((packed, aligned(S))) Any4 { uint32_t v; };
+        struct __attribute__((packed, aligned(S < 2 ? S : 2))) Any2 { uint16_t v; };
+        if (bytes & 8) {
+            const uint2_t a = reinterpret_cast<const Any8*>(src)->v;
+            r[0] = a[0];
+            r[1] = a[1];
+        }
+        if (bytes & 4) r[2] = reinterpret_cast<const Any4*>(src + (bytes & 8))->v;
+        if constexpr (S < 4)
+            if (bytes & 2) r[3] = reinterpret_cast<const Any2*>(src + (bytes & 12))->v;
+        if constexpr (S == 1)
+            if (bytes & 1) r[3] |= (uint32_t)(uint8_t)src[bytes & 14] << (bytes & 2 ? 16 : 0);
+    }
+    return r;
+}
+template <typename T> __device__ __forceinline__ uint4_t join16(uint4_t r, int n) {
+    if (n >= 16 / (int)sizeof(T)) return r;
+    const int bytes = n > 0 ? n * (int)sizeof(T) : 0;
+    const uint32_t x = bytes & 4 ? r[2] : r[3], y = bytes & 4 ? r[3] : 0;
+    return bytes & 8 ? uint4_t{r[0], r[1], x, y} : uint4_t{x, y, 0u, 0u};
 }
 
 // Two floats as the halves of three words: 8 bits of each per word, which together are the floats exactly.
@@ -136,18 +168,6 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int64_t n, 
     store_upto8(e.y, m * e.ld_y + n, e.y_dtype, v, count);
 }
 
-// Eight elements as they lie in memory, so that many loads can be under way before the first is converted.
-template <typename T> __device__ __forceinline__ typename Eight<T>::vec raw_upto8(const T* p, int n) {
-    typename Eight<T>::vec v = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (n >= 8) {
-        v = reinterpret_cast<const typename Eight<T>::Any*>(p)->v;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) v[i] = p[i];
-    }
-    return v;
-}
 template <typename F> __device__ __forceinline__ void with_type(int32_t dtype, F f) {
     if (dtype == LF_DTYPE_F32) f(0.f);
     else if (dtype == LF_DTYPE_BF16) f((__bf16)0.f);
@@ -190,7 +210,7 @@ template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
 #pragma unroll
                 for (int h = 0; h < kRegs; ++h) {
                     if (whole) r[i][h] = load16(src + h * kWide);
-                    else r[i][h] = load16_upto(src + h * kWide, (int)left - at - h * kWide);
+                    else r[i][h] = part16(src + h * kWide, (int)left - at - h * kWide);
                 }
             } else {
                 const Across a(u);
@@ -201,7 +221,7 @@ template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
                     const T* src = base + (k0 + a.k + h) * ld + row;
                     const bool in = whole || a.k + h < left;
                     if (in && n == kWide) r[i][h] = load16(src);
-                    else r[i][h] = load16_upto(src, in ? n : 0);
+                    else r[i][h] = load16_each(src, in ? n : 0);
                 }
             }
         }
@@ -217,7 +237,14 @@ template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
             k = (kl + 8 * (rest / (RU / 8))) * 4;
         }
     };
-    __device__ __forceinline__ void store(uint4_t* lds, int tid) const {
+    // (`left` as it was loaded)
+    __device__ __forceinline__ void store(uint4_t* lds, int64_t left, int tid) {
+        if constexpr (!ACROSS)
+            if (left < kStep)
+#pragma unroll
+                for (int i = 0; i < kMine; ++i)
+#pragma unroll
+                    for (int h = 0; h < kRegs; ++h) r[i][h] = join16<T>(r[i][h], (int)left - (tid + i * THREADS) % kPieces * kElems - h * kWide);
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             const int u = tid + i * THREADS;
@@ -281,6 +308,9 @@ template <int N> __device__ __forceinline__ void activate_all(float8_t (&v)[N], 
         for (int u = 0; u < N; ++u) v[u] = activate(v[u], LF_ACT_SILU);
     }
 }
+// Where four columns, from 4 c on, of a row of WC turned sums stand: even c first, then odd ones, so that lanes that read every second one lie in
+// different banks, as do those that write one c of eight rows.
+template <int WC> __device__ __forceinline__ int turned(int row, int c) { return row * (WC / 4) + (((c & 1) * (WC / 8) + (c >> 1)) ^ (row & 7)); }
 struct None {};
 template <int FM, int FN, int PR, typename Acc, typename Again>
 __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN], uint4_t* lds, int64_t m, int64_t n, Again again) {
@@ -298,7 +328,7 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
         if (e.bias) bias = load_upto8(e.bias, n, e.bias_dtype, count);
         if (e.w_scale) ws = load_upto8(e.w_scale + n, count);
     }
-    auto place = [&](int row, int h) { return lds + row * (WC / 4) + ((2 * piece + h) ^ (row & 7)); };
+    auto place = [&](int row, int h) { return lds + turned<WC>(row, 2 * piece + h); };
     auto sums = [&](int row) {
         const uint4_t a = *place(row, 0), b = *place(row, 1);
         const uint32_t w[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -326,7 +356,7 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
                 const int row = 16 * i + li, c = 4 * j + lg;
-                lds[row * (WC / 4) + (c ^ (row & 7))] = __builtin_bit_cast(uint4_t, acc[FIRST / 16 + i][j]);
+                lds[turned<WC>(row, c)] = __builtin_bit_cast(uint4_t, acc[FIRST / 16 + i][j]);
             }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -437,7 +467,7 @@ __device__ __forceinline__ void tile_of(const Product& g, unsigned id, int& tm, 
 }
 
 template <typename T, bool PX, bool QX, int TM, int TN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN)
+__global__ void __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 4)
 product_kernel(Product g) {
     constexpr int THREADS = 64 * WM * WN, FM = TM / WM / 16, FN = TN / WN / 16;
     using Acc = typename Elem<T>::Acc;
@@ -523,31 +553,33 @@ product_kernel(Product g) {
             p.load((const T*)g.p, g.ld_p, m0, g.m, k, k_last - k, tid);
             q.load((const T*)g.q, g.ld_q, n0, g.n, k, k_last - k, tid);
         };
+        auto store = [&](int64_t s, int buffer) {
+            const int64_t left = k_last - k_first - s * KS;
+            p.store(s_p + buffer * SP, left, tid);
+            q.store(s_q + buffer * SQ, left, tid);
+        };
         load(0);
         if constexpr (NB == 1) {
             for (int64_t s = 0; s < steps; ++s) {
-                p.store(s_p, tid);
-                q.store(s_q, tid);
+                store(s, 0);
                 __syncthreads();
                 if (s + 1 < steps) load(s + 1);
                 multiply(s_p, s_q);
                 __syncthreads();
             }
         } else {
-        p.store(s_p, tid);
-        q.store(s_q, tid);
-        if (steps > 1) load(1);
-        __syncthreads();
-        for (int64_t s = 0; s < steps; ++s) {
-            const int now = (int)(s & 1);
-            multiply(s_p + now * SP, s_q + now * SQ);
-            if (s + 1 < steps) {
-                p.store(s_p + (now ^ 1) * SP, tid);
-                q.store(s_q + (now ^ 1) * SQ, tid);
-                if (s + 2 < steps) load(s + 2);
-            }
+            store(0, 0);
+            if (steps > 1) load(1);
             __syncthreads();
-        }
+            for (int64_t s = 0; s < steps; ++s) {
+                const int now = (int)(s & 1);
+                multiply(s_p + now * SP, s_q + now * SQ);
+                if (s + 1 < steps) {
+                    store(s + 1, now ^ 1);
+                    if (s + 2 < steps) load(s + 2);
+                }
+                __syncthreads();
+            }
         }
     }
 
@@ -653,9 +685,12 @@ template <typename T, bool ACROSS, int ROWS> struct Direct {
                      : "memory", "scc");
     }
     __device__ __forceinline__ void load_last(uint4_t* lds, int left) const {
+        uint4_t r[kLoads];
+        auto count = [&](int i) { return ACROSS ? (at(i) < left ? kElems : 0) : left - at(i); };
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-            lds[(wave + 4 * i) * kLoad + lane] = load16_upto((const T*)(base + off[i]), ACROSS ? (at(i) < left ? kElems : 0) : left - at(i));
+        for (int i = 0; i < kLoads; ++i) r[i] = part16((const T*)(base + off[i]), count(i));
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) lds[(wave + 4 * i) * kLoad + lane] = join16<T>(r[i], count(i));
     }
     // half h of rows `row` .. + 15 of the tile as an operand of the matrix instructions
     __device__ __forceinline__ void read(Frag<T>& f, const uint4_t* lds, int row, int h) const {
