@@ -30,8 +30,60 @@ template <typename T> __device__ __forceinline__ float8_t load8(const T* p) {
 template <typename T> __device__ __forceinline__ void store8(T* p, float8_t f) {
     reinterpret_cast<typename Eight<T>::Any*>(p)->v = __builtin_convertvector(f, typename Eight<T>::vec);
 }
-// The first `n` of them (any n; others read as zero).
+// 16 bytes at any address that suits the type
+template <typename T> __device__ __forceinline__ uint4_t load16(const T* p) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Any { uint4_t v; };
+    return reinterpret_cast<const Any*>(p)->v;
+}
+// The first n elements of them, zeros behind, one by one: loads that nothing waits for.
+template <typename T> __device__ __forceinline__ uint4_t load16_each(const T* p, int n) {
+    constexpr int E = 16 / sizeof(T);
+    if (n >= E) return load16(p);
+    uint4_t r = {0u, 0u, 0u, 0u};
+    for (int i = 0; i < E; ++i)
+        if (i < n) {
+            if constexpr (sizeof(T) == 4) r[i] = __builtin_bit_cast(uint32_t, p[i]);
+            else if constexpr (sizeof(T) == 2) r[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << (16 * (i & 1));
+            else r[i >> 2] |= (uint32_t)__builtin_bit_cast(uint8_t, p[i]) << (8 * (i & 3));
+        }
+    return r;
+}
+// The same as eight, four, two bytes and one, where their number has that bit.  In two steps, so that several
+// such loads can be under way: part16 leaves what it loads beside each other, join16 puts it together.
+template <typename T> __device__ __forceinline__ uint4_t part16(const T* p, int n) {
+    constexpr int S = sizeof(T);
+    uint4_t r = {0u, 0u, 0u, 0u};
+    if (n >= 16 / S) {
+        r = load16(p);
+    } else if (n > 0) {
+        const char* src = (const char*)p;
+        const int bytes = n * S;
+        struct __attribute__((packed, aligned(S))) Any8 { uint2_t v; };
+        struct __attribute__((packed, aligned(S))) Any4 { uint32_t v; };
+        struct __attribute__((packed, aligned(S < 2 ? S : 2))) Any2 { uint16_t v; };
+        if (bytes & 8) {
+            const uint2_t a = reinterpret_cast<const Any8*>(src)->v;
+            r[0] = a[0];
+            r[1] = a[1];
+        }
+        if (bytes & 4) r[2] = reinterpret_cast<const Any4*>(src + (bytes & 8))->v;
+        if constexpr (S < 4)
+            if (bytes & 2) r[3] = reinterpret_cast<const Any2*>(src + (bytes & 12))->v;
+        if constexpr (S == 1)
+            if (bytes & 1) r[3] |= (uint32_t)(uint8_t)src[bytes & 14] << (bytes & 2 ? 16 : 0);
+    }
+    return r;
+}
+template <typename T> __device__ __forceinline__ uint4_t join16(uint4_t r, int n) {
+    if (n >= 16 / (int)sizeof(T)) return r;
+    const int bytes = n > 0 ? n * (int)sizeof(T) : 0;
+    const uint32_t x = bytes & 4 ? r[2] : r[3], y = bytes & 4 ? r[3] : 0;
+    return bytes & 8 ? uint4_t{r[0], r[1], x, y} : uint4_t{x, y, 0u, 0u};
+}
+
+// The first `n` of eight elements (any n; others read as zero).
 template <typename T> __device__ __forceinline__ float8_t load_upto8(const T* p, int n) {
+    if constexpr (sizeof(T) == 2) return __builtin_convertvector(__builtin_bit_cast(typename Eight<T>::vec, join16<T>(part16(p, n), n)), float8_t);
     if (n >= 8) return load8(p);
     float8_t f = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll

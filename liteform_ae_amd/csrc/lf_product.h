@@ -91,57 +91,6 @@ __device__ __forceinline__ float4_t mma_e4m3(uint4_t a0, uint4_t a1, uint4_t b0,
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
 }
 
-// 16 bytes at any address that suits the type
-template <typename T> __device__ __forceinline__ uint4_t load16(const T* p) {
-    struct __attribute__((packed, aligned(sizeof(T)))) Any { uint4_t v; };
-    return reinterpret_cast<const Any*>(p)->v;
-}
-// The first n elements of them, zeros behind, one by one: loads that nothing waits for.
-template <typename T> __device__ __forceinline__ uint4_t load16_each(const T* p, int n) {
-    constexpr int E = 16 / sizeof(T);
-    if (n >= E) return load16(p);
-    uint4_t r = {0u, 0u, 0u, 0u};
-    for (int i = 0; i < E; ++i)
-        if (i < n) {
-            if constexpr (sizeof(T) == 4) r[i] = __builtin_bit_cast(uint32_t, p[i]);
-            else if constexpr (sizeof(T) == 2) r[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << (16 * (i & 1));
-            else r[i >> 2] |= (uint32_t)__builtin_bit_cast(uint8_t, p[i]) << (8 * (i & 3));
-        }
-    return r;
-}
-// The same as eight, four, two bytes and one, where their number has that bit.  In two steps, so that several
-// such loads can be under way: part16 leaves what it loads beside each other, join16 puts it together.
-template <typename T> __device__ __forceinline__ uint4_t part16(const T* p, int n) {
-    constexpr int S = sizeof(T);
-    uint4_t r = {0u, 0u, 0u, 0u};
-    if (n >= 16 / S) {
-        r = load16(p);
-    } else if (n > 0) {
-        const char* src = (const char*)p;
-        const int bytes = n * S;
-        struct __attribute__((packed, aligned(S))) Any8 { uint2_t v; };
-        struct __attribute__((packed, aligned(S))) Any4 { uint32_t v; };
-        struct __attribute__((packed, aligned(S < 2 ? S : 2))) Any2 { uint16_t v; };
-        if (bytes & 8) {
-            const uint2_t a = reinterpret_cast<const Any8*>(src)->v;
-            r[0] = a[0];
-            r[1] = a[1];
-        }
-        if (bytes & 4) r[2] = reinterpret_cast<const Any4*>(src + (bytes & 8))->v;
-        if constexpr (S < 4)
-            if (bytes & 2) r[3] = reinterpret_cast<const Any2*>(src + (bytes & 12))->v;
-        if constexpr (S == 1)
-            if (bytes & 1) r[3] |= (uint32_t)(uint8_t)src[bytes & 14] << (bytes & 2 ? 16 : 0);
-    }
-    return r;
-}
-template <typename T> __device__ __forceinline__ uint4_t join16(uint4_t r, int n) {
-    if (n >= 16 / (int)sizeof(T)) return r;
-    const int bytes = n > 0 ? n * (int)sizeof(T) : 0;
-    const uint32_t x = bytes & 4 ? r[2] : r[3], y = bytes & 4 ? r[3] : 0;
-    return bytes & 8 ? uint4_t{r[0], r[1], x, y} : uint4_t{x, y, 0u, 0u};
-}
-
 // Two floats as the halves of three words: 8 bits of each per word, which together are the floats exactly.
 __device__ __forceinline__ void cut(float a, float b, uint32_t (&w)[3]) {
     const uint32_t top = 0xffff0000u;
@@ -215,13 +164,13 @@ template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
             } else {
                 const Across a(u);
                 const int64_t row = row0 + a.row;
-                const int n = (int)min((int64_t)kWide, rows - row);
+                const int n = (int)max((int64_t)-1, min((int64_t)kWide, rows - row));
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     const T* src = base + (k0 + a.k + h) * ld + row;
                     const bool in = whole || a.k + h < left;
                     if (in && n == kWide) r[i][h] = load16(src);
-                    else r[i][h] = load16_each(src, in ? n : 0);
+                    else r[i][h] = part16(src, in ? n : 0);
                 }
             }
         }
@@ -237,8 +186,8 @@ template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
             k = (kl + 8 * (rest / (RU / 8))) * 4;
         }
     };
-    // (`left` as it was loaded)
-    __device__ __forceinline__ void store(uint4_t* lds, int64_t left, int tid) {
+    // (rows and `left` as they were loaded)
+    __device__ __forceinline__ void store(uint4_t* lds, int64_t row0, int64_t rows, int64_t left, int tid) {
         if constexpr (!ACROSS)
             if (left < kStep)
 #pragma unroll
@@ -264,6 +213,10 @@ template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
             } else {
                 const Across a(u);
                 uint2_t* half = reinterpret_cast<uint2_t*>(lds);
+                const int n = (int)max((int64_t)-1, min((int64_t)kWide, rows - row0 - a.row));
+                if (n < kWide)
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) r[i][h] = join16<T>(r[i][h], n);
 #pragma unroll
                 for (int j = 0; j < kWide; ++j) {
                     const int at = 2 * slot<kPieces>(a.row + j, a.k / kElems) + (a.k / 4 & 1);
@@ -555,8 +508,8 @@ product_kernel(Product g) {
         };
         auto store = [&](int64_t s, int buffer) {
             const int64_t left = k_last - k_first - s * KS;
-            p.store(s_p + buffer * SP, left, tid);
-            q.store(s_q + buffer * SQ, left, tid);
+            p.store(s_p + buffer * SP, m0, g.m, left, tid);
+            q.store(s_q + buffer * SQ, n0, g.n, left, tid);
         };
         load(0);
         if constexpr (NB == 1) {
