@@ -109,6 +109,12 @@ __device__ __forceinline__ void store_upto8(void* p, int64_t at, int32_t dtype, 
     return store_upto8((_Float16*)p + at, f, n);
 }
 
+__device__ __forceinline__ void store_one(void* p, int64_t at, int32_t dtype, float v) {
+    if (dtype == LF_DTYPE_F32) ((float*)p)[at] = v;
+    else if (dtype == LF_DTYPE_BF16) ((__bf16*)p)[at] = (__bf16)v;
+    else ((_Float16*)p)[at] = (_Float16)v;
+}
+
 // Eight values as e4m3 (nearest, ties to even; |v| <= 448 is the caller's, NaN stays NaN).
 __device__ __forceinline__ uint2_t to_e4m3(float8_t v) {
     uint2_t r = {0u, 0u};

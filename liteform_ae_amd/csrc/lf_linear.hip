@@ -141,11 +141,11 @@ few_rows_kernel(Product g) {
 // ---------------------------------------------------------------------------- gradient of the activation
 
 // dz = dy act'(z), in rows of `ld_dz` elements, and the column sums of a slab of rows (before rounding): ACROSS threads of eight columns
-// each, the others take further rows.
+// each, the others take further rows.  A single slab's sums are db.
 template <typename T, int ACROSS>
 __global__ void __launch_bounds__(256)
-activation_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* dz, int64_t ld_dz, float* part, int64_t m, int64_t n, int32_t act,
-                       int64_t slab) {
+activation_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* dz, int64_t ld_dz, float* part, void* db, int32_t db_dtype, int64_t m, int64_t n,
+                       int32_t act, int64_t slab) {
     constexpr int DOWN = 256 / ACROSS;
     __shared__ float s[DOWN][ACROSS][9];
     const int lx = threadIdx.x % ACROSS, ly = threadIdx.x / ACROSS;
@@ -165,7 +165,7 @@ activation_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* 
             if (dz) store_upto8(dz + r * ld_dz + col, d, count);
             sum += d;
         }
-    if (!part) return;
+    if (!part && !db) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[ly][lx][i] = sum[i];
     __syncthreads();
@@ -174,7 +174,8 @@ activation_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* 
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < DOWN; ++i) t += s[i][threadIdx.x >> 3][threadIdx.x & 7];
-    part[(int64_t)blockIdx.y * n + c] = t;
+    if (part) part[(int64_t)blockIdx.y * n + c] = t;
+    else store_one(db, c, db_dtype, t);
 }
 
 // ---------------------------------------------------------------------------- launches
@@ -308,7 +309,7 @@ struct GradWork { size_t dz, sums, parts, total; };
 GradWork grad_work(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act, bool dx, bool dw, bool db) {
     GradWork w{0, 0, 0, 0};
     if (act != LF_ACT_NONE) w.dz = padded((size_t)m * (size_t)ld_dz(n) * dtype_bytes(dtype));
-    if (db) w.sums = padded((size_t)slabs_of(m, n) * (size_t)n * 4);
+    if (db && slabs_of(m, n) > 1) w.sums = padded((size_t)slabs_of(m, n) * (size_t)n * 4);
     if (dx && m && k) w.parts = cut_product(dtype, m, k, n).bytes;
     if (dw && n && k) w.parts = std::max(w.parts, cut_product(dtype, n, k, m).bytes);
     w.total = w.dz + w.sums + w.parts;
@@ -380,17 +381,17 @@ int lf_linear_grad(const lf_linear_grad_args* h_args, void* d_work, size_t work_
     float* sums = w.sums ? (float*)(at + w.dz) : nullptr;
     void* parts = at + w.dz + w.sums;
     const int64_t slabs = slabs_of(a.m, a.n), slab = ceil_div(std::max<int64_t>(a.m, 1), slabs);
-    if ((dz || sums) && a.n > 0) {
+    if ((dz || a.d_db) && a.n > 0) {
         const int across = threads_across(a.n);
         const dim3 grid((unsigned)ceil_div(a.n, 8 * across), (unsigned)slabs);
         auto go = [&](auto t) {
             using T = decltype(t);
             auto kernel = across == 8 ? activation_grad_kernel<T, 8> : across == 16 ? activation_grad_kernel<T, 16> : activation_grad_kernel<T, 32>;
-            kernel<<<grid, 256, 0, st>>>((const T*)a.d_dy, a.ld_dy, (const T*)a.d_z, a.ld_z, (T*)dz, ld_dz(a.n), sums, a.m, a.n, a.activation, slab);
+            kernel<<<grid, 256, 0, st>>>((const T*)a.d_dy, a.ld_dy, (const T*)a.d_z, a.ld_z, (T*)dz, ld_dz(a.n), sums, sums ? nullptr : a.d_db, a.db_dtype, a.m, a.n, a.activation, slab);
         };
         if (a.dtype == LF_DTYPE_F32) go(0.f); else if (a.dtype == LF_DTYPE_BF16) go((__bf16)0.f); else go((_Float16)0.f);
         LF_HIP(hipGetLastError());
-        if (a.d_db) LF_TRY(lf::column_sums(sums, slabs, a.n, a.d_db, a.db_dtype, st));
+        if (sums) LF_TRY(lf::column_sums(sums, slabs, a.n, a.d_db, a.db_dtype, st));
     }
     const void* d = dz ? dz : a.d_dy;
     const int64_t ld = dz ? ld_dz(a.n) : a.ld_dy;

@@ -240,6 +240,7 @@ rms_norm_long_kernel(NormArgs a) {
 
 struct GradArgs {
     const void* dy; const void* h; const void* w; const void* dh; void* dx; float* part;
+    void* dw;                                               // of a single workgroup, which needs no partial sums
     int64_t ldy, ldh, ldd, ldx;
     int64_t rows;
     int32_t dim, w_dtype;
@@ -296,8 +297,11 @@ rms_norm_grad_kernel(GradArgs a) {
             if (p.first < 8) store_piece(dx, p, dim, d);
         }
     }
-    if (!a.part) return;
-    float* part = a.part + (int64_t)blockIdx.x * dim;
+    if (!a.part && !a.dw) return;
+    auto leave = [&](int col, float v) {
+        if (a.part) a.part[(int64_t)blockIdx.x * dim + col] = v;
+        else store_one(a.dw, col, a.w_dtype, v);
+    };
     if constexpr (R > 1) {
         // the sums of a workgroup's row groups, column by column
 #pragma unroll
@@ -311,7 +315,7 @@ rms_norm_grad_kernel(GradArgs a) {
             float v = 0.f;
 #pragma unroll
             for (int g = 0; g < R; ++g) v += s_dw[g * 8 * C * G + j];
-            part[p.at + (j & 7)] = v;
+            leave(p.at + (j & 7), v);
         }
     } else {
 #pragma unroll
@@ -319,7 +323,7 @@ rms_norm_grad_kernel(GradArgs a) {
             const Piece p = piece_of((c * G + lane) * 8, dim);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (i >= p.first && p.at + i < dim) part[p.at + i] = dw[c][i];
+                if (i >= p.first && p.at + i < dim) leave(p.at + i, dw[c][i]);
         }
     }
 }
@@ -379,9 +383,7 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const float* part, in
     v = 0.f;
 #pragma unroll
     for (int i = 0; i < 64; ++i) v += s[i][threadIdx.x];
-    if (dtype == LF_DTYPE_F32) ((float*)out)[col] = v;
-    else if (dtype == LF_DTYPE_BF16) ((__bf16*)out)[col] = (__bf16)v;
-    else ((_Float16*)out)[col] = (_Float16)v;
+    store_one(out, col, dtype, v);
 }
 
 // Threads that hold a row, and pieces of eight of each (more than two: the kernels for long rows).
@@ -434,6 +436,8 @@ constexpr int kNormGroups = 2048, kGradGroups = 1024;
 unsigned grad_groups(int64_t rows, int64_t dim) {
     return std::min(workgroups(rows, shape_of(dim), kGradGroups), (unsigned)std::max<int64_t>(1, (1ll << 26) / dim));
 }
+// Whether a launch of one workgroup leaves dw itself, which saves the second launch's 4 us (long rows keep it in memory meanwhile).
+bool alone(int64_t rows, int64_t dim) { return shape_of(dim).pieces <= 2 && grad_groups(rows, dim) == 1; }
 
 int check_rows(const char* what, int64_t rows, int64_t dim, const void* p, int64_t ld, int32_t dtype) {
     LF_REQUIRE(p || rows == 0, LF_ERR_INVALID, "%s: null pointer", what);
@@ -505,7 +509,7 @@ int lf_quantize_rows(const void* d_x, int64_t ld_x, int32_t x_dtype, int64_t row
 }
 
 size_t lf_rms_norm_grad_work_bytes(int64_t rows, int64_t dim) {
-    if (rows <= 0 || dim < 1 || dim > kMaxDim) return 0;
+    if (rows <= 0 || dim < 1 || dim > kMaxDim || alone(rows, dim)) return 0;
     return (size_t)grad_groups(rows, dim) * (size_t)dim * sizeof(float);
 }
 
@@ -520,7 +524,7 @@ int lf_rms_norm_grad(const void* d_dy, int64_t ld_dy, int32_t dy_dtype, const vo
     const unsigned groups = rows ? grad_groups(rows, dim) : 0;
     if (d_dw) {
         LF_TRY(check_rows("dw", 1, dim, d_dw, dim, weight_dtype));
-        LF_REQUIRE(rows == 0 || (d_work && (uintptr_t)d_work % 16 == 0), LF_ERR_INVALID, "null or unaligned workspace");
+        LF_REQUIRE(rows == 0 || alone(rows, dim) || (d_work && (uintptr_t)d_work % 16 == 0), LF_ERR_INVALID, "null or unaligned workspace");
         LF_REQUIRE(work_bytes >= lf_rms_norm_grad_work_bytes(rows, dim), LF_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", work_bytes,
                    lf_rms_norm_grad_work_bytes(rows, dim));
     }
@@ -531,13 +535,14 @@ int lf_rms_norm_grad(const void* d_dy, int64_t ld_dy, int32_t dy_dtype, const vo
         LF_TRY(check_rows("dx", rows, dim, d_dx, ld_dx, h_dtype));
         if (d_dh) LF_TRY(check_rows("dh", rows, dim, d_dh, ld_dh, h_dtype));
         if (d_weight) LF_TRY(check_rows("weight", 1, dim, d_weight, dim, weight_dtype));
-        const GradArgs a{d_dy, d_h, d_weight, d_dh, d_dx, d_dw ? (float*)d_work : nullptr, ld_dy, ld_h, ld_dh, ld_dx, rows, (int32_t)dim, weight_dtype,
+        const bool one = alone(rows, dim);
+        const GradArgs a{d_dy, d_h, d_weight, d_dh, d_dx, d_dw && !one ? (float*)d_work : nullptr, one ? d_dw : nullptr, ld_dy, ld_h, ld_dh, ld_dx, rows, (int32_t)dim, weight_dtype,
                          eps, (float)(1.0 / (double)dim)};
         auto kernel = of_types(dy_dtype, h_dtype, [&](auto k) { return decltype(k)::grad(s); });
         kernel<<<groups, std::max(s.group, 256), 0, st>>>(a);
         LF_HIP(hipGetLastError());
     }
-    if (d_dw) LF_TRY(lf::column_sums((const float*)d_work, groups, dim, d_dw, weight_dtype, st));
+    if (d_dw && !(rows && alone(rows, dim))) LF_TRY(lf::column_sums((const float*)d_work, groups, dim, d_dw, weight_dtype, st));
     return LF_OK;
 }
 

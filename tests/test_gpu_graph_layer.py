@@ -1,0 +1,106 @@
+"""A graph layer made of the package's operators (graph_layer) against the same layer in 64 bits, forward, in 8 bits and backward."""
+import numpy as np
+import pytest
+
+from helpers import skewed_matrix
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+def dense(g):
+    return torch.from_numpy(np.asarray(g.coo_mtx.todense())).double().cuda()
+
+
+def layer64(A, layer, y, h):
+    """(y, h) of a layer, differentiable in 64 bits."""
+    s = A @ y + h
+    n = s / torch.sqrt((s * s).mean(dim=1, keepdim=True) + layer.eps) * layer.p64[0]
+    z = n @ layer.p64[1].t() + layer.p64[2]
+    return z * torch.special.ndtr(z), s
+
+
+@pytest.fixture(scope="module")
+def setup():
+    from liteform_ae_amd import graph_layer as gl
+    rng = np.random.default_rng(5)
+    g = skewed_matrix(rng, 300, 300, mean_deg=5.0)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    aggregation = gl.Aggregation(g, 64)
+    layers = [gl.GraphLayer(aggregation, 64, generator=gen) for _ in range(3)]
+    for layer in layers:
+        layer.norm += 0.1 * torch.randn(64, device="cuda", generator=gen)
+        layer.bias += 0.1 * torch.randn(64, device="cuda", generator=gen)
+    y, h, target = (torch.randn((300, 64), device="cuda", generator=gen) for _ in range(3))
+    return gl, g, layers, y, h, target
+
+
+def test_forward_and_gradients(setup):
+    gl, g, layers, y, h, target = setup
+    A = dense(g)
+    for layer in layers:
+        layer.p64 = [p.detach().double().requires_grad_() for p in layer.parameters()]
+    v, s = y.double().requires_grad_(), h.double().requires_grad_()
+    a, b = v, s
+    for layer in layers:
+        a, b = layer64(A, layer, a, b)
+    c, d = y, h
+    for layer in layers:
+        c, d = layer.forward(c, d, keep=True)
+    # each of the three layers is off by some 100 roundings of 2^-24 of values near one, and rows of up to 150 neighbours
+    assert float((c.double() - a).norm() / a.norm()) <= 1e-5 and float((d.double() - b).norm() / b.norm()) <= 1e-5
+    dy, dh = torch.randn_like(c), torch.randn_like(d)
+    ((a * dy.double()).sum() + (b * dh.double()).sum()).backward()
+    for layer in reversed(layers):
+        dy, dh, grads = layer.backward(dy, dh)
+        for got, want in zip(grads, layer.p64):
+            assert float((got.double() - want.grad).norm() / want.grad.norm()) <= 2e-5
+    assert float((dy.double() - v.grad).norm() / v.grad.norm()) <= 2e-5
+    assert float((dh.double() - s.grad).norm() / s.grad.norm()) <= 2e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.int8])
+def test_forward_in_8_bits(setup, dtype):
+    gl, g, layers, y, h, target = setup
+    c, d, e, f = y, h, y, h
+    for layer in layers:
+        layer._eight = None
+        c, d = layer.forward(c, d)
+        e, f = layer.forward_8bit(e, f, dtype)
+    # e4m3 rounds by 2^-4 / sqrt 3 of a value at most, both operands of each of three layers; the products' sums average that
+    assert 1e-4 < float((e - c).norm() / c.norm()) < 0.1
+    kept = layers[0]._eight
+    assert kept[0].dtype is dtype
+    layers[0].forward_8bit(y, h)
+    assert layers[0]._eight is kept
+    layers[0].update([torch.zeros_like(p) for p in layers[0].parameters()], 1.0)
+    assert layers[0]._eight is None
+
+
+def test_training_lowers_the_loss(setup):
+    gl, g, layers, y, h, target = setup
+    losses = [float(gl.train_step(layers, y, h, target, 5.0)) for _ in range(6)]
+    assert all(b < a for a, b in zip(losses, losses[1:])), losses
+
+
+def test_bfloat16_layer(setup):
+    gl, g, _, y, h, _ = setup
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    aggregation = gl.Aggregation(g, 64, "bf16")
+    layer = gl.GraphLayer(aggregation, 64, dtype=torch.bfloat16, generator=gen)
+    layer.p64 = [p.double() for p in layer.parameters()]
+    yb, hb = y.bfloat16(), h.bfloat16()
+    a, b = layer64(dense(g), layer, yb.double(), hb.double())
+    c, d = layer.forward(yb, hb)
+    assert c.dtype is d.dtype is torch.bfloat16
+    # three roundings of 2^-9 on average each (n, y; h once)
+    assert float((c.double() - a).norm() / a.norm()) < 1e-2 and float((d.double() - b).norm() / b.norm()) < 4e-3
+    assert layer.forward_8bit(yb, hb)[0].dtype is torch.bfloat16
+
+
+def test_command(capsys):
+    from liteform_ae_amd import graph_layer
+    losses = graph_layer.main(["--synthetic", "cfg2", "--scale", "0.02", "--feat", "64", "--steps", "3", "--rate", "5"])
+    assert losses[2] < losses[1] < losses[0]
+    assert "8 bits" in capsys.readouterr().out
