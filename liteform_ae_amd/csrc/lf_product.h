@@ -264,22 +264,53 @@ template <int N> __device__ __forceinline__ void activate_all(float8_t (&v)[N], 
 // Where four columns, from 4 c on, of a row of WC turned sums stand: even c first, then odd ones, so that lanes that read every second one lie in
 // different banks, as do those that write one c of eight rows.
 template <int WC> __device__ __forceinline__ int turned(int row, int c) { return row * (WC / 4) + (((c & 1) * (WC / 8) + (c >> 1)) ^ (row & 7)); }
+// What the epilogue needs of a tile's rows and columns, loaded before the first operands and kept in LDS: at the end each would be a wait.
+template <int TM, int TN> struct Vectors {
+    float bias[TN], w_scale[TN], x_scale[TM];
+    struct Loaded { float b, w, x; };
+    // (by 256 threads)
+    static __device__ __forceinline__ Loaded load(const Product& g, int64_t m0, int64_t n0) {
+        const int t = threadIdx.x;
+        Loaded l{0.f, 1.f, 1.f};
+        if (g.part) return l;
+        if (t < TN && n0 + t < g.n) {
+            if (g.e.bias) {
+                if (g.e.bias_dtype == LF_DTYPE_F32) l.b = ((const float*)g.e.bias)[n0 + t];
+                else if (g.e.bias_dtype == LF_DTYPE_BF16) l.b = (float)((const __bf16*)g.e.bias)[n0 + t];
+                else l.b = (float)((const _Float16*)g.e.bias)[n0 + t];
+            }
+            if (g.e.w_scale) l.w = g.e.w_scale[n0 + t];
+        }
+        if (g.e.x_scale && t < TM && m0 + t < g.m) l.x = g.e.x_scale[m0 + t];
+        return l;
+    }
+    __device__ __forceinline__ void keep(const Loaded& l) {
+        const int t = threadIdx.x;
+        if (t < TN) {
+            bias[t] = l.b;
+            w_scale[t] = l.w;
+        }
+        if (t < TM) x_scale[t] = l.x;
+    }
+};
 struct None {};
-template <int FM, int FN, int PR, typename Acc, typename Again>
-__device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN], uint4_t* lds, int64_t m, int64_t n, Again again) {
+// (m0, n0): of the tile that `vec` is of
+template <int FM, int FN, int PR, typename Acc, typename Vec, typename Again>
+__device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN], uint4_t* lds, const Vec& vec, int64_t m0, int64_t n0, int row0, int col0, Again again) {
     constexpr int WC = 16 * FN, LANES = WC / 8, AT_ONCE = 64 / LANES, U = PR / AT_ONCE, PHASES = FM * 16 / PR;
     constexpr bool INT = std::is_same_v<Acc, int4v>;
     static_assert(FM * 16 % PR == 0 && PR % AT_ONCE == 0 && PHASES <= 4, "");
     const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
     const int mine = lane / LANES, piece = lane % LANES;
-    n += piece * 8;
+    const int64_t m = m0 + row0, n = n0 + col0 + piece * 8;
     const int count = (int)max((int64_t)0, min((int64_t)8, g.n - n));
     const Epilogue& e = g.e;
     const bool whole = __all(count == 0 || count == 8) && !g.part;
-    float8_t bias = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, ws = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
-    if (!g.part && count) {
-        if (e.bias) bias = load_upto8(e.bias, n, e.bias_dtype, count);
-        if (e.w_scale) ws = load_upto8(e.w_scale + n, count);
+    float8_t bias, ws;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        bias[i] = vec.bias[col0 + piece * 8 + i];
+        ws[i] = vec.w_scale[col0 + piece * 8 + i];
     }
     auto place = [&](int row, int h) { return lds + turned<WC>(row, 2 * piece + h); };
     auto sums = [&](int row) {
@@ -294,7 +325,6 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
         constexpr int FIRST = decltype(number)::value * PR;
         const int64_t top = m + FIRST + mine;                                     // the lane's first row
         uint4_t raw[U][2];
-        const float xs = e.x_scale && whole ? e.x_scale[min(m + FIRST + lane, g.m - 1)] : 1.f;      // (of row `lane`)
         if (whole && e.res && count) {
             const int size = e.res_dtype == LF_DTYPE_F32 ? 4 : 2;
 #pragma unroll
@@ -347,7 +377,7 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
                         if constexpr (INT)
 #pragma unroll
                             for (int i = 0; i < 8; ++i) v[u][i] = (float)__float_as_int(v[u][i]);
-                        if (e.x_scale) v[u] = v[u] * __shfl(xs, r0 + u * AT_ONCE) * ws;
+                        if (e.x_scale) v[u] = v[u] * vec.x_scale[row0 + FIRST + r0 + u * AT_ONCE] * ws;
                         v[u] += bias;
                         const int64_t row = m + FIRST + r0 + u * AT_ONCE;
                         if (e.z && row < g.m && count) store_upto8(e.z, row * e.ld_z + n, e.z_dtype, v[u], 8);
@@ -432,6 +462,7 @@ product_kernel(Product g) {
     constexpr int SP = PL * StageP::kSlots, SQ = PL * StageQ::kSlots;
     __shared__ uint4_t s_all[NB * (SP + SQ)];
     uint4_t *const s_p = s_all, *const s_q = s_all + NB * SP;
+    __shared__ Vectors<TM, TN> s_vec;
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
     int tm, tn;
@@ -498,6 +529,7 @@ product_kernel(Product g) {
     };
 
     const int64_t steps = k_last > k_first ? (k_last - k_first + KS - 1) / KS : 0;
+    const auto vectors = s_vec.load(g, m0, n0);
     if (steps > 0) {
         StageP p;
         StageQ q;
@@ -512,6 +544,7 @@ product_kernel(Product g) {
             q.store(s_q + buffer * SQ, n0, g.n, left, tid);
         };
         load(0);
+        s_vec.keep(vectors);
         if constexpr (NB == 1) {
             for (int64_t s = 0; s < steps; ++s) {
                 store(s, 0);
@@ -536,19 +569,23 @@ product_kernel(Product g) {
         }
     }
 
+    if (steps <= 0) {
+        s_vec.keep(vectors);
+        __syncthreads();
+    }
     // (the last step is behind a barrier: LDS is free)
     constexpr int SLOTS = NB * PL * (StageP::kSlots + StageQ::kSlots) / (WM * WN), WHOLE = FM * 16, FIT = SLOTS / (FN * 4);
     constexpr int PR = 32;                       // (64 would take the registers of the CU's second workgroup)
     static_assert(PR <= FIT && WHOLE % PR == 0, "");
     uint4_t* mine = s_all + wave * SLOTS;
-    const int64_t m = m0 + wm * (TM / WM), n = n0 + wn * (TN / WN);
+    const int row0 = wm * (TM / WM), col0 = wn * (TN / WN);
     if constexpr (PL == 3)
-        leave<FM, FN, PR>(g, acc, mine, m, n, [&](int64_t row, int64_t col) {
+        leave<FM, FN, PR>(g, acc, mine, s_vec, m0, n0, row0, col0, [&](int64_t row, int64_t col) {
             return dot_f32((const float*)g.p + (PX ? k_first * g.ld_p + row : row * g.ld_p + k_first), PX ? g.ld_p : 1,
                            (const float*)g.q + (QX ? k_first * g.ld_q + col : col * g.ld_q + k_first), QX ? g.ld_q : 1, k_last - k_first);
         });
     else
-        leave<FM, FN, PR>(g, acc, mine, m, n, None{});
+        leave<FM, FN, PR>(g, acc, mine, s_vec, m0, n0, row0, col0, None{});
 }
 
 // ---------------------------------------------------------------------------- the tiled product, large tiles
@@ -679,6 +716,7 @@ wide_kernel(Product g) {
     constexpr int KS = 128 / sizeof(T);
     // (arrays of their own: what is read from one must not wait for what is on its way into another)
     __shared__ uint4_t s_p0[Direct<T, PX, 256>::kSlots], s_q0[Direct<T, QX, 256>::kSlots], s_p1[Direct<T, PX, 256>::kSlots], s_q1[Direct<T, QX, 256>::kSlots];
+    __shared__ Vectors<256, 256> s_vec;
     int tm, tn;
     tile_of(g, blockIdx.x, tm, tn);
     const int64_t m0 = (int64_t)tm * 256, n0 = (int64_t)tn * 256;
@@ -715,6 +753,8 @@ wide_kernel(Product g) {
         P.base = p_first + s * P.step_bytes;
         Q.base = q_first + s * Q.step_bytes;
     };
+    const auto vectors = s_vec.load(g, m0, n0);
+    if (steps <= 0) s_vec.keep(vectors);
     if (steps > 0) {
         // (a load past the last step loads that one again, where nobody reads it)
         auto both = [&](uint32_t sp, uint32_t sq) {
@@ -722,6 +762,7 @@ wide_kernel(Product g) {
             for (int n = 0; n < 16; ++n) load(sp, sq, n);
         };
         both(at_p0, at_q0);
+        s_vec.keep(vectors);
         arrived();
         go_to(min((int64_t)1, steps - 1));
         both(at_p1, at_q1);
@@ -780,7 +821,7 @@ wide_kernel(Product g) {
     for (int i = 0; i < 8; ++i) settle(acc[i]);
     __syncthreads();
     uint4_t* mine = P.wave == 0 ? s_p0 : P.wave == 1 ? s_q0 : P.wave == 2 ? s_p1 : s_q1;
-    leave<8, 8, 64>(g, acc, mine, m0 + row_p, n0 + row_q, None{});
+    leave<8, 8, 64>(g, acc, mine, s_vec, m0, n0, row_p, row_q, None{});
 }
 
 // ---------------------------------------------------------------------------- the tiled product, aligned operands, small tiles
@@ -796,6 +837,7 @@ direct_kernel(Product g) {
     using DQ = Direct<T, QX, TILE>;
     constexpr int KS = 128 / sizeof(T), FR = TILE / 32, SB = DP::kSlots + DQ::kSlots;
     __shared__ uint4_t s[BUFFERS * SB];
+    __shared__ Vectors<TILE, TILE> s_vec;
     int tm, tn;
     tile_of(g, blockIdx.x, tm, tn);
     const int64_t m0 = (int64_t)tm * TILE, n0 = (int64_t)tn * TILE;
@@ -841,6 +883,8 @@ direct_kernel(Product g) {
     constexpr int ON_THE_WAY = (BUFFERS - 2) * (DP::kLoads + DQ::kLoads), SIZE = SB * 16;
     static_assert(ON_THE_WAY < 64, "");
     const char *const p_first = P.base, *const q_first = Q.base;
+    const auto vectors = s_vec.load(g, m0, n0);
+    if (steps <= 0) s_vec.keep(vectors);
     if (steps > 0) {
         // (a load past the last step loads that one again, where nobody reads it: the number under way is always the same)
         auto advance = [&](int64_t next) {
@@ -860,6 +904,7 @@ direct_kernel(Product g) {
             load(b * SIZE);
             advance(b + 1);
         }
+        s_vec.keep(vectors);
         wait();
         load((BUFFERS - 1) * SIZE);
         advance(BUFFERS);
@@ -894,7 +939,7 @@ direct_kernel(Product g) {
         multiply(o);
     }
     arrived();
-    leave<FR, FR, TILE / 2 < 32 ? TILE / 2 : 32>(g, acc, s + P.wave * (SB / 2), m0 + row_p, n0 + row_q, None{});
+    leave<FR, FR, TILE / 2 < 32 ? TILE / 2 : 32>(g, acc, s + P.wave * (SB / 2), s_vec, m0, n0, row_p, row_q, None{});
 }
 
 template <typename T, bool PX, bool QX> ProductFn kernel_of(int tile, bool aligned, bool deep) {
