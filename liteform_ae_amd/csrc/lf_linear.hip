@@ -251,6 +251,7 @@ bool aligned_operands(const Product& g, int32_t dtype, bool px, bool qx) {
 
 int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipStream_t st) {
     if (g.m == 0 || g.n == 0) return LF_OK;
+    g.e.stream = g.m * g.n * dtype_bytes(g.e.y_dtype) >= kStreamBytes;
     if (!px && !qx && g.m <= kFewRows) {
         const int64_t groups = ceil_div(g.n, 16);
         LF_REQUIRE(groups < (1ll << 31), LF_ERR_UNSUPPORTED, "too many columns");

@@ -73,14 +73,14 @@ struct Piece {
 template <typename T> __device__ __forceinline__ float8_t load_piece(const T* row, const Piece& p, int dim) {
     return dim >= 8 ? load8(row + p.at) : load_upto8(row, dim);
 }
-template <typename T> __device__ __forceinline__ void store_piece(T* row, const Piece& p, int dim, float8_t v) {
-    if (dim >= 8) store8(row + p.at, v); else store_upto8(row, v, dim);
+template <typename T> __device__ __forceinline__ void store_piece(T* row, const Piece& p, int dim, float8_t v, bool stream) {
+    if (dim >= 8) store8(row + p.at, v, stream); else store_upto8(row, v, dim);
 }
 __device__ __forceinline__ float8_t load_piece(const void* base, int64_t at, int32_t dtype, const Piece& p, int dim) {
     return dim >= 8 ? load_upto8(base, at + p.at, dtype, 8) : load_upto8(base, at, dtype, dim);
 }
-__device__ __forceinline__ void store_piece(void* base, int64_t at, int32_t dtype, const Piece& p, int dim, float8_t v) {
-    if (dim >= 8) store_upto8(base, at + p.at, dtype, v, 8); else store_upto8(base, at, dtype, v, dim);
+__device__ __forceinline__ void store_piece(void* base, int64_t at, int32_t dtype, const Piece& p, int dim, float8_t v, bool stream) {
+    if (dim >= 8) store_upto8(base, at + p.at, dtype, v, 8, stream); else store_upto8(base, at, dtype, v, dim);
 }
 // For rows shorter than eight the one piece counts from 0, and its elements past the row are zeros.
 __device__ __forceinline__ Piece piece_of(int col, int dim) {
@@ -94,6 +94,7 @@ struct NormArgs {
     int64_t ldx, ldr, ldy, ldh;
     int64_t rows;
     int32_t dim, w_dtype, y_dtype, norm;                    // norm 0: rows as they are (quantize_rows)
+    int32_t stream;                                         // outputs past the caches
     float eps, inv_dim;
 };
 
@@ -111,13 +112,14 @@ struct Eighth {
         to = top == 0 || !fine ? 0.f : top8 / (amax * up);
     }
     __device__ __forceinline__ float scale(float s) const { return fine ? amax * s / top8 : __uint_as_float(0x7fc00000u); }
-    __device__ __forceinline__ void store(uint8_t* q, float8_t t, int n) const {
+    __device__ __forceinline__ void store(uint8_t* q, float8_t t, int n, bool stream) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) t[i] = fminf(fmaxf(t[i] * up * to, -top8), top8);        // (NaN goes to -top8)
         const uint2_t b = e4m3 ? to_e4m3(t) : to_int8(t);
         if (n >= 8) {
-            struct __attribute__((packed, aligned(1))) Any { uint2_t v; };
-            reinterpret_cast<Any*>(q)->v = b;
+            typedef uint32_t any2_t __attribute__((ext_vector_type(2), aligned(1)));
+            if (stream) __builtin_nontemporal_store(b, reinterpret_cast<any2_t __attribute__((address_space(1)))*>(reinterpret_cast<uintptr_t>(q)));
+            else *reinterpret_cast<any2_t*>(q) = b;
         } else {
             for (int i = 0; i < n; ++i) q[i] = (uint8_t)(b[i >> 2] >> (8 * (i & 3)));
         }
@@ -169,14 +171,14 @@ rms_norm_kernel(NormArgs a) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const Piece p = piece_of((c * G + lane) * 8, dim);
-                if (p.first < 8) store_piece(hr, p, dim, h[c]);
+                if (p.first < 8) store_piece(hr, p, dim, h[c], a.stream);
             }
         }
         if (!q8) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const Piece p = piece_of((c * G + lane) * 8, dim);
-                if (p.first < 8) store_piece(a.y, row * a.ldy, a.y_dtype, p, dim, h[c] * s * w[c]);
+                if (p.first < 8) store_piece(a.y, row * a.ldy, a.y_dtype, p, dim, h[c] * s * w[c], a.stream);
             }
             continue;
         }
@@ -185,7 +187,7 @@ rms_norm_kernel(NormArgs a) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const Piece p = piece_of((c * G + lane) * 8, dim);
-            if (p.first < 8) q.store((uint8_t*)a.y + row * a.ldy + p.at, h[c] * w[c], dim);
+            if (p.first < 8) q.store((uint8_t*)a.y + row * a.ldy + p.at, h[c] * w[c], dim, a.stream);
         }
     }
 }
@@ -232,7 +234,7 @@ rms_norm_long_kernel(NormArgs a) {
             if (!q8) {
                 store_upto8(a.y, row * a.ldy + col, a.y_dtype, h * s * w, n);
             } else {
-                q.store((uint8_t*)a.y + row * a.ldy + col, h * w, n);
+                q.store((uint8_t*)a.y + row * a.ldy + col, h * w, n, a.stream);
             }
         }
     }
@@ -244,6 +246,7 @@ struct GradArgs {
     int64_t ldy, ldh, ldd, ldx;
     int64_t rows;
     int32_t dim, w_dtype;
+    int32_t stream;
     float eps, inv_dim;
 };
 
@@ -294,7 +297,7 @@ rms_norm_grad_kernel(GradArgs a) {
             float8_t d = (dy[c] * w[c] - h[c] * k) * s;
             if (a.dh) d += load_piece((const HT*)a.dh + row * a.ldd, p, dim);
             dw[c] += dy[c] * h[c] * s;
-            if (p.first < 8) store_piece(dx, p, dim, d);
+            if (p.first < 8) store_piece(dx, p, dim, d, a.stream);
         }
     }
     if (!a.part && !a.dw) return;
@@ -483,7 +486,7 @@ int lf_rms_norm(const void* d_x, int64_t ld_x, int32_t x_dtype, const void* d_re
     }
     if (d_weight) LF_TRY(check_rows("weight", 1, dim, d_weight, dim, weight_dtype));
     const NormArgs a{d_x, d_residual, d_weight, d_y, d_h, d_scale, ld_x, ld_residual, ld_y, ld_h, rows, (int32_t)dim, weight_dtype, y_dtype, 1,
-                     eps, (float)(1.0 / (double)dim)};
+                     rows * dim * (dtype_bytes(y_dtype) + (d_h ? dtype_bytes(residual_dtype) : 0)) >= kStreamBytes, eps, (float)(1.0 / (double)dim)};
     const Shape s = shape_of(dim);
     auto kernel = of_types(x_dtype, d_residual ? residual_dtype : x_dtype, [&](auto k) { return decltype(k)::norm(s); });
     kernel<<<workgroups(rows, s, kNormGroups), std::max(s.group, 256), 0, (hipStream_t)stream>>>(a);
@@ -500,7 +503,8 @@ int lf_quantize_rows(const void* d_x, int64_t ld_x, int32_t x_dtype, int64_t row
     LF_REQUIRE(d_scale, LF_ERR_INVALID, "null pointer");
     LF_TRY(check_rows("x", rows, dim, d_x, ld_x, x_dtype));
     LF_TRY(check_rows("q", rows, dim, d_q, ld_q, q_dtype));
-    const NormArgs a{d_x, nullptr, nullptr, d_q, nullptr, d_scale, ld_x, 0, ld_q, 0, rows, (int32_t)dim, LF_DTYPE_F32, q_dtype, 0, 0.f, 0.f};
+    const NormArgs a{d_x, nullptr, nullptr, d_q, nullptr, d_scale, ld_x, 0, ld_q, 0, rows, (int32_t)dim, LF_DTYPE_F32, q_dtype, 0,
+                     rows * dim >= kStreamBytes, 0.f, 0.f};
     const Shape s = shape_of(dim);
     auto kernel = of_types(x_dtype, x_dtype, [&](auto k) { return decltype(k)::norm(s); });
     kernel<<<workgroups(rows, s, kNormGroups), std::max(s.group, 256), 0, (hipStream_t)stream>>>(a);
@@ -537,7 +541,7 @@ int lf_rms_norm_grad(const void* d_dy, int64_t ld_dy, int32_t dy_dtype, const vo
         if (d_weight) LF_TRY(check_rows("weight", 1, dim, d_weight, dim, weight_dtype));
         const bool one = alone(rows, dim);
         const GradArgs a{d_dy, d_h, d_weight, d_dh, d_dx, d_dw && !one ? (float*)d_work : nullptr, one ? d_dw : nullptr, ld_dy, ld_h, ld_dh, ld_dx, rows, (int32_t)dim, weight_dtype,
-                         eps, (float)(1.0 / (double)dim)};
+                         rows * dim * dtype_bytes(h_dtype) >= kStreamBytes, eps, (float)(1.0 / (double)dim)};
         auto kernel = of_types(dy_dtype, h_dtype, [&](auto k) { return decltype(k)::grad(s); });
         kernel<<<groups, std::max(s.group, 256), 0, st>>>(a);
         LF_HIP(hipGetLastError());

@@ -38,6 +38,7 @@ struct Epilogue {
     void* y; const void* res; void* z; const void* bias; const float* x_scale; const float* w_scale;
     int64_t ld_y, ld_res, ld_z;
     int32_t y_dtype, res_dtype, z_dtype, bias_dtype, act;
+    int32_t stream;                 // y past the caches
 };
 
 struct Product {
@@ -415,7 +416,7 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
                         using Y = decltype(t);
 #pragma unroll
                         for (int u = 0; u < H; ++u)
-                            if (top + (u0 + u) * AT_ONCE < g.m) store8((Y*)e.y + (top + (u0 + u) * AT_ONCE) * e.ld_y + n, v[u]);
+                            if (top + (u0 + u) * AT_ONCE < g.m) store8((Y*)e.y + (top + (u0 + u) * AT_ONCE) * e.ld_y + n, v[u], e.stream);
                     });
             }
         } else {
