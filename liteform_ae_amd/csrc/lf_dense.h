@@ -95,6 +95,15 @@ template <typename T> __device__ __forceinline__ uint4_t join16(uint4_t r, int n
     return bytes & 8 ? uint4_t{r[0], r[1], x, y} : uint4_t{x, y, 0u, 0u};
 }
 
+// 16 bytes without their first d elements, and zeros from the n-th of what is left (any n).
+template <typename T> __device__ __forceinline__ uint4_t move16(uint4_t r, int d, int n) {
+    constexpr int E = 16 / sizeof(T), BITS = 8 * sizeof(T);
+    unsigned __int128 v = __builtin_bit_cast(unsigned __int128, r);
+    v = d >= E ? 0 : v >> (d * BITS);
+    if (n < E) v = n <= 0 ? 0 : v & (((unsigned __int128)1 << (n * BITS)) - 1);
+    return __builtin_bit_cast(uint4_t, v);
+}
+
 // The first `n` of eight elements (any n; others read as zero).
 template <typename T> __device__ __forceinline__ float8_t load_upto8(const T* p, int n) {
     if constexpr (sizeof(T) == 2) return __builtin_convertvector(__builtin_bit_cast(typename Eight<T>::vec, join16<T>(part16(p, n), n)), float8_t);

@@ -146,36 +146,6 @@ template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
     static constexpr int kRegs = ACROSS ? 4 : kPlanes == 3 ? 2 : 1;       // 16-byte registers of a unit
     uint4_t r[kMine][kRegs];
 
-    // `left`: elements of k from this step on (more than a step: the fast way)
-    __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t left, int tid) {
-        const bool whole = left >= kStep;
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-            const int u = tid + i * THREADS;
-            if (kUnits % THREADS && u >= kUnits) continue;
-            if constexpr (!ACROSS) {
-                const int64_t row = min(row0 + u / kPieces, rows - 1);    // (rows past the end are read for the last one and not used)
-                const int at = (u % kPieces) * kElems;
-                const T* src = base + row * ld + k0 + at;
-#pragma unroll
-                for (int h = 0; h < kRegs; ++h) {
-                    if (whole) r[i][h] = load16(src + h * kWide);
-                    else r[i][h] = part16(src + h * kWide, (int)left - at - h * kWide);
-                }
-            } else {
-                const Across a(u);
-                const int64_t row = row0 + a.row;
-                const int n = (int)max((int64_t)-1, min((int64_t)kWide, rows - row));
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const T* src = base + (k0 + a.k + h) * ld + row;
-                    const bool in = whole || a.k + h < left;
-                    if (in && n == kWide) r[i][h] = load16(src);
-                    else r[i][h] = part16(src, in ? n : 0);
-                }
-            }
-        }
-    }
     struct Across {
         int row, k;                                                       // of the unit in the tile
         __device__ __forceinline__ explicit Across(int u) {
@@ -187,14 +157,92 @@ template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
             k = (kl + 8 * (rest / (RU / 8))) * 4;
         }
     };
-    // (rows and `left` as they were loaded)
-    __device__ __forceinline__ void store(uint4_t* lds, int64_t row0, int64_t rows, int64_t left, int tid) {
-        if constexpr (!ACROSS)
+
+    // `left`: elements of k from this step on, to the end of the product's part; `k`: of the matrix.
+    // Along k rows past the end are read for the last one and not used.
+    // Across, every piece is loaded whole: what stands behind a row in memory comes along, as rows of the tile that are never left.  In the last steps a
+    // piece that would pass the end of the matrix is loaded from its last 16 bytes instead, and store() moves its elements to their places and
+    // clears those of k past the end.  (Loaded by their size, in branches of each lane, pieces of bf16 4279 x 3514 by 4279 x 224 waited
+    // for each other at every step: dw 124 us, now 60.  Along k, where branches are of whole wavefronts but in a last step, the same costs 4 %.)
+    // A matrix of less than a piece, which has one step, is loaded one by one.
+    static __device__ __forceinline__ int64_t last_piece(int64_t ld, int64_t rows, int64_t k) { return (k - 1) * ld + rows - kWide; }
+    static __device__ __forceinline__ int64_t across_at(int u, int h, int64_t ld, int64_t row0, int64_t k0, int64_t rows) {
+        const Across a(u);
+        return max((int64_t)0, (k0 + a.k + h) * ld + min(row0 + a.row, rows - 1));   // (one row: ld is any number)
+    }
+    template <bool FIRST> __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t k, int64_t left, int tid) {
+        if constexpr (!ACROSS) {
+            const bool whole = left >= kStep;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int u = tid + i * THREADS;
+                if (kUnits % THREADS && u >= kUnits) continue;
+                const int at = (u % kPieces) * kElems;
+                const T* src = base + min(row0 + u / kPieces, rows - 1) * ld + k0 + at;
+#pragma unroll
+                for (int h = 0; h < kRegs; ++h) {
+                    if (whole) r[i][h] = load16(src + h * kWide);
+                    else r[i][h] = part16(src + h * kWide, (int)left - at - h * kWide);
+                }
+            }
+        } else {
+            // (a piece reaches up to kWide - 1 elements past its row, as many rows of k behind it hold at least; offsets in 32 bits)
+            if (k - k0 >= kStep + kWide && ld < (1 << 20)) {
+                const T* step = base + k0 * ld + row0;
+                const uint32_t last_row = (uint32_t)min((int64_t)ROWS, rows - 1 - row0);
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    const int u = tid + i * THREADS;
+                    if (kUnits % THREADS && u >= kUnits) continue;
+                    const Across a(u);
+                    const uint32_t off = (a.k * (uint32_t)ld + min((uint32_t)a.row, last_row)) * (uint32_t)sizeof(T);
+#pragma unroll
+                    for (int h = 0; h < kRegs; ++h) r[i][h] = load16((const T*)((const char*)(step + h * ld) + off));
+                }
+                return;
+            }
+            asm volatile("" : "+s"(ld));             // (or the addresses of these few steps would stay in registers through all)
+            const int64_t last = last_piece(ld, rows, k);
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int u = tid + i * THREADS;
+                if (kUnits % THREADS && u >= kUnits) continue;
+                if constexpr (FIRST)
+                    if (last < 0) {
+#pragma unroll
+                        for (int h = 0; h < kRegs; ++h) {
+                            const int64_t o = across_at(u, h, ld, row0, k0, rows);
+                            r[i][h] = load16_each(base + min(o, last + kWide), (int)max((int64_t)0, last + kWide - o));
+                        }
+                        continue;
+                    }
+#pragma unroll
+                for (int h = 0; h < kRegs; ++h) r[i][h] = load16(base + min(across_at(u, h, ld, row0, k0, rows), last));
+            }
+        }
+    }
+    // (as it was loaded)
+    __device__ __forceinline__ void store(uint4_t* lds, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t k, int64_t left, int tid) {
+        if constexpr (!ACROSS) {
             if (left < kStep)
 #pragma unroll
                 for (int i = 0; i < kMine; ++i)
 #pragma unroll
                     for (int h = 0; h < kRegs; ++h) r[i][h] = join16<T>(r[i][h], (int)left - (tid + i * THREADS) % kPieces * kElems - h * kWide);
+        } else if (left < kStep + kWide) {
+            asm volatile("" : "+s"(ld));
+            const int64_t last = last_piece(ld, rows, k);
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int u = tid + i * THREADS;
+                if (kUnits % THREADS && u >= kUnits) continue;
+#pragma unroll
+                for (int h = 0; h < kRegs; ++h) {
+                    const int64_t o = across_at(u, h, ld, row0, k0, rows);
+                    r[i][h] = move16<T>(r[i][h], last < 0 ? 0 : (int)min((int64_t)kWide, max((int64_t)0, o - last)), Across(u).k + h < left ? kWide : 0);
+                }
+            }
+        }
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             const int u = tid + i * THREADS;
@@ -214,10 +262,6 @@ template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
             } else {
                 const Across a(u);
                 uint2_t* half = reinterpret_cast<uint2_t*>(lds);
-                const int n = (int)max((int64_t)-1, min((int64_t)kWide, rows - row0 - a.row));
-                if (n < kWide)
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) r[i][h] = join16<T>(r[i][h], n);
 #pragma unroll
                 for (int j = 0; j < kWide; ++j) {
                     const int at = 2 * slot<kPieces>(a.row + j, a.k / kElems) + (a.k / 4 & 1);
@@ -536,15 +580,16 @@ product_kernel(Product g) {
         StageQ q;
         auto load = [&](int64_t s) {
             const int64_t k = k_first + s * KS;
-            p.load((const T*)g.p, g.ld_p, m0, g.m, k, k_last - k, tid);
-            q.load((const T*)g.q, g.ld_q, n0, g.n, k, k_last - k, tid);
+            p.template load<false>((const T*)g.p, g.ld_p, m0, g.m, k, g.k, k_last - k, tid);
+            q.template load<false>((const T*)g.q, g.ld_q, n0, g.n, k, g.k, k_last - k, tid);
         };
         auto store = [&](int64_t s, int buffer) {
-            const int64_t left = k_last - k_first - s * KS;
-            p.store(s_p + buffer * SP, m0, g.m, left, tid);
-            q.store(s_q + buffer * SQ, n0, g.n, left, tid);
+            const int64_t k = k_first + s * KS;
+            p.store(s_p + buffer * SP, g.ld_p, m0, g.m, k, g.k, k_last - k, tid);
+            q.store(s_q + buffer * SQ, g.ld_q, n0, g.n, k, g.k, k_last - k, tid);
         };
-        load(0);
+        p.template load<true>((const T*)g.p, g.ld_p, m0, g.m, k_first, g.k, k_last - k_first, tid);
+        q.template load<true>((const T*)g.q, g.ld_q, n0, g.n, k_first, g.k, k_last - k_first, tid);
         s_vec.keep(vectors);
         if constexpr (NB == 1) {
             for (int64_t s = 0; s < steps; ++s) {

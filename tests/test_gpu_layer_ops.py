@@ -440,6 +440,28 @@ def test_linear_grad_of_many_tiles(lo, x_type):
     check_grad(lo, (4100, 3901, 4005), x_type, None, F32, g, pad=1)
 
 
+@pytest.mark.parametrize("x_type", [F32, BF16, F16])
+def test_linear_grad_at_the_ends_of_matrices(lo, x_type):
+    """Matrices of a few elements and lengths around a step, in buffers that hold NaN behind every row and behind the last one."""
+    g = gen(25)
+
+    def among_nan(rows, cols, pad):
+        flat = torch.full((rows * (cols + pad) + 64,), float("nan"), device="cuda", dtype=x_type)
+        t = flat[:rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+        return t.copy_(normal((rows, cols), x_type, g))
+
+    for m in (1, 2, 9, 17, 31, 32, 33, 36, 40, 41, 63, 64, 65, 70, 72, 73, 137):
+        for n in (1, 3, 8, 17):
+            for k in (1, 2, 7, 8, 65):
+                for pad in (0, 3):
+                    dy, x, w = among_nan(m, n, pad), among_nan(m, k, pad), among_nan(n, k, pad)
+                    dx, dw, _ = lo.linear_grad(dy, x, w)
+                    want = dy.double() @ w.double()
+                    within(dx, want, want.abs() * U[x_type] + (dy.double().abs() @ w.double().abs()) * (n + 24) * E + TINY[x_type], f"dx {(m, n, k, pad)}")
+                    want = dy.double().t() @ x.double()
+                    within(dw, want, want.abs() * U[x_type] + (dy.double().abs().t() @ x.double().abs()) * (m + 24) * E + TINY[x_type], f"dw {(m, n, k, pad)}")
+
+
 def test_linear_grad_of_what_is_wanted(lo):
     g = gen(23)
     x, w, dy = normal((300, 64), BF16, g), normal((128, 64), BF16, g), normal((300, 128), BF16, g)
