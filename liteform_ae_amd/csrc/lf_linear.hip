@@ -69,7 +69,8 @@ template <typename A> int launch_join(const Product& g, hipStream_t st) {
 // ---------------------------------------------------------------------------- few rows
 
 // Up to 16 rows of X: a workgroup takes 16 rows of W, its wavefronts the 128-byte steps of k in turn, and their sums
-// meet in LDS.  W goes from memory into the matrix instructions' registers, 32 consecutive bytes a lane and step.
+// meet in LDS.  W goes from memory into the matrix instructions' registers, 32 consecutive bytes a lane and step.  Bound by the
+// read of W, small ones by the launch: one row, bf16 W of 8192^2 29 us (4.6 TB/s), of 4096^2 9.4 (3.6); 13 rows, int8 W of 1001 x 4000 6.
 template <typename T, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES)
 few_rows_kernel(Product g) {
