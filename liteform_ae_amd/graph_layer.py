@@ -51,7 +51,7 @@ class GraphLayer:
         self.norm = torch.ones(feat_size, dtype=dtype, device="cuda")
         self.weight = (torch.randn((feat_size, feat_size), device="cuda", generator=generator) * feat_size ** -0.5).to(dtype)
         self.bias = torch.zeros(feat_size, dtype=dtype, device="cuda")
-        self._eight = None
+        self._eight = None                          # [q, scale] of the last call in 8 bits; its type is the next one's, unless that names one
         self._kept = None
 
     def parameters(self):
@@ -73,12 +73,25 @@ class GraphLayer:
         dsum, dnorm = lo.rms_norm_grad(dn, h, self.norm, eps=self.eps, dh=dh)
         return self.aggregation.backward(dsum), dsum, [dnorm, dweight, dbias]
 
-    def forward_8bit(self, y, h, dtype=None):
-        """``forward`` with the dense product in 8 bits; the weight's are made for the first call and kept until ``update``."""
-        if self._eight is None:
-            self._eight = lo.quantize_rows(self.weight, dtype)
-        q, scale, h = lo.rms_norm_8bit(self.aggregation.forward(y), self.norm, residual=h, eps=self.eps, dtype=self._eight[0].dtype)
-        return lo.linear_8bit(q, scale, *self._eight, self.bias, activation=self.activation, out_dtype=self.weight.dtype), h
+    def weight_8bit(self, dtype=None):
+        """The weight as it is now in 8 bits, for ``forward_8bit``: ``(q, scale)`` of ``quantize_rows``."""
+        return lo.quantize_rows(self.weight, dtype)
+
+    def forward_8bit(self, y, h, dtype=None, weight=None):
+        """``forward`` with the dense product in 8 bits, ``dtype`` (None: that of the layer's call before, e4m3 for the first one and after
+        ``update``).  The weight is taken into 8 bits in every call, since nothing tells who has written to it meanwhile.  A caller who
+        knows passes ``weight``, what ``weight_8bit`` returned since the last change, and saves that pass over it."""
+        if weight is None:
+            eight = self.weight_8bit(self._eight[0].dtype if dtype is None and self._eight else dtype)
+            if self._eight is None:
+                self._eight = []
+            self._eight[:] = eight
+        elif dtype is not None and weight[0].dtype is not dtype:
+            raise ValueError(f"weight is of {weight[0].dtype}, dtype is {dtype}")
+        else:
+            eight = weight
+        q, scale, h = lo.rms_norm_8bit(self.aggregation.forward(y), self.norm, residual=h, eps=self.eps, dtype=eight[0].dtype)
+        return lo.linear_8bit(q, scale, *eight, self.bias, activation=self.activation, out_dtype=self.weight.dtype), h
 
     def update(self, grads, rate: float):
         for p, d in zip(self.parameters(), grads):
@@ -130,11 +143,12 @@ def main(argv=None):
     def serve(call):
         v, s = y, h
         for layer in layers:
-            v, s = getattr(layer, call)(v, s)
+            v, s = call(layer, v, s)
         return v
 
-    want = serve("forward")
-    for name, call in (("float32", "forward"), ("8 bits", "forward_8bit")):
+    eights = {layer: layer.weight_8bit() for layer in layers}            # (trained weights do not change any more)
+    want = serve(GraphLayer.forward)
+    for name, call in (("float32", GraphLayer.forward), ("8 bits", lambda layer, v, s: layer.forward_8bit(v, s, weight=eights[layer]))):
         best = float("inf")
         for _ in range(5):
             torch.cuda.synchronize()

@@ -104,3 +104,54 @@ def test_command(capsys):
     losses = graph_layer.main(["--synthetic", "cfg2", "--scale", "0.02", "--feat", "64", "--steps", "3", "--rate", "5"])
     assert losses[2] < losses[1] < losses[0]
     assert "8 bits" in capsys.readouterr().out
+
+
+def eight_by_hand(layer, y, h, dtype):
+    from liteform_ae_amd import layer_ops as lo
+    q, scale, s = lo.rms_norm_8bit(layer.aggregation.forward(y), layer.norm, residual=h, eps=layer.eps, dtype=dtype)
+    return lo.linear_8bit(q, scale, *lo.quantize_rows(layer.weight, dtype), layer.bias, activation=layer.activation, out_dtype=layer.weight.dtype), s
+
+
+def test_8_bits_of_the_type_that_is_asked_for(setup):
+    gl, g, layers, y, h, target = setup
+    layer = layers[1]
+    for dtype in (torch.float8_e4m3fn, torch.int8, torch.float8_e4m3fn):
+        for got, want in zip(layer.forward_8bit(y, h, dtype), eight_by_hand(layer, y, h, dtype)):
+            assert torch.equal(got, want)
+    weight = layer.weight_8bit(torch.int8)
+    assert torch.equal(layer.forward_8bit(y, h, weight=weight)[0], eight_by_hand(layer, y, h, torch.int8)[0])
+    assert torch.equal(layer.forward_8bit(y, h, torch.int8, weight)[0], eight_by_hand(layer, y, h, torch.int8)[0])
+    with pytest.raises(ValueError, match="dtype"):
+        layer.forward_8bit(y, h, torch.float8_e4m3fn, weight)
+
+
+def test_8_bits_of_the_weight_as_it_is(setup):
+    """Written to by an optimizer, past autograd's counter of changes, or by a replayed graph."""
+    gl, g, _, y, h, _ = setup
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    layer = gl.GraphLayer(gl.Aggregation(g, 64), 64, generator=gen)
+
+    def check(change):
+        before = layer.forward_8bit(y, h)[0]
+        change()
+        got = layer.forward_8bit(y, h)[0]
+        assert torch.equal(got, eight_by_hand(layer, y, h, torch.float8_e4m3fn)[0])
+        assert not torch.equal(got, before)
+
+    def optimize():
+        for p in layer.parameters():
+            p.grad = torch.randn(p.shape, device="cuda", generator=gen)
+        torch.optim.SGD(layer.parameters(), lr=0.1).step()
+
+    check(optimize)
+    check(lambda: layer.weight.copy_(torch.randn((64, 64), device="cuda", generator=gen)))
+    check(lambda: layer.weight.data.mul_(torch.randn((64, 64), device="cuda", generator=gen)))
+    layer.weight = torch.randn((64, 64), device="cuda", generator=gen)
+    check(lambda: setattr(layer, "weight", torch.randn((64, 64), device="cuda", generator=gen)))
+    turn = torch.randn((64, 64), device="cuda", generator=gen)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer.weight.mul_(turn)
+    for _ in range(3):
+        check(graph.replay)
