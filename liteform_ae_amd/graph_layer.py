@@ -42,7 +42,7 @@ class Aggregation:
 
 
 class GraphLayer:
-    """One layer with its parameters, in float32 or bfloat16.  ``backward`` returns the gradients that ``forward`` kept what for."""
+    """One layer with its parameters, in float32 or bfloat16.  ``backward`` returns the gradients of a call of ``forward`` that kept what they need."""
 
     def __init__(self, aggregation: Aggregation, feat_size: int, activation: str = "gelu", dtype=None, generator=None, eps: float = 1e-6):
         torch = fa._torch()
@@ -52,23 +52,30 @@ class GraphLayer:
         self.weight = (torch.randn((feat_size, feat_size), device="cuda", generator=generator) * feat_size ** -0.5).to(dtype)
         self.bias = torch.zeros(feat_size, dtype=dtype, device="cuda")
         self._eight = None                          # [q, scale] of the last call in 8 bits; its type is the next one's, unless that names one
-        self._kept = None
+        self._kept = []                             # (n, h, z) of calls of forward whose gradients are still to come
 
     def parameters(self):
         return [self.norm, self.weight, self.bias]
 
-    def forward(self, y, h, keep: bool = False):
-        """(y, h) of the next layer from those of this one."""
+    def forward(self, y, h, keep=False):
+        """(y, h) of the next layer from those of this one.  ``keep=True`` keeps what ``backward`` needs, for each call of its own, until
+        that takes it or ``update`` changes the parameters; ``keep=`` a list appends it there instead."""
         n, h = lo.rms_norm(self.aggregation.forward(y), self.norm, residual=h, eps=self.eps, out_dtype=self.weight.dtype)
-        if not keep:
+        kept = keep if isinstance(keep, list) else self._kept if keep else None
+        if kept is None:
             return lo.linear(n, self.weight, self.bias, activation=self.activation), h
         y, z = lo.linear(n, self.weight, self.bias, activation=self.activation, return_preactivation=True)
-        self._kept = (n, h, z)
+        kept.append((n, h, z))
         return y, h
 
-    def backward(self, dy, dh):
-        """Gradients (dy, dh) of the layer's inputs and of its parameters from those of its outputs."""
-        (n, h, z), self._kept = self._kept, None
+    def backward(self, dy, dh, kept=None):
+        """Gradients (dy, dh) of the layer's inputs and of its parameters from those of its outputs.  They are those of the latest
+        ``forward(keep=True)`` that no ``backward`` has had yet, or of the call whose entry of its list is passed as ``kept``."""
+        if kept is None:
+            if not self._kept:
+                raise RuntimeError("no forward(keep=True) since the last update is left to take gradients of")
+            kept = self._kept.pop()
+        n, h, z = kept
         dn, dweight, dbias = lo.linear_grad(dy, n, self.weight, z=z, activation=self.activation, bias_dtype=self.bias.dtype)
         dsum, dnorm = lo.rms_norm_grad(dn, h, self.norm, eps=self.eps, dh=dh)
         return self.aggregation.backward(dsum), dsum, [dnorm, dweight, dbias]
@@ -97,18 +104,23 @@ class GraphLayer:
         for p, d in zip(self.parameters(), grads):
             p.add_(d.to(p.dtype), alpha=-rate)
         self._eight = None
+        self._kept.clear()
 
 
 def train_step(layers, y, h, target, rate: float):
-    """One step of plain gradient descent on mean((y - target)^2); returns the loss before it (a CUDA scalar)."""
+    """One step of plain gradient descent on mean((y - target)^2); returns the loss before it (a CUDA scalar).  A layer may stand in
+    ``layers`` more than once."""
     torch = fa._torch()
     for layer in layers:
         y, h = layer.forward(y, h, keep=True)
     off = y.float() - target
     loss = off.square().mean()
     dy, dh = (off * (2.0 / off.numel())).to(y.dtype), torch.zeros_like(h)
+    sums = {}
     for layer in reversed(layers):
         dy, dh, grads = layer.backward(dy.to(layer.weight.dtype), dh)
+        sums[layer] = [a + b for a, b in zip(sums[layer], grads)] if layer in sums else grads
+    for layer, grads in sums.items():
         layer.update(grads, rate)
     return loss
 

@@ -155,3 +155,55 @@ def test_8_bits_of_the_weight_as_it_is(setup):
         layer.weight.mul_(turn)
     for _ in range(3):
         check(graph.replay)
+
+
+def test_gradients_of_calls_that_wait_for_them(setup):
+    """Two calls before their gradients, newest first or out of lists in any order, are those of each call alone."""
+    gl, g, layers, y, h, target = setup
+    layer = layers[2]
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    inputs = [tuple(torch.randn((300, 64), device="cuda", generator=gen) for _ in range(4)) for _ in range(2)]     # y, h, dy, dh
+    alone = []
+    for a, b, dy, dh in inputs:
+        layer.forward(a, b, keep=True)
+        alone.append(layer.backward(dy, dh))
+
+    def same(got, want):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and all(torch.equal(a, b) for a, b in zip(got[2], want[2]))
+
+    for a, b, _, _ in inputs:
+        layer.forward(a, b, keep=True)
+    for i in (1, 0):
+        same(layer.backward(*inputs[i][2:]), alone[i])
+    with pytest.raises(RuntimeError, match="keep=True"):
+        layer.backward(*inputs[0][2:])
+    kept = []
+    for a, b, _, _ in inputs:
+        layer.forward(a, b, keep=kept)
+    for i in (0, 1):
+        same(layer.backward(*inputs[i][2:], kept[i]), alone[i])
+    layer.forward(*inputs[0][:2], keep=True)
+    layer.update([torch.zeros_like(p) for p in layer.parameters()], 1.0)
+    with pytest.raises(RuntimeError, match="keep=True"):
+        layer.backward(*inputs[0][2:])                                    # (of parameters that are no more)
+
+
+def test_training_with_a_layer_that_stands_twice(setup):
+    gl, g, layers, y, h, target = setup
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    layer, other = (gl.GraphLayer(layers[0].aggregation, 64, generator=gen) for _ in range(2))
+    A, rate = dense(g), 5.0
+    for each in (layer, other):
+        each.p64 = [p.double().requires_grad_() for p in each.parameters()]
+    a, b = y.double(), h.double()
+    for each in (layer, other, layer):
+        a, b = layer64(A, each, a, b)
+    loss = (a - target.double()).square().mean()
+    loss.backward()
+    got = gl.train_step([layer, other, layer], y, h, target, rate)
+    assert float((got.double() - loss.detach()).abs() / loss.detach()) <= 1e-5
+    for each in (layer, other):
+        # the step of a parameter near one is known to half of its last place, 2^-24 of the values' norm at most, and to the gradient's 2e-5
+        for p, p64 in zip(each.parameters(), each.p64):
+            step = rate * p64.grad
+            assert float((p.double() - (p64.detach() - step)).norm()) <= 2e-5 * float(step.norm()) + 2.0 ** -24 * float(p64.detach().norm() + step.norm())
