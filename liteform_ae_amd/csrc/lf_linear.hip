@@ -181,45 +181,6 @@ activation_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* 
 
 // ---------------------------------------------------------------------------- launches
 
-// How a product is cut up: tile, splits of k, bytes of partial sums.
-struct Cut { int tile; int splits; int64_t k_split; size_t bytes; };
-
-// Microseconds of a step (128 bytes of k; float32 32 elements) of all workgroups that are on the GPU at once, `each` of them to a CU, as
-// measured with products of 64 .. 4096 rows and columns on 256 CUs.  Large tiles do the most to an operand's byte, small ones are more: bf16
-// 1024 x 2048 x 2048 in tiles of 128 / 64 takes 25 / 14 us, 4096 x 2048 x 1024 21 / 28, 3000^3 in tiles of 256 / 128 82 / 102.
-double step_us(bool f32, int tile, int64_t each) {
-    static const double k16[2][4] = {{0.23, 0.30, 0.52, 0.80}, {0.65, 1.15, 0, 0}}, k32[2][4] = {{0.70, 1.08, 1.40, 1.74}, {1.80, 2.60, 0, 0}};
-    return tile == kWideTile ? 1.5 : (f32 ? k32 : k16)[tile == 128][each - 1];
-}
-// Of a launch, of an epilogue of a large tile, and of the second kernel where k is split, which reads what the first one wrote at 4 TB/s.
-constexpr double kLaunchUs = 4.0, kWideUs = 8.0, kJoinUs = 5.0, kJoinBytesPerUs = 4e6;
-constexpr int kCus = 256;
-
-Cut cut_product(int32_t dtype, int64_t m, int64_t n, int64_t k) {
-    const bool f32 = dtype == LF_DTYPE_F32;
-    const int step = f32 ? 32 : 128 / dtype_bytes(dtype);
-    const int64_t steps = std::max<int64_t>(1, ceil_div(k, step));
-    Cut best{64, 1, steps * step, 0};
-    double best_us = 1e300;
-    for (const int tile : {64, 128, kWideTile}) {
-        if (tile == kWideTile && f32) continue;
-        const int64_t tiles = ceil_div(m, tile) * ceil_div(n, tile), most = (tile == 64 ? 4 : tile == 128 ? 2 : 1) * kCus;
-        for (int64_t want = 1; want <= 512 && want * 2 <= steps + 1; want += std::max<int64_t>(1, want / 2)) {
-            const int64_t each = ceil_div(steps, want), splits = ceil_div(steps, each);
-            const int64_t groups = tiles * splits, rest = groups % most;
-            if (splits > 1 && groups > 2 * most) break;
-            const double bytes = splits > 1 ? 4.0 * (double)splits * (double)m * (double)n : 0.0;
-            const double us = (double)each * ((double)(groups / most) * step_us(f32, tile, most / kCus) + (rest ? step_us(f32, tile, ceil_div(rest, kCus)) : 0.0)) + kLaunchUs +
-                              (tile == kWideTile ? kWideUs * (double)ceil_div(groups, most) : 0.0) + (splits > 1 ? kJoinUs + 2 * bytes / kJoinBytesPerUs : 0.0);
-            if (us < best_us) {
-                best_us = us;
-                best = {tile, (int)splits, each * step, (size_t)bytes};
-            }
-        }
-    }
-    return best;
-}
-
 ProductFn product_of(int32_t dtype, bool px, bool qx, int tile, bool aligned, bool deep) {
     switch (dtype) {
         case LF_DTYPE_F32: return product_f32(px, qx, tile, aligned, deep);
@@ -239,21 +200,11 @@ template <int WAVES> ProductFn few_rows_of(int32_t dtype) {
     }
 }
 
-constexpr int64_t kFewRows = 16;
-
-// Whether an operand can go straight into LDS: pieces of 16 bytes that are aligned (across k whole ones, too), and the rows of a tile within
-// 32-bit offsets.
-bool aligned_operand(const void* p, int64_t ld, int64_t rows, bool across, int bytes) {
-    return (uintptr_t)p % 16 == 0 && ld * bytes % 16 == 0 && (across ? 64 : 256) * ld * bytes < (1ll << 31) && (!across || rows % 8 == 0);
-}
-bool aligned_operands(const Product& g, int32_t dtype, bool px, bool qx) {
-    return aligned_operand(g.p, g.ld_p, g.m, px, dtype_bytes(dtype)) && aligned_operand(g.q, g.ld_q, g.n, qx, dtype_bytes(dtype));
-}
-
 int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipStream_t st) {
     if (g.m == 0 || g.n == 0) return LF_OK;
     g.e.stream = g.m * g.n * dtype_bytes(g.e.y_dtype) >= kStreamBytes;
-    if (!px && !qx && g.m <= kFewRows) {
+    const Path path = path_of(dtype_bytes(dtype), {g.p, g.ld_p, g.m, px}, {g.q, g.ld_q, g.n, qx}, g.k);
+    if (path.kernel == kPathFewRows) {
         const int64_t groups = ceil_div(g.n, 16);
         LF_REQUIRE(groups < (1ll << 31), LF_ERR_UNSUPPORTED, "too many columns");
         // few workgroups take 16 wavefronts each
@@ -262,9 +213,7 @@ int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipSt
         LF_HIP(hipGetLastError());
         return LF_OK;
     }
-    Cut c = cut_product(dtype, g.m, g.n, g.k);
-    const bool aligned = dtype != LF_DTYPE_F32 && aligned_operands(g, dtype, px, qx);
-    if (c.tile == kWideTile && !aligned) c.tile = 128;
+    const Cut& c = path.cut;
     const int64_t tm = ceil_div(g.m, c.tile), tn = ceil_div(g.n, c.tile);
     LF_REQUIRE(tm < (1ll << 27) && tn < (1ll << 27) && tm * tn < (1ll << 31), LF_ERR_UNSUPPORTED, "too many tiles");
     g.tiles_m = (int32_t)tm;
@@ -272,7 +221,7 @@ int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipSt
     g.splits = c.splits;
     g.k_split = c.k_split;
     g.part = c.splits > 1 ? work : nullptr;
-    product_of(dtype, px, qx, c.tile, aligned, tm * tn * c.splits <= kCus)<<<dim3((unsigned)(tm * tn), (unsigned)c.splits), 256, 0, st>>>(g);
+    product_of(dtype, px, qx, c.tile, path.kernel != kPathProduct, path.deep)<<<dim3((unsigned)(tm * tn), (unsigned)c.splits), 256, 0, st>>>(g);
     LF_HIP(hipGetLastError());
     if (c.splits > 1) {
         LF_TRY(dtype == LF_DTYPE_I8 ? launch_join<int32_t>(g, st) : launch_join<float>(g, st));
@@ -312,8 +261,8 @@ GradWork grad_work(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act, 
     GradWork w{0, 0, 0, 0};
     if (act != LF_ACT_NONE) w.dz = padded((size_t)m * (size_t)ld_dz(n) * dtype_bytes(dtype));
     if (db && slabs_of(m, n) > 1) w.sums = padded((size_t)slabs_of(m, n) * (size_t)n * 4);
-    if (dx && m && k) w.parts = cut_product(dtype, m, k, n).bytes;
-    if (dw && n && k) w.parts = std::max(w.parts, cut_product(dtype, n, k, m).bytes);
+    if (dx && m && k) w.parts = cut_product(dtype_bytes(dtype), m, k, n).bytes;
+    if (dw && n && k) w.parts = std::max(w.parts, cut_product(dtype_bytes(dtype), n, k, m).bytes);
     w.total = w.dz + w.sums + w.parts;
     return w;
 }
@@ -324,7 +273,7 @@ extern "C" {
 
 size_t lf_linear_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype) {
     if (m <= kFewRows || n <= 0 || k <= 0 || !(is_float_dtype(dtype) || is_8bit_dtype(dtype))) return 0;
-    return cut_product(dtype, m, n, k).bytes;
+    return cut_product(dtype_bytes(dtype), m, n, k).bytes;
 }
 
 int lf_linear(const lf_linear_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream) {

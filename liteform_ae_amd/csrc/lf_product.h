@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "lf_cut.h"
 #include "lf_dense.h"
 
 namespace lf {
@@ -55,7 +56,6 @@ using ProductFn = void (*)(Product);
 
 // The kernel for operands of a type: px, qx: P, Q stored across k; tile: 64, 128 or, aligned and not float32, 256 (kWideTile); aligned: pieces of
 // 16 bytes of the operands are, and across k they are whole; deep: few workgroups.
-constexpr int kWideTile = 256;
 ProductFn product_f32(bool px, bool qx, int tile, bool aligned, bool deep);
 ProductFn product_bf16(bool px, bool qx, int tile, bool aligned, bool deep);
 ProductFn product_f16(bool px, bool qx, int tile, bool aligned, bool deep);
