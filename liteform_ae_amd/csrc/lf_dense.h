@@ -156,50 +156,78 @@ __device__ __forceinline__ uint2_t to_int8(float8_t v) {
     return r;
 }
 
-// 1 - Phi(a) for a = |z|, at most 16, and exp(-a^2 / 2) with it: half of erfc(a / sqrt 2) by the rational approximation 7.1.26 of
-// Abramowitz and Stegun, Handbook of Mathematical Functions, which is off by 1.5e-7 at most.  erff takes twice its time, 90 us of the
-// 370 of an e4m3 product of 16k x 4k x 4k.
-__device__ __forceinline__ float normal_tail(float a, float& e) {
-    const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.3275911f * 0.70710678f, 1.f));
-    e = __builtin_amdgcn_exp2f(a * a * -0.72134752f);
-    const float p = fmaf(fmaf(fmaf(fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f), t, 0.5f * 1.421413741f), t, 0.5f * -0.284496736f), t, 0.5f * 0.254829592f);
-    return p * t * e;
+// exp(c (x + x2)), c x of -128 to 0, c a power of two and x2 less than the last place of x: 2^(c x / ln 2) with what the product's rounding, 1 / ln 2 in 32
+// bits and x2 leave, in one more term of exp's series.
+__device__ __forceinline__ float exp_of(float x, float x2, float c) {
+    const float t = x * (c * 1.44269502f);
+    const float rest = fmaf(x2, c * 1.44269502f, fmaf(x, c * 1.92596299e-8f, fmaf(x, c * 1.44269502f, -t)));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, rest * 0.693147181f, e);
 }
-// act(z) and act'(z).  gelu is z Phi(z) with the normal distribution's Phi.
-__device__ __forceinline__ float activate(float z, int32_t act) {
-    const float positive = z < 0.f ? 0.f : z;                            // (NaN stays)
-    if (act == LF_ACT_RELU) return positive;
-    if (act == LF_ACT_GELU) {
-        float e;
-        const float a = fminf(fabsf(z), 16.f);                           // (beyond, the tail is 0 in 32 bits, and Inf has none)
-        return fmaf(-a, normal_tail(a, e), positive);
+// 1 - Phi(a) for a = |z|, at most 16, and exp(-a^2 / 2) with it.  Their ratio goes from 1/2 at 0 as 0.4 / a: a quotient of polynomials in a, fitted over
+// 0 .. 14.5 for the least relative error, so that what gelu leaves of a negative z has its digits too.
+// FINE, for float32: degrees 4 and 5, off by 6e-9, at most 20 roundings of 32 bits with those of its evaluation, among them that of a^2,
+// which exp would take times a^2 / 2.  For 16 bits: degrees 3 and 4, off by 4e-7, and by up to a^2 2^-24 in exp's argument.
+template <bool FINE> __device__ __forceinline__ float normal_tail(float a, float& e) {
+    if constexpr (FINE) {
+        const float sq = a * a;
+        e = exp_of(sq, fmaf(a, a, -sq), -0.5f);
+        const float p = fmaf(fmaf(fmaf(fmaf(4.116355848e-3f, a, 4.063350893e-2f), a, 0.1832359274f), a, 0.4382959418f), a, 0.5f);
+        const float q = fmaf(fmaf(fmaf(fmaf(fmaf(1.031805421e-2f, a, 0.1018595493f), a, 0.4694727291f), a, 1.202506301f), a, 1.674476865f), a, 1.f);
+        return p * __builtin_amdgcn_rcpf(q) * e;
+    } else {
+        e = __builtin_amdgcn_exp2f(a * a * -0.72134752f);
+        const float p = fmaf(fmaf(fmaf(1.717115205e-2f, a, 0.1200515037f), a, 0.3628747862f), a, 0.4999998005f);
+        const float q = fmaf(fmaf(fmaf(fmaf(4.304641672e-2f, a, 0.3007297552f), a, 0.9559268397f), a, 1.523614424f), a, 1.f);
+        return p * __builtin_amdgcn_rcpf(q) * e;
     }
-    if (act == LF_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+}
+// What the kernels take for an activation: for float32 outputs gelu and silu to their last places (kActFine), for 16 bits with fewer instructions.
+// e4m3 16k x 4k x 4k with gelu into float32: 333 us, 312 with those of 16 bits; float32 170k x 128 by 256 138, 129.
+constexpr int32_t kActFine = 8;
+constexpr int32_t activation_of(int32_t act, int32_t dtype) { return dtype == LF_DTYPE_F32 && (act == LF_ACT_GELU || act == LF_ACT_SILU) ? act | kActFine : act; }
+// act(z) and act'(z).  gelu is z Phi(z) with the normal distribution's Phi.
+__device__ __forceinline__ float relu(float z) { return __builtin_elementwise_maximum(z, 0.f); }     // (NaN stays)
+template <bool FINE> __device__ __forceinline__ float gelu(float z) {
+    float e;
+    const float a = fminf(fabsf(z), 16.f);                               // (beyond, the tail is 0 in 32 bits, and Inf has none)
+    return fmaf(-a, normal_tail<FINE>(a, e), relu(z));
+}
+// z s(z), FINE likewise from what is left at -|z|: s(-a) = e / (1 + e), e = exp(-a)
+template <bool FINE> __device__ __forceinline__ float silu(float z) {
+    if constexpr (!FINE) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+    const float a = fminf(fabsf(z), 128.f), e = exp_of(a, 0.f, -1.f);
+    return fmaf(-a, e * __builtin_amdgcn_rcpf(1.f + e), relu(z));
+}
+template <typename V, typename F> __device__ __forceinline__ V each(V z, F f) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(V) / sizeof(float)); ++i) z[i] = f(z[i]);
     return z;
+}
+template <typename V> __device__ __forceinline__ V activate_fine(V z, int32_t act) {
+    return act == (LF_ACT_GELU | kActFine) ? each(z, [](float v) { return gelu<true>(v); }) : each(z, [](float v) { return silu<true>(v); });
 }
 __device__ __forceinline__ float8_t activate(float8_t z, int32_t act) {
-    if (act == LF_ACT_RELU) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = activate(z[i], LF_ACT_RELU);
-    } else if (act == LF_ACT_GELU) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = activate(z[i], LF_ACT_GELU);
-    } else if (act == LF_ACT_SILU) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = activate(z[i], LF_ACT_SILU);
-    }
-    return z;
+    if (act == LF_ACT_RELU) return each(z, [](float v) { return relu(v); });
+    if (act == LF_ACT_GELU) return each(z, [](float v) { return gelu<false>(v); });
+    if (act == LF_ACT_SILU) return each(z, [](float v) { return silu<false>(v); });
+    return act & kActFine ? activate_fine(z, act) : z;
 }
-__device__ __forceinline__ float activate_grad(float z, int32_t act) {
+// FINE: of float32 z
+template <bool FINE> __device__ __forceinline__ float activate_grad(float z, int32_t act) {
     if (act == LF_ACT_RELU) return z > 0.f ? 1.f : 0.f;
     if (act == LF_ACT_GELU) {
         float e;
-        const float a = fminf(fabsf(z), 16.f), tail = normal_tail(a, e), d = fmaf(a * 0.39894228f, e, -tail);
+        const float a = fminf(fabsf(z), 16.f), tail = normal_tail<FINE>(a, e), d = fmaf(a * 0.39894228f, e, -tail);
         return z != z ? z : z < 0.f ? -d : 1.f + d;                      // Phi(z) + z phi(z)
     }
     if (act == LF_ACT_SILU) {
-        const float s = 1.f / (1.f + __expf(-z));
-        return s * (1.f + z * (1.f - s));
+        if constexpr (!FINE) {
+            const float s = 1.f / (1.f + __expf(-z));
+            return s * (1.f + z * (1.f - s));
+        }
+        const float e = exp_of(fminf(fabsf(z), 128.f), 0.f, -1.f), more = __builtin_amdgcn_rcpf(1.f + e), less = e * more;
+        return z < 0.f ? less * fmaf(z, more, 1.f) : more * fmaf(z, less, 1.f);      // s(z) and 1 - s(z) = s(-z), neither as a difference
     }
     return 1.f;
 }

@@ -161,7 +161,7 @@ activation_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* 
             if (act != LF_ACT_NONE) {
                 const float8_t v = load_upto8(z + r * ld_z + col, count);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] *= activate_grad(v[i], act);
+                for (int i = 0; i < 8; ++i) d[i] *= activate_grad<std::is_same_v<T, float>>(v[i], act);
             }
             if (dz) store_upto8(dz + r * ld_dz + col, d, count);
             sum += d;
@@ -296,7 +296,7 @@ int lf_linear(const lf_linear_args* h_args, void* d_work, size_t work_bytes, lf_
     Product g{};
     g.p = a.d_x; g.q = a.d_w; g.ld_p = a.ld_x; g.ld_q = a.ld_w; g.m = a.m; g.n = a.n; g.k = a.k;
     g.e = Epilogue{a.d_y, a.d_residual, a.d_z, a.d_bias, a.d_x_scale, a.d_w_scale, a.ld_y, a.ld_residual, a.ld_z, a.y_dtype, a.residual_dtype, a.z_dtype,
-                   a.bias_dtype, a.activation};
+                   a.bias_dtype, activation_of(a.activation, a.y_dtype)};
     return launch_product(g, a.dtype, false, false, d_work, (hipStream_t)stream);
 }
 

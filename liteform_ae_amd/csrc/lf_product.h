@@ -112,9 +112,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int64_t n, 
     if (e.x_scale) v = v * e.x_scale[m] * load_upto8(e.w_scale + n, count);
     if (e.bias) v += load_upto8(e.bias, n, e.bias_dtype, count);
     if (e.z) store_upto8(e.z, m * e.ld_z + n, e.z_dtype, v, count);
-    if (e.act != LF_ACT_NONE)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = activate(v[i], e.act);
+    v = activate(v, e.act);
     if (e.res) v += load_upto8(e.res, m * e.ld_res + n, e.res_dtype, count);
     store_upto8(e.y, m * e.ld_y + n, e.y_dtype, v, count);
 }
@@ -296,16 +294,13 @@ __device__ __forceinline__ float dot_f32(const float* p, int64_t p_step, const f
 // columns, with pieces of less than eight, take them one by one.
 // float32: `again(row, column)` computes an output from the operands.
 template <int N> __device__ __forceinline__ void activate_all(float8_t (&v)[N], int32_t act) {
-    if (act == LF_ACT_RELU) {
+    auto all = [&](auto f) {
 #pragma unroll
-        for (int u = 0; u < N; ++u) v[u] = activate(v[u], LF_ACT_RELU);
-    } else if (act == LF_ACT_GELU) {
-#pragma unroll
-        for (int u = 0; u < N; ++u) v[u] = activate(v[u], LF_ACT_GELU);
-    } else if (act == LF_ACT_SILU) {
-#pragma unroll
-        for (int u = 0; u < N; ++u) v[u] = activate(v[u], LF_ACT_SILU);
-    }
+        for (int u = 0; u < N; ++u) v[u] = each(v[u], f);
+    };
+    if (act == LF_ACT_RELU) all([](float z) { return relu(z); });
+    else if (act == LF_ACT_GELU) all([](float z) { return gelu<false>(z); });
+    else if (act == LF_ACT_SILU) all([](float z) { return silu<false>(z); });
 }
 // Where four columns, from 4 c on, of a row of WC turned sums stand: even c first, then odd ones, so that lanes that read every second one lie in
 // different banks, as do those that write one c of eight rows.
@@ -404,21 +399,22 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
                     }
             }
         }
-        if (g.part) {
+        if (__builtin_expect(g.part != nullptr, 0)) {
 #pragma unroll 2
             for (int row = mine; row < PR; row += AT_ONCE)
                 if (m + FIRST + row < g.m && count) store_upto8((float*)g.part + ((int64_t)blockIdx.y * g.m + m + FIRST + row) * g.n + n, sums(row), count);
-        } else if (whole) {
+        } else if (__builtin_expect(whole, 1)) {
             // What follows the sums and comes before the residual, in a lane's own places of LDS: a loop, since its code is long and would be read
             // from memory for every tile if it stood there sixteen times (gelu: 44 us of the 285 of an e4m3 product of 16k x 4k x 4k, 25 as a loop)
             constexpr int H = U < 4 ? U : 4;
             const bool first_pass = INT || e.x_scale || e.z || e.act != LF_ACT_NONE;
-            if (first_pass)
+            auto pass = [&](auto rows, auto act) {
+                constexpr int N = decltype(rows)::value;
 #pragma unroll 1
-                for (int r0 = mine; r0 < PR; r0 += H * AT_ONCE) {
-                    float8_t v[H];
+                for (int r0 = mine; r0 < PR; r0 += N * AT_ONCE) {
+                    float8_t v[N];
 #pragma unroll
-                    for (int u = 0; u < H; ++u) {
+                    for (int u = 0; u < N; ++u) {
                         v[u] = sums(r0 + u * AT_ONCE);
                         if constexpr (INT)
 #pragma unroll
@@ -428,13 +424,18 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
                         const int64_t row = m + FIRST + r0 + u * AT_ONCE;
                         if (e.z && row < g.m && count) store_upto8(e.z, row * e.ld_z + n, e.z_dtype, v[u], 8);
                     }
-                    activate_all(v, e.act);
+                    act(v);
 #pragma unroll
-                    for (int u = 0; u < H; ++u) {
+                    for (int u = 0; u < N; ++u) {
                         *place(r0 + u * AT_ONCE, 0) = __builtin_bit_cast(uint4_t, float4_t{v[u][0], v[u][1], v[u][2], v[u][3]});
                         *place(r0 + u * AT_ONCE, 1) = __builtin_bit_cast(uint4_t, float4_t{v[u][4], v[u][5], v[u][6], v[u][7]});
                     }
                 }
+            };
+            // (gelu and silu of float32 outputs are longer still: a row at a time.  What is expected, here and above, is for the order in memory: the
+            // code that large products run has to stay in the instruction cache; with this pass in its midst e4m3 16k x 4k x 4k took 10 to 20 us more)
+            if (__builtin_expect(e.act & kActFine, 0)) pass(std::integral_constant<int, 1>{}, [&](float8_t (&v)[1]) { v[0] = activate_fine(v[0], e.act); });
+            else if (first_pass) pass(std::integral_constant<int, H>{}, [&](float8_t (&v)[H]) { activate_all(v, e.act); });
 #pragma unroll
             for (int u0 = 0; u0 < U; u0 += H) {
                 float8_t v[H];

@@ -631,3 +631,82 @@ def test_refusals_of_the_library(lo):
     assert lib.lf_rms_norm_grad(x.data_ptr(), 64, 0, x.data_ptr(), 64, 0, x.data_ptr(), 0, None, 0, 40, 64, 1e-6, y.data_ptr(), 64, y.data_ptr(), work.data_ptr(),
                                 need - 4, None) == _lib.LF_ERR_WORKSPACE
     torch.cuda.synchronize()
+
+
+# --------------------------------------------------------------------------- activations over their range
+
+
+def phi64(z):
+    """Phi(z); torch.special.ndtr is 1 + erf below -1, with none of the digits of what it leaves."""
+    return 0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+
+
+def gelu64(z, act):
+    return z * phi64(z) if act == "gelu" else act64(z, act)
+
+
+def act_off(z, act, fine):
+    """How far act(z) may be off in 32 bits, roundings counted in E = 2^-24 (a device function's last place: 2).  gelu: the tail 1 - Phi(|z|) is
+    a quotient of polynomials of positive terms (4 and 5 products with sums, each coefficient rounded, a reciprocal, a product) and exp(-z^2 / 2),
+    with the rounding of z^2 made up for: 20 in all.  For 16 bits: fitted to 4e-7, and two roundings of exp's argument, z^2 / 2."""
+    z = z.abs()
+    if act == "gelu":
+        tail = phi64(-z)
+        return z * tail * (20 * E if fine else 4.1e-7 + (20 + z * z) * E)
+    # exp, 1 + exp, product, quotient; without fine its argument z is rounded twice
+    return act64(-z, "silu").abs() * (8 if fine else 10 + 2 * z) * E if act == "silu" else 0.0 * z
+
+
+def act_grad_off(z, act, fine):
+    a = z.abs()
+    if act == "gelu":                                       # a phi(a), with exp as above and three roundings, and the tail
+        phi = a * torch.exp(-a * a / 2) / math.sqrt(2 * math.pi)
+        rest = 0.0 if fine else 4.1e-7 + a * a * E
+        return phi * (10 * E + rest) + phi64(-a) * (20 * E + rest)
+    if act == "silu":                                       # s (1 + z (1 - s)): s and 1 - s to seven roundings, without fine as a difference
+        s, t = torch.sigmoid(z), torch.sigmoid(-z)
+        return s * (a * t + (1 + z * t).abs()) * 9 * E if fine else s * (a * t + 1 + a) * (12 + 2 * a) * E
+    return 0.0 * a
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu", "relu"])
+@pytest.mark.parametrize("x_type", [F32, BF16, F16])
+def test_activations_and_their_gradients_keep_their_digits(lo, x_type, act):
+    """z = x from -10 to 10, as sums of one product: of few rows, of tiles with and without whole pieces of columns, of parts of k."""
+    every = torch.linspace(-10, 10, 40_001, device="cuda").to(x_type)
+    for rows, n, k in [(40_001, 1, 1), (40_001, 8, 8), (9, 3, 5), (70, 16, 40_000)]:
+        z = every[:: 40_001 // rows][:rows]
+        x, w = torch.zeros((rows, k), device="cuda", dtype=x_type), torch.ones((n, k), device="cuda", dtype=x_type)
+        x[:, 0] = z
+        z64 = z.double()[:, None].expand(rows, n)
+        for out in (x_type, F32):
+            y = lo.linear(x, w, activation=act, out_dtype=out)
+            y64 = gelu64(z64, act)
+            within(y, y64, y64.abs() * U[out] + act_off(z64, act, out is F32) + TINY[out], f"{act} {rows, n, k} {out}")
+    one = torch.ones((1, 1), device="cuda", dtype=x_type)
+    z = every[:, None].contiguous()
+    dx, _, db = lo.linear_grad(torch.ones_like(z), z, one, z=z, activation=act, bias_dtype=F32)
+    d = z.double()
+    want = phi64(d) + d * torch.exp(-d * d / 2) / math.sqrt(2 * math.pi) if act == "gelu" else act_grad64(d, act)
+    within(dx, want, want.abs() * U[x_type] + act_grad_off(d, act, x_type is F32) + TINY[x_type], act)
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_activations_of_large_products_keep_their_digits(lo, act):
+    """Through the large tiles, 16 and 8 bits in, 32 and 16 bits out."""
+    m, n = 7001, 4104
+    for x_type, k in [(BF16, 1024), (I8, 2048)]:
+        x, w = torch.zeros((m, k), device="cuda", dtype=x_type), torch.zeros((n, k), device="cuda", dtype=x_type)
+        w[:, 1] = 1
+        if x_type is BF16:
+            x[:, 1] = torch.linspace(-9, 9, m, device="cuda")
+            z64 = x[:, 1:2].double()
+        else:
+            x[:, 1] = torch.arange(m, device="cuda") % 256 - 128
+            z64 = x[:, 1:2].double() / 16
+        scales = [torch.full((m,), 0.25, device="cuda"), torch.full((n,), 0.25, device="cuda")]
+        y64 = gelu64(z64, act)
+        for out in (F32, BF16, F16):
+            y = lo.linear(x, w, activation=act, out_dtype=out) if x_type is BF16 else lo.linear_8bit(x, scales[0], w, scales[1], activation=act, out_dtype=out)
+            assert bool((y == y[:, :1]).all())
+            within(y[:, :1], y64, y64.abs() * U[out] + act_off(z64, act, out is F32) + TINY[out], f"{act} {x_type} {out}")
