@@ -114,7 +114,7 @@ struct Eighth {
         fine = top < 0x7f800000u;
         to = top == 0 || !fine ? 0.f : top8 / (amax * up);
     }
-    __device__ __forceinline__ float scale(float s) const { return fine ? amax * s / top8 : __uint_as_float(0x7fc00000u); }
+    __device__ __forceinline__ float scale(float s) const { return !fine ? __uint_as_float(0x7fc00000u) : amax == 0.f ? 0.f : amax * s / top8; }
     __device__ __forceinline__ void store(uint8_t* q, float8_t t, int n, bool stream) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) t[i] = fminf(fmaxf(t[i] * up * to, -top8), top8);        // (NaN goes to -top8)

@@ -710,3 +710,16 @@ def test_activations_of_large_products_keep_their_digits(lo, act):
             y = lo.linear(x, w, activation=act, out_dtype=out) if x_type is BF16 else lo.linear_8bit(x, scales[0], w, scales[1], activation=act, out_dtype=out)
             assert bool((y == y[:, :1]).all())
             within(y[:, :1], y64, y64.abs() * U[out] + act_off(z64, act, out is F32) + TINY[out], f"{act} {x_type} {out}")
+
+
+# --------------------------------------------------------------------------- rows at the ends of the range
+
+
+@pytest.mark.parametrize("dtype", [E4M3, I8])
+def test_8bit_rows_of_zeros_without_eps(lo, dtype):
+    for dim in (7, 300, 20_001):
+        x = torch.zeros((3, dim), device="cuda")
+        x[1] = torch.arange(dim, device="cuda") + 1.0
+        q, scale = lo.rms_norm_8bit(x, eps=0.0, dtype=dtype)
+        assert scale[0].item() == scale[2].item() == 0 and bool((q[0::2].float() == 0).all())
+        eight_within(q[1:2], scale[1:2], norm_reference(x[1:2], None, None, 0.0)[2], dtype)
