@@ -715,6 +715,36 @@ def test_activations_of_large_products_keep_their_digits(lo, act):
 # --------------------------------------------------------------------------- rows at the ends of the range
 
 
+@pytest.mark.parametrize("dim", [5, 300, 3000, 20_001])
+@pytest.mark.parametrize("x_type", [F32, BF16])
+def test_norm_of_rows_whose_squares_leave_the_range(lo, x_type, dim):
+    """Squares of 1e20 and more overflow 32 bits, those of 1e-25 vanish (eps = 0): y, the stream, the 8-bit form and the gradients are as of any row,
+    and the rows beside them as ever."""
+    g = gen(51)
+    for eps, factors in ((1e-6, (1.0, 1e20, 1e25, 3e36, 1.0)), (0.0, (1.0, 1e-17, 1e-25, 1e-37, 1e30, 1.0))):
+        rows = len(factors)
+        x = normal((rows, dim), F32, g)
+        x = (x / x.abs().amax(dim=1, keepdim=True) * torch.tensor(factors, device="cuda")[:, None]).to(x_type)
+        res = (normal((rows, dim), F32, g).clamp(-3, 3) * torch.tensor(factors, device="cuda")[:, None] * 0.25).to(x_type)
+        w, dy = normal((1, dim), x_type, g)[0], normal((rows, dim), x_type, g)
+        for r in (None, res):
+            h64, _, y64 = norm_reference(x, w, r, eps)
+            y = lo.rms_norm(x, w, residual=r, eps=eps, out_dtype=F32)
+            if r is not None:
+                y, h = y
+                within(h, h64, h64.abs() * (U[x_type] + E) + TINY[x_type], "h")
+            # (x + r is rounded to 32 bits first: a unit, and one of the smallest step where that is all it has)
+            within(y, y64, y64.abs() * (U[F32] + 64 * E) + (TINY[F32] / h64.abs().amax(dim=1, keepdim=True)) * y64.abs().amax(dim=1, keepdim=True), "y")
+            for dtype in (E4M3, I8):
+                q, scale, *_ = lo.rms_norm_8bit(x, w, residual=r, eps=eps, dtype=dtype)
+                eight_within(q, scale, y64, dtype)
+        dx, dw = lo.rms_norm_grad(dy, x, w, eps=eps)
+        dx64, size, dw64, dw_size = grad_reference(dy, x, w, eps, None)
+        fits = dx64.abs() < 3.3e38                                       # (of the smallest rows 16 / 2e-38 does not)
+        within(dx[fits], dx64[fits], (dx64.abs() * U[x_type] + size * 128 * E + TINY[x_type])[fits], "dx")
+        within(dw, dw64, dw64.abs() * U[x_type] + dw_size * (rows + 70) * E, "dw")
+
+
 @pytest.mark.parametrize("dtype", [E4M3, I8])
 def test_8bit_rows_of_zeros_without_eps(lo, dtype):
     for dim in (7, 300, 20_001):
