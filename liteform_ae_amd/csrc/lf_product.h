@@ -720,10 +720,14 @@ template <typename T, bool ACROSS, int ROWS> struct Direct {
     }
     // Load instruction i of a step, into the array of LDS that begins at `lds`.  (In assembly, since the compiler would have every transposing
     // read wait for all loads.  It has no output in registers; arrived() waits for it.)
+    // m0 is declared as written (nothing else here uses it, an access of the compiler's own might); that it belongs to the compiler is known.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
     __device__ __forceinline__ void load(uint32_t lds, int i) const {
         asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[i]), "s"(base), "s"(wave * (kLoad * 16)), "s"(lds + i * (4 * kLoad * 16))
-                     : "memory", "scc");
+                     : "memory", "m0", "scc");
     }
+#pragma clang diagnostic pop
     __device__ __forceinline__ void load_last(uint4_t* lds, int left) const {
         uint4_t r[kLoads];
         auto count = [&](int i) { return ACROSS ? (at(i) < left ? kElems : 0) : left - at(i); };
