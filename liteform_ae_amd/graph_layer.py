@@ -35,9 +35,11 @@ class Aggregation:
         return fa.HybSpMM(fa.build_hyb_format_device(g, widths), feat_size, b_dtype, windows=windows)
 
     def forward(self, y):
+        lo.refuse_graph("y", y)
         return self._forward.run(y if y.dtype is self.dtype else y.to(self.dtype))
 
     def backward(self, dC):
+        lo.refuse_graph("dC", dC)
         return self._backward.run(dC if dC.dtype is self.dtype else dC.to(self.dtype))
 
 

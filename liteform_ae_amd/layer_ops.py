@@ -13,6 +13,9 @@ The reference ends with the sparse product (format_algos.py:388-605) and has no 
 
 Matrices are CUDA tensors (rows, features) whose rows are contiguous; the distance from one row to the next is free, so a
 slice of a wider buffer's columns needs no copy.  float32, bfloat16 and float16, sums in 32 bits.
+
+What is returned is no part of a torch graph: gradients are those of ``rms_norm_grad`` and ``linear_grad``.  Tensors that require
+gradients are taken under ``torch.no_grad()`` only, and refused where torch would expect a graph.
 """
 from __future__ import annotations
 
@@ -39,6 +42,13 @@ def _begin():
     return torch, _lib.load(), torch._C._cuda_getDevice()
 
 
+def refuse_graph(name, t):
+    """ValueError where a gradient that torch is asked for would be lost without a word."""
+    if t.requires_grad and _torch().is_grad_enabled():
+        raise ValueError(f"{name} requires gradients, and what is returned would not lead back to it: call this under torch.no_grad() (or pass "
+                         f"{name}.detach()) and take them from rms_norm_grad and linear_grad")
+
+
 def _matrix(name, t, types, device, rows=None, cols=None):
     """(address, elements from row to row, type) of a matrix operand; ValueError unless it is one of the current device, and of
     (rows, cols) where they are given."""
@@ -48,6 +58,8 @@ def _matrix(name, t, types, device, rows=None, cols=None):
         want = "(rows, features)" if rows is None else (rows, cols)
         raise ValueError(f"{name} must be a tensor of shape {want} on the current device, cuda:{device}, and one of {[str(d) for d in types]}, "
                          f"got {tuple(t.shape)} of {t.dtype} on {t.device}")
+    if t.requires_grad:
+        refuse_graph(name, t)
     across, along = t.stride()
     cols = shape[1]
     if (along != 1 and cols > 1) or (across < cols and shape[0] > 1):
@@ -61,6 +73,8 @@ def _vector(name, t, types, device, size):
     if code is None or len(shape) != 1 or shape[0] != size or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of {size} elements on the current device, cuda:{device}, and one of "
                          f"{[str(d) for d in types]}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+    if t.requires_grad:
+        refuse_graph(name, t)
     return t.data_ptr(), code
 
 

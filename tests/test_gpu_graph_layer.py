@@ -207,3 +207,15 @@ def test_training_with_a_layer_that_stands_twice(setup):
         for p, p64 in zip(each.parameters(), each.p64):
             step = rate * p64.grad
             assert float((p.double() - (p64.detach() - step)).norm()) <= 2e-5 * float(step.norm()) + 2.0 ** -24 * float(p64.detach().norm() + step.norm())
+
+
+def test_inputs_that_require_gradients(setup):
+    gl, g, layers, y, h, target = setup
+    layer = layers[0]
+    want = layer.forward(y, h)
+    for a, b in ((y.clone().requires_grad_(), h), (y, h.clone().requires_grad_())):
+        for call in (layer.forward, layer.forward_8bit):
+            with pytest.raises(ValueError, match="no_grad"):
+                call(a, b)
+        with torch.no_grad():
+            assert all(torch.equal(c, d) for c, d in zip(layer.forward(a, b), want))

@@ -753,3 +753,25 @@ def test_8bit_rows_of_zeros_without_eps(lo, dtype):
         q, scale = lo.rms_norm_8bit(x, eps=0.0, dtype=dtype)
         assert scale[0].item() == scale[2].item() == 0 and bool((q[0::2].float() == 0).all())
         eight_within(q[1:2], scale[1:2], norm_reference(x[1:2], None, None, 0.0)[2], dtype)
+
+
+def test_tensors_that_require_gradients(lo):
+    """Refused where torch would build a graph, as its gradients would end here; taken under no_grad, with the results of any others."""
+    g = gen(61)
+    x, w, b, v, r = normal((20, 64), F32, g), normal((32, 64), F32, g), normal((1, 32), F32, g)[0], normal((1, 64), F32, g)[0], normal((20, 64), F32, g)
+    dy, z, y = normal((20, 32), F32, g), normal((20, 32), F32, g), normal((20, 32), F32, g)
+    q, s = lo.quantize_rows(x)
+    p, t = lo.quantize_rows(w)
+    calls = [(lo.rms_norm, [x, v, r]), (lo.rms_norm_8bit, [x, v, r]), (lo.quantize_rows, [x]), (lo.rms_norm_grad, [r, x, v]),
+             (lambda a, d: lo.rms_norm_grad(r, a, v, dh=d), [x, r]), (lambda *a: lo.linear(*a[:3], "gelu", a[3]), [x, w, b, y]),
+             (lambda a, c, e, f: lo.linear_8bit(q, a, p, c, e, residual=f), [s, t, b, y]), (lambda *a: lo.linear_grad(*a, activation="gelu"), [dy, x, w, z])]
+    for call, args in calls:
+        want = call(*args)
+        for i in range(len(args)):
+            with_graph = [a.clone().requires_grad_() if k == i else a for k, a in enumerate(args)]
+            with pytest.raises(ValueError, match="no_grad"):
+                call(*with_graph)
+            with torch.no_grad():
+                got = call(*with_graph)
+            for a, c in zip(*((r if isinstance(r, tuple) else (r,)) for r in (got, want))):
+                assert a is None and c is None or torch.equal(a.float(), c.float())
