@@ -16,7 +16,7 @@
 //   * float32 has no fast matrix instruction.  A value is cut into three bfloat16 of 8 bits each (exactly: by truncation), and
 //     six of the nine products - all but those below 2^-24 of the largest - go through the bfloat16 one, which is 16 times as fast
 //     as the float32 one: 4096^3 695 us (198 TFLOP/s), the library's float32 product 940.  Bound by the matrix cores there, by memory where
-//     k is short (170k x 128 by 256 117 us, 3.8 TB/s).  Inf and NaN do not survive the cut; outputs that are not finite are computed again from the operands.
+//     k is short (170k x 128 by 256 117 us, 3.8 TB/s).  Inf and NaN do not survive the cut; outputs that are not finite are computed again from the operands (repair).
 //   * Few tiles are cut along k as well: partial sums in 32 bits, added up in a fixed order by a second kernel with the epilogue.
 // Up to 16 rows of X are another problem - W is read once, nothing is shared - and have a kernel of their own.
 #pragma once
@@ -280,11 +280,62 @@ template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
     }
 };
 
-// One output of a float32 product from the operands themselves, whose elements are so far apart.
-__device__ __forceinline__ float dot_f32(const float* p, int64_t p_step, const float* q, int64_t q_step, int64_t k) {
-    float s = 0.f;
-    for (; k > 0; --k, p += p_step, q += q_step) s = fmaf(*p, *q, s);
-    return s;
+// Sums of planes that are not finite: infinities, NaN and values near the ends of the exponents' range do not survive the cut, or leave the range on the
+// way.  Sixteen rows of P with such an output are multiplied again by float32 matrix instructions, operands from memory; finite sums stay as they
+// are.  (Each output by a lane of its own, along k: a NaN in 1024^3 took 525 us where 40 are usual, an operand of NaN in 4096^3 73 ms for 0.7; now 58 us
+// and 2.8 ms.)
+template <bool ACROSS> __device__ __forceinline__ uint4_t four_of(const float* p, int64_t ld, int64_t row, int64_t k, int64_t end) {
+    if constexpr (!ACROSS) return load16_each(p + row * ld + k, (int)max((int64_t)0, min((int64_t)4, end - k)));
+    uint4_t r = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (k + c < end) r[c] = __float_as_uint(p[(k + c) * ld + row]);
+    return r;
+}
+template <bool PX, bool QX, int FM, int FN>
+__device__ __forceinline__ void repair(const Product& g, float4_t (&acc)[FM][FN], int64_t m, int64_t n, int64_t k_first, int64_t k_last) {
+    const int li = threadIdx.x & 15, lg = threadIdx.x >> 4 & 3;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        float none = 0.f;                                                // NaN where a sum is not finite
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) none = fmaf(acc[i][j][v], 0.f, none);
+        if (__builtin_expect(__all(none == 0.f), 1)) continue;
+        bool fine = true;                                                // ... in rows and columns that there are
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) fine = fine && (fabsf(acc[i][j][v]) < __builtin_inff() || n + 16 * j + 4 * lg + v >= g.n);
+        if (__all(fine || m + 16 * i + li >= g.m)) continue;
+        float4_t again[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) again[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+        uint4_t p, q[FN];
+        auto load = [&](int64_t k) {                                     // (sixteen k: four of a lane, the same ones of both operands)
+            p = four_of<PX>((const float*)g.p, g.ld_p, min(m + 16 * i + li, g.m - 1), k + 4 * lg, k_last);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) q[j] = four_of<QX>((const float*)g.q, g.ld_q, min(n + 16 * j + li, g.n - 1), k + 4 * lg, k_last);
+        };
+        load(k_first);
+#pragma unroll 1
+        for (int64_t k = k_first; k < k_last; k += 16) {
+            const uint4_t b = p;
+            uint4_t a[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) a[j] = q[j];
+            load(k + 16);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) again[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j][c]), __uint_as_float(b[c]), again[j], 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) acc[i][j][v] = fabsf(acc[i][j][v]) < __builtin_inff() ? acc[i][j][v] : again[j][v];
+    }
 }
 
 // What a wavefront does with its WC columns of sums from (m, n) on: partial ones go to the work space, others through the epilogue.
@@ -292,7 +343,6 @@ __device__ __forceinline__ float dot_f32(const float* p, int64_t p_step, const f
 // residual is read and the output written in whole lines.  The residual of PR rows is under way while their sums are turned: one after the
 // other, its pieces would wait for memory each (bf16 8192^3, four rows at a time: 889 us).  Wavefronts at the last
 // columns, with pieces of less than eight, take them one by one.
-// float32: `again(row, column)` computes an output from the operands.
 template <int N> __device__ __forceinline__ void activate_all(float8_t (&v)[N], int32_t act) {
     auto all = [&](auto f) {
 #pragma unroll
@@ -334,10 +384,9 @@ template <int TM, int TN> struct Vectors {
         if (t < TM) x_scale[t] = l.x;
     }
 };
-struct None {};
 // (m0, n0): of the tile that `vec` is of
-template <int FM, int FN, int PR, typename Acc, typename Vec, typename Again>
-__device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN], uint4_t* lds, const Vec& vec, int64_t m0, int64_t n0, int row0, int col0, Again again) {
+template <int FM, int FN, int PR, typename Acc, typename Vec>
+__device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN], uint4_t* lds, const Vec& vec, int64_t m0, int64_t n0, int row0, int col0) {
     constexpr int WC = 16 * FN, LANES = WC / 8, AT_ONCE = 64 / LANES, U = PR / AT_ONCE, PHASES = FM * 16 / PR;
     constexpr bool INT = std::is_same_v<Acc, int4v>;
     static_assert(FM * 16 % PR == 0 && PR % AT_ONCE == 0 && PHASES <= 4, "");
@@ -384,21 +433,6 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
             }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        if constexpr (!std::is_same_v<Again, None>) {
-#pragma unroll 1
-            for (int row = mine; row < PR && m + FIRST + row < g.m; row += AT_ONCE) {
-                const float8_t v = sums(row);
-                bool fine = true;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) fine = fine && fabsf(v[i]) < __builtin_inff();
-                if (!fine)
-#pragma unroll 1
-                    for (int i = 0; i < count; ++i) {
-                        float* s = (float*)place(row, i >> 2) + (i & 3);
-                        if (!(fabsf(*s) < __builtin_inff())) *s = again(m + FIRST + row, n + i);
-                    }
-            }
-        }
         if (__builtin_expect(g.part != nullptr, 0)) {
 #pragma unroll 2
             for (int row = mine; row < PR; row += AT_ONCE)
@@ -627,13 +661,8 @@ product_kernel(Product g) {
     static_assert(PR <= FIT && WHOLE % PR == 0, "");
     uint4_t* mine = s_all + wave * SLOTS;
     const int row0 = wm * (TM / WM), col0 = wn * (TN / WN);
-    if constexpr (PL == 3)
-        leave<FM, FN, PR>(g, acc, mine, s_vec, m0, n0, row0, col0, [&](int64_t row, int64_t col) {
-            return dot_f32((const float*)g.p + (PX ? k_first * g.ld_p + row : row * g.ld_p + k_first), PX ? g.ld_p : 1,
-                           (const float*)g.q + (QX ? k_first * g.ld_q + col : col * g.ld_q + k_first), QX ? g.ld_q : 1, k_last - k_first);
-        });
-    else
-        leave<FM, FN, PR>(g, acc, mine, s_vec, m0, n0, row0, col0, None{});
+    if constexpr (PL == 3) repair<PX, QX>(g, acc, m0 + row0, n0 + col0, k_first, k_last);
+    leave<FM, FN, PR>(g, acc, mine, s_vec, m0, n0, row0, col0);
 }
 
 // ---------------------------------------------------------------------------- the tiled product, large tiles
@@ -875,7 +904,7 @@ wide_kernel(Product g) {
     for (int i = 0; i < 8; ++i) settle(acc[i]);
     __syncthreads();
     uint4_t* mine = P.wave == 0 ? s_p0 : P.wave == 1 ? s_q0 : P.wave == 2 ? s_p1 : s_q1;
-    leave<8, 8, 64>(g, acc, mine, s_vec, m0, n0, row_p, row_q, None{});
+    leave<8, 8, 64>(g, acc, mine, s_vec, m0, n0, row_p, row_q);
 }
 
 // ---------------------------------------------------------------------------- the tiled product, aligned operands, small tiles
@@ -994,7 +1023,7 @@ direct_kernel(Product g) {
         multiply(o);
     }
     arrived();
-    leave<FR, FR, TILE / 2 < 32 ? TILE / 2 : 32>(g, acc, s + P.wave * (SB / 2), s_vec, m0, n0, row_p, row_q, None{});
+    leave<FR, FR, TILE / 2 < 32 ? TILE / 2 : 32>(g, acc, s + P.wave * (SB / 2), s_vec, m0, n0, row_p, row_q);
 }
 
 template <typename T, bool PX, bool QX> ProductFn kernel_of(int tile, bool aligned, bool deep) {
