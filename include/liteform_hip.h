@@ -58,7 +58,7 @@ extern "C" {
 
 #define LF_ACT_NONE 0
 #define LF_ACT_RELU 1
-#define LF_ACT_GELU 2           /* z Phi(z), Phi by erf */
+#define LF_ACT_GELU 2           /* z Phi(z), Phi that of the normal distribution */
 #define LF_ACT_SILU 3           /* z / (1 + exp(-z)) */
 
 #define LF_COST_REFERENCE 0     /* format_algos.py:1035-1166 bit for bit */
@@ -441,7 +441,8 @@ int lf_bsr_spmm_trusted_nnz(const int32_t* d_indptr, const int32_t* d_indices, c
  *
  * lf_rms_norm: h = x + residual (NULL: h = x, and d_h is NULL too), y = h / sqrt(mean(h^2) + eps) * weight (NULL: ones).  d_h receives
  * h in the residual's type.  y_dtype LF_DTYPE_E4M3 / LF_DTYPE_I8: q = y / scale to the nearest, with d_scale[row] = max|y| / 448 (/ 127),
- * 0 for a row of zeros, NaN for one with Inf or NaN; d_scale is NULL otherwise.
+ * 0 for a row of zeros, NaN for one with Inf or NaN; d_scale is NULL otherwise.  Rows whose squares overflow or vanish in 32 bits come out as any others
+ * (with eps = 0 y of a row of zeros is 0 / 0).
  * lf_quantize_rows: the same 8-bit form of rows as they are (a weight).
  * lf_rms_norm_grad: from dy and h, dx = gradient of h - x and the residual have the same one - plus d_dh (NULL: none), what comes
  * down the residual stream; dw [dim] in the weight's type (NULL: not wanted; else lf_rms_norm_grad_work_bytes bytes of work space,
@@ -458,7 +459,8 @@ int lf_rms_norm_grad(const void* d_dy, int64_t ld_dy, int32_t dy_dtype, const vo
                      void* d_dw, void* d_work, size_t work_bytes, lf_stream_t stream);
 
 /* y = act(x w^T + bias) + residual for x [m][k], w [n][k] of one type, `dtype`.  float32, bfloat16 and float16; LF_DTYPE_E4M3 and LF_DTYPE_I8 with a
- * scale for every row of x and of w (k < 2^17 for int8).  Sums are in 32 bits (float32: as exact as a float32 product).  bias [n], residual
+ * scale for every row of x and of w (k < 2^17 for int8).  Sums are in 32 bits (float32: as exact as a float32 product of values from 2^-110 on; what
+ * smaller ones have below 2^-126 may be lost).  gelu and silu keep their digits at any z, to some 20 roundings of 32 bits for float32 y and about 1e-5 for others.  bias [n], residual
  * [m][n] and z [m][n], which receives x w^T + bias, may be NULL; they and y are float32, bfloat16 or float16, each of its own.
  * lf_linear_work_bytes bytes of device memory, 16-byte aligned, that no other call uses meanwhile (0: d_work may be NULL).
  *

@@ -42,7 +42,7 @@ template <typename T> __device__ __forceinline__ void store8(T* p, float8_t f, b
     reinterpret_cast<typename Eight<T>::Any*>(p)->v = v;
 }
 // Outputs of this many bytes are stored past the caches: norm of 16k x 4096 into e4m3 90.9 -> 86.2 us, its gradient at 32k x 2048 105.1 -> 102.7,
-// product bf16 8192^3 813 -> 801, e4m3 16k x 4k x 4k 293.5 -> 285.7.  Smaller ones the next operation may find there.
+// e4m3 product of 16k x 4k x 4k 293.5 -> 285.7 (bf16 8192^3: less than its runs differ by).  Smaller ones the next operation may find there.
 constexpr int64_t kStreamBytes = 64ll << 20;
 // 16 bytes at any address that suits the type
 template <typename T> __device__ __forceinline__ uint4_t load16(const T* p) {

@@ -17,7 +17,7 @@
 // A row of a length that is no multiple of eight ends in a piece that reaches back into the piece before it: its elements
 // are read and written twice, with the same values, and summed once.
 //
-// Measured, against a copy of 1 GiB at 5.04 TB/s: float32 170k x 128 with a float32 stream 73 us (4.8 TB/s), bfloat16 16k x 4096 into e4m3 86 (5.5),
+// Measured, against a copy of 1 GiB at 5.04 TB/s: float32 170k x 128 with a float32 stream 70 us (5.0 TB/s), bfloat16 16k x 4096 into e4m3 86 (5.5),
 // gradient of bfloat16 32k x 2048 103 (5.2), of float16 5003 x 1001 in odd rows 12 + 4 (two launches); one row of 4096 features 4.
 #include <algorithm>
 

@@ -16,7 +16,8 @@
 //   * float32 has no fast matrix instruction.  A value is cut into three bfloat16 of 8 bits each (exactly: by truncation), and
 //     six of the nine products - all but those below 2^-24 of the largest - go through the bfloat16 one, which is 16 times as fast
 //     as the float32 one: 4096^3 695 us (198 TFLOP/s), the library's float32 product 940.  Bound by the matrix cores there, by memory where
-//     k is short (170k x 128 by 256 117 us, 3.8 TB/s).  Inf and NaN do not survive the cut; outputs that are not finite are computed again from the operands (repair).
+//     k is short (170k x 128 by 256 116 us, 3.8 TB/s).  Inf and NaN do not survive the cut; outputs that are not finite are computed again from the operands (repair).
+//     What a cut leaves below 2^-126 is lost to the instruction: values below 2^-110 have fewer digits than a float.
 //   * Few tiles are cut along k as well: partial sums in 32 bits, added up in a fixed order by a second kernel with the epilogue.
 // Up to 16 rows of X are another problem - W is read once, nothing is shared - and have a kernel of their own.
 #pragma once
@@ -676,8 +677,8 @@ product_kernel(Product g) {
 // others.  The order of the instructions is the one written here: one of these beside every product or two.  (Left to the compiler's scheduler, reads stood
 // together and products waited for them: bf16 8192^3 999 us.)
 // A last step of less than 128 bytes of k goes through registers, with zeros behind the end.
-// Measured: bf16 8192^3 with bias, silu and residual 800 - 827 us (1340 TFLOP/s; a library product without them 802), matrix cores busy for 70 % of the cycles at
-// a clock of 1.7 GHz; e4m3 16k x 4k x 4k with gelu and residual 286 - 293, 60 - 80 of them epilogue; bf16 across k 4096 x 4096 x 8192 207 - 223.
+// Measured: bf16 8192^3 with bias, silu and residual 800 - 850 us by the clock (1290 - 1370 TFLOP/s; a library product without them 802), matrix cores busy for 70 % of the cycles at
+// a clock of 1.7 GHz; e4m3 16k x 4k x 4k with gelu and residual 285 - 301, 60 - 80 of them epilogue; bf16 across k 4096 x 4096 x 8192 207 - 242.
 
 template <typename T> struct Frag { uint4_t c[2]; };                      // 64 bytes of k of a row: two pieces of a lane
 

@@ -44,7 +44,8 @@ class Aggregation:
 
 
 class GraphLayer:
-    """One layer with its parameters, in float32 or bfloat16.  ``backward`` returns the gradients of a call of ``forward`` that kept what they need."""
+    """One layer with its parameters, in float32 or bfloat16.  ``backward`` returns the gradients of a call of ``forward`` that kept what they need;
+    torch builds no graph through a layer, and one is called under ``torch.no_grad()`` where tensors require gradients."""
 
     def __init__(self, aggregation: Aggregation, feat_size: int, activation: str = "gelu", dtype=None, generator=None, eps: float = 1e-6):
         torch = fa._torch()

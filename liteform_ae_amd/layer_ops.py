@@ -136,7 +136,8 @@ def _norm(torch, lib, device, x, weight, residual, eps, dtype, code, eight):
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-6, out_dtype=None):
     """``y = h / sqrt(mean(h^2) + eps) * weight`` with ``h = x + residual``, by rows.  Returns ``y``, and with a residual
     ``(y, h)``: h, the stream that the next layer adds to, in the residual's type, y in ``out_dtype`` (default: x's).  The
-    norm is of h before that rounding.  x and residual may be of different types (an f32 product, a bf16 stream)."""
+    norm is of h before that rounding.  x and residual may be of different types (an f32 product, a bf16 stream).  Rows whose squares
+    overflow or vanish in 32 bits come out as any others; ``eps=0`` makes y of a row of zeros NaN."""
     torch, lib, device = _begin()
     dtype = x.dtype if out_dtype is None else out_dtype
     y, _, h = _norm(torch, lib, device, x, weight, residual, eps, dtype, _float_type("out_dtype", dtype), False)
@@ -234,7 +235,8 @@ def linear(x, weight, bias=None, activation=None, residual=None, out_dtype=None,
     """``y = act(x weight^T + bias) + residual`` for x (rows, k) and weight (n, k) of one type; ``activation`` is None, "relu",
     "gelu" (by erf) or "silu".  bias and residual are floating tensors of any type, y is of ``out_dtype`` (default: x's).
     ``return_preactivation=True`` returns ``(y, z)`` with z = x weight^T + bias in x's type, which ``linear_grad`` needs behind an
-    activation.  float32 products are as exact as float32 sums of float32 products."""
+    activation.  float32 products are as exact as float32 sums of float32 products of values from 2^-110 (8e-34) on; what smaller ones
+    have below 2^-126 may be lost.  gelu and silu keep their digits at any z (float32 y: some 20 roundings)."""
     torch, lib, device = _begin()
     out = x.dtype if out_dtype is None else out_dtype
     y, z = _linear(torch, lib, device, x, weight, None, None, bias, activation, residual, _FLOATS, out, x.dtype if return_preactivation else None)

@@ -1,4 +1,4 @@
-"""float32 products with many values that are not finite: right as any others, and not much slower."""
+"""float32 products at the ends of the range: with many values that are not finite, right as any others and not much slower; of the smallest ones."""
 import math
 
 import pytest
@@ -78,3 +78,19 @@ def test_an_operand_of_nan_takes_a_few_times_as_long(lo):  # noqa: F811
     bad = torch.full_like(x, math.nan)
     time(x), time(bad)
     assert time(bad) <= 12 * time(x)
+
+
+@pytest.mark.parametrize("power", [-100, -112, -118, -124, -130])
+def test_values_near_the_smallest(lo, power):  # noqa: F811
+    """What a value's three bfloat16 leave below 2^-126 is lost to the matrix instruction, and so is a sum below it at each of its instructions."""
+    g = gen(74)
+    lost = 2.0 ** -126
+    for m, n, k in [(64, 70, 256), (300, 200, 1000), (40, 30, 9000)]:
+        x, w = normal((m, k), F32, g) * 2.0 ** power, normal((n, k), F32, g)
+        x64, w64 = x.double(), w.double()
+        want = x64 @ w64.t()
+        bound = (x64.abs() @ w64.abs().t()) * (k + 24) * E + 1.01 * lost * (x64.abs().sum(dim=1)[:, None] + w64.abs().sum(dim=1)) + 6 * (k // 32 + 1) * lost
+        assert bool(((lo.linear(x, w).double() - want).abs() <= bound).all()), (m, n, k)
+    x, w = normal((16, 300), F32, g) * 2.0 ** power, normal((40, 300), F32, g)         # (few rows: float32 instructions)
+    x64, w64 = x.double(), w.double()
+    assert bool(((lo.linear(x, w).double() - x64 @ w64.t()).abs() <= (x64.abs() @ w64.abs().t()) * 324 * E + TINY[F32]).all())
