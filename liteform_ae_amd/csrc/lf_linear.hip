@@ -253,7 +253,7 @@ size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // Threads across a row (of eight columns each), and slabs of rows whose column sums are kept apart: enough workgroups to fill the GPU.
 int threads_across(int64_t n) { return n <= 64 ? 8 : n <= 128 ? 16 : 32; }
 int64_t slabs_of(int64_t m, int64_t n) {
-    return std::max<int64_t>(1, std::min(ceil_div(m, 64), ceil_div(512, std::min<int64_t>(4, ceil_div(n, 256)))));
+    return std::max<int64_t>(1, std::min(ceil_div(m, 64), ceil_div(512, std::clamp<int64_t>(ceil_div(n, 256), 1, 4))));
 }
 
 struct GradWork { size_t dz, sums, parts, total; };

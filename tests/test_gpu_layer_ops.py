@@ -775,3 +775,25 @@ def test_tensors_that_require_gradients(lo):
                 got = call(*with_graph)
             for a, c in zip(*((r if isinstance(r, tuple) else (r,)) for r in (got, want))):
                 assert a is None and c is None or torch.equal(a.float(), c.float())
+
+
+@pytest.mark.parametrize("x_type", [F32, BF16])
+def test_products_of_sizes_of_zero(lo, x_type):
+    """No rows, no features out, none in, in every combination: sums of nothing are 0."""
+    g = gen(81)
+    for m in (0, 1, 40, 700):
+        for n in (0, 1, 24, 300):
+            for k in (0, 1, 40, 300):
+                if m and n and k:
+                    continue
+                x, w, dy, z = normal((m, k), x_type, g), normal((n, k), x_type, g), normal((m, n), x_type, g), normal((m, n), x_type, g)
+                b = normal((1, n), F32, g)[0]
+                y = lo.linear(x, w, b, activation="relu", residual=dy)
+                y64 = b.double().clamp_min(0) + dy.double()
+                within(y, y64, y64.abs() * (U[x_type] + 4 * E), f"y {(m, n, k)}")
+                for act in ACTS:
+                    dx, dw, db = lo.linear_grad(dy, x, w, z=z, activation=act, bias_dtype=F32)
+                    assert dx.shape == (m, k) and dw.shape == (n, k) and db.shape == (n,)
+                    assert bool((dx == 0).all()) and bool((dw == 0).all())
+                    dz = dy.double() if act is None else dy.double() * act_grad64(z.double(), act)
+                    within(db, dz.sum(dim=0), (dz.abs() + dy.double().abs()).sum(dim=0) * (m + 40) * E, f"db {(m, n, k)}")

@@ -30,3 +30,17 @@ def test_tiled_products_keep_their_sums_in_registers(kernels):  # noqa: F811
     assert len([n for n in tiled if "wide_kernel" in n]) == 8
     # (large tiles: a few words outside the loop over k, whose 256 sums and operands take all 512 registers)
     assert {n: v for n, v in tiled.items() if v[1] > (64 if "wide_kernel" in n else 0)} == {}
+
+
+def test_work_bytes_of_sizes_of_zero():
+    from liteform_ae_amd import _lib
+    lib = _lib.load()
+    for m in (0, 1, 700):
+        for n in (0, 1, 300):
+            for k in (0, 1, 300):
+                lib.lf_linear_work_bytes(m, n, k, _lib.LF_DTYPE_BF16)
+                for act in (_lib.LF_ACT_NONE, _lib.LF_ACT_GELU):
+                    need = lib.lf_linear_grad_work_bytes(m, n, k, _lib.LF_DTYPE_BF16, act, 1, 1, 1)
+                    assert need == 0 or m * n > 0
+    for rows, dim in ((0, 8), (8, 0), (0, 0), (-1, 8), (8, -1)):
+        assert lib.lf_rms_norm_grad_work_bytes(rows, dim) == 0
