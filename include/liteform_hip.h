@@ -484,6 +484,68 @@ int lf_linear(const lf_linear_args* h_args, void* d_work, size_t work_bytes, lf_
 size_t lf_linear_grad_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t activation, int32_t want_dx, int32_t want_dw, int32_t want_db);
 int lf_linear_grad(const lf_linear_grad_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream);
 
+/* The gated product: z = x w^T + bias for w [2 n][k] and bias [2 n]; y [m][n] = act(z[:, :n]) z[:, n:], the first n rows of w being the gate's.  z
+ * [m][2 n] may be NULL, as bias; d_residual is.  Types, scales and work space as for lf_linear.
+ *
+ * lf_gated_linear_grad: from dy [m][n] and z [m][2 n], dz = [dy z[:, n:] act'(z[:, :n]) | dy act(z[:, :n])]; dx = dz w, dw [2 n][k] = dz^T x,
+ * db [2 n] = column sums of dz; any of the three may be NULL. */
+size_t lf_gated_linear_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype);
+int lf_gated_linear(const lf_linear_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream);
+size_t lf_gated_linear_grad_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t want_dx, int32_t want_dw, int32_t want_db);
+int lf_gated_linear_grad(const lf_linear_grad_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream);
+
+/* lf_layer_norm: h = x + residual (NULL: h = x, and d_h is NULL too), y = (h - mean(h)) / sqrt(var(h) + eps) * weight + bias (NULL: ones, zeros), by rows; var is
+ * the mean of (h - mean)^2.  The rest as for lf_rms_norm: d_h receives h in the residual's type, 8-bit y come with d_scale, rows whose sums overflow
+ * come out as any others.
+ * lf_layer_norm_grad: from dy and h, dx = gradient of h plus d_dh (NULL: none); dw [dim] in the weight's type and db [dim], sums over the rows
+ * (NULL: not wanted; work space where one is).  dx and d_dh have h's type. */
+typedef struct lf_layer_norm_args {
+    const void* d_x; const void* d_residual; const void* d_weight; const void* d_bias; void* d_y; float* d_scale; void* d_h;
+    int64_t ld_x, ld_residual, ld_y, ld_h, rows, dim;
+    int32_t x_dtype, residual_dtype, weight_dtype, bias_dtype, y_dtype;
+    float eps;
+} lf_layer_norm_args;
+typedef struct lf_layer_norm_grad_args {
+    const void* d_dy; const void* d_h; const void* d_weight; const void* d_dh; void* d_dx; void* d_dw; void* d_db;
+    int64_t ld_dy, ld_h, ld_dh, ld_dx, rows, dim;
+    int32_t dy_dtype, h_dtype, weight_dtype, db_dtype;
+    float eps;
+} lf_layer_norm_grad_args;
+int lf_layer_norm(const lf_layer_norm_args* h_args, lf_stream_t stream);
+size_t lf_layer_norm_grad_work_bytes(int64_t rows, int64_t dim);
+int lf_layer_norm_grad(const lf_layer_norm_grad_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream);
+
+/* lf_embedding: y[i] = scale * table[id_i], a row of zeros for an id outside 0 .. rows - 1 (padding).  n ids of ids_bits = 32 or 64 bits, ids_stride elements
+ * apart (0: one id for all); n and rows below 2^31.
+ * lf_embedding_grad: grad[v] = scale * sum over i with id_i = v of dy[i], in order of i, all rows of it; work space as lf_embedding_grad_work_bytes says, 16-byte aligned. */
+typedef struct lf_embedding_args {
+    const void* d_ids; const void* d_table; void* d_y;
+    int64_t ids_stride, ld_table, ld_y, n, rows, dim;
+    int32_t ids_bits, table_dtype, y_dtype;
+    float scale;
+} lf_embedding_args;
+typedef struct lf_embedding_grad_args {
+    const void* d_dy; const void* d_ids; void* d_grad;
+    int64_t ids_stride, ld_dy, ld_grad, n, rows, dim;
+    int32_t ids_bits, dy_dtype, grad_dtype;
+    float scale;
+} lf_embedding_grad_args;
+int lf_embedding(const lf_embedding_args* h_args, lf_stream_t stream);
+size_t lf_embedding_grad_work_bytes(int64_t n, int64_t rows, int64_t dim);
+int lf_embedding_grad(const lf_embedding_grad_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream);
+
+/* lf_clip_gradients: *d_norm (device memory) = sqrt(sum over n tensors of their elements' squares), added in 64 bits; each d_dst = d_src * min(1, most / (norm + eps)),
+ * which is 1 for a norm of 0.  A norm that is NaN leaves NaN, an infinite one zeros and, of the infinities, NaN.  d_dst NULL in all tensors: the norm alone.  d_dst may be
+ * d_src (with its ld), but may lie on no other tensor: LF_ERR_INVALID.  The tensors are read before the call returns; nothing is copied to
+ * the GPU.  Work space as lf_clip_work_bytes says, 16-byte aligned. */
+typedef struct lf_tensor_desc {
+    const void* d_src; void* d_dst;
+    int64_t rows, cols, ld_src, ld_dst;
+    int64_t dtype;
+} lf_tensor_desc;
+size_t lf_clip_work_bytes(int32_t n);
+int lf_clip_gradients(const lf_tensor_desc* h_tensors, int32_t n, float most, float eps, float* d_norm, void* d_work, size_t work_bytes, lf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

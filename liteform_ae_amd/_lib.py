@@ -63,6 +63,37 @@ class LinearGradArgs(C.Structure):
                 + [(n, C.c_int32) for n in ("dtype", "db_dtype", "activation")])
 
 
+class LayerNormArgs(C.Structure):
+    """struct lf_layer_norm_args"""
+    _fields_ = ([(n, vp) for n in ("x", "residual", "weight", "bias", "y", "scale", "h")]
+                + [(n, C.c_int64) for n in ("ld_x", "ld_residual", "ld_y", "ld_h", "rows", "dim")]
+                + [(n, C.c_int32) for n in ("x_dtype", "residual_dtype", "weight_dtype", "bias_dtype", "y_dtype")] + [("eps", C.c_float)])
+
+
+class LayerNormGradArgs(C.Structure):
+    """struct lf_layer_norm_grad_args"""
+    _fields_ = ([(n, vp) for n in ("dy", "h", "weight", "dh", "dx", "dw", "db")]
+                + [(n, C.c_int64) for n in ("ld_dy", "ld_h", "ld_dh", "ld_dx", "rows", "dim")]
+                + [(n, C.c_int32) for n in ("dy_dtype", "h_dtype", "weight_dtype", "db_dtype")] + [("eps", C.c_float)])
+
+
+class EmbeddingArgs(C.Structure):
+    """struct lf_embedding_args"""
+    _fields_ = ([(n, vp) for n in ("ids", "table", "y")] + [(n, C.c_int64) for n in ("ids_stride", "ld_table", "ld_y", "n", "rows", "dim")]
+                + [(n, C.c_int32) for n in ("ids_bits", "table_dtype", "y_dtype")] + [("scale", C.c_float)])
+
+
+class EmbeddingGradArgs(C.Structure):
+    """struct lf_embedding_grad_args"""
+    _fields_ = ([(n, vp) for n in ("dy", "ids", "grad")] + [(n, C.c_int64) for n in ("ids_stride", "ld_dy", "ld_grad", "n", "rows", "dim")]
+                + [(n, C.c_int32) for n in ("ids_bits", "dy_dtype", "grad_dtype")] + [("scale", C.c_float)])
+
+
+class TensorDesc(C.Structure):
+    """struct lf_tensor_desc"""
+    _fields_ = [(n, vp) for n in ("src", "dst")] + [(n, C.c_int64) for n in ("rows", "cols", "ld_src", "ld_dst", "dtype")]
+
+
 # name -> (restype, argtypes); one entry per function declared in the header
 SIGNATURES = {
     "lf_version": (C.c_int, []),
@@ -125,6 +156,18 @@ SIGNATURES = {
     "lf_linear": (C.c_int, [vp, vp, C.c_size_t, vp]),
     "lf_linear_grad_work_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "lf_linear_grad": (C.c_int, [vp, vp, C.c_size_t, vp]),
+    "lf_gated_linear_work_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64, C.c_int32]),
+    "lf_gated_linear": (C.c_int, [vp, vp, C.c_size_t, vp]),
+    "lf_gated_linear_grad_work_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "lf_gated_linear_grad": (C.c_int, [vp, vp, C.c_size_t, vp]),
+    "lf_layer_norm": (C.c_int, [vp, vp]),
+    "lf_layer_norm_grad_work_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
+    "lf_layer_norm_grad": (C.c_int, [vp, vp, C.c_size_t, vp]),
+    "lf_embedding": (C.c_int, [vp, vp]),
+    "lf_embedding_grad_work_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),
+    "lf_embedding_grad": (C.c_int, [vp, vp, C.c_size_t, vp]),
+    "lf_clip_work_bytes": (C.c_size_t, [C.c_int32]),
+    "lf_clip_gradients": (C.c_int, [vp, C.c_int32, C.c_float, C.c_float, vp, vp, C.c_size_t, vp]),
 }
 
 _lock = threading.Lock()

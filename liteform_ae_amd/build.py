@@ -18,7 +18,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblfhip.so")
 
 SOURCES = ["lf_error.cpp", "lf_search.cpp", "lf_format.hip", "lf_spmm.hip", "lf_csr.hip", "lf_cells.hip", "lf_bsr.hip", "lf_ingest.hip",
-           "lf_norm.hip", "lf_linear.hip", "lf_product_f32.hip", "lf_product_bf16.hip", "lf_product_f16.hip", "lf_product_8bit.hip"]
+           "lf_norm.hip", "lf_layer_norm.hip", "lf_embedding.hip", "lf_clip.hip", "lf_linear.hip", "lf_product_f32.hip", "lf_product_bf16.hip", "lf_product_f16.hip", "lf_product_8bit.hip"]
 
 # -ffp-contract=off: the width search must add and multiply doubles exactly like CPython.
 # packed-fp32-ops is switched off for device code on purpose (scalar fp32 FMAs only).

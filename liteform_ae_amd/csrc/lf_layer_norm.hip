@@ -1,0 +1,580 @@
+// Layer norm of rows of features with the addition of the residual stream, its output in the stream's types or in 8 bits with a
+// scale a row, and its gradient.
+//
+//     h = x + r;  mu = mean(h);  s = 1 / sqrt(mean((h - mu)^2) + eps);  t = (h - mu) s;  y = t w + b
+//     8 bits: a = max|y| of the row: q = round(y (T / a)), scale = a / T, T = 448 (e4m3) or 127 (int8)
+//     gradient, g = dy w:  dh = s (g - mean(g) - t mean(g t)) + dh_in;  dw = sum over rows of dy t;  db = sum over rows of dy
+//
+// Bound by memory, as the norms of lf_norm.hip and in their layout: a row is read once and stays in the registers of G neighbouring threads, workgroups
+// walk over the rows with weight and bias in registers, partial rows of dw and db are added up by a second kernel in a fixed order.
+// Two sums over the row one after the other: that of h, then those of d = h - mu and d^2 (and, in the gradient, of g and g d).  The second
+// look at the mean takes off what the rounding of the first has left, so that rows far from zero keep their digits: mu is off by less than
+// a rounding of the largest |h - mu|, not of |mu|.
+// Rows whose sums overflow are summed again times 2^-100, those whose squares vanish after the subtraction times 2^100.
+#include "lf_rows.h"
+
+namespace {
+
+// Sums of N numbers over the G threads of a row; `s` holds N G / 64 words where G > 64.
+template <int G, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* s) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = dpp_add<(G < 64 ? G : 64)>(v[n]);
+    if constexpr (G > 64) {
+        constexpr int W = G / 64;
+        __syncthreads();                                   // what was there before has been read
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int n = 0; n < N; ++n) s[n * W + (threadIdx.x >> 6)] = v[n];
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            v[n] = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) v[n] += s[n * W + w];
+        }
+    }
+}
+template <int G> __device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t* s) {
+    m = lanes_max<G>(m);
+    if constexpr (G > 64) {
+        constexpr int W = G / 64;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) m = max(m, s[w]);
+    }
+    return m;
+}
+
+__device__ __forceinline__ bool counts(const Piece& p, int i, int dim) { return i >= p.first && p.at + i < dim; }
+
+struct LayerArgs {
+    const void* x; const void* res; const void* w; const void* b; void* y; void* h; float* scale;
+    int64_t ldx, ldr, ldy, ldh;
+    int64_t rows;
+    int32_t dim, w_dtype, b_dtype, y_dtype;
+    int32_t stream;                                         // outputs past the caches
+    float eps, inv_dim;
+};
+
+// A row's statistics: t = ((h up - mean) late - less) inv.  Powers of two: up for sums that overflow, late for squares that vanish.
+struct Centre {
+    float mean, less, inv, up, late;
+    // first: () -> sum of h up.  second: (d, dd) <- sums of (h up - mean) late and of its squares
+    template <typename FIRST, typename SECOND> __device__ __forceinline__ void find(float eps, float inv_dim, FIRST first, SECOND second) {
+        up = late = 1.f;
+        auto variance = [&] {
+            float d, dd;
+            second(d, dd);
+            less = d * inv_dim;
+            const float v = fmaf(dd, inv_dim, -(less * less));
+            return v < 0.f ? 0.f : v;                                    // (a NaN stays)
+        };
+        mean = first() * inv_dim;
+        float var = variance() + eps;
+        if (__builtin_expect(!(var >= kTiny && var < __builtin_inff()), 0)) {      // (the same for all threads of the row)
+            if (var < kTiny) {
+                late = 1.f / kTiny;
+                var = variance() + eps * late * late;
+            } else {
+                // (the mean once more: here eps, far below what is left of its rounding, would not hide it)
+                up = kTiny;
+                mean = first() * inv_dim;
+                variance();
+                mean += less;
+                var = variance();
+                if (eps > 0.f && var < kTiny) var = kTiny;
+            }
+        }
+        inv = 1.f / sqrtf(var);
+    }
+    __device__ __forceinline__ float8_t of(float8_t h) const { return ((h * up - mean) * late - less) * inv; }
+};
+
+template <typename XT, typename RT, int G, int C>
+__global__ void __launch_bounds__(G < 256 ? 256 : G)
+layer_norm_kernel(LayerArgs a) {
+    constexpr int T = G < 256 ? 256 : G, R = T / G;
+    __shared__ float s_red[2 * (G > 64 ? G / 64 : 1)];
+    const int lane = threadIdx.x % G, group = threadIdx.x / G, dim = a.dim;
+    const bool q8 = a.scale != nullptr;
+    float8_t w[C], b[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const Piece p = piece_of((c * G + lane) * 8, dim);
+        w[c] = float8_t{1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        b[c] = float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (a.w) w[c] = load_piece(a.w, 0, a.w_dtype, p, dim);
+        if (a.b) b[c] = load_piece(a.b, 0, a.b_dtype, p, dim);
+    }
+    for (int64_t row = (int64_t)blockIdx.x * R + group; row < a.rows; row += (int64_t)gridDim.x * R) {
+        float8_t h[C];
+        const XT* x = (const XT*)a.x + row * a.ldx;
+#pragma unroll
+        for (int c = 0; c < C; ++c) h[c] = load_piece(x, piece_of((c * G + lane) * 8, dim), dim);
+        if (a.res) {
+            const RT* r = (const RT*)a.res + row * a.ldr;
+            float8_t v[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) v[c] = load_piece(r, piece_of((c * G + lane) * 8, dim), dim);
+#pragma unroll
+            for (int c = 0; c < C; ++c) h[c] += v[c];
+        }
+        Centre m;
+        auto each_of = [&](auto f) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const Piece p = piece_of((c * G + lane) * 8, dim);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (counts(p, i, dim)) f(h[c][i]);
+            }
+        };
+        m.find(a.eps, a.inv_dim,
+               [&] {
+                   float v[1] = {0.f};
+                   each_of([&](float x) { v[0] += x * m.up; });
+                   row_sums<G>(v, s_red);
+                   return v[0];
+               },
+               [&](float& d, float& dd) {
+                   float v[2] = {0.f, 0.f};
+                   each_of([&](float x) {
+                       const float t = (x * m.up - m.mean) * m.late;
+                       v[0] += t;
+                       v[1] = fmaf(t, t, v[1]);
+                   });
+                   row_sums<G>(v, s_red);
+                   d = v[0];
+                   dd = v[1];
+               });
+        if (a.res) {
+            RT* hr = (RT*)a.h + row * a.ldh;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const Piece p = piece_of((c * G + lane) * 8, dim);
+                if (p.first < 8) store_piece(hr, p, dim, h[c], a.stream);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) h[c] = m.of(h[c]) * w[c] + b[c];
+        if (!q8) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const Piece p = piece_of((c * G + lane) * 8, dim);
+                if (p.first < 8) store_piece(a.y, row * a.ldy, a.y_dtype, p, dim, h[c], a.stream);
+            }
+            continue;
+        }
+        uint32_t top = 0;
+        each_of([&](float x) { top = max(top, __float_as_uint(x) & 0x7fffffffu); });
+        const Eighth q(row_max<G>(top, (uint32_t*)s_red), a.y_dtype);
+        if (lane == 0) a.scale[row] = q.scale(1.f);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const Piece p = piece_of((c * G + lane) * 8, dim);
+            if (p.first < 8) q.store((uint8_t*)a.y + row * a.ldy + p.at, h[c], dim, a.stream);
+        }
+    }
+}
+
+// Rows that no workgroup holds in its registers: read for the sum, for the squares, in 8 bits for the largest, and for the output.
+template <typename XT, typename RT>
+__global__ void __launch_bounds__(1024)
+layer_norm_long_kernel(LayerArgs a) {
+    __shared__ float s_red[32];
+    const int dim = a.dim;
+    const bool q8 = a.scale != nullptr;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const XT* x = (const XT*)a.x + row * a.ldx;
+        const RT* r = (const RT*)a.res + row * a.ldr;
+        auto sum8 = [&](int col, int n) {
+            float8_t h = load_upto8(x + col, n);
+            if (a.res) h += load_upto8(r + col, n);
+            return h;
+        };
+        auto pieces = [&](auto f) {
+            for (int col = threadIdx.x * 8; col < dim; col += 8192) {
+                const int n = min(8, dim - col);
+                f(col, n, sum8(col, n));
+            }
+        };
+        Centre m;
+        m.find(a.eps, a.inv_dim,
+               [&] {
+                   float v[1] = {0.f};
+                   pieces([&](int, int, float8_t h) {                    // (zeros behind the end)
+#pragma unroll
+                       for (int i = 0; i < 8; ++i) v[0] += h[i] * m.up;
+                   });
+                   row_sums<1024>(v, s_red);
+                   return v[0];
+               },
+               [&](float& d, float& dd) {
+                   float v[2] = {0.f, 0.f};
+                   pieces([&](int, int n, float8_t h) {
+#pragma unroll
+                       for (int i = 0; i < 8; ++i) {
+                           const float t = i < n ? (h[i] * m.up - m.mean) * m.late : 0.f;
+                           v[0] += t;
+                           v[1] = fmaf(t, t, v[1]);
+                       }
+                   });
+                   row_sums<1024>(v, s_red);
+                   d = v[0];
+                   dd = v[1];
+               });
+        auto out = [&](int col, int n, float8_t h) {
+            float8_t y = m.of(h);
+            if (a.w) y *= load_upto8(a.w, col, a.w_dtype, n);
+            if (a.b) y += load_upto8(a.b, col, a.b_dtype, n);
+            return y;
+        };
+        uint32_t top = 0;
+        if (q8) {
+            pieces([&](int col, int n, float8_t h) {
+                const float8_t y = out(col, n, h);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = max(top, i < n ? __float_as_uint(y[i]) & 0x7fffffffu : 0u);
+            });
+            top = row_max<1024>(top, (uint32_t*)s_red);
+        }
+        const Eighth q(top, a.y_dtype);
+        if (q8 && threadIdx.x == 0) a.scale[row] = q.scale(1.f);
+        pieces([&](int col, int n, float8_t h) {
+            const float8_t y = out(col, n, h);
+            if (a.res) store_upto8((RT*)a.h + row * a.ldh + col, h, n);
+            if (q8) q.store((uint8_t*)a.y + row * a.ldy + col, y, n, a.stream);
+            else store_upto8(a.y, row * a.ldy + col, a.y_dtype, y, n);
+        });
+    }
+}
+
+struct LayerGradArgs {
+    const void* dy; const void* h; const void* w; const void* dh; void* dx;
+    float* part;                                            // [workgroups][2][dim]: of dw and db
+    void* dw; void* db;
+    int64_t ldy, ldh, ldd, ldx;
+    int64_t rows;
+    int32_t dim, w_dtype, db_dtype;
+    int32_t stream;
+    float eps, inv_dim;
+    // `which` 0: dw, 1: db
+    __device__ __forceinline__ bool wants(int which) const { return which ? db != nullptr : dw != nullptr; }
+    __device__ __forceinline__ void leave(int which, int col, float v) const {
+        if (part) part[((int64_t)blockIdx.x * 2 + which) * dim + col] = v;
+        else if (which) store_one(db, col, db_dtype, v);
+        else store_one(dw, col, w_dtype, v);
+    }
+};
+
+template <typename DT, typename HT, int G, int C>
+__global__ void __launch_bounds__(G < 256 ? 256 : G)
+layer_norm_grad_kernel(LayerGradArgs a) {
+    constexpr int T = G < 256 ? 256 : G, R = T / G;
+    __shared__ float s_red[4 * (G > 64 ? G / 64 : 1)];
+    __shared__ float s_sum[R > 1 ? T * 8 * C : 1];
+    const int lane = threadIdx.x % G, group = threadIdx.x / G, dim = a.dim;
+    float8_t w[C], sums[2][C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        w[c] = float8_t{1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        sums[0][c] = sums[1][c] = float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (a.w) w[c] = load_piece(a.w, 0, a.w_dtype, piece_of((c * G + lane) * 8, dim), dim);
+    }
+    for (int64_t row = (int64_t)blockIdx.x * R + group; row < a.rows; row += (int64_t)gridDim.x * R) {
+        float8_t h[C], dy[C];
+        const HT* hr = (const HT*)a.h + row * a.ldh;
+        const DT* dr = (const DT*)a.dy + row * a.ldy;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const Piece p = piece_of((c * G + lane) * 8, dim);
+            h[c] = load_piece(hr, p, dim);
+            dy[c] = load_piece(dr, p, dim);
+        }
+        auto each_of = [&](auto f) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const Piece p = piece_of((c * G + lane) * 8, dim);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (counts(p, i, dim)) f(h[c][i], dy[c][i] * w[c][i]);
+            }
+        };
+        Centre m;
+        float g_sum, g_dot;                                              // of g and g (h up - mean) late
+        m.find(a.eps, a.inv_dim,
+               [&] {
+                   float v[1] = {0.f};
+                   each_of([&](float x, float) { v[0] += x * m.up; });
+                   row_sums<G>(v, s_red);
+                   return v[0];
+               },
+               [&](float& d, float& dd) {
+                   float v[4] = {0.f, 0.f, 0.f, 0.f};
+                   each_of([&](float x, float g) {
+                       const float t = (x * m.up - m.mean) * m.late;
+                       v[0] += t;
+                       v[1] = fmaf(t, t, v[1]);
+                       v[2] += g;
+                       v[3] = fmaf(g, t, v[3]);
+                   });
+                   row_sums<G>(v, s_red);
+                   d = v[0];
+                   dd = v[1];
+                   g_sum = v[2];
+                   g_dot = v[3];
+               });
+        const float g_mean = g_sum * a.inv_dim, along = fmaf(-m.less, g_sum, g_dot) * m.inv * a.inv_dim, s = m.inv * m.late * m.up;
+        HT* dx = (HT*)a.dx + row * a.ldx;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const Piece p = piece_of((c * G + lane) * 8, dim);
+            const float8_t t = m.of(h[c]);
+            float8_t d = (dy[c] * w[c] - g_mean - t * along) * s;
+            if (a.dh) d += load_piece((const HT*)a.dh + row * a.ldd, p, dim);
+            sums[0][c] += dy[c] * t;
+            sums[1][c] += dy[c];
+            if (p.first < 8) store_piece(dx, p, dim, d, a.stream);
+        }
+    }
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        if (!a.wants(which)) continue;
+        if constexpr (R > 1) {
+            // the sums of a workgroup's row groups, column by column
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s_sum[(group * C + c) * 8 * G + lane * 8 + i] = sums[which][c][i];
+            __syncthreads();
+            for (int j = threadIdx.x; j < 8 * C * G; j += T) {
+                const Piece p = piece_of(j & ~7, dim);
+                if (!counts(p, j & 7, dim)) continue;
+                float v = 0.f;
+#pragma unroll
+                for (int g = 0; g < R; ++g) v += s_sum[g * 8 * C * G + j];
+                a.leave(which, p.at + (j & 7), v);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const Piece p = piece_of((c * G + lane) * 8, dim);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (counts(p, i, dim)) a.leave(which, p.at + i, sums[which][c][i]);
+            }
+        }
+    }
+}
+
+template <typename DT, typename HT>
+__global__ void __launch_bounds__(1024)
+layer_norm_grad_long_kernel(LayerGradArgs a) {
+    __shared__ float s_red[64];
+    const int dim = a.dim;
+    bool first_row = true;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const HT* hr = (const HT*)a.h + row * a.ldh;
+        const DT* dr = (const DT*)a.dy + row * a.ldy;
+        auto pieces = [&](auto f) {
+            for (int col = threadIdx.x * 8; col < dim; col += 8192) {
+                const int n = min(8, dim - col);
+                f(col, n, load_upto8(hr + col, n), load_upto8(dr + col, n));
+            }
+        };
+        auto weighted = [&](float8_t dy, int col, int n) { return a.w ? dy * load_upto8(a.w, col, a.w_dtype, n) : dy; };
+        Centre m;
+        float g_sum, g_dot;
+        m.find(a.eps, a.inv_dim,
+               [&] {
+                   float v[1] = {0.f};
+                   pieces([&](int, int, float8_t h, float8_t) {
+#pragma unroll
+                       for (int i = 0; i < 8; ++i) v[0] += h[i] * m.up;
+                   });
+                   row_sums<1024>(v, s_red);
+                   return v[0];
+               },
+               [&](float& d, float& dd) {
+                   float v[4] = {0.f, 0.f, 0.f, 0.f};
+                   pieces([&](int col, int n, float8_t h, float8_t dy) {
+                       const float8_t g = weighted(dy, col, n);
+#pragma unroll
+                       for (int i = 0; i < 8; ++i) {
+                           if (i >= n) continue;
+                           const float t = (h[i] * m.up - m.mean) * m.late;
+                           v[0] += t;
+                           v[1] = fmaf(t, t, v[1]);
+                           v[2] += g[i];
+                           v[3] = fmaf(g[i], t, v[3]);
+                       }
+                   });
+                   row_sums<1024>(v, s_red);
+                   d = v[0];
+                   dd = v[1];
+                   g_sum = v[2];
+                   g_dot = v[3];
+               });
+        const float g_mean = g_sum * a.inv_dim, along = fmaf(-m.less, g_sum, g_dot) * m.inv * a.inv_dim, s = m.inv * m.late * m.up;
+        pieces([&](int col, int n, float8_t h, float8_t dy) {
+            const float8_t t = m.of(h);
+            float8_t d = (weighted(dy, col, n) - g_mean - t * along) * s;
+            if (a.dh) d += load_upto8((const HT*)a.dh + row * a.ldd + col, n);
+            store_upto8((HT*)a.dx + row * a.ldx + col, d, n);
+            if (!a.part) return;
+            // (a thread's own columns of the partial rows, from row to row)
+            float* part = a.part + (int64_t)blockIdx.x * 2 * dim + col;
+            float8_t dw = dy * t, db = dy;
+            if (!first_row) {
+                dw += load_upto8(part, n);
+                db += load_upto8(part + dim, n);
+            }
+            store_upto8(part, dw, n);
+            store_upto8(part + dim, db, n);
+        });
+        first_row = false;
+    }
+}
+
+// Columns of [n][2][dim] partial sums into dw and db (blockIdx.y): 16 columns to a workgroup, every 64th row to a thread, then the threads in order.
+__global__ void __launch_bounds__(1024) layer_norm_sums_kernel(const float* part, int64_t n, int32_t dim, void* dw, int32_t w_dtype, void* db, int32_t db_dtype) {
+    __shared__ float s[64][17];
+    void* out = blockIdx.y ? db : dw;
+    if (!out) return;
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
+    const float* src = part + (int64_t)blockIdx.y * dim + min(col, dim - 1);
+    float v = 0.f;
+#pragma unroll 8
+    for (int64_t r = slice; r < n; r += 64) v += src[r * 2 * dim];
+    s[slice][threadIdx.x & 15] = v;
+    __syncthreads();
+    if (slice || col >= dim) return;
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v += s[i][threadIdx.x];
+    store_one(out, col, blockIdx.y ? db_dtype : w_dtype, v);
+}
+
+template <typename A, typename B> struct Kernels {
+    using Norm = void (*)(LayerArgs);
+    using Grad = void (*)(LayerGradArgs);
+    static Norm norm(Shape s) {
+        switch (s.group) {
+            case 8: return layer_norm_kernel<A, B, 8, 1>;
+            case 16: return layer_norm_kernel<A, B, 16, 1>;
+            case 32: return layer_norm_kernel<A, B, 32, 1>;
+            case 64: return s.pieces == 1 ? layer_norm_kernel<A, B, 64, 1> : layer_norm_kernel<A, B, 64, 2>;
+            case 256: return s.pieces == 1 ? layer_norm_kernel<A, B, 256, 1> : layer_norm_kernel<A, B, 256, 2>;
+            case 512: return layer_norm_kernel<A, B, 512, 2>;
+            default: return s.pieces == 2 ? layer_norm_kernel<A, B, 1024, 2> : layer_norm_long_kernel<A, B>;
+        }
+    }
+    static Grad grad(Shape s) {
+        switch (s.group) {
+            case 8: return layer_norm_grad_kernel<A, B, 8, 1>;
+            case 16: return layer_norm_grad_kernel<A, B, 16, 1>;
+            case 32: return layer_norm_grad_kernel<A, B, 32, 1>;
+            case 64: return s.pieces == 1 ? layer_norm_grad_kernel<A, B, 64, 1> : layer_norm_grad_kernel<A, B, 64, 2>;
+            case 256: return s.pieces == 1 ? layer_norm_grad_kernel<A, B, 256, 1> : layer_norm_grad_kernel<A, B, 256, 2>;
+            case 512: return layer_norm_grad_kernel<A, B, 512, 2>;
+            default: return s.pieces == 2 ? layer_norm_grad_kernel<A, B, 1024, 2> : layer_norm_grad_long_kernel<A, B>;
+        }
+    }
+};
+template <typename F> auto of_types(int32_t a, int32_t b, F f) {
+    auto second = [&](auto x) {
+        using X = decltype(x);
+        return b == LF_DTYPE_F32 ? f(Kernels<X, float>{}) : b == LF_DTYPE_BF16 ? f(Kernels<X, __bf16>{}) : f(Kernels<X, _Float16>{});
+    };
+    return a == LF_DTYPE_F32 ? second(0.f) : a == LF_DTYPE_BF16 ? second((__bf16)0.f) : second((_Float16)0.f);
+}
+
+// Workgroups of 256 threads, as for the norms of lf_norm.hip.
+constexpr int kNormGroups = 3072, kGradGroups = 1024;
+unsigned grad_groups(int64_t rows, int64_t dim) {
+    return std::min(workgroups(rows, shape_of(dim), kGradGroups), (unsigned)std::max<int64_t>(1, (1ll << 25) / dim));
+}
+// Whether a launch of one workgroup leaves dw and db itself (long rows keep them in memory meanwhile).
+bool alone(int64_t rows, int64_t dim) { return shape_of(dim).pieces <= 2 && grad_groups(rows, dim) == 1; }
+
+}  // namespace
+
+extern "C" {
+
+int lf_layer_norm(const lf_layer_norm_args* h_args, lf_stream_t stream) {
+    LF_REQUIRE(h_args, LF_ERR_INVALID, "null argument");
+    const lf_layer_norm_args& a = *h_args;
+    LF_TRY(check_shape(a.rows, a.dim));
+    LF_REQUIRE(is_float_dtype(a.x_dtype) && (!a.d_residual || is_float_dtype(a.residual_dtype)) && (!a.d_weight || is_float_dtype(a.weight_dtype)) &&
+                   (!a.d_bias || is_float_dtype(a.bias_dtype)), LF_ERR_UNSUPPORTED, "x, residual, weight and bias are float32, bfloat16 or float16");
+    LF_REQUIRE(is_float_dtype(a.y_dtype) || is_8bit_dtype(a.y_dtype), LF_ERR_UNSUPPORTED, "unknown type of y");
+    LF_REQUIRE(is_8bit_dtype(a.y_dtype) == (a.d_scale != nullptr) || a.rows == 0, LF_ERR_INVALID, "8-bit rows, and only they, come with scales");
+    LF_REQUIRE(a.eps >= 0.f, LF_ERR_INVALID, "eps must not be negative");
+    LF_REQUIRE(!a.d_residual == !a.d_h || a.rows == 0, LF_ERR_INVALID, "the residual and h = x + residual come together");
+    if (a.rows == 0) return LF_OK;
+    LF_TRY(check_rows("x", a.rows, a.dim, a.d_x, a.ld_x, a.x_dtype));
+    LF_TRY(check_rows("y", a.rows, a.dim, a.d_y, a.ld_y, a.y_dtype));
+    if (a.d_residual) {
+        LF_TRY(check_rows("residual", a.rows, a.dim, a.d_residual, a.ld_residual, a.residual_dtype));
+        LF_TRY(check_rows("h", a.rows, a.dim, a.d_h, a.ld_h, a.residual_dtype));
+    }
+    if (a.d_weight) LF_TRY(check_rows("weight", 1, a.dim, a.d_weight, a.dim, a.weight_dtype));
+    if (a.d_bias) LF_TRY(check_rows("bias", 1, a.dim, a.d_bias, a.dim, a.bias_dtype));
+    const LayerArgs k{a.d_x, a.d_residual, a.d_weight, a.d_bias, a.d_y, a.d_h, a.d_scale, a.ld_x, a.ld_residual, a.ld_y, a.ld_h, a.rows, (int32_t)a.dim, a.weight_dtype,
+                      a.bias_dtype, a.y_dtype, a.rows * a.dim * (dtype_bytes(a.y_dtype) + (a.d_h ? dtype_bytes(a.residual_dtype) : 0)) >= kStreamBytes, a.eps,
+                      (float)(1.0 / (double)a.dim)};
+    const Shape s = shape_of(a.dim);
+    auto kernel = of_types(a.x_dtype, a.d_residual ? a.residual_dtype : a.x_dtype, [&](auto t) { return decltype(t)::norm(s); });
+    kernel<<<workgroups(a.rows, s, kNormGroups), std::max(s.group, 256), 0, (hipStream_t)stream>>>(k);
+    LF_HIP(hipGetLastError());
+    return LF_OK;
+}
+
+size_t lf_layer_norm_grad_work_bytes(int64_t rows, int64_t dim) {
+    if (rows <= 0 || dim < 1 || dim > kMaxDim || alone(rows, dim)) return 0;
+    return (size_t)grad_groups(rows, dim) * 2 * (size_t)dim * sizeof(float);
+}
+
+int lf_layer_norm_grad(const lf_layer_norm_grad_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream) {
+    LF_REQUIRE(h_args, LF_ERR_INVALID, "null argument");
+    const lf_layer_norm_grad_args& a = *h_args;
+    LF_TRY(check_shape(a.rows, a.dim));
+    LF_REQUIRE(is_float_dtype(a.dy_dtype) && is_float_dtype(a.h_dtype) && ((!a.d_weight && !a.d_dw) || is_float_dtype(a.weight_dtype)) &&
+                   (!a.d_db || is_float_dtype(a.db_dtype)), LF_ERR_UNSUPPORTED, "dy, h, weight and db are float32, bfloat16 or float16");
+    LF_REQUIRE(a.eps >= 0.f, LF_ERR_INVALID, "eps must not be negative");
+    const Shape s = shape_of(a.dim);
+    const unsigned groups = a.rows ? grad_groups(a.rows, a.dim) : 0;
+    const bool sums = a.d_dw || a.d_db, one = a.rows && alone(a.rows, a.dim);
+    if (a.d_dw) LF_TRY(check_rows("dw", 1, a.dim, a.d_dw, a.dim, a.weight_dtype));
+    if (a.d_db) LF_TRY(check_rows("db", 1, a.dim, a.d_db, a.dim, a.db_dtype));
+    if (sums) {
+        LF_REQUIRE(a.rows == 0 || one || (d_work && (uintptr_t)d_work % 16 == 0), LF_ERR_INVALID, "null or unaligned workspace");
+        LF_REQUIRE(work_bytes >= lf_layer_norm_grad_work_bytes(a.rows, a.dim), LF_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", work_bytes,
+                   lf_layer_norm_grad_work_bytes(a.rows, a.dim));
+    }
+    hipStream_t st = (hipStream_t)stream;
+    if (a.rows) {
+        LF_TRY(check_rows("dy", a.rows, a.dim, a.d_dy, a.ld_dy, a.dy_dtype));
+        LF_TRY(check_rows("h", a.rows, a.dim, a.d_h, a.ld_h, a.h_dtype));
+        LF_TRY(check_rows("dx", a.rows, a.dim, a.d_dx, a.ld_dx, a.h_dtype));
+        if (a.d_dh) LF_TRY(check_rows("dh", a.rows, a.dim, a.d_dh, a.ld_dh, a.h_dtype));
+        if (a.d_weight) LF_TRY(check_rows("weight", 1, a.dim, a.d_weight, a.dim, a.weight_dtype));
+        const LayerGradArgs k{a.d_dy, a.d_h, a.d_weight, a.d_dh, a.d_dx, sums && !one ? (float*)d_work : nullptr, a.d_dw, a.d_db, a.ld_dy, a.ld_h, a.ld_dh, a.ld_dx, a.rows,
+                              (int32_t)a.dim, a.weight_dtype, a.db_dtype, a.rows * a.dim * dtype_bytes(a.h_dtype) >= kStreamBytes, a.eps, (float)(1.0 / (double)a.dim)};
+        auto kernel = of_types(a.dy_dtype, a.h_dtype, [&](auto t) { return decltype(t)::grad(s); });
+        kernel<<<groups, std::max(s.group, 256), 0, st>>>(k);
+        LF_HIP(hipGetLastError());
+    }
+    if (sums && !one) {
+        layer_norm_sums_kernel<<<dim3((unsigned)ceil_div(a.dim, 16), 2), 1024, 0, st>>>((const float*)d_work, groups, (int32_t)a.dim, a.d_dw, a.weight_dtype, a.d_db,
+                                                                                        a.db_dtype);
+        LF_HIP(hipGetLastError());
+    }
+    return LF_OK;
+}
+
+}  // extern "C"

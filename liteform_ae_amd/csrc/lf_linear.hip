@@ -179,6 +179,68 @@ activation_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* 
     else store_one(db, c, db_dtype, t);
 }
 
+// ---------------------------------------------------------------------------- gate
+
+// y = act(g) u from sums [m][2 n] of which the first n of a row are g: scales and biases as finish() has them.
+__global__ void __launch_bounds__(256) gate_kernel(const float* sums, int64_t m, int64_t n, Epilogue e) {
+    const int64_t across = (n + 7) / 8, unit = (int64_t)blockIdx.x * 256 + threadIdx.x, row = unit / across, col = (unit % across) * 8;
+    if (row >= m) return;
+    const int count = (int)min((int64_t)8, n - col);
+    float8_t v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        v[h] = load_upto8(sums + row * 2 * n + h * n + col, count);
+        if (e.x_scale) v[h] = v[h] * e.x_scale[row] * load_upto8(e.w_scale + h * n + col, count);
+        if (e.bias) v[h] += load_upto8(e.bias, h * n + col, e.bias_dtype, count);
+        if (e.z) store_upto8(e.z, row * e.ld_z + h * n + col, e.z_dtype, v[h], count);
+    }
+    store_upto8(e.y, row * e.ld_y + col, e.y_dtype, activate(v[0], e.act) * v[1], count);
+}
+
+// dz = [dy u act'(g) | dy act(g)] of z = [g | u], in rows of `ld_dz`, and the column sums of a slab of rows, as activation_grad_kernel has them.
+template <typename T, int ACROSS>
+__global__ void __launch_bounds__(256)
+gate_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* dz, int64_t ld_dz, float* part, void* db, int32_t db_dtype, int64_t m, int64_t n, int32_t act,
+                 int64_t slab) {
+    constexpr int DOWN = 256 / ACROSS;
+    constexpr bool FINE = std::is_same_v<T, float>;
+    __shared__ float s[DOWN][ACROSS][9];
+    const int lx = threadIdx.x % ACROSS, ly = threadIdx.x / ACROSS;
+    const int64_t col = ((int64_t)blockIdx.x * ACROSS + lx) * 8;
+    const int count = (int)min((int64_t)8, n - col);
+    const int64_t r1 = min(m, ((int64_t)blockIdx.y + 1) * slab);
+    float8_t sum[2];
+    sum[0] = sum[1] = float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (count > 0)
+#pragma unroll 2
+        for (int64_t r = (int64_t)blockIdx.y * slab + ly; r < r1; r += DOWN) {
+            const float8_t d = load_upto8(dy + r * ld_dy + col, count), g = load_upto8(z + r * ld_z + col, count), u = load_upto8(z + r * ld_z + n + col, count);
+            const float8_t du = d * activate(g, activation_of(act, FINE ? LF_DTYPE_F32 : LF_DTYPE_BF16));
+            float8_t dg = d * u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dg[i] *= activate_grad<FINE>(g[i], act);
+            store_upto8(dz + r * ld_dz + col, dg, count);
+            store_upto8(dz + r * ld_dz + n + col, du, count);
+            sum[0] += dg;
+            sum[1] += du;
+        }
+    if (!part && !db) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[ly][lx][i] = sum[h][i];
+        __syncthreads();
+        const int64_t c = (int64_t)blockIdx.x * ACROSS * 8 + threadIdx.x;
+        if (threadIdx.x >= ACROSS * 8 || c >= n) continue;
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < DOWN; ++i) t += s[i][threadIdx.x >> 3][threadIdx.x & 7];
+        if (part) part[((int64_t)blockIdx.y * 2 + h) * n + c] = t;
+        else store_one(db, h * n + c, db_dtype, t);
+    }
+}
+
 // ---------------------------------------------------------------------------- launches
 
 ProductFn product_of(int32_t dtype, bool px, bool qx, int tile, bool aligned, bool deep) {
@@ -267,6 +329,31 @@ GradWork grad_work(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act, 
     return w;
 }
 
+// Of the gated product, whose dz has 2 n columns.
+GradWork gated_work(int64_t m, int64_t n, int64_t k, int32_t dtype, bool dx, bool dw, bool db) {
+    GradWork w = grad_work(m, 2 * n, k, dtype, LF_ACT_SILU, dx, dw, false);
+    if (db && slabs_of(m, n) > 1) w.sums = padded((size_t)slabs_of(m, n) * 2 * (size_t)n * 4);
+    w.total += w.sums;
+    return w;
+}
+
+// dx = dz w and dw = dz^T x for dz of `n` columns.
+int two_products(const lf_linear_grad_args& a, int64_t n, const void* dz, int64_t ld, void* parts, hipStream_t st) {
+    if (a.d_dx) {
+        Product g{};
+        g.p = dz; g.ld_p = ld; g.q = a.d_w; g.ld_q = a.ld_w; g.m = a.m; g.n = a.k; g.k = n;
+        g.e.y = a.d_dx; g.e.ld_y = a.ld_dx; g.e.y_dtype = a.dtype;
+        LF_TRY(launch_product(g, a.dtype, false, true, parts, st));
+    }
+    if (a.d_dw) {
+        Product g{};
+        g.p = dz; g.ld_p = ld; g.q = a.d_x; g.ld_q = a.ld_x; g.m = n; g.n = a.k; g.k = a.m;
+        g.e.y = a.d_dw; g.e.ld_y = a.ld_dw; g.e.y_dtype = a.dtype;
+        LF_TRY(launch_product(g, a.dtype, true, true, parts, st));
+    }
+    return LF_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -344,21 +431,89 @@ int lf_linear_grad(const lf_linear_grad_args* h_args, void* d_work, size_t work_
         LF_HIP(hipGetLastError());
         if (sums) LF_TRY(lf::column_sums(sums, slabs, a.n, a.d_db, a.db_dtype, st));
     }
-    const void* d = dz ? dz : a.d_dy;
-    const int64_t ld = dz ? ld_dz(a.n) : a.ld_dy;
-    if (a.d_dx) {
-        Product g{};
-        g.p = d; g.ld_p = ld; g.q = a.d_w; g.ld_q = a.ld_w; g.m = a.m; g.n = a.k; g.k = a.n;
-        g.e.y = a.d_dx; g.e.ld_y = a.ld_dx; g.e.y_dtype = a.dtype;
-        LF_TRY(launch_product(g, a.dtype, false, true, parts, st));
-    }
-    if (a.d_dw) {
-        Product g{};
-        g.p = d; g.ld_p = ld; g.q = a.d_x; g.ld_q = a.ld_x; g.m = a.n; g.n = a.k; g.k = a.m;
-        g.e.y = a.d_dw; g.e.ld_y = a.ld_dw; g.e.y_dtype = a.dtype;
-        LF_TRY(launch_product(g, a.dtype, true, true, parts, st));
-    }
+    return two_products(a, a.n, dz ? dz : a.d_dy, dz ? ld_dz(a.n) : a.ld_dy, parts, st);
+}
+
+size_t lf_gated_linear_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype) {
+    if (m <= 0 || n <= 0 || k < 0 || !(is_float_dtype(dtype) || is_8bit_dtype(dtype))) return 0;
+    return padded((size_t)m * (size_t)n * 8) + lf_linear_work_bytes(m, 2 * n, k, dtype);
+}
+
+int lf_gated_linear(const lf_linear_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream) {
+    LF_REQUIRE(h_args, LF_ERR_INVALID, "null argument");
+    const lf_linear_args& a = *h_args;
+    LF_TRY(check_sizes(a.m, 2 * a.n, a.k, a.dtype, a.activation));
+    LF_REQUIRE(is_float_dtype(a.y_dtype) && (!a.d_bias || is_float_dtype(a.bias_dtype)) && (!a.d_z || is_float_dtype(a.z_dtype)), LF_ERR_UNSUPPORTED,
+               "y, z and bias are float32, bfloat16 or float16");
+    LF_REQUIRE(!a.d_residual, LF_ERR_INVALID, "a gated product has no residual");
+    if (a.m == 0 || a.n == 0) return LF_OK;
+    LF_TRY(check_matrix("x", a.d_x, a.m, a.k, a.ld_x, a.dtype));
+    LF_TRY(check_matrix("w", a.d_w, 2 * a.n, a.k, a.ld_w, a.dtype));
+    LF_TRY(check_matrix("y", a.d_y, a.m, a.n, a.ld_y, a.y_dtype));
+    if (a.d_z) LF_TRY(check_matrix("z", a.d_z, a.m, 2 * a.n, a.ld_z, a.z_dtype));
+    if (a.d_bias) LF_TRY(check_matrix("bias", a.d_bias, 1, 2 * a.n, 2 * a.n, a.bias_dtype));
+    LF_REQUIRE(!a.d_x_scale == !a.d_w_scale && is_8bit_dtype(a.dtype) == (a.d_x_scale != nullptr), LF_ERR_INVALID, "8-bit operands, and only they, come with scales");
+    const size_t need = lf_gated_linear_work_bytes(a.m, a.n, a.k, a.dtype);
+    LF_REQUIRE(need == 0 || (d_work && (uintptr_t)d_work % 16 == 0), LF_ERR_INVALID, "null or unaligned workspace");
+    LF_REQUIRE(work_bytes >= need, LF_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", work_bytes, need);
+    const size_t sums = padded((size_t)a.m * (size_t)a.n * 8);
+    Product g{};
+    g.p = a.d_x; g.q = a.d_w; g.ld_p = a.ld_x; g.ld_q = a.ld_w; g.m = a.m; g.n = 2 * a.n; g.k = a.k;
+    g.e.y = d_work; g.e.ld_y = 2 * a.n; g.e.y_dtype = LF_DTYPE_F32;
+    LF_TRY(launch_product(g, a.dtype, false, false, (char*)d_work + sums, (hipStream_t)stream));
+    const Epilogue e{a.d_y, nullptr, a.d_z, a.d_bias, a.d_x_scale, a.d_w_scale, a.ld_y, 0, a.ld_z, a.y_dtype, 0, a.z_dtype, a.bias_dtype, activation_of(a.activation, a.y_dtype)};
+    const int64_t groups = ceil_div(a.m * ceil_div(a.n, 8), 256);
+    LF_REQUIRE(groups < (1ll << 31), LF_ERR_UNSUPPORTED, "too many outputs");
+    gate_kernel<<<(unsigned)groups, 256, 0, (hipStream_t)stream>>>((const float*)d_work, a.m, a.n, e);
+    LF_HIP(hipGetLastError());
     return LF_OK;
+}
+
+size_t lf_gated_linear_grad_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t want_dx, int32_t want_dw, int32_t want_db) {
+    if (m <= 0 || n <= 0 || k < 0 || !is_float_dtype(dtype)) return 0;
+    return gated_work(m, n, k, dtype, want_dx, want_dw, want_db).total;
+}
+
+int lf_gated_linear_grad(const lf_linear_grad_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream) {
+    LF_REQUIRE(h_args, LF_ERR_INVALID, "null argument");
+    const lf_linear_grad_args& a = *h_args;
+    LF_TRY(check_sizes(a.m, 2 * a.n, a.k, a.dtype, a.activation));
+    LF_REQUIRE(is_float_dtype(a.dtype) && (!a.d_db || is_float_dtype(a.db_dtype)), LF_ERR_UNSUPPORTED, "gradients are of float32, bfloat16 or float16");
+    LF_TRY(check_matrix("dy", a.d_dy, a.m, a.n, a.ld_dy, a.dtype));
+    LF_TRY(check_matrix("z", a.d_z, a.m, 2 * a.n, a.ld_z, a.dtype));
+    if (a.d_dw) {
+        LF_TRY(check_matrix("x", a.d_x, a.m, a.k, a.ld_x, a.dtype));
+        LF_TRY(check_matrix("dw", a.d_dw, 2 * a.n, a.k, a.ld_dw, a.dtype));
+    }
+    if (a.d_dx) {
+        LF_TRY(check_matrix("w", a.d_w, 2 * a.n, a.k, a.ld_w, a.dtype));
+        LF_TRY(check_matrix("dx", a.d_dx, a.m, a.k, a.ld_dx, a.dtype));
+    }
+    if (a.d_db) LF_TRY(check_matrix("db", a.d_db, 1, 2 * a.n, 2 * a.n, a.db_dtype));
+    if (a.n == 0 && a.k == 0) return LF_OK;
+    const GradWork w = gated_work(a.m, a.n, a.k, a.dtype, a.d_dx, a.d_dw, a.d_db);
+    LF_REQUIRE(w.total == 0 || (d_work && (uintptr_t)d_work % 16 == 0), LF_ERR_INVALID, "null or unaligned workspace");
+    LF_REQUIRE(work_bytes >= w.total, LF_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", work_bytes, w.total);
+    hipStream_t st = (hipStream_t)stream;
+    char* at = (char*)d_work;
+    void* dz = at;
+    float* sums = w.sums ? (float*)(at + w.dz) : nullptr;
+    void* parts = at + w.dz + w.sums;
+    const int64_t slabs = slabs_of(a.m, a.n), slab = ceil_div(std::max<int64_t>(a.m, 1), slabs);
+    if (a.n > 0) {
+        const int across = threads_across(a.n);
+        const dim3 grid((unsigned)ceil_div(a.n, 8 * across), (unsigned)slabs);
+        auto go = [&](auto t) {
+            using T = decltype(t);
+            auto kernel = across == 8 ? gate_grad_kernel<T, 8> : across == 16 ? gate_grad_kernel<T, 16> : gate_grad_kernel<T, 32>;
+            kernel<<<grid, 256, 0, st>>>((const T*)a.d_dy, a.ld_dy, (const T*)a.d_z, a.ld_z, (T*)dz, ld_dz(2 * a.n), sums, sums ? nullptr : a.d_db, a.db_dtype, a.m, a.n, a.activation,
+                                         slab);
+        };
+        if (a.dtype == LF_DTYPE_F32) go(0.f); else if (a.dtype == LF_DTYPE_BF16) go((__bf16)0.f); else go((_Float16)0.f);
+        LF_HIP(hipGetLastError());
+        if (sums && a.d_db) LF_TRY(lf::column_sums(sums, slabs, 2 * a.n, a.d_db, a.db_dtype, st));
+    }
+    return two_products(a, 2 * a.n, dz, ld_dz(2 * a.n), parts, st);
 }
 
 }  // extern "C"

@@ -31,6 +31,10 @@ _EIGHTS = {}
 # struct lf_linear_args and lf_linear_grad_args in one call each: a field at a time they cost as much as the launch
 _LINEAR_ARGS = struct.Struct("8Q8q6i").pack
 _LINEAR_GRAD_ARGS = struct.Struct("7Q9q3i4x").pack
+_LAYER_NORM_ARGS = struct.Struct("7Q6q5if").pack
+_LAYER_NORM_GRAD_ARGS = struct.Struct("7Q6q4if4x").pack
+_EMBEDDING_ARGS = struct.Struct("3Q6q3if").pack
+_TENSOR_DESC = struct.Struct("2Q5q").pack
 
 
 def _begin():
@@ -198,6 +202,83 @@ def rms_norm_grad(dy, h, weight=None, eps: float = 1e-6, dh=None):
     return dx, dw
 
 
+# --------------------------------------------------------------------------- layer norm
+
+
+def _layer_norm(lib, device, x, weight, bias, residual, eps, dtype, code, eight):
+    torch = _torch()
+    xp, ldx, xt = _matrix("x", x, _FLOATS, device)
+    rows, dim = x.shape
+    wp, wt = (0, 0) if weight is None else _vector("weight", weight, _FLOATS, device, dim)
+    bp, bt = (0, 0) if bias is None else _vector("bias", bias, _FLOATS, device, dim)
+    h = scale = None
+    rp = ldr = rt = hp = sp = 0
+    if residual is not None:
+        rp, ldr, rt = _matrix("residual", residual, _FLOATS, device, rows, dim)
+        h = residual.new_empty((rows, dim))
+        hp = h.data_ptr()
+    y = _new(x, (rows, dim), dtype)
+    if eight:
+        scale = _new(x, (rows,), torch.float32)
+        sp = scale.data_ptr()
+    rc = lib.lf_layer_norm(_LAYER_NORM_ARGS(xp, rp, wp, bp, y.data_ptr(), sp, hp, ldx, ldr, dim, dim, rows, dim, xt, rt, wt, bt, code, eps), _stream())
+    if rc:
+        _lib.check(rc)
+    return y, scale, h
+
+
+def layer_norm(x, weight=None, bias=None, residual=None, eps: float = 1e-5, out_dtype=None):
+    """``y = (h - mean(h)) / sqrt(var(h) + eps) * weight + bias`` with ``h = x + residual``, by rows; ``var`` is the mean of ``(h - mean)^2``.  Returns
+    ``y``, and with a residual ``(y, h)``, types and rounding as ``rms_norm`` has them.  A row of equal elements comes out as the bias (with ``eps=0`` it is
+    not defined); one that holds Inf or NaN as NaN."""
+    torch, lib, device = _begin()
+    dtype = x.dtype if out_dtype is None else out_dtype
+    y, _, h = _layer_norm(lib, device, x, weight, bias, residual, eps, dtype, _float_type("out_dtype", dtype), False)
+    return y if residual is None else (y, h)
+
+
+def layer_norm_8bit(x, weight=None, bias=None, residual=None, eps: float = 1e-5, dtype=None):
+    """``layer_norm`` with y in 8 bits: ``(q, scale)``, and with a residual ``(q, scale, h)``, as ``rms_norm_8bit`` has them."""
+    torch, lib, device = _begin()
+    dtype, code = _eight(torch, dtype)
+    q, scale, h = _layer_norm(lib, device, x, weight, bias, residual, eps, dtype, code, True)
+    return (q, scale) if residual is None else (q, scale, h)
+
+
+def layer_norm_grad(dy, h, weight=None, eps: float = 1e-5, dh=None, bias_dtype=None):
+    """``(dx, dweight, dbias)`` of ``layer_norm`` from the gradient ``dy`` of y and the ``h`` that it returned (x where there was no residual).  dx, in h's
+    type, is the gradient of x and of the residual alike; ``dh``, of h's type, is added to it.  dweight, in the weight's type, is None
+    without a weight; dbias is of ``bias_dtype`` (None: not computed)."""
+    torch, lib, device = _begin()
+    hp, ldh, ht = _matrix("h", h, _FLOATS, device)
+    rows, dim = h.shape
+    gp, ldg, gt = _matrix("dy", dy, _FLOATS, device, rows, dim)
+    wp, wt = (0, 0) if weight is None else _vector("weight", weight, _FLOATS, device, dim)
+    dp = ldd = dwp = dbp = bt = nbytes = 0
+    if dh is not None:
+        dp, ldd, dt = _matrix("dh", dh, _FLOATS, device, rows, dim)
+        if dt != ht:
+            raise ValueError(f"dh must have h's type {h.dtype}, got {dh.dtype}")
+    dx = h.new_empty((rows, dim))
+    dw = db = kp = None
+    if weight is not None:
+        dw = weight.new_empty((dim,))
+        dwp = dw.data_ptr()
+    if bias_dtype is not None:
+        bt = _float_type("bias_dtype", bias_dtype)
+        db = _new(h, (dim,), bias_dtype)
+        dbp = db.data_ptr()
+    if dwp or dbp:
+        nbytes = lib.lf_layer_norm_grad_work_bytes(rows, dim)
+        if nbytes:
+            work = h.new_empty((nbytes,), dtype=torch.uint8)
+            kp = work.data_ptr()
+    rc = lib.lf_layer_norm_grad(_LAYER_NORM_GRAD_ARGS(gp, hp, wp, dp, dx.data_ptr(), dwp, dbp, ldg, ldh, ldd, dim, rows, dim, gt, ht, wt, bt, eps), kp, nbytes, _stream())
+    if rc:
+        _lib.check(rc)
+    return dx, dw, db
+
+
 # --------------------------------------------------------------------------- product
 
 
@@ -295,3 +376,200 @@ def linear_grad(dy, x, weight, z=None, activation=None, bias_dtype=None, want_dx
     if rc:
         _lib.check(rc)
     return dx, dw, db
+
+
+# --------------------------------------------------------------------------- gated product
+
+
+def _gated_weight(x, weight):
+    rows, k = weight.shape if weight.dim() == 2 else (1, -1)
+    if weight.dtype is not x.dtype or k != x.shape[1] or rows % 2:
+        raise ValueError(f"weight must be (2 features out, {x.shape[1]}) of {x.dtype}, the gate's rows first, got {tuple(weight.shape)} of {weight.dtype}")
+    return rows // 2
+
+
+def _gated(torch, lib, device, x, weight, x_scale, w_scale, bias, activation, types, out_dtype, z_dtype):
+    act = _activation(activation)
+    xp, ldx, xt = _matrix("x", x, types, device)
+    m, k = x.shape
+    n = _gated_weight(x, weight)
+    wp, ldw, _ = _matrix("weight", weight, types, device)
+    xs = ws = bp = bt = zp = zt = 0
+    if types is _EIGHTS:
+        xs, ws = _scales(torch, "x_scale", x_scale, device, m), _scales(torch, "weight_scale", w_scale, device, 2 * n)
+    if bias is not None:
+        bp, bt = _vector("bias", bias, _FLOATS, device, 2 * n)
+    yt = _float_type("out_dtype", out_dtype)
+    y, z, kp = _new(x, (m, n), out_dtype), None, None
+    if z_dtype is not None:
+        z = _new(x, (m, 2 * n), z_dtype)
+        zp, zt = z.data_ptr(), _FLOATS[z_dtype]
+    nbytes = lib.lf_gated_linear_work_bytes(m, n, k, xt)
+    if nbytes:
+        work = x.new_empty((nbytes,), dtype=torch.uint8)
+        kp = work.data_ptr()
+    rc = lib.lf_gated_linear(_LINEAR_ARGS(xp, wp, xs, ws, bp, 0, y.data_ptr(), zp, ldx, ldw, 0, n, 2 * n, m, n, k, xt, bt, 0, yt, zt, act), kp, nbytes, _stream())
+    if rc:
+        _lib.check(rc)
+    return y, z
+
+
+def gated_linear(x, weight, bias=None, activation="silu", out_dtype=None, return_preactivation: bool = False):
+    """``y = act(g) * u`` with ``z = x weight^T + bias = [g | u]``: both projections of a gated feed-forward block, its activation and the product, for x (rows, k) and
+    weight (2 n, k) of one type, the gate's n rows first; bias (2 n).  y (rows, n) is of ``out_dtype`` (default: x's).  ``return_preactivation=True`` returns
+    ``(y, z)`` with z (rows, 2 n) in x's type, which ``gated_linear_grad`` needs.  The block's second layer is ``linear(y, ...)``.  Activations, types and
+    their limits are those of ``linear``."""
+    torch, lib, device = _begin()
+    out = x.dtype if out_dtype is None else out_dtype
+    y, z = _gated(torch, lib, device, x, weight, None, None, bias, activation, _FLOATS, out, x.dtype if return_preactivation else None)
+    return (y, z) if return_preactivation else y
+
+
+def gated_linear_8bit(x, x_scale, weight, weight_scale, bias=None, activation="silu", out_dtype=None):
+    """``gated_linear`` of rows in 8 bits with their scales, as ``linear_8bit`` takes them; weight_scale (2 n).  y is of ``out_dtype`` (default bfloat16)."""
+    torch, lib, device = _begin()
+    out = torch.bfloat16 if out_dtype is None else out_dtype
+    return _gated(torch, lib, device, x, weight, x_scale, weight_scale, bias, activation, _EIGHTS, out, None)[0]
+
+
+def gated_linear_grad(dy, x, weight, z, activation="silu", bias_dtype=None, want_dx: bool = True, want_dweight: bool = True):
+    """``(dx, dweight, dbias)`` of ``gated_linear`` from the gradient ``dy`` (rows, n) of y and the ``z`` that it returned: dz = [dy u act'(g) | dy act(g)], dx = dz
+    weight, dweight (2 n, k) = dz^T x, dbias (2 n) = column sums of dz.  All of one type but dbias, which is of ``bias_dtype`` (None: not computed).
+    Gradients that are not wanted are None.  dz is rounded to the operands' type before the products."""
+    torch, lib, device = _begin()
+    act = _activation(activation)
+    xp, ldx, xt = _matrix("x", x, _FLOATS, device)
+    m, k = x.shape
+    n = _gated_weight(x, weight)
+    wp, ldw, _ = _matrix("weight", weight, _FLOATS, device)
+    gp, ldg, gt = _matrix("dy", dy, _FLOATS, device, m, n)
+    zp, ldz, zt = _matrix("z", z, _FLOATS, device, m, 2 * n)
+    if gt != xt or zt != xt:
+        raise ValueError(f"dy and z must have x's type {x.dtype}, got {dy.dtype} and {z.dtype}")
+    dxp = dwp = dbp = bt = 0
+    dx = dw = db = kp = None
+    if want_dx:
+        dx = x.new_empty((m, k))
+        dxp = dx.data_ptr()
+    if want_dweight:
+        dw = x.new_empty((2 * n, k))
+        dwp = dw.data_ptr()
+    if bias_dtype is not None:
+        bt = _float_type("bias_dtype", bias_dtype)
+        db = _new(x, (2 * n,), bias_dtype)
+        dbp = db.data_ptr()
+    nbytes = lib.lf_gated_linear_grad_work_bytes(m, n, k, xt, want_dx, want_dweight, db is not None)
+    if nbytes:
+        work = x.new_empty((nbytes,), dtype=torch.uint8)
+        kp = work.data_ptr()
+    rc = lib.lf_gated_linear_grad(_LINEAR_GRAD_ARGS(gp, zp, xp, wp, dxp, dwp, dbp, ldg, ldz, ldx, ldw, k, k, m, n, k, xt, bt, act), kp, nbytes, _stream())
+    if rc:
+        _lib.check(rc)
+    return dx, dw, db
+
+
+# --------------------------------------------------------------------------- embedding
+
+
+def _ids(torch, ids, device, size=None):
+    """(address, elements from one to the next, bits of each, number)."""
+    bits = 64 if ids.dtype is torch.int64 else 32 if ids.dtype is torch.int32 else 0
+    if not bits or ids.dim() != 1 or ids.get_device() != device or (size is not None and ids.shape[0] != size):
+        raise ValueError(f"ids must be a tensor of shape {'(n,)' if size is None else (size,)} on the current device, cuda:{device}, of int64 or int32, "
+                         f"got {tuple(ids.shape)} of {ids.dtype} on {ids.device}")
+    return ids.data_ptr(), ids.stride(0), bits, ids.shape[0]
+
+
+def embedding(ids, table, scale: float = 1.0, out_dtype=None):
+    """Rows of ``table`` (rows, features) by id, times ``scale``: y (n, features) of ``out_dtype`` (default: the table's).  ids (n,) are int64 or int32, any
+    number of elements apart; one outside 0 .. rows - 1 (padding, such as -1) gives a row of zeros."""
+    torch, lib, device = _begin()
+    ip, step, bits, n = _ids(torch, ids, device)
+    tp, ldt, tt = _matrix("table", table, _FLOATS, device)
+    rows, dim = table.shape
+    dtype = table.dtype if out_dtype is None else out_dtype
+    yt = _float_type("out_dtype", dtype)
+    y = _new(table, (n, dim), dtype)
+    rc = lib.lf_embedding(_EMBEDDING_ARGS(ip, tp, y.data_ptr(), step, ldt, dim, n, rows, dim, bits, tt, yt, scale), _stream())
+    if rc:
+        _lib.check(rc)
+    return y
+
+
+def embedding_grad(dy, ids, rows: int, scale: float = 1.0, out_dtype=None):
+    """The gradient (rows, features) of ``embedding``'s table from that of y, ``dy`` (n, features): ``scale`` times the sum of dy's rows of each id, in 32 bits and in their
+    order, zeros for ids that do not occur.  It is of ``out_dtype`` (default: dy's); ids outside 0 .. rows - 1 have none."""
+    torch, lib, device = _begin()
+    gp, ldg, gt = _matrix("dy", dy, _FLOATS, device)
+    n, dim = dy.shape
+    ip, step, bits, _ = _ids(torch, ids, device, n)
+    dtype = dy.dtype if out_dtype is None else out_dtype
+    wt = _float_type("out_dtype", dtype)
+    if rows < 0:
+        raise ValueError(f"rows must not be negative, got {rows}")
+    dw, kp = _new(dy, (rows, dim), dtype), None
+    nbytes = lib.lf_embedding_grad_work_bytes(n, rows, dim)
+    if nbytes:
+        work = dy.new_empty((nbytes,), dtype=torch.uint8)
+        kp = work.data_ptr()
+    rc = lib.lf_embedding_grad(_EMBEDDING_ARGS(gp, ip, dw.data_ptr(), step, ldg, dim, n, rows, dim, bits, gt, wt, scale), kp, nbytes, _stream())
+    if rc:
+        _lib.check(rc)
+    return dw
+
+
+# --------------------------------------------------------------------------- norm of all gradients
+
+
+def _dense_rows(name, t, device):
+    """(rows, columns, elements from row to row, type) of a contiguous tensor, or of a matrix with contiguous rows."""
+    code = _FLOATS.get(t.dtype)
+    if code is None or t.get_device() != device:
+        raise ValueError(f"{name} must be on the current device, cuda:{device}, and one of {[str(d) for d in _FLOATS]}, got {t.dtype} on {t.device}")
+    if t.requires_grad:
+        refuse_graph(name, t)
+    if t.is_contiguous():
+        return 1, t.numel(), 0, code
+    if t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1) and t.stride(0) >= t.shape[1]:
+        return t.shape[0], t.shape[1], t.stride(0), code
+    raise ValueError(f"{name} must be contiguous, or a matrix whose rows are contiguous and do not overlap, got {tuple(t.shape)} with strides {t.stride()}")
+
+
+def _clip(grads, most, eps, in_place, want):
+    torch, lib, device = _begin()
+    grads = list(grads)
+    layouts = [_dense_rows(f"gradient {i}", g, device) for i, g in enumerate(grads)]
+    out = grads
+    if want and not in_place:
+        # one allocation to a type
+        sizes = {}
+        for g in grads:
+            sizes.setdefault(g.dtype, []).append(g.numel())
+        parts = {t: iter(torch.empty(sum(s), dtype=t, device=f"cuda:{device}").split(s)) for t, s in sizes.items()}
+        out = [next(parts[g.dtype]).view(g.shape) for g in grads]
+    descs = b"".join(_TENSOR_DESC(g.data_ptr(), o.data_ptr() if want else 0, rows, cols, ld, ld if o is g else cols, code)
+                     for g, o, (rows, cols, ld, code) in zip(grads, out, layouts))
+    norm = torch.empty((), dtype=torch.float32, device=f"cuda:{device}")
+    nbytes = lib.lf_clip_work_bytes(len(grads))
+    work = torch.empty(nbytes, dtype=torch.uint8, device=norm.device) if nbytes else None
+    rc = lib.lf_clip_gradients(descs, len(grads), most, eps, norm.data_ptr(), work.data_ptr() if nbytes else None, nbytes, _stream())
+    if rc:
+        _lib.check(rc)
+    if want and in_place:
+        torch.autograd.graph.increment_version(out)
+    return out, norm
+
+
+def gradient_norm(grads):
+    """The square root of the sum of the squares of all elements of all tensors in ``grads`` (float32, a CUDA scalar): the norm of a step's gradients together.  Squares
+    are added in 64 bits.  Tensors of float32, bfloat16 and float16 may stand side by side."""
+    return _clip(grads, 0.0, 0.0, False, False)[1]
+
+
+def clip_gradients(grads, max_norm: float, eps: float = 1e-6, in_place: bool = False):
+    """``(clipped, norm)``: the tensors of ``grads`` times ``min(1, max_norm / (norm + eps))`` and their ``gradient_norm`` before.  ``in_place=True`` writes
+    them where they are (a tensor that shares elements with another is refused), and leaves them alone where nothing is to be cut.  A norm that is NaN
+    makes all of them NaN; look at it first where that may be."""
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    return _clip(grads, max_norm, eps, in_place, True)
