@@ -531,7 +531,7 @@ typedef struct lf_embedding_grad_args {
     float scale;
 } lf_embedding_grad_args;
 int lf_embedding(const lf_embedding_args* h_args, lf_stream_t stream);
-size_t lf_embedding_grad_work_bytes(int64_t n, int64_t rows, int64_t dim);
+size_t lf_embedding_grad_work_bytes(int64_t n, int64_t rows, int64_t dim, int32_t dy_dtype);
 int lf_embedding_grad(const lf_embedding_grad_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream);
 
 /* lf_clip_gradients: *d_norm (device memory) = sqrt(sum over n tensors of their elements' squares), added in 64 bits; each d_dst = d_src * min(1, most / (norm + eps)),

@@ -164,7 +164,7 @@ SIGNATURES = {
     "lf_layer_norm_grad_work_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
     "lf_layer_norm_grad": (C.c_int, [vp, vp, C.c_size_t, vp]),
     "lf_embedding": (C.c_int, [vp, vp]),
-    "lf_embedding_grad_work_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),
+    "lf_embedding_grad_work_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64, C.c_int32]),
     "lf_embedding_grad": (C.c_int, [vp, vp, C.c_size_t, vp]),
     "lf_clip_work_bytes": (C.c_size_t, [C.c_int32]),
     "lf_clip_gradients": (C.c_int, [vp, C.c_int32, C.c_float, C.c_float, vp, vp, C.c_size_t, vp]),

@@ -508,7 +508,7 @@ def embedding_grad(dy, ids, rows: int, scale: float = 1.0, out_dtype=None):
     if rows < 0:
         raise ValueError(f"rows must not be negative, got {rows}")
     dw, kp = _new(dy, (rows, dim), dtype), None
-    nbytes = lib.lf_embedding_grad_work_bytes(n, rows, dim)
+    nbytes = lib.lf_embedding_grad_work_bytes(n, rows, dim, gt)
     if nbytes:
         work = dy.new_empty((nbytes,), dtype=torch.uint8)
         kp = work.data_ptr()

@@ -100,7 +100,7 @@ def test_embedding_refusals():
         refused(call(**change), _lib.LF_ERR_UNSUPPORTED)
     assert call(n=0, ids=None, y=None) == 0
     good = dict(dy=AT, ids=AT, grad=AT * 2, ids_stride=1, ld_dy=8, ld_grad=8, n=4, rows=5, dim=8, ids_bits=32, scale=1.0)
-    need = lib.lf_embedding_grad_work_bytes(4, 5, 8)
+    need = lib.lf_embedding_grad_work_bytes(4, 5, 8, F32)
 
     def grad(work=AT, size=need, **change):
         return lib.lf_embedding_grad(C.byref(_lib.EmbeddingGradArgs(**{**good, **change})), work, size, None)
@@ -110,7 +110,7 @@ def test_embedding_refusals():
     refused(grad(size=need - 1), _lib.LF_ERR_WORKSPACE)
     assert grad(rows=0, grad=None) == 0
     for n, rows in ((0, 5), (4, 0), (-1, 5), (4, -1), (1 << 31, 5), (4, 1 << 31)):
-        assert lib.lf_embedding_grad_work_bytes(n, rows, 8) == 0
+        assert lib.lf_embedding_grad_work_bytes(n, rows, 8, F32) == 0
 
 
 def descs(*tensors):
