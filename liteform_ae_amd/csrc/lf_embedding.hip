@@ -48,7 +48,7 @@ embedding_kernel(Ids ids, const WT* w, int64_t ld_w, int64_t dim, float scale, v
 // ---------------------------------------------------------------------------- sorting
 
 struct Entry { uint32_t key, at; };                         // id and position
-constexpr int kMostBits = 11, kMostDigits = 1 << kMostBits, kTile = 4096;
+constexpr int kMostBits = 11, kMostDigits = 1 << kMostBits, kTile = 2048, kSortThreads = 512;
 
 struct Passes { int passes, bits; };
 // of keys 0 .. rows
@@ -65,22 +65,35 @@ struct SortArgs {
     const Entry* from; Entry* to;
     uint32_t* counts;                                       // [workgroup][digit]: entries, then the entries of that digit before them
     uint32_t* totals;                                       // [digit]
+    uint8_t* present;                                       // [row]: the first pass clears it, the last one marks the ids that occur
     int64_t n, each;                                        // entries; to a workgroup
-    int32_t bits, shift, groups;
+    int32_t bits, shift, groups, first, last;
     __device__ __forceinline__ Entry entry(int64_t i) const { return from ? from[i] : Entry{(uint32_t)ids.at(i), (uint32_t)i}; }
     __device__ __forceinline__ uint32_t digit(uint32_t key) const { return key >> shift & ((1u << bits) - 1); }
 };
 
-__global__ void __launch_bounds__(256) sort_count_kernel(SortArgs a) {
+__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs a) {
     __shared__ uint32_t s_count[kMostDigits];
     const int digits = 1 << a.bits;
-    for (int d = threadIdx.x; d < digits; d += 256) s_count[d] = 0;
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) s_count[d] = 0;
+    if (a.first)                                            // (in pieces of 16 bytes, which there is room for)
+        for (int64_t i = (int64_t)blockIdx.x * kSortThreads + threadIdx.x; i * 16 < a.ids.rows; i += (int64_t)gridDim.x * kSortThreads)
+            reinterpret_cast<uint4_t*>(a.present)[i] = uint4_t{0u, 0u, 0u, 0u};
     __syncthreads();
     const int64_t first = (int64_t)blockIdx.x * a.each, last = min(a.n, first + a.each);
-#pragma unroll 4
-    for (int64_t i = first + threadIdx.x; i < last; i += 256) atomicAdd(&s_count[a.digit(a.entry(i).key)], 1u);
+    for (int64_t tile = first; tile < last; tile += kTile) {
+        uint32_t d[kTile / kSortThreads];
+#pragma unroll
+        for (int r = 0; r < kTile / kSortThreads; ++r) {
+            const int64_t i = tile + threadIdx.x + r * kSortThreads;
+            d[r] = i < last ? a.digit(a.entry(i).key) : ~0u;
+        }
+#pragma unroll
+        for (int r = 0; r < kTile / kSortThreads; ++r)
+            if (d[r] != ~0u) atomicAdd(&s_count[d[r]], 1u);
+    }
     __syncthreads();
-    for (int d = threadIdx.x; d < digits; d += 256) a.counts[(int64_t)blockIdx.x * digits + d] = s_count[d];
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) a.counts[(int64_t)blockIdx.x * digits + d] = s_count[d];
 }
 
 // 16 digits to a workgroup; 64 threads share the workgroups' counts of one.
@@ -98,11 +111,16 @@ __global__ void __launch_bounds__(1024) sort_offsets_kernel(SortArgs a) {
     for (int i = 0; i < slice; ++i) before += s[i][threadIdx.x & 15];
     if (d >= digits) return;
     if (slice == 63) a.totals[d] = before + sum;
-    for (int g = first; g < last; ++g) {
-        uint32_t* c = a.counts + (int64_t)g * digits + d;
-        const uint32_t v = *c;
-        *c = before;
-        before += v;
+    for (int g0 = first; g0 < last; g0 += 8) {
+        uint32_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = g0 + i < last ? a.counts[(int64_t)(g0 + i) * digits + d] : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (g0 + i < last) {
+                a.counts[(int64_t)(g0 + i) * digits + d] = before;
+                before += v[i];
+            }
     }
 }
 
@@ -129,16 +147,50 @@ template <typename C> __device__ __forceinline__ uint32_t rank_in_wave(C* count,
     return seen + before;
 }
 
-__global__ void __launch_bounds__(256) sort_move_kernel(SortArgs a) {
-    constexpr int WAVES = 4, ROUNDS = kTile / 256;
+// Up to so many workgroups add up one another's counts themselves, which spares a launch (and 32 loads a digit take as long as one).
+constexpr int kFewGroups = 32;
+
+// FEW: `counts` is what sort_count_kernel left
+template <bool FEW>
+__global__ void __launch_bounds__(kSortThreads) sort_move_kernel(SortArgs a) {
+    constexpr int WAVES = kSortThreads / 64, ROUNDS = kTile / kSortThreads, MINE = kMostDigits / kSortThreads;
     __shared__ uint32_t s_base[kMostDigits], s_count[WAVES][kMostDigits], s_wave[WAVES];
     const int digits = 1 << a.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t end = min(a.n, ((int64_t)blockIdx.x + 1) * a.each);
+    int64_t mine = (int64_t)blockIdx.x * a.each + wave * (64 * ROUNDS) + lane;
+    Entry e[ROUNDS];
+    auto load = [&] {
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r)
+            if (mine + r * 64 < end) e[r] = a.entry(mine + r * 64);
+    };
+    load();
     // where each digit begins: the digits below it, and this digit's entries of the workgroups before
     {
-        const int each = (digits + 255) / 256, first = threadIdx.x * each;
-        uint32_t sum = 0;
-        for (int d = first; d < min(digits, first + each); ++d) sum += a.totals[d];
+        uint32_t total[MINE], sum = 0;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const int d = threadIdx.x * MINE + i;
+            total[i] = 0;
+            if (d >= digits) continue;
+            if constexpr (FEW) {
+                uint32_t before = 0;
+#pragma unroll 8
+                for (int g = 0; g < a.groups; ++g) {
+                    const uint32_t v = a.counts[g * digits + d];
+                    before += g < (int)blockIdx.x ? v : 0;
+                    total[i] += v;
+                }
+                s_base[d] = before;
+            } else {
+                total[i] = a.totals[d];
+                s_base[d] = a.counts[(int64_t)blockIdx.x * digits + d];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) sum += total[i];
         uint32_t upto = sum;
+#pragma unroll
         for (int o = 1; o < 64; o *= 2) {
             const uint32_t v = __shfl_up((int)upto, o);
             if (lane >= o) upto += v;
@@ -147,31 +199,26 @@ __global__ void __launch_bounds__(256) sort_move_kernel(SortArgs a) {
         __syncthreads();
         uint32_t before = upto - sum;
         for (int w = 0; w < wave; ++w) before += s_wave[w];
-        for (int d = first; d < min(digits, first + each); ++d) {
-            s_base[d] = before + a.counts[(int64_t)blockIdx.x * digits + d];
-            before += a.totals[d];
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const int d = threadIdx.x * MINE + i;
+            if (d < digits) s_base[d] += before;
+            before += total[i];
         }
     }
-    const int64_t end = min(a.n, ((int64_t)blockIdx.x + 1) * a.each);
-    for (int64_t tile = (int64_t)blockIdx.x * a.each; tile < end; tile += kTile) {
+    for (int64_t tile = (int64_t)blockIdx.x * a.each;;) {
         for (int w = 0; w < WAVES; ++w)
-            for (int d = threadIdx.x; d < digits; d += 256) s_count[w][d] = 0;
-        Entry e[ROUNDS];
-        uint32_t rank[ROUNDS];
-        const int64_t mine = tile + wave * (64 * ROUNDS) + lane;
-#pragma unroll
-        for (int r = 0; r < ROUNDS; ++r)
-            if (mine + r * 64 < end) e[r] = a.entry(mine + r * 64);
+            for (int d = threadIdx.x; d < digits; d += kSortThreads) s_count[w][d] = 0;
         __syncthreads();
         // a wavefront's entries in order, 64 at a time: those of the digit before, and among the 64
+        uint32_t rank[ROUNDS];
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
             const bool on = mine + r * 64 < end;
-            const uint32_t d = on ? a.digit(e[r].key) : 0;
-            rank[r] = rank_in_wave(s_count[wave], d, a.bits, on);
+            rank[r] = rank_in_wave(s_count[wave], on ? a.digit(e[r].key) : 0, a.bits, on);
         }
         __syncthreads();
-        for (int d = threadIdx.x; d < digits; d += 256) {
+        for (int d = threadIdx.x; d < digits; d += kSortThreads) {
             uint32_t at = s_base[d];
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
@@ -184,7 +231,14 @@ __global__ void __launch_bounds__(256) sort_move_kernel(SortArgs a) {
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r)
-            if (mine + r * 64 < end) a.to[s_count[wave][a.digit(e[r].key)] + rank[r]] = e[r];
+            if (mine + r * 64 < end) {
+                a.to[s_count[wave][a.digit(e[r].key)] + rank[r]] = e[r];
+                if (a.last && e[r].key < (uint32_t)a.ids.rows) a.present[e[r].key] = 1;
+            }
+        tile += kTile;
+        if (tile >= end) return;
+        mine += kTile;
+        load();
         __syncthreads();
     }
 }
@@ -277,17 +331,28 @@ __device__ __forceinline__ int64_t first_of(const Entry* e, int64_t n, uint32_t 
     return lo;
 }
 
-// G threads take `each` sorted entries one after the other, eight columns a thread.  An id that begins and ends among them is done there; of one that does not
-// they leave what they have of it: `head` where it begins before them, `tail` where it begins among them.
+// The first entry before `hi` that is not of the id that entry `lo` has, or hi.
+__device__ __forceinline__ int end_of(const Entry* e, int lo, int hi, uint32_t key) {
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (e[mid].key == key) lo = mid; else hi = mid;
+    }
+    return hi;
+}
+
+// A workgroup takes a span of sorted entries, G threads of it `each` one after the other, eight columns a thread.  Ids that go on from these G threads to the next are
+// put together in LDS; of one that goes on from a workgroup to the next, `tail` is what the one that it begins in has of it, `head` what each of the others has.
+constexpr int kSumThreads = 512, kMostEach = 64;
 template <typename S> struct Sums {
     const Entry* e;
+    const uint8_t* present;                                 // of each row, whether its id occurs; NULL: it is looked for
     const void* dy; void* dw;
-    S* part;                                                // [chunk][head, tail][ld_part]
-    int64_t n, ld_dy, rows, dim, ld_dw, ld_part, chunks;
-    int32_t dw_dtype, each, sum_groups;
+    S* part;                                                // [workgroup][head, tail][ld_part]
+    int64_t n, ld_dy, rows, dim, ld_dw, ld_part;
+    int32_t dw_dtype, each, sum_groups, fill_rows, stream;
     float scale;
-    __device__ __forceinline__ S* head(int64_t chunk) const { return part + chunk * 2 * ld_part; }
-    __device__ __forceinline__ S* tail(int64_t chunk) const { return head(chunk) + ld_part; }
+    __device__ __forceinline__ S* head(int64_t group) const { return part + group * 2 * ld_part; }
+    __device__ __forceinline__ S* tail(int64_t group) const { return head(group) + ld_part; }
 };
 template <typename S> struct Eight8 { typedef S vec __attribute__((ext_vector_type(8))); };
 
@@ -295,134 +360,187 @@ template <typename S> __device__ __forceinline__ float8_t scaled(typename Eight8
     return __builtin_convertvector(v * (S)scale, float8_t);
 }
 
-template <typename DT, typename S, int G>
-__global__ void __launch_bounds__(256) embedding_sums_kernel(Sums<S> a) {
-    using V = typename Eight8<S>::vec;
-    constexpr int U = 8;
-    const int lane = threadIdx.x % G, team = threadIdx.x / G;
-    const int64_t col = ((int64_t)blockIdx.y * G + lane) * 8;
-    const int count = (int)min((int64_t)8, a.dim - col);
-    if ((int)blockIdx.x >= a.sum_groups) {
-        // Rows of ids that do not occur: 64 to a wavefront, each looked for by a lane.
-        const int64_t base = ((int64_t)(blockIdx.x - a.sum_groups) * 4 + (threadIdx.x >> 6)) * 64;
-        const int64_t row = base + (threadIdx.x & 63);
-        bool absent = false;
-        if (row < a.rows) {
+// Rows of ids that do not occur: `fill_rows` to a wavefront, a row's id to a lane.
+template <typename S, int G> __device__ __forceinline__ void fill_rows(const Sums<S>& a, int64_t col, int count) {
+    const int64_t base = ((int64_t)(blockIdx.x - a.sum_groups) * (kSumThreads / 64) + (threadIdx.x >> 6)) * a.fill_rows;
+    const int64_t row = base + (threadIdx.x & 63);
+    bool absent = false;
+    if (row < min(a.rows, base + a.fill_rows)) {
+        if (a.present) {
+            absent = !a.present[row];
+        } else {
             const int64_t at = first_of(a.e, a.n, (uint32_t)row);
             absent = at >= a.n || a.e[at].key != (uint32_t)row;
         }
-        const uint64_t zeros = __ballot(absent);
-        constexpr int AT_ONCE = 64 / G;
-        const int mine = (threadIdx.x & 63) / G;
-        if (count > 0)
-            for (int r = mine; r < 64; r += AT_ONCE)
-                if (zeros >> r & 1) store_upto8(a.dw, (base + r) * a.ld_dw + col, a.dw_dtype, float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, count);
-        return;
     }
-    const int64_t chunk = (int64_t)blockIdx.x * (256 / G) + team, first = chunk * a.each, last = min(a.n, first + a.each);
-    if (first >= a.n || count <= 0) return;
-    const uint32_t none = (uint32_t)a.rows, before = first > 0 ? a.e[first - 1].key : none, after = last < a.n ? a.e[last].key : none;
-    uint32_t key = a.e[first].key;
-    V sum = V{0, 0, 0, 0, 0, 0, 0, 0};
-    auto leave = [&](bool end) {
-        if (key == none) return;
-        S* part = key == before ? a.head(chunk) : end && key == after ? a.tail(chunk) : nullptr;     // (sorted: `before` is the key of the chunk's first id or of none)
-        if (part) *reinterpret_cast<V*>(part + col) = sum;
-        else store_upto8(a.dw, (int64_t)key * a.ld_dw + col, a.dw_dtype, scaled<S>(sum, a.scale), count);
-    };
-    for (int64_t i = first; i < last; i += U) {
-        Entry e[U];
-        float8_t v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) e[u] = i + u < last ? a.e[i + u] : Entry{none, 0};
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = e[u].key != none ? load_upto8((const DT*)a.dy + (int64_t)e[u].at * a.ld_dy + col, count) : float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i + u < last && e[u].key != key) {
-                leave(false);
-                key = e[u].key;
-                sum = V{0, 0, 0, 0, 0, 0, 0, 0};
-            }
-            sum += __builtin_convertvector(v[u], V);
-        }
-    }
-    leave(true);
+    const uint64_t zeros = __ballot(absent);
+    if (count <= 0) return;
+    for (int r = (threadIdx.x & 63) / G; r < a.fill_rows; r += 64 / G)
+        if (zeros >> r & 1) store_upto8(a.dw, (base + r) * a.ld_dw + col, a.dw_dtype, float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, count, a.stream);
 }
 
-// What the chunks left of ids that go on from one to the next: G threads look after the end of a chunk; where an id begins in it that goes on, they add
-// up its parts, in order.  Ids of more than kFewParts parts are left to all threads of the workgroup.
-constexpr int kFewParts = 64;
+template <typename DT, typename S, int G>
+__global__ void __launch_bounds__(kSumThreads) embedding_sums_kernel(Sums<S> a) {
+    using V = typename Eight8<S>::vec;
+    constexpr int U = 8, TEAMS = kSumThreads / G;
+    const int lane = threadIdx.x % G, team = threadIdx.x / G;
+    const int64_t col = ((int64_t)blockIdx.y * G + lane) * 8;
+    const int count = (int)min((int64_t)8, a.dim - col);
+    if ((int)blockIdx.x >= a.sum_groups) return fill_rows<S, G>(a, col, count);
+    __shared__ Entry s_e[TEAMS * kMostEach + 2];            // with the entry before, and that behind
+    __shared__ S s_head[TEAMS][8][G];                       // what G threads have of an id that begins before theirs
+    const uint32_t none = (uint32_t)a.rows;
+    const int64_t from0 = (int64_t)blockIdx.x * TEAMS * a.each - 1;
+    for (int j = threadIdx.x; j < TEAMS * a.each + 2; j += kSumThreads) s_e[j] = from0 + j >= 0 && from0 + j < a.n ? a.e[from0 + j] : Entry{none, 0};
+    __syncthreads();
+    auto key_at = [&](int i) { return s_e[i].key; };
+    // rows of dy of the entries `from` to `to` of s_e; between(key, sum) before each is added
+    auto add = [&](int from, int to, auto between) {
+        V sum = V{0, 0, 0, 0, 0, 0, 0, 0};
+        if (count > 0)
+            for (int i = from; i < to; i += U) {
+                Entry e[U];
+                float8_t v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) e[u] = i + u < to ? s_e[i + u] : Entry{none, 0};
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    v[u] = e[u].key != none ? load_upto8((const DT*)a.dy + (int64_t)e[u].at * a.ld_dy + col, count) : float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (i + u < to) between(e[u].key, sum);
+                    sum += __builtin_convertvector(v[u], V);
+                }
+            }
+        return sum;
+    };
+    auto leave = [&](uint32_t key, V sum) {
+        if (key != none && count > 0) store_upto8(a.dw, (int64_t)key * a.ld_dw + col, a.dw_dtype, scaled<S>(sum, a.scale), count, a.stream);
+    };
+    int first = 1 + team * a.each;
+    const int last = first + a.each;                        // (entries past the end have no id)
+    const uint32_t key0 = key_at(first), key1 = key_at(last - 1);
+    const bool from_before = key0 != none && key_at(first - 1) == key0, goes_on = key1 != none && key_at(last) == key1;
+    if (from_before) {
+        const int end = end_of(s_e, first, last, key0);
+        const V sum = add(first, end, [](uint32_t, V&) {});
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s_head[team][i][lane] = sum[i];
+        first = end;
+    }
+    V rest = V{0, 0, 0, 0, 0, 0, 0, 0};
+    const bool begins = first < last;
+    if (begins) {
+        uint32_t key = key_at(first);
+        rest = add(first, last, [&](uint32_t next, V& sum) {
+            if (next == key) return;
+            leave(key, sum);
+            key = next;
+            sum = V{0, 0, 0, 0, 0, 0, 0, 0};
+        });
+        if (!goes_on) leave(key, rest);
+    }
+    __syncthreads();
+    // adds what the threads from `t` on have of the id `key`; true: it goes on behind the workgroup's entries
+    auto follow = [&](V& sum, uint32_t key, int t) {
+        for (;; ++t) {
+            if (t == TEAMS) return true;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += s_head[t][i][lane];
+            const int next = 1 + (t + 1) * a.each;
+            if (key_at(next - 1) != key || key_at(next) != key) return false;
+        }
+    };
+    auto keep = [&](S* part, V sum) {
+        if (count > 0) *reinterpret_cast<V*>(part + col) = sum;
+    };
+    if (begins && goes_on) {
+        if (follow(rest, key1, team + 1)) keep(a.tail(blockIdx.x), rest);
+        else leave(key1, rest);
+    }
+    if (team == 0 && from_before) {
+        V sum = V{0, 0, 0, 0, 0, 0, 0, 0};
+        follow(sum, key0, 0);
+        keep(a.head(blockIdx.x), sum);
+    }
+}
+
+// What the workgroups left of ids that go on from one to the next: G threads look after the end of one; where an id begins in it that goes on, they add up its
+// parts, in order.  Ids of more than kFewParts parts are left to all threads of the workgroup.
+constexpr int kFewParts = 16;
 template <typename S, int G>
 __global__ void __launch_bounds__(1024) embedding_join_kernel(Sums<S> a) {
     using V = typename Eight8<S>::vec;
     typedef double D8 __attribute__((ext_vector_type(8)));
     constexpr int TEAMS = 1024 / G;
     __shared__ int s_parts[TEAMS];
-    __shared__ double s_sum[TEAMS][G][8];
+    __shared__ double s_sum[TEAMS][8][G];
     const int lane = threadIdx.x % G, team = threadIdx.x / G;
-    const int64_t col = ((int64_t)blockIdx.y * G + lane) * 8;
+    const int64_t col = ((int64_t)blockIdx.y * G + lane) * 8, span = kSumThreads / G * a.each;
     const int count = (int)min((int64_t)8, a.dim - col);
-    const int64_t chunk0 = (int64_t)blockIdx.x * TEAMS;
+    const int group0 = blockIdx.x * TEAMS;
     auto key_at = [&](int64_t i) { return a.e[i].key; };
-    // parts behind the tail of the chunk's last id; 0: it does not go on, or begins before
-    auto parts_of = [&](int64_t chunk) -> int {
-        const int64_t first = chunk * a.each, next = first + a.each;
+    // parts behind the tail of the group's last id; 0: it does not go on, or begins before
+    auto parts_of = [&](int group) -> int {
+        const int64_t first = group * span, next = first + span;
         if (next >= a.n) return 0;
-        const uint32_t key = key_at(next - 1);
-        if (key >= (uint32_t)a.rows || key_at(next) != key || (first > 0 && key_at(first - 1) == key)) return 0;
-        // the last chunk whose first entry is of this id: by steps of 1, 2, 4 .., then between
-        int64_t lo = chunk + 1, step = 1;
-        while (lo + step < a.chunks && key_at((lo + step) * a.each) == key) {
-            lo += step;
-            step *= 2;
+        const uint32_t key = key_at(next - 1), behind = key_at(next), own = key_at(first), before = key_at(max(first, (int64_t)1) - 1);
+        if (key >= (uint32_t)a.rows || behind != key || (first > 0 && before == key && own == key)) return 0;
+        // the last group whose first entry is of this id: G at a time, then in steps of G, G * G ..
+        int64_t lo = group + 1, step = 1;
+        for (;;) {
+            const int64_t c = lo + (lane + 1) * step;
+            const bool same = c < a.sum_groups && key_at(c * span) == key;
+            const uint64_t all = __ballot(same) >> (threadIdx.x & 63 & ~(G - 1));
+            const int those = __popcll(G < 64 ? all & ((1ull << (G & 63)) - 1) : all);
+            lo += those * step;
+            if (those == G) step *= G;
+            else if (step == 1) break;
+            else step /= G;
         }
-        int64_t hi = min(lo + step, a.chunks);
-        while (hi - lo > 1) {
-            const int64_t mid = (lo + hi) >> 1;
-            if (key_at(mid * a.each) == key) lo = mid; else hi = mid;
-        }
-        return (int)(lo - chunk);
+        return (int)(lo - group);
     };
-    auto add_heads = [&](D8& sum, int64_t from, int64_t to) {
+    auto add_heads = [&](D8& sum, int from, int to) {
         if (count <= 0) return;
 #pragma unroll 8
-        for (int64_t c = from; c < to; ++c) sum += __builtin_convertvector(*reinterpret_cast<const V*>(a.head(c) + col), D8);
+        for (int c = from; c < to; ++c) sum += __builtin_convertvector(*reinterpret_cast<const V*>(a.head(c) + col), D8);
     };
-    auto leave = [&](int64_t chunk, D8 sum) {
-        if (count > 0)
-            store_upto8(a.dw, (int64_t)key_at((chunk + 1) * a.each) * a.ld_dw + col, a.dw_dtype, __builtin_convertvector(sum * (double)a.scale, float8_t), count);
+    auto leave = [&](int group, D8 sum) {
+        if (count > 0) store_upto8(a.dw, (int64_t)key_at((group + 1) * span) * a.ld_dw + col, a.dw_dtype, __builtin_convertvector(sum * (double)a.scale, float8_t), count);
     };
-    auto tail_of = [&](int64_t chunk) {
+    auto tail_of = [&](int group) {
         D8 sum = D8{0, 0, 0, 0, 0, 0, 0, 0};
-        if (count > 0) sum = __builtin_convertvector(*reinterpret_cast<const V*>(a.tail(chunk) + col), D8);
+        if (count > 0) sum = __builtin_convertvector(*reinterpret_cast<const V*>(a.tail(group) + col), D8);
         return sum;
     };
-    const int64_t chunk = chunk0 + team;
-    const int parts = chunk < a.chunks ? parts_of(chunk) : 0;
+    const int group = group0 + team, parts = group < a.sum_groups ? parts_of(group) : 0;
     if (lane == 0) s_parts[team] = parts;
     if (parts > 0 && parts <= kFewParts) {
-        D8 sum = tail_of(chunk);
-        add_heads(sum, chunk + 1, chunk + 1 + parts);
-        leave(chunk, sum);
+        D8 sum = tail_of(group);
+        add_heads(sum, group + 1, group + 1 + parts);
+        leave(group, sum);
     }
     __syncthreads();
     for (int t = 0; t < TEAMS; ++t) {
         const int n = s_parts[t];                           // (the same for all threads)
         if (n <= kFewParts) continue;
-        const int64_t c = chunk0 + t;
-        const int each = (n + TEAMS - 1) / TEAMS, from = min(n, team * each), to = min(n, from + each);
+        const int c = group0 + t, each = (n + TEAMS - 1) / TEAMS, from = min(n, team * each), to = min(n, from + each);
         D8 sum = D8{0, 0, 0, 0, 0, 0, 0, 0};
         if (team == 0) sum = tail_of(c);
         add_heads(sum, c + 1 + from, c + 1 + to);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s_sum[team][lane][i] = sum[i];
+        for (int i = 0; i < 8; ++i) s_sum[team][i][lane] = sum[i];
         __syncthreads();
-        if (team == 0) {
-#pragma unroll 4
-            for (int o = 1; o < TEAMS; ++o)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum[i] += s_sum[o][lane][i];
+        for (int half = TEAMS / 2; half > 0; half /= 2) {
+            if (team < half)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s_sum[team][i][lane] += s_sum[team + half][i][lane];
+            __syncthreads();
+        }
+        if (team == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] = s_sum[0][i][lane];
             leave(c, sum);
         }
         __syncthreads();
@@ -435,30 +553,35 @@ template <typename F> void of_type(int32_t t, F f) {
 
 inline size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // Entries that some threads take one after the other: enough of them for 8192 wavefronts.
-int64_t entries_each(int64_t n, int64_t dim) {
+int entries_each(int64_t n, int64_t dim) {
     const int64_t waves = n * ceil_div(dim, 8 * group_of(dim)) * group_of(dim) / 64;
-    return waves <= 16 * 8192 ? 16 : waves <= 32 * 8192 ? 32 : 64;
+    return waves <= 16 * 8192 ? 16 : waves <= 32 * 8192 ? 32 : kMostEach;
 }
+int64_t sum_groups(int64_t n, int64_t dim) { return ceil_div(n, (int64_t)entries_each(n, dim) * (kSumThreads / group_of(dim))); }
 inline int sum_bytes(int32_t dtype) { return dtype == LF_DTYPE_F32 ? 8 : 4; }
-struct GradWork { size_t entries, counts, totals, parts, total; };
+struct GradWork { size_t entries, counts, totals, present, parts, total; };
 GradWork grad_work(int64_t n, int64_t rows, int64_t dim, int32_t dtype) {
     const Passes p = passes_of(rows, kMostBits);
-    const int64_t chunks = ceil_div(n, entries_each(n, dim));
-    GradWork w{padded((size_t)n * sizeof(Entry)), 0, 0, 0, 0};
+    const int64_t groups = sum_groups(n, dim);
+    GradWork w{padded((size_t)n * sizeof(Entry)), 0, 0, 0, 0, 0};
     if (n > kSmall) {
         w.counts = padded(((size_t)sort_groups(n) << p.bits) * 4);
         w.totals = padded(4 << p.bits);
+        w.present = padded(rows);
     }
-    if (chunks > 1) w.parts = (size_t)chunks * 2 * (size_t)(ceil_div(dim, 8) * 8) * sum_bytes(dtype);
-    w.total = (n > kSmall ? 2 : 1) * w.entries + w.counts + w.totals + w.parts;
+    if (groups > 1) w.parts = (size_t)groups * 2 * (size_t)(ceil_div(dim, 8) * 8) * sum_bytes(dtype);
+    w.total = (n > kSmall ? 2 : 1) * w.entries + w.counts + w.totals + w.present + w.parts;
     return w;
 }
-template <typename DT, typename S, int G> int launch_sums(const Sums<S>& a, hipStream_t st) {
-    const unsigned slices = (unsigned)ceil_div(a.dim, 8 * G);
-    embedding_sums_kernel<DT, S, G><<<dim3((unsigned)(a.sum_groups + ceil_div(a.rows, 256)), slices), 256, 0, st>>>(a);
+template <typename DT, typename S, int G> int launch_sums(Sums<S> a, hipStream_t st) {
+    const int64_t slices = ceil_div(a.dim, 8 * G);
+    // rows to a wavefront: 64, or fewer for enough of them
+    a.fill_rows = a.rows * slices >= 64 * 4096 ? 64 : 16;
+    const int64_t fill = ceil_div(a.rows, (int64_t)a.fill_rows * (kSumThreads / 64));
+    embedding_sums_kernel<DT, S, G><<<dim3((unsigned)(a.sum_groups + fill), (unsigned)slices), kSumThreads, 0, st>>>(a);
     LF_HIP(hipGetLastError());
-    if (a.chunks > 1) {
-        embedding_join_kernel<S, G><<<dim3((unsigned)ceil_div(a.chunks, 1024 / G), slices), 1024, 0, st>>>(a);
+    if (a.sum_groups > 1) {
+        embedding_join_kernel<S, G><<<dim3((unsigned)ceil_div(a.sum_groups, 1024 / G), (unsigned)slices), 1024, 0, st>>>(a);
         LF_HIP(hipGetLastError());
     }
     return LF_OK;
@@ -522,10 +645,11 @@ int lf_embedding_grad(const lf_embedding_grad_args* h_args, void* d_work, size_t
     LF_REQUIRE(work_bytes >= need, LF_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", work_bytes, need);
     hipStream_t st = (hipStream_t)stream;
     const Entry* sorted = nullptr;
+    const uint8_t* present = nullptr;
     char* at = (char*)d_work;
     if (a.n) {
         const GradWork w = grad_work(a.n, a.rows, a.dim, a.dy_dtype);
-        SortArgs s{{a.d_ids, a.ids_stride, a.n, a.rows, a.ids_bits == 64}, nullptr, (Entry*)at, nullptr, nullptr, a.n, kTile * tiles_each(a.n), 0, 0, (int32_t)sort_groups(a.n)};
+        SortArgs s{{a.d_ids, a.ids_stride, a.n, a.rows, a.ids_bits == 64}, nullptr, (Entry*)at, nullptr, nullptr, nullptr, a.n, kTile * tiles_each(a.n), 0, 0, (int32_t)sort_groups(a.n), 0, 0};
         if (a.n <= kSmall) {
             const Passes p = passes_of(a.rows, kSmallBits);
             s.bits = p.bits;
@@ -539,30 +663,35 @@ int lf_embedding_grad(const lf_embedding_grad_args* h_args, void* d_work, size_t
             Entry* turn[2] = {(Entry*)at, (Entry*)(at + w.entries)};
             s.counts = (uint32_t*)(at + 2 * w.entries);
             s.totals = (uint32_t*)(at + 2 * w.entries + w.counts);
+            present = s.present = (uint8_t*)(at + 2 * w.entries + w.counts + w.totals);
             s.bits = p.bits;
             for (int pass = 0; pass < p.passes; ++pass) {
                 s.from = sorted;
                 s.to = turn[pass & 1];
                 s.shift = pass * p.bits;
-                sort_count_kernel<<<s.groups, 256, 0, st>>>(s);
+                s.first = pass == 0;
+                s.last = pass == p.passes - 1;
+                sort_count_kernel<<<s.groups, kSortThreads, 0, st>>>(s);
                 LF_HIP(hipGetLastError());
-                sort_offsets_kernel<<<(unsigned)ceil_div(1 << p.bits, 16), 1024, 0, st>>>(s);
-                LF_HIP(hipGetLastError());
-                sort_move_kernel<<<s.groups, 256, 0, st>>>(s);
+                const bool few = s.groups <= kFewGroups;
+                if (!few) {
+                    sort_offsets_kernel<<<(unsigned)ceil_div(1 << p.bits, 16), 1024, 0, st>>>(s);
+                    LF_HIP(hipGetLastError());
+                }
+                (few ? sort_move_kernel<true> : sort_move_kernel<false>)<<<s.groups, kSortThreads, 0, st>>>(s);
                 LF_HIP(hipGetLastError());
                 sorted = s.to;
             }
-            at += 2 * w.entries + w.counts + w.totals;
+            at += 2 * w.entries + w.counts + w.totals + w.present;
         }
     }
     const int group = group_of(a.dim);
-    const int64_t each = entries_each(a.n, a.dim), chunks = ceil_div(a.n, each);
     int rc = LF_OK;
     of_type(a.dy_dtype, [&](auto t) {
         using T = decltype(t);
         using S = std::conditional_t<std::is_same_v<T, float>, double, float>;
-        const Sums<S> k{sorted, a.d_dy, a.d_grad, (S*)at, a.n, a.ld_dy, a.rows, a.dim, a.ld_grad, ceil_div(a.dim, 8) * 8, chunks, a.grad_dtype, (int32_t)each,
-                        (int32_t)ceil_div(chunks, 256 / group), a.scale};
+        const Sums<S> k{sorted, present, a.d_dy, a.d_grad, (S*)at, a.n, a.ld_dy, a.rows, a.dim, a.ld_grad, ceil_div(a.dim, 8) * 8, a.grad_dtype, entries_each(a.n, a.dim),
+                        (int32_t)sum_groups(a.n, a.dim), 0, a.rows * a.dim * dtype_bytes(a.grad_dtype) >= kStreamBytes, a.scale};
         rc = group == 8 ? launch_sums<T, S, 8>(k, st) : group == 16 ? launch_sums<T, S, 16>(k, st) : group == 32 ? launch_sums<T, S, 32>(k, st) : launch_sums<T, S, 64>(k, st);
     });
     return rc;
