@@ -71,21 +71,23 @@ template <typename A> int launch_join(const Product& g, hipStream_t st) {
 // Up to 16 rows of X: a workgroup takes 16 rows of W, its wavefronts the 128-byte steps of k in turn, and their sums
 // meet in LDS.  W goes from memory into the matrix instructions' registers, 32 consecutive bytes a lane and step.  Bound by the
 // read of W, small ones by the launch: one row, bf16 W of 8192^2 29 us (4.6 TB/s), of 4096^2 9.4 (3.6); 13 rows, int8 W of 1001 x 4000 6.
-template <typename T, int WAVES>
+template <typename T, int WAVES, bool GATED = false>
 __global__ void __launch_bounds__(64 * WAVES)
 few_rows_kernel(Product g) {
     constexpr int KS = 128 / sizeof(T), MINE = 32 / sizeof(T), E = 16 / sizeof(T);
     using Acc = typename Elem<T>::Acc;
     using S = std::conditional_t<std::is_same_v<Acc, int4v>, int32_t, float>;
-    __shared__ S s_sum[WAVES][16][17];
+    constexpr int HALVES = GATED ? 2 : 1;
+    __shared__ S s_sum[HALVES][WAVES][16][17];
     const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t n0 = (int64_t)blockIdx.x * 16;
     const T* w = (const T*)g.q + min(n0 + li, g.n - 1) * g.ld_q + lg * MINE;
     const bool on = li < g.m;
     const T* x = (const T*)g.p + (on ? li : 0) * g.ld_p + lg * MINE;
-    Acc acc = {0, 0, 0, 0};
-    auto multiply = [&](const uint4_t (&a)[2], const uint4_t (&b)[2]) {
+    const int64_t half = g.n * g.ld_q;                          // from the gate's rows to those of the other half
+    Acc acc[HALVES] = {};
+    auto multiply = [&](Acc& acc, const uint4_t (&a)[2], const uint4_t (&b)[2]) {
         if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -97,46 +99,57 @@ few_rows_kernel(Product g) {
             acc = mma(a[1], b[1], acc, T{});
         }
     };
-    constexpr int U = 4;                                        // steps under way at once
+    constexpr int U = GATED && WAVES == 16 ? 2 : 4;             // steps under way at once (as many as there are registers for)
     const int64_t steps = g.k / KS;
     int64_t s = wave;
     for (; s + (U - 1) * WAVES < steps; s += U * WAVES) {
-        uint4_t a[U][2], b[U][2];
+        uint4_t a[HALVES][U][2], b[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                a[u][h] = load16(w + (s + u * WAVES) * KS + h * E);
+#pragma unroll
+                for (int v = 0; v < HALVES; ++v) a[v][u][h] = load16(w + v * half + (s + u * WAVES) * KS + h * E);
                 b[u][h] = uint4_t{0u, 0u, 0u, 0u};
                 if (on) b[u][h] = load16(x + (s + u * WAVES) * KS + h * E);
             }
 #pragma unroll
-        for (int u = 0; u < U; ++u) multiply(a[u], b[u]);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int v = 0; v < HALVES; ++v) multiply(acc[v], a[v][u], b[u]);
     }
     for (; s < steps + (g.k % KS != 0); s += WAVES) {
-        uint4_t a[2], b[2];
+        uint4_t a[HALVES][2], b[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int left = (int)min((int64_t)E, g.k - s * KS - lg * MINE - h * E);
-            a[h] = load16_each(w + s * KS + h * E, left);
+#pragma unroll
+            for (int v = 0; v < HALVES; ++v) a[v][h] = load16_each(w + v * half + s * KS + h * E, left);
             b[h] = load16_each(x + s * KS + h * E, on ? left : 0);
         }
-        multiply(a, b);
+#pragma unroll
+        for (int v = 0; v < HALVES; ++v) multiply(acc[v], a[v], b);
     }
 #pragma unroll
-    for (int v = 0; v < 4; ++v) s_sum[wave][li][lg * 4 + v] = acc[v];
+    for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s_sum[h][wave][li][lg * 4 + v] = acc[h][v];
     __syncthreads();
     const int m = threadIdx.x >> 1, at = (threadIdx.x & 1) * 8;
     if (m >= g.m || n0 + at >= g.n) return;
-    float8_t out;
+    float8_t out[HALVES];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        S t = 0;
+    for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-        for (int u = 0; u < WAVES; ++u) t += s_sum[u][m][at + i];
-        out[i] = (float)t;
-    }
-    finish(g.e, m, n0 + at, (int)min((int64_t)8, g.n - n0 - at), out);
+        for (int i = 0; i < 8; ++i) {
+            S t = 0;
+#pragma unroll
+            for (int u = 0; u < WAVES; ++u) t += s_sum[h][u][m][at + i];
+            out[h][i] = (float)t;
+        }
+    const int count = (int)min((int64_t)8, g.n - n0 - at);
+    if constexpr (GATED) finish_gated(g.e, m, n0 + at, g.n, count, out);
+    else finish(g.e, m, n0 + at, count, out[0]);
 }
 
 // ---------------------------------------------------------------------------- gradient of the activation
@@ -181,20 +194,72 @@ activation_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* 
 
 // ---------------------------------------------------------------------------- gate
 
-// y = act(g) u from sums [m][2 n] of which the first n of a row are g: scales and biases as finish() has them.
-__global__ void __launch_bounds__(256) gate_kernel(const float* sums, int64_t m, int64_t n, Epilogue e) {
-    const int64_t across = (n + 7) / 8, unit = (int64_t)blockIdx.x * 256 + threadIdx.x, row = unit / across, col = (unit % across) * 8;
-    if (row >= m) return;
-    const int count = (int)min((int64_t)8, n - col);
-    float8_t v[2];
+// join_kernel of a gated product: the splits' partial sums [splits][m][2 n] in order, and its epilogue.
+template <typename A, int SLICES>
+__global__ void __launch_bounds__(256) gated_join_kernel(const A* part, int64_t m, int64_t n, int32_t splits, Epilogue e) {
+    constexpr int UNITS = 256 / SLICES;
+    __shared__ A s_sum[2][SLICES][UNITS][9];
+    const int64_t across = (n + 7) / 8, u = (int64_t)blockIdx.x * UNITS + threadIdx.x % UNITS;
+    const int slice = threadIdx.x / UNITS;
+    const int64_t row = u / across, col = (u % across) * 8;
+    const int count = row < m ? (int)min((int64_t)8, n - col) : 0;
+    A sum[2][8] = {};
+    struct __attribute__((packed, aligned(4))) Any { A v[8]; };
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        v[h] = load_upto8(sums + row * 2 * n + h * n + col, count);
-        if (e.x_scale) v[h] = v[h] * e.x_scale[row] * load_upto8(e.w_scale + h * n + col, count);
-        if (e.bias) v[h] += load_upto8(e.bias, h * n + col, e.bias_dtype, count);
-        if (e.z) store_upto8(e.z, row * e.ld_z + h * n + col, e.z_dtype, v[h], count);
+        const A* src = part + row * 2 * n + h * n + col;
+        if (count == 8) {
+#pragma unroll 4
+            for (int s = slice; s < splits; s += SLICES) {
+                const Any v = *reinterpret_cast<const Any*>(src + (int64_t)s * m * 2 * n);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[h][i] += v.v[i];
+            }
+        } else if (count > 0) {
+#pragma unroll 2
+            for (int s = slice; s < splits; s += SLICES)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[h][i] += src[(int64_t)s * m * 2 * n + min(i, count - 1)];
+        }
     }
-    store_upto8(e.y, row * e.ld_y + col, e.y_dtype, activate(v[0], e.act) * v[1], count);
+    if constexpr (SLICES > 1) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s_sum[h][slice][threadIdx.x % UNITS][i] = sum[h][i];
+        __syncthreads();
+        // a thread adds up the slices of some outputs
+        constexpr int OUT = 2 * UNITS * 8;
+        for (int o = threadIdx.x; o < OUT; o += 256) {
+            const int h = o / (UNITS * 8), unit = o / 8 % UNITS, i = o % 8;
+            A t = s_sum[h][0][unit][i];
+#pragma unroll
+            for (int v = 1; v < SLICES; ++v) t += s_sum[h][v][unit][i];
+            s_sum[h][0][unit][i] = t;
+        }
+        __syncthreads();
+        if (slice) return;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[h][i] = s_sum[h][0][threadIdx.x][i];
+    }
+    if (count == 0) return;
+    float8_t v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[h][i] = (float)sum[h][i];
+    finish_gated(e, row, col, n, count, v);
+}
+template <typename A> int launch_gated_join(const Product& g, hipStream_t st) {
+    const int slices = g.splits <= 4 ? 1 : g.splits <= 32 ? 8 : 32;
+    const int64_t groups = ceil_div(g.m * ceil_div(g.n, 8), 256 / slices);
+    LF_REQUIRE(groups < (1ll << 31), LF_ERR_UNSUPPORTED, "too many outputs");
+    auto kernel = slices == 1 ? gated_join_kernel<A, 1> : slices == 8 ? gated_join_kernel<A, 8> : gated_join_kernel<A, 32>;
+    kernel<<<(unsigned)groups, 256, 0, st>>>((const A*)g.part, g.m, g.n, g.splits, g.e);
+    LF_HIP(hipGetLastError());
+    return LF_OK;
 }
 
 // dz = [dy u act'(g) | dy act(g)] of z = [g | u], in rows of `ld_dz`, and the column sums of a slab of rows, as activation_grad_kernel has them.
@@ -252,43 +317,54 @@ ProductFn product_of(int32_t dtype, bool px, bool qx, int tile, bool aligned, bo
         default: return product_i8(px, qx, tile, aligned, deep);
     }
 }
-template <int WAVES> ProductFn few_rows_of(int32_t dtype) {
+ProductFn gated_of(int32_t dtype, int tile, bool aligned, bool deep) {
     switch (dtype) {
-        case LF_DTYPE_F32: return few_rows_kernel<float, WAVES>;
-        case LF_DTYPE_BF16: return few_rows_kernel<__bf16, WAVES>;
-        case LF_DTYPE_F16: return few_rows_kernel<_Float16, WAVES>;
-        case LF_DTYPE_E4M3: return few_rows_kernel<e4m3_t, WAVES>;
-        default: return few_rows_kernel<int8_t, WAVES>;
+        case LF_DTYPE_F32: return gated_f32(tile, aligned, deep);
+        case LF_DTYPE_BF16: return gated_bf16(tile, aligned, deep);
+        case LF_DTYPE_F16: return gated_f16(tile, aligned, deep);
+        case LF_DTYPE_E4M3: return gated_e4m3(tile, aligned, deep);
+        default: return gated_i8(tile, aligned, deep);
+    }
+}
+template <int WAVES, bool GATED> ProductFn few_rows_of(int32_t dtype) {
+    switch (dtype) {
+        case LF_DTYPE_F32: return few_rows_kernel<float, WAVES, GATED>;
+        case LF_DTYPE_BF16: return few_rows_kernel<__bf16, WAVES, GATED>;
+        case LF_DTYPE_F16: return few_rows_kernel<_Float16, WAVES, GATED>;
+        case LF_DTYPE_E4M3: return few_rows_kernel<e4m3_t, WAVES, GATED>;
+        default: return few_rows_kernel<int8_t, WAVES, GATED>;
     }
 }
 
-int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipStream_t st) {
+// gated: g.n outputs, of 2 g.n rows of Q
+int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipStream_t st, bool gated = false) {
     if (g.m == 0 || g.n == 0) return LF_OK;
-    g.e.stream = g.m * g.n * dtype_bytes(g.e.y_dtype) >= kStreamBytes;
-    const Path path = path_of(dtype_bytes(dtype), {g.p, g.ld_p, g.m, px}, {g.q, g.ld_q, g.n, qx}, g.k);
+    const int64_t q_rows = gated ? 2 * g.n : g.n;
+    g.e.stream = g.m * (g.n * dtype_bytes(g.e.y_dtype) + (gated && g.e.z ? q_rows * dtype_bytes(g.e.z_dtype) : 0)) >= kStreamBytes;
+    const Path path = path_of(dtype_bytes(dtype), {g.p, g.ld_p, g.m, px}, {g.q, g.ld_q, q_rows, qx}, g.k);
     if (path.kernel == kPathFewRows) {
         const int64_t groups = ceil_div(g.n, 16);
         LF_REQUIRE(groups < (1ll << 31), LF_ERR_UNSUPPORTED, "too many columns");
         // few workgroups take 16 wavefronts each
-        if (groups <= 256) few_rows_of<16>(dtype)<<<(unsigned)groups, 1024, 0, st>>>(g);
-        else few_rows_of<8>(dtype)<<<(unsigned)groups, 512, 0, st>>>(g);
+        if (groups <= 256) (gated ? few_rows_of<16, true>(dtype) : few_rows_of<16, false>(dtype))<<<(unsigned)groups, 1024, 0, st>>>(g);
+        else (gated ? few_rows_of<8, true>(dtype) : few_rows_of<8, false>(dtype))<<<(unsigned)groups, 512, 0, st>>>(g);
         LF_HIP(hipGetLastError());
         return LF_OK;
     }
     const Cut& c = path.cut;
-    const int64_t tm = ceil_div(g.m, c.tile), tn = ceil_div(g.n, c.tile);
+    const int64_t tm = ceil_div(g.m, c.tile), tn = ceil_div(q_rows, c.tile);
     LF_REQUIRE(tm < (1ll << 27) && tn < (1ll << 27) && tm * tn < (1ll << 31), LF_ERR_UNSUPPORTED, "too many tiles");
     g.tiles_m = (int32_t)tm;
     g.tiles_n = (int32_t)tn;
     g.splits = c.splits;
     g.k_split = c.k_split;
     g.part = c.splits > 1 ? work : nullptr;
-    product_of(dtype, px, qx, c.tile, path.kernel != kPathProduct, path.deep)<<<dim3((unsigned)(tm * tn), (unsigned)c.splits), 256, 0, st>>>(g);
+    const bool aligned = path.kernel != kPathProduct;
+    (gated ? gated_of(dtype, c.tile, aligned, path.deep) : product_of(dtype, px, qx, c.tile, aligned, path.deep))<<<dim3((unsigned)(tm * tn), (unsigned)c.splits), 256, 0, st>>>(g);
     LF_HIP(hipGetLastError());
-    if (c.splits > 1) {
-        LF_TRY(dtype == LF_DTYPE_I8 ? launch_join<int32_t>(g, st) : launch_join<float>(g, st));
-    }
-    return LF_OK;
+    if (c.splits == 1) return LF_OK;
+    if (gated) return dtype == LF_DTYPE_I8 ? launch_gated_join<int32_t>(g, st) : launch_gated_join<float>(g, st);
+    return dtype == LF_DTYPE_I8 ? launch_join<int32_t>(g, st) : launch_join<float>(g, st);
 }
 
 constexpr int64_t kMostRows = 1ll << 40, kMostFeatures = 1ll << 24;
@@ -435,8 +511,7 @@ int lf_linear_grad(const lf_linear_grad_args* h_args, void* d_work, size_t work_
 }
 
 size_t lf_gated_linear_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype) {
-    if (m <= 0 || n <= 0 || k < 0 || !(is_float_dtype(dtype) || is_8bit_dtype(dtype))) return 0;
-    return padded((size_t)m * (size_t)n * 8) + lf_linear_work_bytes(m, 2 * n, k, dtype);
+    return lf_linear_work_bytes(m, 2 * n, k, dtype);
 }
 
 int lf_gated_linear(const lf_linear_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream) {
@@ -456,17 +531,10 @@ int lf_gated_linear(const lf_linear_args* h_args, void* d_work, size_t work_byte
     const size_t need = lf_gated_linear_work_bytes(a.m, a.n, a.k, a.dtype);
     LF_REQUIRE(need == 0 || (d_work && (uintptr_t)d_work % 16 == 0), LF_ERR_INVALID, "null or unaligned workspace");
     LF_REQUIRE(work_bytes >= need, LF_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", work_bytes, need);
-    const size_t sums = padded((size_t)a.m * (size_t)a.n * 8);
     Product g{};
-    g.p = a.d_x; g.q = a.d_w; g.ld_p = a.ld_x; g.ld_q = a.ld_w; g.m = a.m; g.n = 2 * a.n; g.k = a.k;
-    g.e.y = d_work; g.e.ld_y = 2 * a.n; g.e.y_dtype = LF_DTYPE_F32;
-    LF_TRY(launch_product(g, a.dtype, false, false, (char*)d_work + sums, (hipStream_t)stream));
-    const Epilogue e{a.d_y, nullptr, a.d_z, a.d_bias, a.d_x_scale, a.d_w_scale, a.ld_y, 0, a.ld_z, a.y_dtype, 0, a.z_dtype, a.bias_dtype, activation_of(a.activation, a.y_dtype)};
-    const int64_t groups = ceil_div(a.m * ceil_div(a.n, 8), 256);
-    LF_REQUIRE(groups < (1ll << 31), LF_ERR_UNSUPPORTED, "too many outputs");
-    gate_kernel<<<(unsigned)groups, 256, 0, (hipStream_t)stream>>>((const float*)d_work, a.m, a.n, e);
-    LF_HIP(hipGetLastError());
-    return LF_OK;
+    g.p = a.d_x; g.q = a.d_w; g.ld_p = a.ld_x; g.ld_q = a.ld_w; g.m = a.m; g.n = a.n; g.k = a.k;
+    g.e = Epilogue{a.d_y, nullptr, a.d_z, a.d_bias, a.d_x_scale, a.d_w_scale, a.ld_y, 0, a.ld_z, a.y_dtype, 0, a.z_dtype, a.bias_dtype, activation_of(a.activation, a.y_dtype)};
+    return launch_product(g, a.dtype, false, false, d_work, (hipStream_t)stream, true);
 }
 
 size_t lf_gated_linear_grad_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t want_dx, int32_t want_dw, int32_t want_db) {

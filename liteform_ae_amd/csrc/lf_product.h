@@ -20,6 +20,10 @@
 //     What a cut leaves below 2^-126 is lost to the instruction: values below 2^-110 have fewer digits than a float.
 //   * Few tiles are cut along k as well: partial sums in 32 bits, added up in a fixed order by a second kernel with the epilogue.
 // Up to 16 rows of X are another problem - W is read once, nothing is shared - and have a kernel of their own.
+//
+// The gated product, Y = act(X Wg^T + bg) (X Wu^T + bu), is one product with Q = [Wg; Wu], of 2 n rows.  A tile takes 16 rows of Wg and 16 of Wu in turn (gated_row), so
+// that a wavefront holds both sums of an output and the epilogue (leave_gated) needs no second pass over them: z is written only where it is asked
+// for.  bf16 8192 x 4096 by 2 x 8192 with silu and z: see wide_kernel.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -62,6 +66,12 @@ ProductFn product_bf16(bool px, bool qx, int tile, bool aligned, bool deep);
 ProductFn product_f16(bool px, bool qx, int tile, bool aligned, bool deep);
 ProductFn product_e4m3(bool px, bool qx, int tile, bool aligned, bool deep);
 ProductFn product_i8(bool px, bool qx, int tile, bool aligned, bool deep);
+// The same of the gated product, whose Q has 2 n rows (both operands along k).
+ProductFn gated_f32(int tile, bool aligned, bool deep);
+ProductFn gated_bf16(int tile, bool aligned, bool deep);
+ProductFn gated_f16(int tile, bool aligned, bool deep);
+ProductFn gated_e4m3(int tile, bool aligned, bool deep);
+ProductFn gated_i8(int tile, bool aligned, bool deep);
 
 }  // namespace lf
 
@@ -118,6 +128,22 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int64_t n, 
     store_upto8(e.y, m * e.ld_y + n, e.y_dtype, v, count);
 }
 
+// ... of a gated product of n outputs: v[0] and v[1] are sums of the gate and of the other half
+__device__ __forceinline__ void finish_gated(const Epilogue& e, int64_t m, int64_t col, int64_t n, int count, float8_t (&v)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (e.x_scale) v[h] = v[h] * e.x_scale[m] * load_upto8(e.w_scale + h * n + col, count);
+        if (e.bias) v[h] += load_upto8(e.bias, h * n + col, e.bias_dtype, count);
+        if (e.z) store_upto8(e.z, m * e.ld_z + h * n + col, e.z_dtype, v[h], count);
+    }
+    store_upto8(e.y, m * e.ld_y + col, e.y_dtype, activate(v[0], e.act) * v[1], count);
+}
+// Row r of a gated product's tile of Q: of which half it is, and which of the tile's outputs it belongs to.
+struct GatedRow {
+    int half, out;
+    __device__ __forceinline__ explicit GatedRow(int r) : half(r >> 4 & 1), out((r >> 5) * 16 + (r & 15)) {}
+};
+
 template <typename F> __device__ __forceinline__ void with_type(int32_t dtype, F f) {
     if (dtype == LF_DTYPE_F32) f(0.f);
     else if (dtype == LF_DTYPE_BF16) f((__bf16)0.f);
@@ -133,7 +159,7 @@ template <int PIECES> __device__ __forceinline__ int slot(int row, int c) {
 }
 
 // One operand's tile of ROWS x (a step of k): global memory -> registers -> LDS.
-template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
+template <typename T, bool ACROSS, int ROWS, int THREADS, bool GATED = false> struct Stage {
     static constexpr int kPlanes = Elem<T>::kPlanes;
     static constexpr int kStep = sizeof(T) == 4 ? 32 : 128 / sizeof(T);   // elements of k
     static constexpr int kPieces = sizeof(T) == 4 ? 4 : 8;                // pieces of a row in LDS (of each plane)
@@ -178,7 +204,12 @@ template <typename T, bool ACROSS, int ROWS, int THREADS> struct Stage {
                 const int u = tid + i * THREADS;
                 if (kUnits % THREADS && u >= kUnits) continue;
                 const int at = (u % kPieces) * kElems;
-                const T* src = base + min(row0 + u / kPieces, rows - 1) * ld + k0 + at;
+                int64_t row = min(row0 + u / kPieces, rows - 1);
+                if constexpr (GATED) {
+                    const GatedRow g(u / kPieces);
+                    row = g.half * rows + min(row0 + g.out, rows - 1);
+                }
+                const T* src = base + row * ld + k0 + at;
 #pragma unroll
                 for (int h = 0; h < kRegs; ++h) {
                     if (whole) r[i][h] = load16(src + h * kWide);
@@ -293,9 +324,10 @@ template <bool ACROSS> __device__ __forceinline__ uint4_t four_of(const float* p
         if (k + c < end) r[c] = __float_as_uint(p[(k + c) * ld + row]);
     return r;
 }
-template <bool PX, bool QX, int FM, int FN>
+template <bool PX, bool QX, bool GATED, int FM, int FN>
 __device__ __forceinline__ void repair(const Product& g, float4_t (&acc)[FM][FN], int64_t m, int64_t n, int64_t k_first, int64_t k_last) {
     const int li = threadIdx.x & 15, lg = threadIdx.x >> 4 & 3;
+    auto first_of = [&](int j) { return n + 16 * (GATED ? j >> 1 : j); };         // output of the j-th sixteen
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
         float none = 0.f;                                                // NaN where a sum is not finite
@@ -308,7 +340,7 @@ __device__ __forceinline__ void repair(const Product& g, float4_t (&acc)[FM][FN]
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) fine = fine && (fabsf(acc[i][j][v]) < __builtin_inff() || n + 16 * j + 4 * lg + v >= g.n);
+            for (int v = 0; v < 4; ++v) fine = fine && (fabsf(acc[i][j][v]) < __builtin_inff() || first_of(j) + 4 * lg + v >= g.n);
         if (__all(fine || m + 16 * i + li >= g.m)) continue;
         float4_t again[FN];
 #pragma unroll
@@ -317,7 +349,7 @@ __device__ __forceinline__ void repair(const Product& g, float4_t (&acc)[FM][FN]
         auto load = [&](int64_t k) {                                     // (sixteen k: four of a lane, the same ones of both operands)
             p = four_of<PX>((const float*)g.p, g.ld_p, min(m + 16 * i + li, g.m - 1), k + 4 * lg, k_last);
 #pragma unroll
-            for (int j = 0; j < FN; ++j) q[j] = four_of<QX>((const float*)g.q, g.ld_q, min(n + 16 * j + li, g.n - 1), k + 4 * lg, k_last);
+            for (int j = 0; j < FN; ++j) q[j] = four_of<QX>((const float*)g.q, g.ld_q, (GATED && j & 1 ? g.n : 0) + min(first_of(j) + li, g.n - 1), k + 4 * lg, k_last);
         };
         load(k_first);
 #pragma unroll 1
@@ -357,7 +389,7 @@ template <int N> __device__ __forceinline__ void activate_all(float8_t (&v)[N], 
 // different banks, as do those that write one c of eight rows.
 template <int WC> __device__ __forceinline__ int turned(int row, int c) { return row * (WC / 4) + (((c & 1) * (WC / 8) + (c >> 1)) ^ (row & 7)); }
 // What the epilogue needs of a tile's rows and columns, loaded before the first operands and kept in LDS: at the end each would be a wait.
-template <int TM, int TN> struct Vectors {
+template <int TM, int TN, bool GATED = false> struct Vectors {
     float bias[TN], w_scale[TN], x_scale[TM];
     struct Loaded { float b, w, x; };
     // (by 256 threads)
@@ -365,13 +397,15 @@ template <int TM, int TN> struct Vectors {
         const int t = threadIdx.x;
         Loaded l{0.f, 1.f, 1.f};
         if (g.part) return l;
-        if (t < TN && n0 + t < g.n) {
+        const GatedRow r(t);
+        const int64_t out = n0 + (GATED ? r.out : t), at = GATED ? r.half * g.n + out : out;
+        if (t < TN && out < g.n) {
             if (g.e.bias) {
-                if (g.e.bias_dtype == LF_DTYPE_F32) l.b = ((const float*)g.e.bias)[n0 + t];
-                else if (g.e.bias_dtype == LF_DTYPE_BF16) l.b = (float)((const __bf16*)g.e.bias)[n0 + t];
-                else l.b = (float)((const _Float16*)g.e.bias)[n0 + t];
+                if (g.e.bias_dtype == LF_DTYPE_F32) l.b = ((const float*)g.e.bias)[at];
+                else if (g.e.bias_dtype == LF_DTYPE_BF16) l.b = (float)((const __bf16*)g.e.bias)[at];
+                else l.b = (float)((const _Float16*)g.e.bias)[at];
             }
-            if (g.e.w_scale) l.w = g.e.w_scale[n0 + t];
+            if (g.e.w_scale) l.w = g.e.w_scale[at];
         }
         if (g.e.x_scale && t < TM && m0 + t < g.m) l.x = g.e.x_scale[m0 + t];
         return l;
@@ -519,6 +553,137 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
     if constexpr (PHASES > 3) phase(std::integral_constant<int, 3>{});
 }
 
+// The same of a gated product: a wavefront's WC columns of sums are those of WC / 2 outputs, sixteen of the gate and sixteen of the other half in turn.
+// A lane takes eight outputs of a row: four pieces of 16 bytes of the turned sums, each kind of which lies together in a row, and rows so that both the
+// 16 lanes that write one of 16 rows and those that read some rows meet different banks.
+template <int WC> __device__ __forceinline__ int turned_gated(int row, int c) {
+    constexpr int LANES = WC / 16;
+    const int kind = (c >> 2 & 1) * 2 + (c & 1), piece = (c >> 3) * 2 + (c >> 1 & 1);
+    const int r = LANES == 2 ? row >> 1 : row;              // (rows of eight pieces already lie two to all banks)
+    constexpr int ROWS = LANES == 2 ? 4 : 16 / LANES;
+    return row * (4 * LANES) + ((kind * LANES + piece) ^ (r % ROWS * LANES + r / ROWS % LANES));
+}
+template <int FM, int FN, int PR, typename Acc, typename Vec>
+__device__ __forceinline__ void leave_gated(const Product& g, const Acc (&acc)[FM][FN], uint4_t* lds, const Vec& vec, int64_t m0, int64_t n0, int row0, int col0) {
+    constexpr int WC = 16 * FN, LANES = WC / 16, AT_ONCE = 64 / LANES, PHASES = FM * 16 / PR;
+    constexpr bool INT = std::is_same_v<Acc, int4v>;
+    static_assert(FM * 16 % PR == 0 && PR % AT_ONCE == 0, "");
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    const int mine = lane / LANES, piece = lane % LANES;
+    const int64_t m = m0 + row0, n = n0 + col0 / 2 + piece * 8;
+    const int count = (int)max((int64_t)0, min((int64_t)8, g.n - n));
+    const Epilogue& e = g.e;
+    const bool whole = __all(count == 0 || count == 8) && !g.part;
+    const int at = col0 + (piece >> 1) * 32 + (piece & 1) * 8;            // of the gate in the tile's vectors
+    float8_t bias[2], ws[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            bias[h][i] = vec.bias[at + 16 * h + i];
+            ws[h][i] = vec.w_scale[at + 16 * h + i];
+        }
+    auto sums = [&](int row, float8_t (&v)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = (piece >> 1) * 8 + h * 4 + (piece & 1) * 2;
+            const uint4_t a = lds[turned_gated<WC>(row, c)], b = lds[turned_gated<WC>(row, c + 1)];
+            const uint32_t w[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[h][i] = __uint_as_float(w[i]);
+        }
+    };
+    auto as_floats = [&](float8_t (&v)[2]) {
+        if constexpr (INT)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[h][i] = (float)__float_as_int(v[h][i]);
+    };
+    auto phase = [&](auto number) {
+        constexpr int FIRST = decltype(number)::value * PR;
+#pragma unroll
+        for (int i = 0; i < PR / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) lds[turned_gated<WC>(16 * i + li, 4 * j + lg)] = __builtin_bit_cast(uint4_t, acc[FIRST / 16 + i][j]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (__builtin_expect(g.part != nullptr, 0)) {
+#pragma unroll 1
+            for (int row = mine; row < PR; row += AT_ONCE) {
+                float8_t v[2];
+                sums(row, v);
+                if (m + FIRST + row < g.m && count)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) store_upto8((float*)g.part + ((int64_t)blockIdx.y * g.m + m + FIRST + row) * 2 * g.n + h * g.n + n, v[h], count);
+            }
+        } else if (__builtin_expect(whole, 1)) {
+            // (a loop, for the instruction cache; two rows at a time, whose activations fill one another's waits)
+            constexpr int H = PR / AT_ONCE < 2 ? PR / AT_ONCE : 2;
+            auto pass = [&](auto act) {
+#pragma unroll 1
+                for (int r0 = mine; r0 < PR; r0 += H * AT_ONCE) {
+                    float8_t v[H][2], y[H];
+#pragma unroll
+                    for (int u = 0; u < H; ++u) {
+                        sums(r0 + u * AT_ONCE, v[u]);
+                        as_floats(v[u]);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (e.x_scale) v[u][h] = v[u][h] * vec.x_scale[row0 + FIRST + r0 + u * AT_ONCE] * ws[h];
+                            v[u][h] += bias[h];
+                        }
+                        y[u] = v[u][0];
+                    }
+                    if (e.z)
+                        with_type(e.z_dtype, [&](auto t) {
+                            using Z = decltype(t);
+#pragma unroll
+                            for (int u = 0; u < H; ++u) {
+                                const int64_t row = m + FIRST + r0 + u * AT_ONCE;
+                                if (row < g.m && count)
+#pragma unroll
+                                    for (int h = 0; h < 2; ++h) store8((Z*)e.z + row * e.ld_z + h * g.n + n, v[u][h], e.stream);
+                            }
+                        });
+                    act(y);
+#pragma unroll
+                    for (int u = 0; u < H; ++u) y[u] *= v[u][1];
+                    with_type(e.y_dtype, [&](auto t) {
+                        using Y = decltype(t);
+#pragma unroll
+                        for (int u = 0; u < H; ++u) {
+                            const int64_t row = m + FIRST + r0 + u * AT_ONCE;
+                            if (row < g.m && count) store8((Y*)e.y + row * e.ld_y + n, y[u], e.stream);
+                        }
+                    });
+                }
+            };
+            if (__builtin_expect(e.act & kActFine, 0))
+                pass([&](float8_t (&y)[H]) {
+#pragma unroll
+                    for (int u = 0; u < H; ++u) y[u] = activate_fine(y[u], e.act);
+                });
+            else pass([&](float8_t (&y)[H]) { activate_all(y, e.act); });
+        } else {
+#pragma unroll 1
+            for (int row = mine; row < PR; row += AT_ONCE) {
+                float8_t v[2];
+                sums(row, v);
+                as_floats(v);
+                if (m + FIRST + row < g.m && count) finish_gated(e, m + FIRST + row, n, g.n, count, v);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    static_assert(PHASES <= 4, "");
+    phase(std::integral_constant<int, 0>{});
+    if constexpr (PHASES > 1) phase(std::integral_constant<int, 1>{});
+    if constexpr (PHASES > 2) phase(std::integral_constant<int, 2>{});
+    if constexpr (PHASES > 3) phase(std::integral_constant<int, 3>{});
+}
+
 // The tile of a workgroup.  Workgroups go to the eight XCDs in turn: each XCD gets a run of neighbouring tiles, eight rows of
 // tiles deep, so that what its L2 holds of both operands is used by its 32 CUs at once.
 __device__ __forceinline__ void tile_of(const Product& g, unsigned id, int& tm, int& tn) {
@@ -531,25 +696,24 @@ __device__ __forceinline__ void tile_of(const Product& g, unsigned id, int& tm, 
     tn = (int)(t / deep);
 }
 
-template <typename T, bool PX, bool QX, int TM, int TN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 4)
-product_kernel(Product g) {
+template <typename T, bool PX, bool QX, int TM, int TN, int WM, int WN, bool GATED>
+__device__ __forceinline__ void product_tile(const Product& g) {
     constexpr int THREADS = 64 * WM * WN, FM = TM / WM / 16, FN = TN / WN / 16;
     using Acc = typename Elem<T>::Acc;
     using StageP = Stage<T, PX, TM, THREADS>;
-    using StageQ = Stage<T, QX, TN, THREADS>;
+    using StageQ = Stage<T, QX, TN, THREADS, GATED>;
     constexpr int PL = StageP::kPlanes, PC = StageP::kPieces, KS = StageP::kStep;
     // float32 takes three planes: one buffer, so that a CU holds two workgroups, one of which multiplies while the other stores
     constexpr int NB = PL == 3 ? 1 : 2;
     constexpr int SP = PL * StageP::kSlots, SQ = PL * StageQ::kSlots;
     __shared__ uint4_t s_all[NB * (SP + SQ)];
     uint4_t *const s_p = s_all, *const s_q = s_all + NB * SP;
-    __shared__ Vectors<TM, TN> s_vec;
+    __shared__ Vectors<TM, TN, GATED> s_vec;
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
     int tm, tn;
     tile_of(g, blockIdx.x, tm, tn);
-    const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * TN;
+    const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * (GATED ? TN / 2 : TN);
     const int64_t k_first = (int64_t)blockIdx.y * g.k_split, k_last = min(g.k, k_first + g.k_split);
 
     Acc acc[FM][FN];
@@ -662,9 +826,14 @@ product_kernel(Product g) {
     static_assert(PR <= FIT && WHOLE % PR == 0, "");
     uint4_t* mine = s_all + wave * SLOTS;
     const int row0 = wm * (TM / WM), col0 = wn * (TN / WN);
-    if constexpr (PL == 3) repair<PX, QX>(g, acc, m0 + row0, n0 + col0, k_first, k_last);
-    leave<FM, FN, PR>(g, acc, mine, s_vec, m0, n0, row0, col0);
+    if constexpr (PL == 3) repair<PX, QX, GATED>(g, acc, m0 + row0, n0 + (GATED ? col0 / 2 : col0), k_first, k_last);
+    if constexpr (GATED) leave_gated<FM, FN, PR>(g, acc, mine, s_vec, m0, n0, row0, col0);
+    else leave<FM, FN, PR>(g, acc, mine, s_vec, m0, n0, row0, col0);
 }
+template <typename T, bool PX, bool QX, int TM, int TN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 4) product_kernel(Product g) { product_tile<T, PX, QX, TM, TN, WM, WN, false>(g); }
+template <typename T, int TILE>
+__global__ void __launch_bounds__(256, TILE == 128 ? 2 : 4) gated_product_kernel(Product g) { product_tile<T, false, false, TILE, TILE, 2, 2, true>(g); }
 
 // ---------------------------------------------------------------------------- the tiled product, large tiles
 
@@ -729,7 +898,8 @@ template <typename T, bool ACROSS, int ROWS> struct Direct {
         const int n = kPairs * (wave + 4 * i) + lane / kPair;
         return 2 * ((n & 16) | (n >> 1 & 3) * 4 | (n >> 3 & 1) * 2 | (n & 1)) + (lane & 1);
     }
-    __device__ __forceinline__ Direct(const void* p, int64_t ld, int64_t row0, int64_t rows, int64_t k0) {
+    // gated: a load instruction's eight rows are of one half, which its wavefront has in common
+    __device__ __forceinline__ Direct(const void* p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, bool gated = false) {
         lane = threadIdx.x & 63;
         li = lane & 15;
         lg = lane >> 4;
@@ -738,6 +908,12 @@ template <typename T, bool ACROSS, int ROWS> struct Direct {
         if constexpr (!ACROSS) {
             base = (const char*)p + (row0 * ld + k0) * sizeof(T);
             step_bytes = 128;
+            if (gated) {
+                base += (wave >> 1) * rows * ld * (int64_t)sizeof(T);
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) off[i] = (uint32_t)min((int64_t)GatedRow(8 * (wave + 4 * i) + (lane >> 3)).out, rows - 1 - row0) * ld_bytes + at(i) * (int)sizeof(T);
+                return;
+            }
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) off[i] = (uint32_t)min((int64_t)(8 * (wave + 4 * i) + (lane >> 3)), rows - 1 - row0) * ld_bytes + at(i) * (int)sizeof(T);
         } else {
@@ -792,23 +968,22 @@ __device__ __forceinline__ void arrived() {
     asm volatile("" ::: "memory");
 }
 
-template <typename T, bool PX, bool QX>
-__global__ void __launch_bounds__(256)
-wide_kernel(Product g) {
+template <typename T, bool PX, bool QX, bool GATED>
+__device__ __forceinline__ void wide_tile(const Product& g) {
     using Acc = typename Elem<T>::Acc;
     using F = Frag<T>;
     constexpr int KS = 128 / sizeof(T);
     // (arrays of their own: what is read from one must not wait for what is on its way into another)
     __shared__ uint4_t s_p0[Direct<T, PX, 256>::kSlots], s_q0[Direct<T, QX, 256>::kSlots], s_p1[Direct<T, PX, 256>::kSlots], s_q1[Direct<T, QX, 256>::kSlots];
-    __shared__ Vectors<256, 256> s_vec;
+    __shared__ Vectors<256, 256, GATED> s_vec;
     int tm, tn;
     tile_of(g, blockIdx.x, tm, tn);
-    const int64_t m0 = (int64_t)tm * 256, n0 = (int64_t)tn * 256;
+    const int64_t m0 = (int64_t)tm * 256, n0 = (int64_t)tn * (GATED ? 128 : 256);
     const int64_t k_first = (int64_t)blockIdx.y * g.k_split, k_last = min(g.k, k_first + g.k_split);
     using DP = Direct<T, PX, 256>;
     using DQ = Direct<T, QX, 256>;
     DP P(g.p, g.ld_p, m0, g.m, k_first);
-    DQ Q(g.q, g.ld_q, n0, g.n, k_first);
+    DQ Q(g.q, g.ld_q, n0, g.n, k_first, GATED);
     const int wm = P.wave & 1, wn = P.wave >> 1, row_p = wm * 128, row_q = wn * 128;
 
     Acc acc[8][8];
@@ -905,8 +1080,11 @@ wide_kernel(Product g) {
     for (int i = 0; i < 8; ++i) settle(acc[i]);
     __syncthreads();
     uint4_t* mine = P.wave == 0 ? s_p0 : P.wave == 1 ? s_q0 : P.wave == 2 ? s_p1 : s_q1;
-    leave<8, 8, 64>(g, acc, mine, s_vec, m0, n0, row_p, row_q);
+    if constexpr (GATED) leave_gated<8, 8, 64>(g, acc, mine, s_vec, m0, n0, row_p, row_q);
+    else leave<8, 8, 64>(g, acc, mine, s_vec, m0, n0, row_p, row_q);
 }
+template <typename T, bool PX, bool QX> __global__ void __launch_bounds__(256) wide_kernel(Product g) { wide_tile<T, PX, QX, false>(g); }
+template <typename T> __global__ void __launch_bounds__(256) gated_wide_kernel(Product g) { wide_tile<T, false, false, true>(g); }
 
 // ---------------------------------------------------------------------------- the tiled product, aligned operands, small tiles
 
@@ -914,21 +1092,20 @@ wide_kernel(Product g) {
 // of this one, the order of the instructions left to the compiler.  With two buffers a CU holds two (four) workgroups, whose wavefronts
 // cover one another's waits; where there are too few workgroups for that, four buffers have more steps on their way.
 // bf16 2000^3 28 us, through registers (rows at odd addresses) 40; the tile of 64 and that of 128: see step_us().
-template <typename T, bool PX, bool QX, int TILE, int BUFFERS>
-__global__ void __launch_bounds__(256, BUFFERS == 4 ? 1 : TILE == 128 ? 2 : 4)
-direct_kernel(Product g) {
+template <typename T, bool PX, bool QX, int TILE, int BUFFERS, bool GATED>
+__device__ __forceinline__ void direct_tile(const Product& g) {
     using Acc = typename Elem<T>::Acc;
     using DP = Direct<T, PX, TILE>;
     using DQ = Direct<T, QX, TILE>;
     constexpr int KS = 128 / sizeof(T), FR = TILE / 32, SB = DP::kSlots + DQ::kSlots;
     __shared__ uint4_t s[BUFFERS * SB];
-    __shared__ Vectors<TILE, TILE> s_vec;
+    __shared__ Vectors<TILE, TILE, GATED> s_vec;
     int tm, tn;
     tile_of(g, blockIdx.x, tm, tn);
-    const int64_t m0 = (int64_t)tm * TILE, n0 = (int64_t)tn * TILE;
+    const int64_t m0 = (int64_t)tm * TILE, n0 = (int64_t)tn * (GATED ? TILE / 2 : TILE);
     const int64_t k_first = (int64_t)blockIdx.y * g.k_split, k_last = min(g.k, k_first + g.k_split);
     DP P(g.p, g.ld_p, m0, g.m, k_first);
-    DQ Q(g.q, g.ld_q, n0, g.n, k_first);
+    DQ Q(g.q, g.ld_q, n0, g.n, k_first, GATED);
     const int row_p = (P.wave & 1) * (TILE / 2), row_q = (P.wave >> 1) * (TILE / 2);
     Acc acc[FR][FR];
 #pragma unroll
@@ -1024,8 +1201,14 @@ direct_kernel(Product g) {
         multiply(o);
     }
     arrived();
-    leave<FR, FR, TILE / 2 < 32 ? TILE / 2 : 32>(g, acc, s + P.wave * (SB / 2), s_vec, m0, n0, row_p, row_q);
+    constexpr int PR = TILE / 2 < 32 ? TILE / 2 : 32;
+    if constexpr (GATED) leave_gated<FR, FR, PR>(g, acc, s + P.wave * (SB / 2), s_vec, m0, n0, row_p, row_q);
+    else leave<FR, FR, PR>(g, acc, s + P.wave * (SB / 2), s_vec, m0, n0, row_p, row_q);
 }
+template <typename T, bool PX, bool QX, int TILE, int BUFFERS>
+__global__ void __launch_bounds__(256, BUFFERS == 4 ? 1 : TILE == 128 ? 2 : 4) direct_kernel(Product g) { direct_tile<T, PX, QX, TILE, BUFFERS, false>(g); }
+template <typename T, int TILE, int BUFFERS>
+__global__ void __launch_bounds__(256, BUFFERS == 4 ? 1 : TILE == 128 ? 2 : 4) gated_direct_kernel(Product g) { direct_tile<T, false, false, TILE, BUFFERS, true>(g); }
 
 template <typename T, bool PX, bool QX> ProductFn kernel_of(int tile, bool aligned, bool deep) {
     if constexpr (!std::is_same_v<T, float>)
@@ -1034,6 +1217,13 @@ template <typename T, bool PX, bool QX> ProductFn kernel_of(int tile, bool align
         if (aligned) return tile == 128 ? (deep ? direct_kernel<T, PX, QX, 128, 4> : direct_kernel<T, PX, QX, 128, 2>)
                                : deep ? direct_kernel<T, PX, QX, 64, 4> : direct_kernel<T, PX, QX, 64, 2>;
     return tile == 128 ? product_kernel<T, PX, QX, 128, 128, 2, 2> : product_kernel<T, PX, QX, 64, 64, 2, 2>;
+}
+template <typename T> ProductFn gated_of(int tile, bool aligned, bool deep) {
+    if constexpr (!std::is_same_v<T, float>) {
+        if (tile == kWideTile) return gated_wide_kernel<T>;
+        if (aligned) return tile == 128 ? (deep ? gated_direct_kernel<T, 128, 4> : gated_direct_kernel<T, 128, 2>) : deep ? gated_direct_kernel<T, 64, 4> : gated_direct_kernel<T, 64, 2>;
+    }
+    return tile == 128 ? gated_product_kernel<T, 128> : gated_product_kernel<T, 64>;
 }
 template <typename T> ProductFn kernel_of(bool px, bool qx, int tile, bool aligned, bool deep) {
     return px ? kernel_of<T, true, true>(tile, aligned, deep) : qx ? kernel_of<T, false, true>(tile, aligned, deep) : kernel_of<T, false, false>(tile, aligned, deep);
