@@ -16,7 +16,7 @@ using namespace lf;
 
 constexpr int kTensors = 64;                                // to a launch
 constexpr int64_t kChunk = 16384;                           // elements to a workgroup
-constexpr int kMostParts = 1024;                            // partial sums of a call
+constexpr int kMostParts = 2048;                            // partial sums of a call
 
 struct Tensor { const void* src; void* dst; int64_t rows, cols, ld_src, ld_dst; };
 struct List {
@@ -34,13 +34,31 @@ __device__ __forceinline__ int tensor_of(const List& l, int chunk) {
     }
     return lo;
 }
+// Eight pieces of eight elements to a thread, all under way at once: f(piece, element of src, of dst, count) for each.
+constexpr int kMine = (int)(kChunk / 8 / 256);
 template <typename F> __device__ __forceinline__ void pieces_of(const Tensor& t, int64_t chunk, F f) {
-    // pieces of eight of a row
-    const int64_t across = (t.cols + 7) / 8, end = min(across * t.rows, (chunk + 1) * (kChunk / 8));
-    for (int64_t u = chunk * (kChunk / 8) + threadIdx.x; u < end; u += 256) {
-        const int64_t row = u / across, col = (u - row * across) * 8;
-        f(row, col, (int)min((int64_t)8, t.cols - col));
+    const int64_t u0 = chunk * (kChunk / 8) + threadIdx.x;
+    if (t.rows == 1) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int64_t col = (u0 + i * 256) * 8;
+            f(i, col, col, (int)max((int64_t)0, min((int64_t)8, t.cols - col)));
+        }
+        return;
     }
+    const int64_t across = (t.cols + 7) / 8, end = across * t.rows;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int64_t u = u0 + i * 256, row = u / across, col = (u - row * across) * 8;
+        f(i, row * t.ld_src + col, row * t.ld_dst + col, u < end ? (int)min((int64_t)8, t.cols - col) : 0);
+    }
+}
+template <typename F> __device__ __forceinline__ void of_type(int32_t dtype, F f) {
+    if (dtype == LF_DTYPE_F32) f(0.f); else if (dtype == LF_DTYPE_BF16) f((__bf16)0.f); else f((_Float16)0.f);
+}
+template <typename T> using Raw = typename Eight<T>::vec;
+template <typename T> __device__ __forceinline__ Raw<T> load_raw(const T* p, int n) {
+    return n >= 8 ? reinterpret_cast<const typename Eight<T>::Any*>(p)->v : __builtin_convertvector(load_upto8(p, n), Raw<T>);
 }
 __device__ __forceinline__ double sum_of_workgroup(double v) {
     __shared__ double s[4];
@@ -56,10 +74,22 @@ __global__ void __launch_bounds__(256) squares_kernel(List l, double* part) {
     for (int chunk = blockIdx.x; chunk < l.first[l.n]; chunk += gridDim.x) {
         const int i = tensor_of(l, chunk);
         const Tensor& t = l.t[i];
-        pieces_of(t, chunk - l.first[i], [&](int64_t row, int64_t col, int n) {
-            const float8_t v = load_upto8(t.src, row * t.ld_src + col, l.dtype[i], n);
+        of_type(l.dtype[i], [&](auto z) {
+            using T = decltype(z);
+            Raw<T> raw[kMine];
+            pieces_of(t, chunk - l.first[i], [&](int u, int64_t at, int64_t, int n) { raw[u] = load_raw((const T*)t.src + at, n); });
+            double mine[kMine];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fma((double)v[j], (double)v[j], sum);
+            for (int u = 0; u < kMine; ++u) {
+                mine[u] = 0.0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const double v = (double)(float)raw[u][j];
+                    mine[u] = fma(v, v, mine[u]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kMine; ++u) sum += mine[u];
         });
     }
     sum = sum_of_workgroup(sum);
@@ -67,7 +97,7 @@ __global__ void __launch_bounds__(256) squares_kernel(List l, double* part) {
 }
 
 // (every workgroup adds up the partial sums, all in one order)
-__global__ void __launch_bounds__(256) clip_kernel(List l, const double* part, int32_t parts, float most, float eps, float* norm, int32_t write_norm) {
+__global__ void __launch_bounds__(256) clip_kernel(List l, const double* part, int32_t parts, float most, float eps, float* norm, int32_t write_norm, int32_t stream) {
     double sum = 0.0;
     for (int i = threadIdx.x; i < parts; i += 256) sum += part[i];
     const float total = (float)sqrt(sum_of_workgroup(sum));
@@ -77,9 +107,13 @@ __global__ void __launch_bounds__(256) clip_kernel(List l, const double* part, i
         const int i = tensor_of(l, chunk);
         const Tensor& t = l.t[i];
         if (c == 1.f && t.src == t.dst) continue;
-        pieces_of(t, chunk - l.first[i], [&](int64_t row, int64_t col, int n) {
-            const float8_t v = load_upto8(t.src, row * t.ld_src + col, l.dtype[i], n);
-            store_upto8(t.dst, row * t.ld_dst + col, l.dtype[i], v * c, n);
+        of_type(l.dtype[i], [&](auto z) {
+            using T = decltype(z);
+            Raw<T> raw[kMine];
+            pieces_of(t, chunk - l.first[i], [&](int u, int64_t at, int64_t, int n) { raw[u] = load_raw((const T*)t.src + at, n); });
+            pieces_of(t, chunk - l.first[i], [&](int u, int64_t, int64_t at, int n) {
+                store_upto8((T*)t.dst + at, __builtin_convertvector(raw[u], float8_t) * c, n, stream);
+            });
         });
     }
 }
@@ -162,6 +196,9 @@ int clip(const lf_tensor_desc* t, int32_t n, float most, float eps, float* d_nor
                                                                                                                               : t[i].rows * ceil_div(t[i].cols, 8);
         if (pieces) add(c, t[i], ceil_div(pieces, kChunk / 8));
     }
+    int64_t bytes = 0;
+    for (int32_t i = 0; i < n; ++i) bytes += t[i].rows * t[i].cols * dtype_bytes((int32_t)t[i].dtype);
+    const int32_t stream = bytes >= kStreamBytes;
     double* part = (double*)d_work;
     int32_t parts = 0;
     for (const List& l : c.lists) {
@@ -172,13 +209,13 @@ int clip(const lf_tensor_desc* t, int32_t n, float most, float eps, float* d_nor
     }
     if (c.lists.empty() || !out) {
         List none{};
-        clip_kernel<<<1, 256, 0, st>>>(none, part, parts, most, eps, d_norm, 1);
+        clip_kernel<<<1, 256, 0, st>>>(none, part, parts, most, eps, d_norm, 1, 0);
         LF_HIP(hipGetLastError());
         return LF_OK;
     }
     for (size_t i = 0; i < c.lists.size(); ++i) {
         const List& l = c.lists[i];
-        clip_kernel<<<(unsigned)std::min(l.first[l.n], 4096), 256, 0, st>>>(l, part, parts, most, eps, d_norm, i == 0);
+        clip_kernel<<<(unsigned)std::min(l.first[l.n], 4096), 256, 0, st>>>(l, part, parts, most, eps, d_norm, i == 0, stream);
         LF_HIP(hipGetLastError());
     }
     return LF_OK;

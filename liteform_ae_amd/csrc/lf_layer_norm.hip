@@ -270,6 +270,13 @@ struct LayerGradArgs {
     }
 };
 
+// A piece as it lies in memory: what is loaded a row ahead takes no more registers than that.
+template <typename T> __device__ __forceinline__ typename Eight<T>::vec load_raw(const T* row, const Piece& p, int dim) {
+    return dim >= 8 ? reinterpret_cast<const typename Eight<T>::Any*>(row + p.at)->v : __builtin_convertvector(load_upto8(row, dim), typename Eight<T>::vec);
+}
+
+// A workgroup's next row is loaded before the sums of this one, whose barriers it fills (bf16 32k x 2048: 117 us without).  Not where the registers for it would
+// take the place of other wavefronts.
 template <typename DT, typename HT, int G, int C>
 __global__ void __launch_bounds__(G < 256 ? 256 : G)
 layer_norm_grad_kernel(LayerGradArgs a) {
@@ -284,16 +291,31 @@ layer_norm_grad_kernel(LayerGradArgs a) {
         sums[0][c] = sums[1][c] = float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (a.w) w[c] = load_piece(a.w, 0, a.w_dtype, piece_of((c * G + lane) * 8, dim), dim);
     }
-    for (int64_t row = (int64_t)blockIdx.x * R + group; row < a.rows; row += (int64_t)gridDim.x * R) {
-        float8_t h[C], dy[C];
-        const HT* hr = (const HT*)a.h + row * a.ldh;
-        const DT* dr = (const DT*)a.dy + row * a.ldy;
+    constexpr bool AHEAD = G < 1024 && C * (sizeof(DT) + 2 * sizeof(HT)) <= 12;
+    typename Eight<HT>::vec raw_h[C], raw_dh[C];
+    typename Eight<DT>::vec raw_dy[C];
+    auto load = [&](int64_t row) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const Piece p = piece_of((c * G + lane) * 8, dim);
-            h[c] = load_piece(hr, p, dim);
-            dy[c] = load_piece(dr, p, dim);
+            raw_h[c] = load_raw((const HT*)a.h + row * a.ldh, p, dim);
+            raw_dy[c] = load_raw((const DT*)a.dy + row * a.ldy, p, dim);
+            if (a.dh && AHEAD) raw_dh[c] = load_raw((const HT*)a.dh + row * a.ldd, p, dim);
         }
+    };
+    const int64_t step = (int64_t)gridDim.x * R;
+    int64_t row = (int64_t)blockIdx.x * R + group;
+    if (AHEAD && row < a.rows) load(row);
+    for (; row < a.rows; row += step) {
+        if (!AHEAD) load(row);
+        float8_t h[C], dy[C], dh[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            h[c] = __builtin_convertvector(raw_h[c], float8_t);
+            dy[c] = __builtin_convertvector(raw_dy[c], float8_t);
+            if (AHEAD) dh[c] = __builtin_convertvector(raw_dh[c], float8_t);
+        }
+        if (AHEAD && row + step < a.rows) load(row + step);
         auto each_of = [&](auto f) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
@@ -334,7 +356,7 @@ layer_norm_grad_kernel(LayerGradArgs a) {
             const Piece p = piece_of((c * G + lane) * 8, dim);
             const float8_t t = m.of(h[c]);
             float8_t d = (dy[c] * w[c] - g_mean - t * along) * s;
-            if (a.dh) d += load_piece((const HT*)a.dh + row * a.ldd, p, dim);
+            if (a.dh) d += AHEAD ? dh[c] : load_piece((const HT*)a.dh + row * a.ldd, p, dim);
             sums[0][c] += dy[c] * t;
             sums[1][c] += dy[c];
             if (p.first < 8) store_piece(dx, p, dim, d, a.stream);
@@ -440,23 +462,35 @@ layer_norm_grad_long_kernel(LayerGradArgs a) {
     }
 }
 
-// Columns of [n][2][dim] partial sums into dw and db (blockIdx.y): 16 columns to a workgroup, every 64th row to a thread, then the threads in order.
+// Columns of [n][2][dim] partial sums into dw and db (blockIdx.y): 32 columns to a workgroup, two to a thread (a line of 128 bytes of a row), every 64th row,
+// then the threads in order.
 __global__ void __launch_bounds__(1024) layer_norm_sums_kernel(const float* part, int64_t n, int32_t dim, void* dw, int32_t w_dtype, void* db, int32_t db_dtype) {
-    __shared__ float s[64][17];
+    typedef float any2_t __attribute__((ext_vector_type(2), aligned(4)));
+    __shared__ float s[64][33];
     void* out = blockIdx.y ? db : dw;
     if (!out) return;
-    const int col = blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
-    const float* src = part + (int64_t)blockIdx.y * dim + min(col, dim - 1);
-    float v = 0.f;
+    const int col0 = blockIdx.x * 32, col = col0 + (threadIdx.x & 15) * 2, slice = threadIdx.x >> 4;
+    const float* src = part + (int64_t)blockIdx.y * dim;
+    float a = 0.f, b = 0.f;
+    if (col + 1 < dim) {
 #pragma unroll 8
-    for (int64_t r = slice; r < n; r += 64) v += src[r * 2 * dim];
-    s[slice][threadIdx.x & 15] = v;
+        for (int64_t r = slice; r < n; r += 64) {
+            const any2_t v = *reinterpret_cast<const any2_t*>(src + r * 2 * dim + col);
+            a += v[0];
+            b += v[1];
+        }
+    } else if (col < dim) {
+#pragma unroll 8
+        for (int64_t r = slice; r < n; r += 64) a += src[r * 2 * dim + col];
+    }
+    s[slice][(threadIdx.x & 15) * 2] = a;
+    s[slice][(threadIdx.x & 15) * 2 + 1] = b;
     __syncthreads();
-    if (slice || col >= dim) return;
-    v = 0.f;
+    if (threadIdx.x >= 32 || col0 + (int)threadIdx.x >= dim) return;
+    float v = 0.f;
 #pragma unroll
     for (int i = 0; i < 64; ++i) v += s[i][threadIdx.x];
-    store_one(out, col, blockIdx.y ? db_dtype : w_dtype, v);
+    store_one(out, col0 + threadIdx.x, blockIdx.y ? db_dtype : w_dtype, v);
 }
 
 template <typename A, typename B> struct Kernels {
@@ -570,7 +604,7 @@ int lf_layer_norm_grad(const lf_layer_norm_grad_args* h_args, void* d_work, size
         LF_HIP(hipGetLastError());
     }
     if (sums && !one) {
-        layer_norm_sums_kernel<<<dim3((unsigned)ceil_div(a.dim, 16), 2), 1024, 0, st>>>((const float*)d_work, groups, (int32_t)a.dim, a.d_dw, a.weight_dtype, a.d_db,
+        layer_norm_sums_kernel<<<dim3((unsigned)ceil_div(a.dim, 32), 2), 1024, 0, st>>>((const float*)d_work, groups, (int32_t)a.dim, a.d_dw, a.weight_dtype, a.d_db,
                                                                                         a.db_dtype);
         LF_HIP(hipGetLastError());
     }

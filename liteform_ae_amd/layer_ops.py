@@ -521,38 +521,40 @@ def embedding_grad(dy, ids, rows: int, scale: float = 1.0, out_dtype=None):
 # --------------------------------------------------------------------------- norm of all gradients
 
 
-def _dense_rows(name, t, device):
-    """(rows, columns, elements from row to row, type) of a contiguous tensor, or of a matrix with contiguous rows."""
-    code = _FLOATS.get(t.dtype)
-    if code is None or t.get_device() != device:
-        raise ValueError(f"{name} must be on the current device, cuda:{device}, and one of {[str(d) for d in _FLOATS]}, got {t.dtype} on {t.device}")
-    if t.requires_grad:
-        refuse_graph(name, t)
-    if t.is_contiguous():
-        return 1, t.numel(), 0, code
-    if t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1) and t.stride(0) >= t.shape[1]:
-        return t.shape[0], t.shape[1], t.stride(0), code
-    raise ValueError(f"{name} must be contiguous, or a matrix whose rows are contiguous and do not overlap, got {tuple(t.shape)} with strides {t.stride()}")
-
-
 def _clip(grads, most, eps, in_place, want):
     torch, lib, device = _begin()
     grads = list(grads)
-    layouts = [_dense_rows(f"gradient {i}", g, device) for i, g in enumerate(grads)]
-    out = grads
-    if want and not in_place:
-        # one allocation to a type
-        sizes = {}
-        for g in grads:
-            sizes.setdefault(g.dtype, []).append(g.numel())
-        parts = {t: iter(torch.empty(sum(s), dtype=t, device=f"cuda:{device}").split(s)) for t, s in sizes.items()}
-        out = [next(parts[g.dtype]).view(g.shape) for g in grads]
-    descs = b"".join(_TENSOR_DESC(g.data_ptr(), o.data_ptr() if want else 0, rows, cols, ld, ld if o is g else cols, code)
-                     for g, o, (rows, cols, ld, code) in zip(grads, out, layouts))
+    types, at, layouts = _FLOATS, {}, []
+    for i, g in enumerate(grads):
+        code = types.get(g.dtype)
+        if code is None or g.get_device() != device:
+            raise ValueError(f"gradient {i} must be on the current device, cuda:{device}, and one of {[str(d) for d in types]}, got {g.dtype} on {g.device}")
+        if g.requires_grad:
+            refuse_graph(f"gradient {i}", g)
+        n = g.numel()
+        if g.is_contiguous():
+            rows, cols, ld = 1, n, 0
+        elif g.dim() == 2 and (g.shape[1] == 1 or g.stride(1) == 1) and g.stride(0) >= g.shape[1]:
+            (rows, cols), ld = g.shape, g.stride(0)
+        else:
+            raise ValueError(f"gradient {i} must be contiguous, or a matrix whose rows are contiguous and do not overlap, got {tuple(g.shape)} with strides {g.stride()}")
+        # outputs of one type lie behind each other, each at a multiple of 16 bytes
+        start = at.get(code, 0)
+        at[code] = start + (n + 7 & -8)
+        layouts.append((rows, cols, ld, code, start))
     norm = torch.empty((), dtype=torch.float32, device=f"cuda:{device}")
+    out, flat = grads, {}
+    if want and not in_place:
+        flat = {code: norm.new_empty(at[code], dtype=dtype) for dtype, code in types.items() if code in at}
+        out = [flat[code].as_strided(g.shape, g.stride(), start) if not ld else flat[code][start:start + rows * cols].view(rows, cols)
+               for g, (rows, cols, ld, code, start) in zip(grads, layouts)]
+        base = {code: (t.data_ptr(), t.element_size()) for code, t in flat.items()}
+        descs = [_TENSOR_DESC(g.data_ptr(), base[code][0] + start * base[code][1], rows, cols, ld, cols, code) for g, (rows, cols, ld, code, start) in zip(grads, layouts)]
+    else:
+        descs = [_TENSOR_DESC(p, p if want else 0, rows, cols, ld, ld, code) for p, (rows, cols, ld, code, _) in zip([g.data_ptr() for g in grads], layouts)]
     nbytes = lib.lf_clip_work_bytes(len(grads))
-    work = torch.empty(nbytes, dtype=torch.uint8, device=norm.device) if nbytes else None
-    rc = lib.lf_clip_gradients(descs, len(grads), most, eps, norm.data_ptr(), work.data_ptr() if nbytes else None, nbytes, _stream())
+    work = norm.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    rc = lib.lf_clip_gradients(b"".join(descs), len(grads), most, eps, norm.data_ptr(), work.data_ptr() if nbytes else None, nbytes, _stream())
     if rc:
         _lib.check(rc)
     if want and in_place:
