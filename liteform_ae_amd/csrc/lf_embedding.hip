@@ -147,8 +147,8 @@ template <typename C> __device__ __forceinline__ uint32_t rank_in_wave(C* count,
     return seen + before;
 }
 
-// Up to so many workgroups add up one another's counts themselves, which spares a launch (and 32 loads a digit take as long as one).
-constexpr int kFewGroups = 32;
+// With so few counts workgroups add up one another's themselves, which spares a launch (32 loads a thread take as long as one; 84 took 20 us, in two launches 14).
+constexpr int kFewCounts = 32 * kSortThreads;
 
 // FEW: `counts` is what sort_count_kernel left
 template <bool FEW>
@@ -342,7 +342,7 @@ __device__ __forceinline__ int end_of(const Entry* e, int lo, int hi, uint32_t k
 
 // A workgroup takes a span of sorted entries, G threads of it `each` one after the other, eight columns a thread.  Ids that go on from these G threads to the next are
 // put together in LDS; of one that goes on from a workgroup to the next, `tail` is what the one that it begins in has of it, `head` what each of the others has.
-constexpr int kSumThreads = 512, kMostEach = 64;
+constexpr int kSumThreads = 256, kMostEach = 64;
 template <typename S> struct Sums {
     const Entry* e;
     const uint8_t* present;                                 // of each row, whether its id occurs; NULL: it is looked for
@@ -356,12 +356,22 @@ template <typename S> struct Sums {
 };
 template <typename S> struct Eight8 { typedef S vec __attribute__((ext_vector_type(8))); };
 
+// A thread's eight columns.  The last ones of a row whose length is no multiple of eight reach back into those before, which two threads then
+// compute and write, alike; rows of less than eight have `count` columns.
+struct Columns {
+    int64_t col;
+    int count;
+    bool on;
+    __device__ __forceinline__ Columns(int64_t first, int64_t dim) : col(dim < 8 ? 0 : min(first, dim - 8)), count((int)min(dim, (int64_t)8)), on(first < dim) {}
+};
+template <typename S> struct AnyEight { struct __attribute__((packed, aligned(sizeof(S)))) type { typename Eight8<S>::vec v; }; };
+
 template <typename S> __device__ __forceinline__ float8_t scaled(typename Eight8<S>::vec v, float scale) {
     return __builtin_convertvector(v * (S)scale, float8_t);
 }
 
 // Rows of ids that do not occur: `fill_rows` to a wavefront, a row's id to a lane.
-template <typename S, int G> __device__ __forceinline__ void fill_rows(const Sums<S>& a, int64_t col, int count) {
+template <typename S, int G> __device__ __forceinline__ void fill_rows(const Sums<S>& a, const Columns& at) {
     const int64_t base = ((int64_t)(blockIdx.x - a.sum_groups) * (kSumThreads / 64) + (threadIdx.x >> 6)) * a.fill_rows;
     const int64_t row = base + (threadIdx.x & 63);
     bool absent = false;
@@ -374,20 +384,20 @@ template <typename S, int G> __device__ __forceinline__ void fill_rows(const Sum
         }
     }
     const uint64_t zeros = __ballot(absent);
-    if (count <= 0) return;
+    if (!at.on) return;
     for (int r = (threadIdx.x & 63) / G; r < a.fill_rows; r += 64 / G)
-        if (zeros >> r & 1) store_upto8(a.dw, (base + r) * a.ld_dw + col, a.dw_dtype, float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, count, a.stream);
+        if (zeros >> r & 1) store_upto8(a.dw, (base + r) * a.ld_dw + at.col, a.dw_dtype, float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, at.count, a.stream);
 }
 
 template <typename DT, typename S, int G>
 __global__ void __launch_bounds__(kSumThreads) embedding_sums_kernel(Sums<S> a) {
     using V = typename Eight8<S>::vec;
-    constexpr int U = 8, TEAMS = kSumThreads / G;
+    using R = typename Eight<DT>::vec;                      // (eight elements as they lie in memory: floats of them would take twice the registers)
+    constexpr int U = sizeof(DT) == 4 ? 4 : 8, TEAMS = kSumThreads / G;
     const int lane = threadIdx.x % G, team = threadIdx.x / G;
-    const int64_t col = ((int64_t)blockIdx.y * G + lane) * 8;
-    const int count = (int)min((int64_t)8, a.dim - col);
-    if ((int)blockIdx.x >= a.sum_groups) return fill_rows<S, G>(a, col, count);
-    __shared__ Entry s_e[TEAMS * kMostEach + 2];            // with the entry before, and that behind
+    const Columns at(((int64_t)blockIdx.y * G + lane) * 8, a.dim);
+    if ((int)blockIdx.x >= a.sum_groups) return fill_rows<S, G>(a, at);
+    extern __shared__ Entry s_e[];                          // [TEAMS * each + 2]: with the entry before, and that behind
     __shared__ S s_head[TEAMS][8][G];                       // what G threads have of an id that begins before theirs
     const uint32_t none = (uint32_t)a.rows;
     const int64_t from0 = (int64_t)blockIdx.x * TEAMS * a.each - 1;
@@ -397,25 +407,39 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sums_kernel(Sums<S> a) 
     // rows of dy of the entries `from` to `to` of s_e; between(key, sum) before each is added
     auto add = [&](int from, int to, auto between) {
         V sum = V{0, 0, 0, 0, 0, 0, 0, 0};
-        if (count > 0)
-            for (int i = from; i < to; i += U) {
-                Entry e[U];
-                float8_t v[U];
+        if (!at.on) return sum;
+        auto row = [&](const Entry& e) { return (const DT*)a.dy + (int64_t)e.at * a.ld_dy + at.col; };
+        if (a.dim < 8) {
+#pragma unroll 1
+            for (int i = from; i < to; ++i) {
+                const Entry e = s_e[i];
+                between(e.key, sum);
+                if (e.key != none)
 #pragma unroll
-                for (int u = 0; u < U; ++u) e[u] = i + u < to ? s_e[i + u] : Entry{none, 0};
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    v[u] = e[u].key != none ? load_upto8((const DT*)a.dy + (int64_t)e[u].at * a.ld_dy + col, count) : float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (i + u < to) between(e[u].key, sum);
-                    sum += __builtin_convertvector(v[u], V);
-                }
+                    for (int c = 0; c < 7; ++c)
+                        if (c < at.count) sum[c] += (S)(float)row(e)[c];
             }
+            return sum;
+        }
+#pragma unroll 1
+        for (int i = from; i < to; i += U) {
+            R v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const Entry e = i + u < to ? s_e[i + u] : Entry{none, 0};
+                v[u] = R{};
+                if (e.key != none) v[u] = reinterpret_cast<const typename Eight<DT>::Any*>(row(e))->v;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i + u < to) between(key_at(i + u), sum);
+                sum += __builtin_convertvector(__builtin_convertvector(v[u], float8_t), V);
+            }
+        }
         return sum;
     };
     auto leave = [&](uint32_t key, V sum) {
-        if (key != none && count > 0) store_upto8(a.dw, (int64_t)key * a.ld_dw + col, a.dw_dtype, scaled<S>(sum, a.scale), count, a.stream);
+        if (key != none && at.on) store_upto8(a.dw, (int64_t)key * a.ld_dw + at.col, a.dw_dtype, scaled<S>(sum, a.scale), at.count, a.stream);
     };
     int first = 1 + team * a.each;
     const int last = first + a.each;                        // (entries past the end have no id)
@@ -452,7 +476,7 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sums_kernel(Sums<S> a) 
         }
     };
     auto keep = [&](S* part, V sum) {
-        if (count > 0) *reinterpret_cast<V*>(part + col) = sum;
+        if (at.on) reinterpret_cast<typename AnyEight<S>::type*>(part + at.col)->v = sum;
     };
     if (begins && goes_on) {
         if (follow(rest, key1, team + 1)) keep(a.tail(blockIdx.x), rest);
@@ -470,14 +494,13 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sums_kernel(Sums<S> a) 
 constexpr int kFewParts = 16;
 template <typename S, int G>
 __global__ void __launch_bounds__(1024) embedding_join_kernel(Sums<S> a) {
-    using V = typename Eight8<S>::vec;
     typedef double D8 __attribute__((ext_vector_type(8)));
     constexpr int TEAMS = 1024 / G;
     __shared__ int s_parts[TEAMS];
     __shared__ double s_sum[TEAMS][8][G];
     const int lane = threadIdx.x % G, team = threadIdx.x / G;
-    const int64_t col = ((int64_t)blockIdx.y * G + lane) * 8, span = kSumThreads / G * a.each;
-    const int count = (int)min((int64_t)8, a.dim - col);
+    const Columns at(((int64_t)blockIdx.y * G + lane) * 8, a.dim);
+    const int64_t span = kSumThreads / G * a.each;
     const int group0 = blockIdx.x * TEAMS;
     auto key_at = [&](int64_t i) { return a.e[i].key; };
     // parts behind the tail of the group's last id; 0: it does not go on, or begins before
@@ -501,16 +524,16 @@ __global__ void __launch_bounds__(1024) embedding_join_kernel(Sums<S> a) {
         return (int)(lo - group);
     };
     auto add_heads = [&](D8& sum, int from, int to) {
-        if (count <= 0) return;
-#pragma unroll 8
-        for (int c = from; c < to; ++c) sum += __builtin_convertvector(*reinterpret_cast<const V*>(a.head(c) + col), D8);
+        if (!at.on) return;
+#pragma unroll 4
+        for (int c = from; c < to; ++c) sum += __builtin_convertvector(reinterpret_cast<const typename AnyEight<S>::type*>(a.head(c) + at.col)->v, D8);
     };
     auto leave = [&](int group, D8 sum) {
-        if (count > 0) store_upto8(a.dw, (int64_t)key_at((group + 1) * span) * a.ld_dw + col, a.dw_dtype, __builtin_convertvector(sum * (double)a.scale, float8_t), count);
+        if (at.on) store_upto8(a.dw, (int64_t)key_at((group + 1) * span) * a.ld_dw + at.col, a.dw_dtype, __builtin_convertvector(sum * (double)a.scale, float8_t), at.count);
     };
     auto tail_of = [&](int group) {
         D8 sum = D8{0, 0, 0, 0, 0, 0, 0, 0};
-        if (count > 0) sum = __builtin_convertvector(*reinterpret_cast<const V*>(a.tail(group) + col), D8);
+        if (at.on) sum = __builtin_convertvector(reinterpret_cast<const typename AnyEight<S>::type*>(a.tail(group) + at.col)->v, D8);
         return sum;
     };
     const int group = group0 + team, parts = group < a.sum_groups ? parts_of(group) : 0;
@@ -520,7 +543,7 @@ __global__ void __launch_bounds__(1024) embedding_join_kernel(Sums<S> a) {
         add_heads(sum, group + 1, group + 1 + parts);
         leave(group, sum);
     }
-    __syncthreads();
+    if (!__syncthreads_or(parts > kFewParts)) return;
     for (int t = 0; t < TEAMS; ++t) {
         const int n = s_parts[t];                           // (the same for all threads)
         if (n <= kFewParts) continue;
@@ -578,7 +601,7 @@ template <typename DT, typename S, int G> int launch_sums(Sums<S> a, hipStream_t
     // rows to a wavefront: 64, or fewer for enough of them
     a.fill_rows = a.rows * slices >= 64 * 4096 ? 64 : 16;
     const int64_t fill = ceil_div(a.rows, (int64_t)a.fill_rows * (kSumThreads / 64));
-    embedding_sums_kernel<DT, S, G><<<dim3((unsigned)(a.sum_groups + fill), (unsigned)slices), kSumThreads, 0, st>>>(a);
+    embedding_sums_kernel<DT, S, G><<<dim3((unsigned)(a.sum_groups + fill), (unsigned)slices), kSumThreads, (kSumThreads / G * a.each + 2) * sizeof(Entry), st>>>(a);
     LF_HIP(hipGetLastError());
     if (a.sum_groups > 1) {
         embedding_join_kernel<S, G><<<dim3((unsigned)ceil_div(a.sum_groups, 1024 / G), (unsigned)slices), 1024, 0, st>>>(a);
@@ -673,7 +696,7 @@ int lf_embedding_grad(const lf_embedding_grad_args* h_args, void* d_work, size_t
                 s.last = pass == p.passes - 1;
                 sort_count_kernel<<<s.groups, kSortThreads, 0, st>>>(s);
                 LF_HIP(hipGetLastError());
-                const bool few = s.groups <= kFewGroups;
+                const bool few = (s.groups << p.bits) <= kFewCounts;
                 if (!few) {
                     sort_offsets_kernel<<<(unsigned)ceil_div(1 << p.bits, 16), 1024, 0, st>>>(s);
                     LF_HIP(hipGetLastError());
