@@ -10,7 +10,7 @@
 // Two sums over the row one after the other: that of h, then those of d = h - mu and d^2 (and, in the gradient, of g and g d).  The second
 // look at the mean takes off what the rounding of the first has left, so that rows far from zero keep their digits: mu is off by less than
 // a rounding of the largest |h - mu|, not of |mu|.
-// Rows whose sums overflow are summed again times 2^-100, those whose squares vanish after the subtraction times 2^100.
+// Rows whose sums overflow are taken times 2^-100 and summed again, those whose squares vanish after the subtraction times 2^100.
 #include "lf_rows.h"
 
 namespace {
@@ -59,12 +59,14 @@ struct LayerArgs {
     float eps, inv_dim;
 };
 
-// A row's statistics: t = ((h up - mean) late - less) inv.  Powers of two: up for sums that overflow, late for squares that vanish.
+// A row's statistics: t = (h - mean - less) inv.  Where sums overflow or squares vanish the row is changed first, h -> (h - off) by, and what is said here is of
+// the row as it is then; by: the power of two.
 struct Centre {
-    float mean, less, inv, up, late;
-    // first: () -> sum of h up.  second: (d, dd) <- sums of (h up - mean) late and of its squares
-    template <typename FIRST, typename SECOND> __device__ __forceinline__ void find(float eps, float inv_dim, FIRST first, SECOND second) {
-        up = late = 1.f;
+    float mean, less, inv, by;
+    // first: () -> sum of h.  second: (d, dd) <- sums of h - mean and of its squares.  change(off, by): changes the row
+    template <typename FIRST, typename SECOND, typename CHANGE>
+    __device__ __forceinline__ void find(float eps, float inv_dim, FIRST first, SECOND second, CHANGE change) {
+        by = 1.f;
         auto variance = [&] {
             float d, dd;
             second(d, dd);
@@ -76,11 +78,14 @@ struct Centre {
         float var = variance() + eps;
         if (__builtin_expect(!(var >= kTiny && var < __builtin_inff()), 0)) {      // (the same for all threads of the row)
             if (var < kTiny) {
-                late = 1.f / kTiny;
-                var = variance() + eps * late * late;
+                by = 1.f / kTiny;
+                change(mean, by);
+                mean = 0.f;
+                var = variance() + eps * by * by;
             } else {
                 // (the mean once more: here eps, far below what is left of its rounding, would not hide it)
-                up = kTiny;
+                by = kTiny;
+                change(0.f, by);
                 mean = first() * inv_dim;
                 variance();
                 mean += less;
@@ -90,7 +95,7 @@ struct Centre {
         }
         inv = 1.f / sqrtf(var);
     }
-    __device__ __forceinline__ float8_t of(float8_t h) const { return ((h * up - mean) * late - less) * inv; }
+    template <typename V> __device__ __forceinline__ V of(V h) const { return (h - mean - less) * inv; }
 };
 
 template <typename XT, typename RT, int G, int C>
@@ -122,34 +127,22 @@ layer_norm_kernel(LayerArgs a) {
 #pragma unroll
             for (int c = 0; c < C; ++c) h[c] += v[c];
         }
-        Centre m;
+        const bool whole = dim % 8 == 0;                                 // (then no element needs to be looked at by itself)
         auto each_of = [&](auto f) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const Piece p = piece_of((c * G + lane) * 8, dim);
+                if (whole) {
+                    if (p.first == 0)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (counts(p, i, dim)) f(h[c][i]);
+                        for (int i = 0; i < 8; ++i) f(h[c][i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (counts(p, i, dim)) f(h[c][i]);
+                }
             }
         };
-        m.find(a.eps, a.inv_dim,
-               [&] {
-                   float v[1] = {0.f};
-                   each_of([&](float x) { v[0] += x * m.up; });
-                   row_sums<G>(v, s_red);
-                   return v[0];
-               },
-               [&](float& d, float& dd) {
-                   float v[2] = {0.f, 0.f};
-                   each_of([&](float x) {
-                       const float t = (x * m.up - m.mean) * m.late;
-                       v[0] += t;
-                       v[1] = fmaf(t, t, v[1]);
-                   });
-                   row_sums<G>(v, s_red);
-                   d = v[0];
-                   dd = v[1];
-               });
         if (a.res) {
             RT* hr = (RT*)a.h + row * a.ldh;
 #pragma unroll
@@ -158,6 +151,29 @@ layer_norm_kernel(LayerArgs a) {
                 if (p.first < 8) store_piece(hr, p, dim, h[c], a.stream);
             }
         }
+        Centre m;
+        m.find(a.eps, a.inv_dim,
+               [&] {
+                   float v[1] = {0.f};
+                   each_of([&](float x) { v[0] += x; });
+                   row_sums<G>(v, s_red);
+                   return v[0];
+               },
+               [&](float& d, float& dd) {
+                   float v[2] = {0.f, 0.f};
+                   each_of([&](float x) {
+                       const float t = x - m.mean;
+                       v[0] += t;
+                       v[1] = fmaf(t, t, v[1]);
+                   });
+                   row_sums<G>(v, s_red);
+                   d = v[0];
+                   dd = v[1];
+               },
+               [&](float off, float by) {
+#pragma unroll
+                   for (int c = 0; c < C; ++c) h[c] = (h[c] - off) * by;
+               });
 #pragma unroll
         for (int c = 0; c < C; ++c) h[c] = m.of(h[c]) * w[c] + b[c];
         if (!q8) {
@@ -201,13 +217,14 @@ layer_norm_long_kernel(LayerArgs a) {
                 f(col, n, sum8(col, n));
             }
         };
+        float off = 0.f, by = 1.f;                                       // (read again, the row is changed again)
         Centre m;
         m.find(a.eps, a.inv_dim,
                [&] {
                    float v[1] = {0.f};
-                   pieces([&](int, int, float8_t h) {                    // (zeros behind the end)
+                   pieces([&](int, int, float8_t h) {                    // (zeros behind the end: only `second` changes by an offset)
 #pragma unroll
-                       for (int i = 0; i < 8; ++i) v[0] += h[i] * m.up;
+                       for (int i = 0; i < 8; ++i) v[0] += h[i] * by;
                    });
                    row_sums<1024>(v, s_red);
                    return v[0];
@@ -217,7 +234,7 @@ layer_norm_long_kernel(LayerArgs a) {
                    pieces([&](int, int n, float8_t h) {
 #pragma unroll
                        for (int i = 0; i < 8; ++i) {
-                           const float t = i < n ? (h[i] * m.up - m.mean) * m.late : 0.f;
+                           const float t = i < n ? (h[i] - off) * by - m.mean : 0.f;
                            v[0] += t;
                            v[1] = fmaf(t, t, v[1]);
                        }
@@ -225,9 +242,13 @@ layer_norm_long_kernel(LayerArgs a) {
                    row_sums<1024>(v, s_red);
                    d = v[0];
                    dd = v[1];
+               },
+               [&](float o, float b) {
+                   off = o;
+                   by = b;
                });
         auto out = [&](int col, int n, float8_t h) {
-            float8_t y = m.of(h);
+            float8_t y = m.of((h - off) * by);
             if (a.w) y *= load_upto8(a.w, col, a.w_dtype, n);
             if (a.b) y += load_upto8(a.b, col, a.b_dtype, n);
             return y;
@@ -316,28 +337,35 @@ layer_norm_grad_kernel(LayerGradArgs a) {
             if (AHEAD) dh[c] = __builtin_convertvector(raw_dh[c], float8_t);
         }
         if (AHEAD && row + step < a.rows) load(row + step);
+        const bool whole = dim % 8 == 0;
         auto each_of = [&](auto f) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const Piece p = piece_of((c * G + lane) * 8, dim);
+                if (whole) {
+                    if (p.first == 0)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (counts(p, i, dim)) f(h[c][i], dy[c][i] * w[c][i]);
+                        for (int i = 0; i < 8; ++i) f(h[c][i], dy[c][i] * w[c][i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (counts(p, i, dim)) f(h[c][i], dy[c][i] * w[c][i]);
+                }
             }
         };
         Centre m;
-        float g_sum, g_dot;                                              // of g and g (h up - mean) late
+        float g_sum, g_dot;                                              // of g and g (h - mean)
         m.find(a.eps, a.inv_dim,
                [&] {
                    float v[1] = {0.f};
-                   each_of([&](float x, float) { v[0] += x * m.up; });
+                   each_of([&](float x, float) { v[0] += x; });
                    row_sums<G>(v, s_red);
                    return v[0];
                },
                [&](float& d, float& dd) {
                    float v[4] = {0.f, 0.f, 0.f, 0.f};
                    each_of([&](float x, float g) {
-                       const float t = (x * m.up - m.mean) * m.late;
+                       const float t = x - m.mean;
                        v[0] += t;
                        v[1] = fmaf(t, t, v[1]);
                        v[2] += g;
@@ -348,8 +376,12 @@ layer_norm_grad_kernel(LayerGradArgs a) {
                    dd = v[1];
                    g_sum = v[2];
                    g_dot = v[3];
+               },
+               [&](float off, float by) {
+#pragma unroll
+                   for (int c = 0; c < C; ++c) h[c] = (h[c] - off) * by;
                });
-        const float g_mean = g_sum * a.inv_dim, along = fmaf(-m.less, g_sum, g_dot) * m.inv * a.inv_dim, s = m.inv * m.late * m.up;
+        const float g_mean = g_sum * a.inv_dim, along = fmaf(-m.less, g_sum, g_dot) * m.inv * a.inv_dim, s = m.inv * m.by;
         HT* dx = (HT*)a.dx + row * a.ldx;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -409,6 +441,7 @@ layer_norm_grad_long_kernel(LayerGradArgs a) {
             }
         };
         auto weighted = [&](float8_t dy, int col, int n) { return a.w ? dy * load_upto8(a.w, col, a.w_dtype, n) : dy; };
+        float off = 0.f, by = 1.f;
         Centre m;
         float g_sum, g_dot;
         m.find(a.eps, a.inv_dim,
@@ -416,7 +449,7 @@ layer_norm_grad_long_kernel(LayerGradArgs a) {
                    float v[1] = {0.f};
                    pieces([&](int, int, float8_t h, float8_t) {
 #pragma unroll
-                       for (int i = 0; i < 8; ++i) v[0] += h[i] * m.up;
+                       for (int i = 0; i < 8; ++i) v[0] += h[i] * by;
                    });
                    row_sums<1024>(v, s_red);
                    return v[0];
@@ -428,7 +461,7 @@ layer_norm_grad_long_kernel(LayerGradArgs a) {
 #pragma unroll
                        for (int i = 0; i < 8; ++i) {
                            if (i >= n) continue;
-                           const float t = (h[i] * m.up - m.mean) * m.late;
+                           const float t = (h[i] - off) * by - m.mean;
                            v[0] += t;
                            v[1] = fmaf(t, t, v[1]);
                            v[2] += g[i];
@@ -440,10 +473,14 @@ layer_norm_grad_long_kernel(LayerGradArgs a) {
                    dd = v[1];
                    g_sum = v[2];
                    g_dot = v[3];
+               },
+               [&](float o, float b) {
+                   off = o;
+                   by = b;
                });
-        const float g_mean = g_sum * a.inv_dim, along = fmaf(-m.less, g_sum, g_dot) * m.inv * a.inv_dim, s = m.inv * m.late * m.up;
+        const float g_mean = g_sum * a.inv_dim, along = fmaf(-m.less, g_sum, g_dot) * m.inv * a.inv_dim, s = m.inv * m.by;
         pieces([&](int col, int n, float8_t h, float8_t dy) {
-            const float8_t t = m.of(h);
+            const float8_t t = m.of((h - off) * by);
             float8_t d = (weighted(dy, col, n) - g_mean - t * along) * s;
             if (a.dh) d += load_upto8((const HT*)a.dh + row * a.ldd + col, n);
             store_upto8((HT*)a.dx + row * a.ldx + col, d, n);
