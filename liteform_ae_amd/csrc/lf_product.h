@@ -421,7 +421,7 @@ template <int TM, int TN, bool GATED = false> struct Vectors {
 };
 // (m0, n0): of the tile that `vec` is of
 template <int FM, int FN, int PR, typename Acc, typename Vec>
-__device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN], uint4_t* lds, const Vec& vec, int64_t m0, int64_t n0, int row0, int col0) {
+__device__ __forceinline__ void leave(const Product& g, int split, const Acc (&acc)[FM][FN], uint4_t* lds, const Vec& vec, int64_t m0, int64_t n0, int row0, int col0) {
     constexpr int WC = 16 * FN, LANES = WC / 8, AT_ONCE = 64 / LANES, U = PR / AT_ONCE, PHASES = FM * 16 / PR;
     constexpr bool INT = std::is_same_v<Acc, int4v>;
     static_assert(FM * 16 % PR == 0 && PR % AT_ONCE == 0 && PHASES <= 4, "");
@@ -471,7 +471,7 @@ __device__ __forceinline__ void leave(const Product& g, const Acc (&acc)[FM][FN]
         if (__builtin_expect(g.part != nullptr, 0)) {
 #pragma unroll 2
             for (int row = mine; row < PR; row += AT_ONCE)
-                if (m + FIRST + row < g.m && count) store_upto8((float*)g.part + ((int64_t)blockIdx.y * g.m + m + FIRST + row) * g.n + n, sums(row), count);
+                if (m + FIRST + row < g.m && count) store_upto8((float*)g.part + ((int64_t)split * g.m + m + FIRST + row) * g.n + n, sums(row), count);
         } else if (__builtin_expect(whole, 1)) {
             // What follows the sums and comes before the residual, in a lane's own places of LDS: a loop, since its code is long and would be read
             // from memory for every tile if it stood there sixteen times (gelu: 44 us of the 285 of an e4m3 product of 16k x 4k x 4k, 25 as a loop)
@@ -564,7 +564,7 @@ template <int WC> __device__ __forceinline__ int turned_gated(int row, int c) {
     return row * (4 * LANES) + ((kind * LANES + piece) ^ (r % ROWS * LANES + r / ROWS % LANES));
 }
 template <int FM, int FN, int PR, typename Acc, typename Vec>
-__device__ __forceinline__ void leave_gated(const Product& g, const Acc (&acc)[FM][FN], uint4_t* lds, const Vec& vec, int64_t m0, int64_t n0, int row0, int col0) {
+__device__ __forceinline__ void leave_gated(const Product& g, int split, const Acc (&acc)[FM][FN], uint4_t* lds, const Vec& vec, int64_t m0, int64_t n0, int row0, int col0) {
     constexpr int WC = 16 * FN, LANES = WC / 16, AT_ONCE = 64 / LANES, PHASES = FM * 16 / PR;
     constexpr bool INT = std::is_same_v<Acc, int4v>;
     static_assert(FM * 16 % PR == 0 && PR % AT_ONCE == 0, "");
@@ -615,7 +615,7 @@ __device__ __forceinline__ void leave_gated(const Product& g, const Acc (&acc)[F
                 sums(row, v);
                 if (m + FIRST + row < g.m && count)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) store_upto8((float*)g.part + ((int64_t)blockIdx.y * g.m + m + FIRST + row) * 2 * g.n + h * g.n + n, v[h], count);
+                    for (int h = 0; h < 2; ++h) store_upto8((float*)g.part + ((int64_t)split * g.m + m + FIRST + row) * 2 * g.n + h * g.n + n, v[h], count);
             }
         } else if (__builtin_expect(whole, 1)) {
             // (a loop, for the instruction cache; two rows at a time, whose activations fill one another's waits)
@@ -684,16 +684,32 @@ __device__ __forceinline__ void leave_gated(const Product& g, const Acc (&acc)[F
     if constexpr (PHASES > 3) phase(std::integral_constant<int, 3>{});
 }
 
-// The tile of a workgroup.  Workgroups go to the eight XCDs in turn: each XCD gets a run of neighbouring tiles, eight rows of
-// tiles deep, so that what its L2 holds of both operands is used by its 32 CUs at once.
-__device__ __forceinline__ void tile_of(const Product& g, unsigned id, int& tm, int& tn) {
-    const unsigned n = (unsigned)g.tiles_m * g.tiles_n, xcd = id % 8, each = n / 8, more = n % 8;
-    unsigned t = xcd * each + min(xcd, more) + id / 8;
+// The tile of a workgroup, and its part of k.  Workgroups go to the eight XCDs in turn: each XCD gets a run of neighbouring tiles, eight rows of
+// tiles deep, so that what its L2 holds of both operands is used by its 32 CUs at once.  From eight parts of k on each XCD takes all tiles of every eighth
+// part instead: an operand's rows are then fetched by one L2 and not by as many as there are tiles across them (gradients of bf16 170k x 256 by 256 107 us,
+// of 100k x 1000 by 64 127; with the parts spread over all XCDs 125 and 145.  float32, which cuts its operands meanwhile: no difference).
+struct Place { int tm, tn, split; };
+__device__ __forceinline__ Place place_of(const Product& g) {
+    const unsigned n = (unsigned)g.tiles_m * g.tiles_n;
+    unsigned t;
+    Place p;
+    if (g.splits < 8) {
+        const unsigned id = blockIdx.x, xcd = id % 8, each = n / 8, more = n % 8;
+        t = xcd * each + min(xcd, more) + id / 8;
+        p.split = blockIdx.y;
+    } else {
+        const unsigned id = blockIdx.y * n + blockIdx.x, even = (unsigned)g.splits / 8 * 8, turn = id / 8;
+        const bool rest = id >= even * n;
+        const unsigned at = rest ? id - even * n : turn;
+        p.split = (int)(rest ? even + at / n : at / n * 8 + id % 8);
+        t = at % n;
+    }
     constexpr unsigned kDeep = 8;
     const unsigned band = t / (kDeep * g.tiles_n), first = band * kDeep, deep = min(kDeep, (unsigned)g.tiles_m - first);
     t -= band * kDeep * g.tiles_n;
-    tm = (int)(first + t % deep);
-    tn = (int)(t / deep);
+    p.tm = (int)(first + t % deep);
+    p.tn = (int)(t / deep);
+    return p;
 }
 
 template <typename T, bool PX, bool QX, int TM, int TN, int WM, int WN, bool GATED>
@@ -711,10 +727,10 @@ __device__ __forceinline__ void product_tile(const Product& g) {
     __shared__ Vectors<TM, TN, GATED> s_vec;
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
-    int tm, tn;
-    tile_of(g, blockIdx.x, tm, tn);
+    const Place at_tile = place_of(g);
+    const int tm = at_tile.tm, tn = at_tile.tn;
     const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * (GATED ? TN / 2 : TN);
-    const int64_t k_first = (int64_t)blockIdx.y * g.k_split, k_last = min(g.k, k_first + g.k_split);
+    const int64_t k_first = (int64_t)at_tile.split * g.k_split, k_last = min(g.k, k_first + g.k_split);
 
     Acc acc[FM][FN];
 #pragma unroll
@@ -827,8 +843,8 @@ __device__ __forceinline__ void product_tile(const Product& g) {
     uint4_t* mine = s_all + wave * SLOTS;
     const int row0 = wm * (TM / WM), col0 = wn * (TN / WN);
     if constexpr (PL == 3) repair<PX, QX, GATED>(g, acc, m0 + row0, n0 + (GATED ? col0 / 2 : col0), k_first, k_last);
-    if constexpr (GATED) leave_gated<FM, FN, PR>(g, acc, mine, s_vec, m0, n0, row0, col0);
-    else leave<FM, FN, PR>(g, acc, mine, s_vec, m0, n0, row0, col0);
+    if constexpr (GATED) leave_gated<FM, FN, PR>(g, at_tile.split, acc, mine, s_vec, m0, n0, row0, col0);
+    else leave<FM, FN, PR>(g, at_tile.split, acc, mine, s_vec, m0, n0, row0, col0);
 }
 template <typename T, bool PX, bool QX, int TM, int TN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, TM == 128 ? 2 : 4) product_kernel(Product g) { product_tile<T, PX, QX, TM, TN, WM, WN, false>(g); }
@@ -976,10 +992,10 @@ __device__ __forceinline__ void wide_tile(const Product& g) {
     // (arrays of their own: what is read from one must not wait for what is on its way into another)
     __shared__ uint4_t s_p0[Direct<T, PX, 256>::kSlots], s_q0[Direct<T, QX, 256>::kSlots], s_p1[Direct<T, PX, 256>::kSlots], s_q1[Direct<T, QX, 256>::kSlots];
     __shared__ Vectors<256, 256, GATED> s_vec;
-    int tm, tn;
-    tile_of(g, blockIdx.x, tm, tn);
+    const Place at_tile = place_of(g);
+    const int tm = at_tile.tm, tn = at_tile.tn;
     const int64_t m0 = (int64_t)tm * 256, n0 = (int64_t)tn * (GATED ? 128 : 256);
-    const int64_t k_first = (int64_t)blockIdx.y * g.k_split, k_last = min(g.k, k_first + g.k_split);
+    const int64_t k_first = (int64_t)at_tile.split * g.k_split, k_last = min(g.k, k_first + g.k_split);
     using DP = Direct<T, PX, 256>;
     using DQ = Direct<T, QX, 256>;
     DP P(g.p, g.ld_p, m0, g.m, k_first);
@@ -1080,8 +1096,8 @@ __device__ __forceinline__ void wide_tile(const Product& g) {
     for (int i = 0; i < 8; ++i) settle(acc[i]);
     __syncthreads();
     uint4_t* mine = P.wave == 0 ? s_p0 : P.wave == 1 ? s_q0 : P.wave == 2 ? s_p1 : s_q1;
-    if constexpr (GATED) leave_gated<8, 8, 64>(g, acc, mine, s_vec, m0, n0, row_p, row_q);
-    else leave<8, 8, 64>(g, acc, mine, s_vec, m0, n0, row_p, row_q);
+    if constexpr (GATED) leave_gated<8, 8, 64>(g, at_tile.split, acc, mine, s_vec, m0, n0, row_p, row_q);
+    else leave<8, 8, 64>(g, at_tile.split, acc, mine, s_vec, m0, n0, row_p, row_q);
 }
 template <typename T, bool PX, bool QX> __global__ void __launch_bounds__(256) wide_kernel(Product g) { wide_tile<T, PX, QX, false>(g); }
 template <typename T> __global__ void __launch_bounds__(256) gated_wide_kernel(Product g) { wide_tile<T, false, false, true>(g); }
@@ -1100,10 +1116,10 @@ __device__ __forceinline__ void direct_tile(const Product& g) {
     constexpr int KS = 128 / sizeof(T), FR = TILE / 32, SB = DP::kSlots + DQ::kSlots;
     __shared__ uint4_t s[BUFFERS * SB];
     __shared__ Vectors<TILE, TILE, GATED> s_vec;
-    int tm, tn;
-    tile_of(g, blockIdx.x, tm, tn);
+    const Place at_tile = place_of(g);
+    const int tm = at_tile.tm, tn = at_tile.tn;
     const int64_t m0 = (int64_t)tm * TILE, n0 = (int64_t)tn * (GATED ? TILE / 2 : TILE);
-    const int64_t k_first = (int64_t)blockIdx.y * g.k_split, k_last = min(g.k, k_first + g.k_split);
+    const int64_t k_first = (int64_t)at_tile.split * g.k_split, k_last = min(g.k, k_first + g.k_split);
     DP P(g.p, g.ld_p, m0, g.m, k_first);
     DQ Q(g.q, g.ld_q, n0, g.n, k_first, GATED);
     const int row_p = (P.wave & 1) * (TILE / 2), row_q = (P.wave >> 1) * (TILE / 2);
@@ -1202,8 +1218,8 @@ __device__ __forceinline__ void direct_tile(const Product& g) {
     }
     arrived();
     constexpr int PR = TILE / 2 < 32 ? TILE / 2 : 32;
-    if constexpr (GATED) leave_gated<FR, FR, PR>(g, acc, s + P.wave * (SB / 2), s_vec, m0, n0, row_p, row_q);
-    else leave<FR, FR, PR>(g, acc, s + P.wave * (SB / 2), s_vec, m0, n0, row_p, row_q);
+    if constexpr (GATED) leave_gated<FR, FR, PR>(g, at_tile.split, acc, s + P.wave * (SB / 2), s_vec, m0, n0, row_p, row_q);
+    else leave<FR, FR, PR>(g, at_tile.split, acc, s + P.wave * (SB / 2), s_vec, m0, n0, row_p, row_q);
 }
 template <typename T, bool PX, bool QX, int TILE, int BUFFERS>
 __global__ void __launch_bounds__(256, BUFFERS == 4 ? 1 : TILE == 128 ? 2 : 4) direct_kernel(Product g) { direct_tile<T, PX, QX, TILE, BUFFERS, false>(g); }
