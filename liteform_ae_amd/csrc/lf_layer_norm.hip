@@ -143,20 +143,23 @@ layer_norm_kernel(LayerArgs a) {
                 }
             }
         };
-        if (a.res) {
-            RT* hr = (RT*)a.h + row * a.ldh;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const Piece p = piece_of((c * G + lane) * 8, dim);
-                if (p.first < 8) store_piece(hr, p, dim, h[c], a.stream);
-            }
-        }
+        bool left = !a.res;
         Centre m;
         m.find(a.eps, a.inv_dim,
                [&] {
                    float v[1] = {0.f};
                    each_of([&](float x) { v[0] += x; });
                    row_sums<G>(v, s_red);
+                   // (behind the sums' barriers: h may be the residual itself, and the end of a row reaches back into what another wavefront reads)
+                   if (!left) {
+                       RT* hr = (RT*)a.h + row * a.ldh;
+#pragma unroll
+                       for (int c = 0; c < C; ++c) {
+                           const Piece p = piece_of((c * G + lane) * 8, dim);
+                           if (p.first < 8) store_piece(hr, p, dim, h[c], a.stream);
+                       }
+                       left = true;
+                   }
                    return v[0];
                },
                [&](float& d, float& dd) {

@@ -155,6 +155,23 @@ def test_layer_norm_of_no_rows(lo):
     assert dx.shape == (0, 64) and bool((dw == 0).all()) and bool((db == 0).all()) and db.dtype is BF16
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layer_norm_where_h_is_the_residual(lo, dtype):
+    """The library may write h where the residual was; rows whose end reaches back into the piece before, which another wavefront may hold."""
+    import ctypes as C
+    from liteform_ae_amd import _lib
+    lib, code = _lib.load(), {F32: _lib.LF_DTYPE_F32, BF16: _lib.LF_DTYPE_BF16}[dtype]
+    g = gen(10)
+    for dim in (5, 63, 513, 1025, 1540, 2049, 2050, 4095, 4097, 6150, 8191, 10_001, 16_383, 20_001):
+        x, res = normal((700, dim), dtype, g), normal((700, dim), dtype, g)
+        y, h = lo.layer_norm(x, residual=res, eps=1e-5)
+        y2 = torch.empty_like(y)
+        a = _lib.LayerNormArgs(x=x.data_ptr(), residual=res.data_ptr(), y=y2.data_ptr(), h=res.data_ptr(), ld_x=dim, ld_residual=dim, ld_y=dim, ld_h=dim, rows=700, dim=dim,
+                               x_dtype=code, residual_dtype=code, y_dtype=code, eps=1e-5)
+        _lib.check(lib.lf_layer_norm(C.byref(a), torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(res, h) and torch.equal(y2, y), dim
+
+
 def check_layer_grad(lo, dy, h, w, eps, dh, what, bias=F32, dy4=False):
     if dy4:
         dy = dy[:4]
@@ -462,7 +479,7 @@ def check_embedding_grad(lo, ids, rows, dim, dy_type, out, scale, g, pad=0, offs
 
 #       ids, rows: none, one; one and more digits of the sort; one tile of it, some, and more workgroups than one
 GRADS = [(0, 10), (1, 1), (1, 70_000), (5, 3), (63, 1000), (64, 2047), (65, 2048), (700, 5), (1000, 4000), (4095, 100), (4096, 3_000_000), (4097, 2_000), (8192, 70_000), (8193, 70_000),
-         (20_000, 50_000), (100_001, 30_000), (300_000, 1), (300_000, 9)]
+         (20_000, 50_000), (100_001, 30_000), (300_000, 1), (300_000, 9), (9000, 5_000_000), (2_500_001, 1_000_000)]
 
 
 @pytest.mark.parametrize("dy_type,out", [(F32, F32), (BF16, BF16), (F16, F16), (BF16, F32), (F32, BF16)])
