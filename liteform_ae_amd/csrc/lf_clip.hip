@@ -16,7 +16,8 @@ using namespace lf;
 
 constexpr int kTensors = 64;                                // to a launch
 constexpr int64_t kChunk = 16384;                           // elements to a workgroup
-constexpr int kMostParts = 2048;                            // partial sums of a call
+constexpr int kMostParts = 2048;                            // partial sums of a launch
+constexpr int64_t kMostElements = 1ll << 40;                // of all tensors: chunks are counted in 32 bits
 
 struct Tensor { const void* src; void* dst; int64_t rows, cols, ld_src, ld_dst; };
 struct List {
@@ -157,7 +158,7 @@ bool overlapping(const lf_tensor_desc* t, int32_t n) {
 
 struct Call { std::vector<List> lists; };
 void add(Call& c, const lf_tensor_desc& d, int64_t chunks) {
-    if (c.lists.empty() || c.lists.back().n == kTensors || c.lists.back().first[c.lists.back().n] + chunks >= (1ll << 31)) {
+    if (c.lists.empty() || c.lists.back().n == kTensors) {
         c.lists.emplace_back();
         c.lists.back().n = 0;
         c.lists.back().first[0] = 0;
@@ -172,18 +173,21 @@ void add(Call& c, const lf_tensor_desc& d, int64_t chunks) {
 
 int clip(const lf_tensor_desc* t, int32_t n, float most, float eps, float* d_norm, void* d_work, size_t work_bytes, hipStream_t st) {
     bool out = false;
+    int64_t elements = 0;
     for (int32_t i = 0; i < n; ++i) {
         const lf_tensor_desc& d = t[i];
         LF_REQUIRE(is_float_dtype((int32_t)d.dtype), LF_ERR_UNSUPPORTED, "tensor %d: gradients are of float32, bfloat16 or float16", i);
         LF_REQUIRE(d.rows >= 0 && d.cols >= 0, LF_ERR_INVALID, "tensor %d: %lld x %lld", i, (long long)d.rows, (long long)d.cols);
         if (!d.rows || !d.cols) continue;
-        LF_REQUIRE(d.rows < (1ll << 40) && d.cols < (1ll << 40) && d.rows * ((d.cols + 7) / 8) < (1ll << 41), LF_ERR_UNSUPPORTED, "tensor %d: %lld x %lld", i, (long long)d.rows,
-                   (long long)d.cols);
+        LF_REQUIRE(d.cols <= kMostElements && d.rows <= kMostElements / (ceil_div(d.cols, 8) * 8) && d.ld_src <= kMostElements && d.ld_dst <= kMostElements, LF_ERR_UNSUPPORTED,
+                   "tensor %d: %lld x %lld", i, (long long)d.rows, (long long)d.cols);
+        elements += d.rows * d.cols;
         LF_REQUIRE(d.d_src, LF_ERR_INVALID, "tensor %d: null pointer", i);
         LF_REQUIRE((uintptr_t)d.d_src % dtype_bytes((int32_t)d.dtype) == 0 && (uintptr_t)d.d_dst % dtype_bytes((int32_t)d.dtype) == 0, LF_ERR_INVALID, "tensor %d: not aligned to its elements", i);
         LF_REQUIRE(d.rows <= 1 || (d.ld_src >= d.cols && (!d.d_dst || d.ld_dst >= d.cols)), LF_ERR_INVALID, "tensor %d: rows of %lld elements overlap", i, (long long)d.cols);
         LF_REQUIRE(!out || d.d_dst, LF_ERR_INVALID, "outputs are for all tensors or for none");
         out = d.d_dst != nullptr;
+        LF_REQUIRE(elements <= kMostElements, LF_ERR_UNSUPPORTED, "more elements than any GPU holds");
     }
     const size_t need = lf_clip_work_bytes(n);
     LF_REQUIRE(need == 0 || (d_work && (uintptr_t)d_work % 16 == 0), LF_ERR_INVALID, "null or unaligned workspace");
@@ -225,7 +229,7 @@ int clip(const lf_tensor_desc* t, int32_t n, float most, float eps, float* d_nor
 
 extern "C" {
 
-size_t lf_clip_work_bytes(int32_t n) { return n <= 0 ? 0 : (size_t)n * kMostParts * sizeof(double); }
+size_t lf_clip_work_bytes(int32_t n) { return n <= 0 ? 0 : (size_t)ceil_div(n, kTensors) * kMostParts * sizeof(double); }
 
 int lf_clip_gradients(const lf_tensor_desc* h_tensors, int32_t n, float most, float eps, float* d_norm, void* d_work, size_t work_bytes, lf_stream_t stream) {
     LF_REQUIRE(n >= 0 && (h_tensors || n == 0) && d_norm, LF_ERR_INVALID, "null argument");

@@ -87,6 +87,7 @@ def test_training_step_with_clipped_gradients(gl):
         loss64.backward()
         norm64 = math.sqrt(sum(float(p.grad.square().sum()) for each in ps.values() for p in each))
         factor, rate = min(1.0, most / (norm64 + 1e-6)), 0.5
+        loss64 = loss64.detach()
         loss, norm = gl.train_step([layers[0], layers[1], layers[0]], ids, h, target, rate, max_norm=most, embedding=embedding)
         assert abs(float(loss) - float(loss64)) <= 1e-5 * float(loss64) and abs(float(norm) - norm64) <= 2e-5 * norm64
         for layer, each in ps.items():

@@ -135,6 +135,9 @@ def test_clip_refusals():
     for bad in (dict(src=None), dict(src=AT + 2), dict(dst=AT + 1), dict(rows=-1), dict(cols=-1), dict(rows=3, ld_src=99, ld_dst=100), dict(rows=3, ld_src=100, ld_dst=99)):
         refused(clip(lib, descs(bad)))
     refused(clip(lib, descs(dict(dtype=E4M3))), _lib.LF_ERR_UNSUPPORTED)
+    for huge in (dict(cols=1 << 62), dict(rows=1 << 62, cols=1), dict(rows=1 << 40, cols=1 << 40), dict(rows=2, ld_src=1 << 62, ld_dst=100), dict(rows=2, ld_src=100, ld_dst=1 << 62)):
+        refused(clip(lib, descs(huge)), _lib.LF_ERR_UNSUPPORTED)
+    refused(clip(lib, descs(*[dict(cols=1 << 39, src=AT, dst=AT + (i << 42)) for i in range(3)])), _lib.LF_ERR_UNSUPPORTED)
     refused(clip(lib, descs({}, dict(src=AT + 4096, dst=None))), text="for all tensors or for none")
     assert lib.lf_clip_work_bytes(0) == 0 and lib.lf_clip_work_bytes(-3) == 0 and lib.lf_clip_work_bytes(100) >= 100 * 8
 
