@@ -350,6 +350,8 @@ template <typename S> struct Sums {
     S* part;                                                // [workgroup][head, tail][ld_part]
     int64_t n, ld_dy, rows, dim, ld_dw, ld_part;
     int32_t dw_dtype, each, sum_groups, fill_rows, stream;
+    uint32_t slices, groups;                                // of a row's columns; of all that adds up and fills
+    int32_t by_slice;                                       // one slice after the other
     float scale;
     __device__ __forceinline__ S* head(int64_t group) const { return part + group * 2 * ld_part; }
     __device__ __forceinline__ S* tail(int64_t group) const { return head(group) + ld_part; }
@@ -371,8 +373,8 @@ template <typename S> __device__ __forceinline__ float8_t scaled(typename Eight8
 }
 
 // Rows of ids that do not occur: `fill_rows` to a wavefront, a row's id to a lane.
-template <typename S, int G> __device__ __forceinline__ void fill_rows(const Sums<S>& a, const Columns& at) {
-    const int64_t base = ((int64_t)(blockIdx.x - a.sum_groups) * (kSumThreads / 64) + (threadIdx.x >> 6)) * a.fill_rows;
+template <typename S, int G> __device__ __forceinline__ void fill_rows(const Sums<S>& a, int group, const Columns& at) {
+    const int64_t base = ((int64_t)group * (kSumThreads / 64) + (threadIdx.x >> 6)) * a.fill_rows;
     const int64_t row = base + (threadIdx.x & 63);
     bool absent = false;
     if (row < min(a.rows, base + a.fill_rows)) {
@@ -395,12 +397,14 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sums_kernel(Sums<S> a) 
     using R = typename Eight<DT>::vec;                      // (eight elements as they lie in memory: floats of them would take twice the registers)
     constexpr int U = sizeof(DT) == 4 ? 4 : 8, TEAMS = kSumThreads / G;
     const int lane = threadIdx.x % G, team = threadIdx.x / G;
-    const Columns at(((int64_t)blockIdx.y * G + lane) * 8, a.dim);
-    if ((int)blockIdx.x >= a.sum_groups) return fill_rows<S, G>(a, at);
+    const uint32_t slice = a.by_slice ? blockIdx.x / a.groups : blockIdx.x % a.slices;
+    const int group = (int)(a.by_slice ? blockIdx.x % a.groups : blockIdx.x / a.slices);
+    const Columns at(((int64_t)slice * G + lane) * 8, a.dim);
+    if (group >= a.sum_groups) return fill_rows<S, G>(a, group - a.sum_groups, at);
     extern __shared__ Entry s_e[];                          // [TEAMS * each + 2]: with the entry before, and that behind
     __shared__ S s_head[TEAMS][8][G];                       // what G threads have of an id that begins before theirs
     const uint32_t none = (uint32_t)a.rows;
-    const int64_t from0 = (int64_t)blockIdx.x * TEAMS * a.each - 1;
+    const int64_t from0 = (int64_t)group * TEAMS * a.each - 1;
     for (int j = threadIdx.x; j < TEAMS * a.each + 2; j += kSumThreads) s_e[j] = from0 + j >= 0 && from0 + j < a.n ? a.e[from0 + j] : Entry{none, 0};
     __syncthreads();
     auto key_at = [&](int i) { return s_e[i].key; };
@@ -479,13 +483,13 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sums_kernel(Sums<S> a) 
         if (at.on) reinterpret_cast<typename AnyEight<S>::type*>(part + at.col)->v = sum;
     };
     if (begins && goes_on) {
-        if (follow(rest, key1, team + 1)) keep(a.tail(blockIdx.x), rest);
+        if (follow(rest, key1, team + 1)) keep(a.tail(group), rest);
         else leave(key1, rest);
     }
     if (team == 0 && from_before) {
         V sum = V{0, 0, 0, 0, 0, 0, 0, 0};
         follow(sum, key0, 0);
-        keep(a.head(blockIdx.x), sum);
+        keep(a.head(group), sum);
     }
 }
 
@@ -575,10 +579,10 @@ template <typename F> void of_type(int32_t t, F f) {
 }
 
 inline size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
-// Entries that some threads take one after the other: enough of them for 8192 wavefronts.
+// Entries that some threads take one after the other: enough of them for 8192 wavefronts, and few where there are few (1440 ids of 16 columns 17 us, in sixteens 22).
 int entries_each(int64_t n, int64_t dim) {
     const int64_t waves = n * ceil_div(dim, 8 * group_of(dim)) * group_of(dim) / 64;
-    return waves <= 16 * 8192 ? 16 : waves <= 32 * 8192 ? 32 : kMostEach;
+    return waves <= 8 * 1024 ? 8 : waves <= 16 * 8192 ? 16 : waves <= 32 * 8192 ? 32 : kMostEach;
 }
 int64_t sum_groups(int64_t n, int64_t dim) { return ceil_div(n, (int64_t)entries_each(n, dim) * (kSumThreads / group_of(dim))); }
 inline int sum_bytes(int32_t dtype) { return dtype == LF_DTYPE_F32 ? 8 : 4; }
@@ -601,7 +605,14 @@ template <typename DT, typename S, int G> int launch_sums(Sums<S> a, hipStream_t
     // rows to a wavefront: 64, or fewer for enough of them
     a.fill_rows = a.rows * slices >= 64 * 4096 ? 64 : 16;
     const int64_t fill = ceil_div(a.rows, (int64_t)a.fill_rows * (kSumThreads / 64));
-    embedding_sums_kernel<DT, S, G><<<dim3((unsigned)(a.sum_groups + fill), (unsigned)slices), kSumThreads, (kSumThreads / G * a.each + 2) * sizeof(Entry), st>>>(a);
+    a.slices = (uint32_t)slices;
+    a.groups = (uint32_t)(a.sum_groups + fill);
+    // Neighbouring workgroups take the slices of a row, so that it is read and written whole by what is on the GPU at once (16,384 ids of 32,000 x 4096
+    // bf16 104 us, one slice after the other 128; 17 ids of 28,215 x 3824 f32 98 and 109).  Slices of float32 are 2 KB, and among many ids the
+    // wavefronts that add up are few: there filling one slice had better lie between adding up two (19,908 ids of 24,964 x 1792 106, else 121).
+    a.by_slice = sizeof(DT) == 4 && a.n >= a.rows / 4;
+    LF_REQUIRE((a.sum_groups + fill) * slices < (1ll << 32) / kSumThreads, LF_ERR_UNSUPPORTED, "too many rows");
+    embedding_sums_kernel<DT, S, G><<<(unsigned)((a.sum_groups + fill) * slices), kSumThreads, (kSumThreads / G * a.each + 2) * sizeof(Entry), st>>>(a);
     LF_HIP(hipGetLastError());
     if (a.sum_groups > 1) {
         embedding_join_kernel<S, G><<<dim3((unsigned)ceil_div(a.sum_groups, 1024 / G), (unsigned)slices), 1024, 0, st>>>(a);
@@ -714,7 +725,7 @@ int lf_embedding_grad(const lf_embedding_grad_args* h_args, void* d_work, size_t
         using T = decltype(t);
         using S = std::conditional_t<std::is_same_v<T, float>, double, float>;
         const Sums<S> k{sorted, present, a.d_dy, a.d_grad, (S*)at, a.n, a.ld_dy, a.rows, a.dim, a.ld_grad, ceil_div(a.dim, 8) * 8, a.grad_dtype, entries_each(a.n, a.dim),
-                        (int32_t)sum_groups(a.n, a.dim), 0, a.rows * a.dim * dtype_bytes(a.grad_dtype) >= kStreamBytes, a.scale};
+                        (int32_t)sum_groups(a.n, a.dim), 0, a.rows * a.dim * dtype_bytes(a.grad_dtype) >= kStreamBytes, 0, 0, 0, a.scale};
         rc = group == 8 ? launch_sums<T, S, 8>(k, st) : group == 16 ? launch_sums<T, S, 16>(k, st) : group == 32 ? launch_sums<T, S, 32>(k, st) : launch_sums<T, S, 64>(k, st);
     });
     return rc;
