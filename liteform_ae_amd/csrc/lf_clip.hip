@@ -4,6 +4,9 @@
 //
 // Squares are added in 64 bits: none overflows or vanishes, whatever the type, and the sum is good to the last place of the norm's 32.
 // Tensors are handed to the kernels as arguments, a few dozen to a launch, so that nothing is copied to the GPU.
+//
+// Bound by memory, three passes of it: the norm has to be known before the first output.  403M elements of bfloat16 141 + 297 us (5.7 and 5.4 TB/s; with one piece of
+// eight elements under way a thread, not eight, the norm took 215); 150k of float32 5 + 8.
 #include <algorithm>
 #include <new>
 #include <vector>

@@ -5,7 +5,14 @@
 // An id outside 0 .. rows - 1 (padding) stands for a row of zeros, and has no gradient.
 //
 // The gradient sorts the ids, by digits of up to 11 bits and stably, so that a row's terms are added in the order in which they were
-// looked up, whatever the scheduling; no two threads add to one address.
+// looked up, whatever the scheduling; no two threads add to one address.  Then equal parts of the sorted entries are added up, whatever ids they are of, and what
+// parts have of one id is put together, in LDS and (from a workgroup to the next) through memory.  Sums of float32 are in 64 bits, of 16-bit types in 32, and
+// in 64 from part to part: an id may have all rows.
+//
+// Measured with inputs that no cache holds: 57,001 rows of 2.45M x 128 f16 8 us; gradient of 16,384 ids of 32,000 x 4096 bf16, most of them a few ids, 104 us: sort
+// 25 in four launches, sums and rows of zeros 75 (396 MB: 5.3 TB/s), join 6.  Bound by memory where rows are long; else by launches and by
+// the latency of each pass (100,000 ids of 16 columns: 59 us).  Counts of the next digit made with atomic additions while the entries move, a launch less: 94 us
+// became 110, 72 (432k ids of 82) became 95.
 #include <algorithm>
 
 #include "lf_dense.h"

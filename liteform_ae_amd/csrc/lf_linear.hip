@@ -71,6 +71,7 @@ template <typename A> int launch_join(const Product& g, hipStream_t st) {
 // Up to 16 rows of X: a workgroup takes 16 rows of W, its wavefronts the 128-byte steps of k in turn, and their sums
 // meet in LDS.  W goes from memory into the matrix instructions' registers, 32 consecutive bytes a lane and step.  Bound by the
 // read of W, small ones by the launch: one row, bf16 W of 8192^2 29 us (4.6 TB/s), of 4096^2 9.4 (3.6); 13 rows, int8 W of 1001 x 4000 6.
+// Gated: 16 rows of each half, and both sums in the same lane; one row, bf16 of 2 x 8192 x 4096 28 out of the memory-side cache, 31 from memory (4.3 TB/s).
 template <typename T, int WAVES, bool GATED = false>
 __global__ void __launch_bounds__(64 * WAVES)
 few_rows_kernel(Product g) {
@@ -263,6 +264,8 @@ template <typename A> int launch_gated_join(const Product& g, hipStream_t st) {
 }
 
 // dz = [dy u act'(g) | dy act(g)] of z = [g | u], in rows of `ld_dz`, and the column sums of a slab of rows, as activation_grad_kernel has them.
+// Bound by memory: bf16 8192 x 4096 67 us (335 MB at 5.0 TB/s), float32 57,001 x 200 50 (228 MB at 4.6).  dz is rounded to the operands' type, since the products
+// take it so.
 template <typename T, int ACROSS>
 __global__ void __launch_bounds__(256)
 gate_grad_kernel(const T* dy, int64_t ld_dy, const T* z, int64_t ld_z, T* dz, int64_t ld_dz, float* part, void* db, int32_t db_dtype, int64_t m, int64_t n, int32_t act,

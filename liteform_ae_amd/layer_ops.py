@@ -8,13 +8,18 @@ addition, and the dense transform with its epilogue - forward, in 8 bits, and ba
     q, s, h = rms_norm_8bit(C, w, residual=h)                     # the same layer served in 8 bits
     y = linear_8bit(q, s, Wq, Ws, b, activation="gelu")           # Wq, Ws = quantize_rows(W), once
 
+    y = embedding(ids, table, scale)                              # a stack from node ids: what its first layer reads
+    n, h = layer_norm(C, w, b, residual=h)                        # a layer with a gated feed-forward block
+    y = linear(gated_linear(n, W2, b2, activation="silu"), W1, b1)
+    grads, norm = clip_gradients(grads, 1.0, in_place=True)       # before a training step's update
+
 The reference ends with the sparse product (format_algos.py:388-605) and has no counterpart.  Everything runs in
 ``liblfhip.so`` (``lf_rms_norm``, ``lf_linear``, ...) on the current stream of the current device; there is no CPU path.
 
 Matrices are CUDA tensors (rows, features) whose rows are contiguous; the distance from one row to the next is free, so a
 slice of a wider buffer's columns needs no copy.  float32, bfloat16 and float16, sums in 32 bits.
 
-What is returned is no part of a torch graph: gradients are those of ``rms_norm_grad`` and ``linear_grad``.  Tensors that require
+What is returned is no part of a torch graph: gradients are those of the functions named ``..._grad``.  Tensors that require
 gradients are taken under ``torch.no_grad()`` only, and refused where torch would expect a graph.
 """
 from __future__ import annotations
@@ -50,7 +55,7 @@ def refuse_graph(name, t):
     """ValueError where a gradient that torch is asked for would be lost without a word."""
     if t.requires_grad and _torch().is_grad_enabled():
         raise ValueError(f"{name} requires gradients, and what is returned would not lead back to it: call this under torch.no_grad() (or pass "
-                         f"{name}.detach()) and take them from rms_norm_grad and linear_grad")
+                         f"{name}.detach()) and take them from the function's _grad")
 
 
 def _matrix(name, t, types, device, rows=None, cols=None):
