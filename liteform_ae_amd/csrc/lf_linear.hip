@@ -71,24 +71,23 @@ template <typename A> int launch_join(const Product& g, hipStream_t st) {
 // Up to 16 rows of X: a workgroup takes 16 rows of W, its wavefronts the 128-byte steps of k in turn, and their sums
 // meet in LDS.  W goes from memory into the matrix instructions' registers, 32 consecutive bytes a lane and step.  Bound by the
 // read of W, small ones by the launch: one row, bf16 W of 8192^2 29 us (4.6 TB/s), of 4096^2 9.4 (3.6); 13 rows, int8 W of 1001 x 4000 6.
-// Gated: 16 rows of each half, and both sums in the same lane; one row, bf16 of 2 x 8192 x 4096 28 out of the memory-side cache, 31 from memory (4.3 TB/s).
-template <typename T, int WAVES, bool GATED = false>
+// Gated: eight rows of each half, so that a workgroup reads as much as one of 16 outputs does; one row, bf16 of 2 x 8192 x 4096 from memory 26 - 28 us (4.8 - 5.2 TB/s),
+// with 16 rows of each half, half as many workgroups of more registers, 31.  16 rows take 39 (36 so): X comes from L2 for every workgroup.
+template <typename T, int WAVES, bool GATED>
 __global__ void __launch_bounds__(64 * WAVES)
 few_rows_kernel(Product g) {
-    constexpr int KS = 128 / sizeof(T), MINE = 32 / sizeof(T), E = 16 / sizeof(T);
+    constexpr int KS = 128 / sizeof(T), MINE = 32 / sizeof(T), E = 16 / sizeof(T), OUT = GATED ? 8 : 16;
     using Acc = typename Elem<T>::Acc;
     using S = std::conditional_t<std::is_same_v<Acc, int4v>, int32_t, float>;
-    constexpr int HALVES = GATED ? 2 : 1;
-    __shared__ S s_sum[HALVES][WAVES][16][17];
+    __shared__ S s_sum[WAVES][16][17];
     const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t n0 = (int64_t)blockIdx.x * 16;
-    const T* w = (const T*)g.q + min(n0 + li, g.n - 1) * g.ld_q + lg * MINE;
+    const int64_t n0 = (int64_t)blockIdx.x * OUT, row = GATED ? (li >> 3) * g.n + min(n0 + (li & 7), g.n - 1) : min(n0 + li, g.n - 1);
+    const T* w = (const T*)g.q + row * g.ld_q + lg * MINE;
     const bool on = li < g.m;
     const T* x = (const T*)g.p + (on ? li : 0) * g.ld_p + lg * MINE;
-    const int64_t half = g.n * g.ld_q;                          // from the gate's rows to those of the other half
-    Acc acc[HALVES] = {};
-    auto multiply = [&](Acc& acc, const uint4_t (&a)[2], const uint4_t (&b)[2]) {
+    Acc acc = {0, 0, 0, 0};
+    auto multiply = [&](const uint4_t (&a)[2], const uint4_t (&b)[2]) {
         if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -100,57 +99,51 @@ few_rows_kernel(Product g) {
             acc = mma(a[1], b[1], acc, T{});
         }
     };
-    constexpr int U = GATED && WAVES == 16 ? 2 : 4;             // steps under way at once (as many as there are registers for)
+    constexpr int U = 4;                                        // steps under way at once
     const int64_t steps = g.k / KS;
     int64_t s = wave;
     for (; s + (U - 1) * WAVES < steps; s += U * WAVES) {
-        uint4_t a[HALVES][U][2], b[U][2];
+        uint4_t a[U][2], b[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int v = 0; v < HALVES; ++v) a[v][u][h] = load16(w + v * half + (s + u * WAVES) * KS + h * E);
+                a[u][h] = load16(w + (s + u * WAVES) * KS + h * E);
                 b[u][h] = uint4_t{0u, 0u, 0u, 0u};
                 if (on) b[u][h] = load16(x + (s + u * WAVES) * KS + h * E);
             }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int v = 0; v < HALVES; ++v) multiply(acc[v], a[v][u], b[u]);
+        for (int u = 0; u < U; ++u) multiply(a[u], b[u]);
     }
     for (; s < steps + (g.k % KS != 0); s += WAVES) {
-        uint4_t a[HALVES][2], b[2];
+        uint4_t a[2], b[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int left = (int)min((int64_t)E, g.k - s * KS - lg * MINE - h * E);
-#pragma unroll
-            for (int v = 0; v < HALVES; ++v) a[v][h] = load16_each(w + v * half + s * KS + h * E, left);
+            a[h] = load16_each(w + s * KS + h * E, left);
             b[h] = load16_each(x + s * KS + h * E, on ? left : 0);
         }
-#pragma unroll
-        for (int v = 0; v < HALVES; ++v) multiply(acc[v], a[v], b);
+        multiply(a, b);
     }
 #pragma unroll
-    for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) s_sum[h][wave][li][lg * 4 + v] = acc[h][v];
+    for (int v = 0; v < 4; ++v) s_sum[wave][li][lg * 4 + v] = acc[v];
     __syncthreads();
-    const int m = threadIdx.x >> 1, at = (threadIdx.x & 1) * 8;
-    if (m >= g.m || n0 + at >= g.n) return;
-    float8_t out[HALVES];
+    const int m = threadIdx.x >> 1, half = threadIdx.x & 1;
+    if (m >= g.m || (!GATED && n0 + half * 8 >= g.n)) return;
+    float8_t out[2];                                            // (gated: the gate's, from the first of the two threads, and the other half's)
 #pragma unroll
-    for (int h = 0; h < HALVES; ++h)
+    for (int i = 0; i < 8; ++i) {
+        S t = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            S t = 0;
-#pragma unroll
-            for (int u = 0; u < WAVES; ++u) t += s_sum[h][u][m][at + i];
-            out[h][i] = (float)t;
-        }
-    const int count = (int)min((int64_t)8, g.n - n0 - at);
-    if constexpr (GATED) finish_gated(g.e, m, n0 + at, g.n, count, out);
-    else finish(g.e, m, n0 + at, count, out[0]);
+        for (int u = 0; u < WAVES; ++u) t += s_sum[u][m][half * 8 + i];
+        out[0][i] = (float)t;
+        if constexpr (GATED) out[1][i] = __shfl_xor(out[0][i], 1);
+    }
+    if constexpr (GATED) {
+        if (!half) finish_gated(g.e, m, n0, g.n, (int)min((int64_t)8, g.n - n0), out);
+    } else {
+        finish(g.e, m, n0 + half * 8, (int)min((int64_t)8, g.n - n0 - half * 8), out[0]);
+    }
 }
 
 // ---------------------------------------------------------------------------- gradient of the activation
@@ -346,7 +339,7 @@ int launch_product(Product g, int32_t dtype, bool px, bool qx, void* work, hipSt
     g.e.stream = g.m * (g.n * dtype_bytes(g.e.y_dtype) + (gated && g.e.z ? q_rows * dtype_bytes(g.e.z_dtype) : 0)) >= kStreamBytes;
     const Path path = path_of(dtype_bytes(dtype), {g.p, g.ld_p, g.m, px}, {g.q, g.ld_q, q_rows, qx}, g.k);
     if (path.kernel == kPathFewRows) {
-        const int64_t groups = ceil_div(g.n, 16);
+        const int64_t groups = ceil_div(g.n, gated ? 8 : 16);
         LF_REQUIRE(groups < (1ll << 31), LF_ERR_UNSUPPORTED, "too many columns");
         // few workgroups take 16 wavefronts each
         if (groups <= 256) (gated ? few_rows_of<16, true>(dtype) : few_rows_of<16, false>(dtype))<<<(unsigned)groups, 1024, 0, st>>>(g);
