@@ -175,7 +175,7 @@ void add(Call& c, const lf_tensor_desc& d, int64_t chunks) {
 }
 
 int clip(const lf_tensor_desc* t, int32_t n, float most, float eps, float* d_norm, void* d_work, size_t work_bytes, hipStream_t st) {
-    bool out = false;
+    bool out = false, any = false;
     int64_t elements = 0;
     for (int32_t i = 0; i < n; ++i) {
         const lf_tensor_desc& d = t[i];
@@ -188,7 +188,8 @@ int clip(const lf_tensor_desc* t, int32_t n, float most, float eps, float* d_nor
         LF_REQUIRE(d.d_src, LF_ERR_INVALID, "tensor %d: null pointer", i);
         LF_REQUIRE((uintptr_t)d.d_src % dtype_bytes((int32_t)d.dtype) == 0 && (uintptr_t)d.d_dst % dtype_bytes((int32_t)d.dtype) == 0, LF_ERR_INVALID, "tensor %d: not aligned to its elements", i);
         LF_REQUIRE(d.rows <= 1 || (d.ld_src >= d.cols && (!d.d_dst || d.ld_dst >= d.cols)), LF_ERR_INVALID, "tensor %d: rows of %lld elements overlap", i, (long long)d.cols);
-        LF_REQUIRE(!out || d.d_dst, LF_ERR_INVALID, "outputs are for all tensors or for none");
+        LF_REQUIRE(!any || out == (d.d_dst != nullptr), LF_ERR_INVALID, "outputs are for all tensors or for none");
+        any = true;
         out = d.d_dst != nullptr;
         LF_REQUIRE(elements <= kMostElements, LF_ERR_UNSUPPORTED, "more elements than any GPU holds");
     }

@@ -142,6 +142,16 @@ def test_clip_refusals():
     assert lib.lf_clip_work_bytes(0) == 0 and lib.lf_clip_work_bytes(-3) == 0 and lib.lf_clip_work_bytes(100) >= 100 * 8
 
 
+# (the first without an output: its address would be null)
+@pytest.mark.parametrize("nones", [(0,), (1,), (2,), (0, 1), (0, 2), (1, 2)])
+def test_clip_refuses_some_outputs_without_the_others(nones):
+    lib = _lib.load()
+    some = [dict(src=AT + 4096 * i, dst=None if i in nones else AT * 2 + 4096 * i) for i in range(3)]
+    refused(clip(lib, descs(*some)), text="for all tensors or for none")
+    empty = dict(src=None, dst=None, rows=0)
+    refused(clip(lib, descs(empty, *some, empty)), text="for all tensors or for none")
+
+
 #  float32 elements of 4 bytes: 100 of them take 400
 LIES = [
     [dict(src=AT, dst=AT), dict(src=AT, dst=AT)],                                                        # the same one twice
