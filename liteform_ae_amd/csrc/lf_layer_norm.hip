@@ -572,7 +572,7 @@ template <typename F> auto of_types(int32_t a, int32_t b, F f) {
 }
 
 // Workgroups of 256 threads, as for the norms of lf_norm.hip.
-constexpr int kNormGroups = 3072, kGradGroups = 1024;
+constexpr int kNormGroups = 12 * 256, kGradGroups = 4 * 256;
 unsigned grad_groups(int64_t rows, int64_t dim) {
     return std::min(workgroups(rows, shape_of(dim), kGradGroups), (unsigned)std::max<int64_t>(1, (1ll << 25) / dim));
 }
