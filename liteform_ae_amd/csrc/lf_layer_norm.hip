@@ -14,7 +14,8 @@
 // with its stream 99 (5.4), gradient of bfloat16 32k x 2048 108 + 5 (5.0); one row of 4096 features 4.6.
 // The gradient has five sums over a row and four barriers where a workgroup shares one.  Two barriers, or products and sums in one operation, made no difference; rows of 2048
 // in one wavefront, without barriers, took 139 us.
-// Rows whose sums overflow are taken times 2^-100 and summed again, those whose squares vanish after the subtraction times 2^100.
+// Rows whose sums overflow are taken times 2^-100 and summed again, those whose squares vanish after the subtraction times 2^100.  Where the variance is less than
+// what the correction takes off - equal elements, or such as differ in their last places - the mean is corrected first and the squares are summed once more.
 #include "lf_rows.h"
 
 namespace {
@@ -63,38 +64,54 @@ struct LayerArgs {
     float eps, inv_dim;
 };
 
+// What changes a row.
+struct Change {
+    float off, by;
+    template <typename V> __device__ __forceinline__ V operator()(V x) const { return (x - off) * by; }
+};
+
 // A row's statistics: t = (h - mean - less) inv.  Where sums overflow or squares vanish the row is changed first, h -> (h - off) by, and what is said here is of
 // the row as it is then; by: the power of two.
 struct Centre {
     float mean, less, inv, by;
-    // first: () -> sum of h.  second: (d, dd) <- sums of h - mean and of its squares.  change(off, by): changes the row
+    // sum: of h.  first(f): that of f(h).  second(f, d, dd): d, dd <- sums of f(h) - mean and of its squares.  change(f): h <- f(h)
     template <typename FIRST, typename SECOND, typename CHANGE>
-    __device__ __forceinline__ void find(float eps, float inv_dim, FIRST first, SECOND second, CHANGE change) {
+    __device__ __forceinline__ void find(float eps, float inv_dim, float sum, FIRST first, SECOND second, CHANGE change) {
         by = 1.f;
-        auto variance = [&] {
+        float var, more = eps;                              // mean((h - mean)^2) - less^2, and what is added to it
+        auto look = [&](auto f) {
             float d, dd;
-            second(d, dd);
+            second(f, d, dd);
             less = d * inv_dim;
             const float v = fmaf(dd, inv_dim, -(less * less));
-            return v < 0.f ? 0.f : v;                                    // (a NaN stays)
+            var = (v < 0.f ? 0.f : v) + more;                            // (a NaN stays)
         };
-        mean = first() * inv_dim;
-        float var = variance() + eps;
-        if (__builtin_expect(!(var >= kTiny && var < __builtin_inff()), 0)) {      // (the same for all threads of the row)
-            if (var < kTiny) {
-                by = 1.f / kTiny;
-                change(mean, by);
-                mean = 0.f;
-                var = variance() + eps * by * by;
-            } else {
-                // (the mean once more: here eps, far below what is left of its rounding, would not hide it)
-                by = kTiny;
-                change(0.f, by);
-                mean = first() * inv_dim;
-                variance();
-                mean += less;
-                var = variance();
-                if (eps > 0.f && var < kTiny) var = kTiny;
+        mean = sum * inv_dim;
+        look([](float x) { return x; });
+        if (__builtin_expect(!(var >= fmaxf(kTiny, less * less) && var < __builtin_inff()), 0)) {      // (the same for all threads of the row)
+            // Where the variance is less than what was taken off - rows far from zero that differ in their last places, or not at all - the mean moves to the float
+            // nearest to the true one, beside which such differences are not small; equal elements then leave 0.
+            Change f{0.f, 1.f};
+#pragma unroll 1
+            for (int moves = 0;;) {
+                if (less * less > var && moves < 3) {
+                    ++moves;
+                    mean += less;
+                } else if (f.by == 1.f && !(var >= kTiny && var < __builtin_inff())) {
+                    moves = 0;
+                    f = var < kTiny ? Change{mean, 1.f / kTiny} : Change{0.f, kTiny};
+                    more = var < kTiny ? eps * f.by * f.by : 0.f;        // (eps is nothing beside squares that overflow)
+                    mean = first(f) * inv_dim;
+                } else {
+                    break;
+                }
+                look(f);
+            }
+            change(f);
+            by = f.by;
+            if (by < 1.f && var == 0.f && eps > 0.f) {
+                by = 1.f;
+                var = eps;
             }
         }
         inv = 1.f / sqrtf(var);
@@ -147,29 +164,28 @@ layer_norm_kernel(LayerArgs a) {
                 }
             }
         };
-        bool left = !a.res;
-        Centre m;
-        m.find(a.eps, a.inv_dim,
-               [&] {
-                   float v[1] = {0.f};
-                   each_of([&](float x) { v[0] += x; });
-                   row_sums<G>(v, s_red);
-                   // (behind the sums' barriers: h may be the residual itself, and the end of a row reaches back into what another wavefront reads)
-                   if (!left) {
-                       RT* hr = (RT*)a.h + row * a.ldh;
+        auto first = [&](auto f) {
+            float v[1] = {0.f};
+            each_of([&](float x) { v[0] += f(x); });
+            row_sums<G>(v, s_red);
+            return v[0];
+        };
+        const float sum = first([](float x) { return x; });
+        // (behind the sum's barriers: h may be the residual itself, and the end of a row reaches back into what another wavefront reads)
+        if (a.res) {
+            RT* hr = (RT*)a.h + row * a.ldh;
 #pragma unroll
-                       for (int c = 0; c < C; ++c) {
-                           const Piece p = piece_of((c * G + lane) * 8, dim);
-                           if (p.first < 8) store_piece(hr, p, dim, h[c], a.stream);
-                       }
-                       left = true;
-                   }
-                   return v[0];
-               },
-               [&](float& d, float& dd) {
+            for (int c = 0; c < C; ++c) {
+                const Piece p = piece_of((c * G + lane) * 8, dim);
+                if (p.first < 8) store_piece(hr, p, dim, h[c], a.stream);
+            }
+        }
+        Centre m;
+        m.find(a.eps, a.inv_dim, sum, first,
+               [&](auto f, float& d, float& dd) {
                    float v[2] = {0.f, 0.f};
                    each_of([&](float x) {
-                       const float t = x - m.mean;
+                       const float t = f(x) - m.mean;
                        v[0] += t;
                        v[1] = fmaf(t, t, v[1]);
                    });
@@ -177,9 +193,9 @@ layer_norm_kernel(LayerArgs a) {
                    d = v[0];
                    dd = v[1];
                },
-               [&](float off, float by) {
+               [&](auto f) {
 #pragma unroll
-                   for (int c = 0; c < C; ++c) h[c] = (h[c] - off) * by;
+                   for (int c = 0; c < C; ++c) h[c] = f(h[c]);
                });
 #pragma unroll
         for (int c = 0; c < C; ++c) h[c] = m.of(h[c]) * w[c] + b[c];
@@ -225,23 +241,24 @@ layer_norm_long_kernel(LayerArgs a) {
             }
         };
         float off = 0.f, by = 1.f;                                       // (read again, the row is changed again)
-        Centre m;
-        m.find(a.eps, a.inv_dim,
-               [&] {
-                   float v[1] = {0.f};
-                   pieces([&](int, int, float8_t h) {                    // (zeros behind the end: only `second` changes by an offset)
+        auto first = [&](auto f) {
+            float v[1] = {0.f};
+            pieces([&](int, int n, float8_t h) {
 #pragma unroll
-                       for (int i = 0; i < 8; ++i) v[0] += h[i] * by;
-                   });
-                   row_sums<1024>(v, s_red);
-                   return v[0];
-               },
-               [&](float& d, float& dd) {
+                for (int i = 0; i < 8; ++i) v[0] += i < n ? f(h[i]) : 0.f;
+            });
+            row_sums<1024>(v, s_red);
+            return v[0];
+        };
+        const float sum = first([](float x) { return x; });
+        Centre m;
+        m.find(a.eps, a.inv_dim, sum, first,
+               [&](auto f, float& d, float& dd) {
                    float v[2] = {0.f, 0.f};
                    pieces([&](int, int n, float8_t h) {
 #pragma unroll
                        for (int i = 0; i < 8; ++i) {
-                           const float t = i < n ? (h[i] - off) * by - m.mean : 0.f;
+                           const float t = i < n ? f(h[i]) - m.mean : 0.f;
                            v[0] += t;
                            v[1] = fmaf(t, t, v[1]);
                        }
@@ -250,9 +267,9 @@ layer_norm_long_kernel(LayerArgs a) {
                    d = v[0];
                    dd = v[1];
                },
-               [&](float o, float b) {
-                   off = o;
-                   by = b;
+               [&](auto f) {
+                   off = f.off;
+                   by = f.by;
                });
         auto out = [&](int col, int n, float8_t h) {
             float8_t y = m.of((h - off) * by);
@@ -312,12 +329,20 @@ layer_norm_grad_kernel(LayerGradArgs a) {
     __shared__ float s_red[4 * (G > 64 ? G / 64 : 1)];
     __shared__ float s_sum[R > 1 ? T * 8 * C : 1];
     const int lane = threadIdx.x % G, group = threadIdx.x / G, dim = a.dim;
+    // A workgroup of 1024 threads has 128 registers a thread.  With a stream of float32 the weight exceeds them by 11 words: read again from the caches it takes 80 us for
+    // 900 x 16,384, not 84; with one of 16 bits by 3, and there 57 us become 61.
+    constexpr bool HELD = G < 1024 || sizeof(HT) == 2;
     float8_t w[C], sums[2][C];
+    auto weight = [&](int c) {
+        uintptr_t at = (uintptr_t)a.w;
+        if (!HELD) asm volatile("" : "+s"(at));            // (for every row, not once before them all)
+        const void* p = (const void*)(const __attribute__((address_space(1))) char*)at;
+        return at ? load_piece(p, 0, a.w_dtype, piece_of((c * G + lane) * 8, dim), dim) : float8_t{1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+    };
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        w[c] = float8_t{1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        if (HELD) w[c] = weight(c);
         sums[0][c] = sums[1][c] = float8_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (a.w) w[c] = load_piece(a.w, 0, a.w_dtype, piece_of((c * G + lane) * 8, dim), dim);
     }
     constexpr bool AHEAD = G < 1024 && C * (sizeof(DT) + 2 * sizeof(HT)) <= 12;
     typename Eight<HT>::vec raw_h[C], raw_dh[C];
@@ -349,6 +374,7 @@ layer_norm_grad_kernel(LayerGradArgs a) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const Piece p = piece_of((c * G + lane) * 8, dim);
+                if (!HELD) w[c] = weight(c);
                 if (whole) {
                     if (p.first == 0)
 #pragma unroll
@@ -362,17 +388,18 @@ layer_norm_grad_kernel(LayerGradArgs a) {
         };
         Centre m;
         float g_sum, g_dot;                                              // of g and g (h - mean)
-        m.find(a.eps, a.inv_dim,
-               [&] {
-                   float v[1] = {0.f};
-                   each_of([&](float x, float) { v[0] += x; });
-                   row_sums<G>(v, s_red);
-                   return v[0];
-               },
-               [&](float& d, float& dd) {
+        auto first = [&](auto f) {
+            float v[1] = {0.f};
+            each_of([&](float x, float) { v[0] += f(x); });
+            row_sums<G>(v, s_red);
+            return v[0];
+        };
+        const float sum = first([](float x) { return x; });
+        m.find(a.eps, a.inv_dim, sum, first,
+               [&](auto f, float& d, float& dd) {
                    float v[4] = {0.f, 0.f, 0.f, 0.f};
                    each_of([&](float x, float g) {
-                       const float t = x - m.mean;
+                       const float t = f(x) - m.mean;
                        v[0] += t;
                        v[1] = fmaf(t, t, v[1]);
                        v[2] += g;
@@ -384,15 +411,16 @@ layer_norm_grad_kernel(LayerGradArgs a) {
                    g_sum = v[2];
                    g_dot = v[3];
                },
-               [&](float off, float by) {
+               [&](auto f) {
 #pragma unroll
-                   for (int c = 0; c < C; ++c) h[c] = (h[c] - off) * by;
+                   for (int c = 0; c < C; ++c) h[c] = f(h[c]);
                });
         const float g_mean = g_sum * a.inv_dim, along = fmaf(-m.less, g_sum, g_dot) * m.inv * a.inv_dim, s = m.inv * m.by;
         HT* dx = (HT*)a.dx + row * a.ldx;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const Piece p = piece_of((c * G + lane) * 8, dim);
+            if (!HELD) w[c] = weight(c);
             const float8_t t = m.of(h[c]);
             float8_t d = (dy[c] * w[c] - g_mean - t * along) * s;
             if (a.dh) d += AHEAD ? dh[c] : load_piece((const HT*)a.dh + row * a.ldd, p, dim);
@@ -451,24 +479,25 @@ layer_norm_grad_long_kernel(LayerGradArgs a) {
         float off = 0.f, by = 1.f;
         Centre m;
         float g_sum, g_dot;
-        m.find(a.eps, a.inv_dim,
-               [&] {
-                   float v[1] = {0.f};
-                   pieces([&](int, int, float8_t h, float8_t) {
+        auto first = [&](auto f) {
+            float v[1] = {0.f};
+            pieces([&](int, int n, float8_t h, float8_t) {
 #pragma unroll
-                       for (int i = 0; i < 8; ++i) v[0] += h[i] * by;
-                   });
-                   row_sums<1024>(v, s_red);
-                   return v[0];
-               },
-               [&](float& d, float& dd) {
+                for (int i = 0; i < 8; ++i) v[0] += i < n ? f(h[i]) : 0.f;
+            });
+            row_sums<1024>(v, s_red);
+            return v[0];
+        };
+        const float sum = first([](float x) { return x; });
+        m.find(a.eps, a.inv_dim, sum, first,
+               [&](auto f, float& d, float& dd) {
                    float v[4] = {0.f, 0.f, 0.f, 0.f};
                    pieces([&](int col, int n, float8_t h, float8_t dy) {
                        const float8_t g = weighted(dy, col, n);
 #pragma unroll
                        for (int i = 0; i < 8; ++i) {
                            if (i >= n) continue;
-                           const float t = (h[i] - off) * by - m.mean;
+                           const float t = f(h[i]) - m.mean;
                            v[0] += t;
                            v[1] = fmaf(t, t, v[1]);
                            v[2] += g[i];
@@ -481,9 +510,9 @@ layer_norm_grad_long_kernel(LayerGradArgs a) {
                    g_sum = v[2];
                    g_dot = v[3];
                },
-               [&](float o, float b) {
-                   off = o;
-                   by = b;
+               [&](auto f) {
+                   off = f.off;
+                   by = f.by;
                });
         const float g_mean = g_sum * a.inv_dim, along = fmaf(-m.less, g_sum, g_dot) * m.inv * a.inv_dim, s = m.inv * m.by;
         pieces([&](int col, int n, float8_t h, float8_t dy) {
