@@ -106,7 +106,8 @@ __global__ void __launch_bounds__(256) clip_kernel(List l, const double* part, i
     for (int i = threadIdx.x; i < parts; i += 256) sum += part[i];
     const float total = (float)sqrt(sum_of_workgroup(sum));
     if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
-    const float by = most / (total + eps), c = by > 1.f || total == 0.f ? 1.f : by;      // (a norm of NaN leaves NaN)
+    // (a norm of NaN leaves NaN; a limit that is infinite cuts nothing, not even an infinite norm)
+    const float by = most / (total + eps), c = by > 1.f || total == 0.f || (most == __builtin_inff() && total == total) ? 1.f : by;
     for (int chunk = blockIdx.x; chunk < l.first[l.n]; chunk += gridDim.x) {
         const int i = tensor_of(l, chunk);
         const Tensor& t = l.t[i];

@@ -576,7 +576,7 @@ def gradient_norm(grads):
 def clip_gradients(grads, max_norm: float, eps: float = 1e-6, in_place: bool = False):
     """``(clipped, norm)``: the tensors of ``grads`` times ``min(1, max_norm / (norm + eps))`` and their ``gradient_norm`` before.  ``in_place=True`` writes
     them where they are (a tensor that shares elements with another is refused), and leaves them alone where nothing is to be cut.  A norm that is NaN
-    makes all of them NaN; look at it first where that may be."""
+    makes all of them NaN, an infinite one zeros (NaN where they are infinite); look at it first where that may be.  ``max_norm=inf`` cuts nothing."""
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     return _clip(grads, max_norm, eps, in_place, True)
