@@ -189,7 +189,7 @@ class NodeEmbedding:
     def forward(self, ids, keep=False):
         kept = keep if isinstance(keep, list) else self._kept if keep else None
         if kept is not None:
-            kept.append(ids)
+            kept.append(ids.clone())                # (the caller may read the next batch into them)
         return lo.embedding(ids, self.table, scale=self.scale)
 
     def backward(self, dy, kept=None):

@@ -1,4 +1,4 @@
-"""Limits of clipping that cut nothing."""
+"""Limits of clipping that cut nothing, and what node embeddings keep of a call."""
 import math
 
 import pytest
@@ -50,3 +50,20 @@ def test_a_finite_limit_and_an_infinite_norm(lo):
             clipped, norm = lo.clip_gradients(grads, most, in_place=in_place)
             assert float(norm) == math.inf and bool(torch.isnan(clipped[0][7])) and int(torch.isnan(clipped[0]).sum()) == 1
             assert bool((torch.nan_to_num(clipped[0]) == 0).all()) and bool((clipped[1] == 0).all())
+
+
+def test_ids_that_change_between_forward_and_backward():
+    """A buffer of ids that the next batch is read into: each call's gradient is of the ids that it had."""
+    from liteform_ae_amd import graph_layer, layer_ops as lo
+    g = gen(82)
+    embedding = graph_layer.NodeEmbedding(50, 24, generator=g)
+    first, second = (torch.randint(0, 50, (300,), device="cuda", generator=g) for _ in range(2))
+    dy = torch.randn((300, 24), device="cuda", generator=g)
+    want = [lo.embedding_grad(dy, ids, 50) for ids in (first, second)]
+    ids, some = first.clone(), []
+    embedding.forward(ids, keep=True)
+    embedding.forward(ids, keep=some)
+    ids.copy_(second)
+    embedding.forward(ids, keep=True)
+    ids.zero_()
+    assert torch.equal(embedding.backward(dy)[0], want[1]) and torch.equal(embedding.backward(dy)[0], want[0]) and torch.equal(embedding.backward(dy, some[0])[0], want[0])
