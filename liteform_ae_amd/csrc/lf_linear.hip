@@ -381,6 +381,9 @@ int check_sizes(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act) {
     return LF_OK;
 }
 
+// Rows of a gated weight; sizes that are refused stay as they are (twice INT64_MIN would be 0).
+int64_t both_halves(int64_t n) { return n < 0 || n > kMostFeatures ? n : 2 * n; }
+
 // Rows of dz are padded to a multiple of 16 bytes.
 int64_t ld_dz(int64_t n) { return ceil_div(n, 8) * 8; }
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -507,13 +510,13 @@ int lf_linear_grad(const lf_linear_grad_args* h_args, void* d_work, size_t work_
 }
 
 size_t lf_gated_linear_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype) {
-    return lf_linear_work_bytes(m, 2 * n, k, dtype);
+    return n > kMostFeatures ? 0 : lf_linear_work_bytes(m, both_halves(n), k, dtype);
 }
 
 int lf_gated_linear(const lf_linear_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream) {
     LF_REQUIRE(h_args, LF_ERR_INVALID, "null argument");
     const lf_linear_args& a = *h_args;
-    LF_TRY(check_sizes(a.m, 2 * a.n, a.k, a.dtype, a.activation));
+    LF_TRY(check_sizes(a.m, both_halves(a.n), a.k, a.dtype, a.activation));
     LF_REQUIRE(is_float_dtype(a.y_dtype) && (!a.d_bias || is_float_dtype(a.bias_dtype)) && (!a.d_z || is_float_dtype(a.z_dtype)), LF_ERR_UNSUPPORTED,
                "y, z and bias are float32, bfloat16 or float16");
     LF_REQUIRE(!a.d_residual, LF_ERR_INVALID, "a gated product has no residual");
@@ -534,14 +537,14 @@ int lf_gated_linear(const lf_linear_args* h_args, void* d_work, size_t work_byte
 }
 
 size_t lf_gated_linear_grad_work_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t want_dx, int32_t want_dw, int32_t want_db) {
-    if (m <= 0 || n <= 0 || k < 0 || !is_float_dtype(dtype)) return 0;
+    if (m <= 0 || n <= 0 || n > kMostFeatures || k < 0 || !is_float_dtype(dtype)) return 0;
     return gated_work(m, n, k, dtype, want_dx, want_dw, want_db).total;
 }
 
 int lf_gated_linear_grad(const lf_linear_grad_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream) {
     LF_REQUIRE(h_args, LF_ERR_INVALID, "null argument");
     const lf_linear_grad_args& a = *h_args;
-    LF_TRY(check_sizes(a.m, 2 * a.n, a.k, a.dtype, a.activation));
+    LF_TRY(check_sizes(a.m, both_halves(a.n), a.k, a.dtype, a.activation));
     LF_REQUIRE(is_float_dtype(a.dtype) && (!a.d_db || is_float_dtype(a.db_dtype)), LF_ERR_UNSUPPORTED, "gradients are of float32, bfloat16 or float16");
     LF_TRY(check_matrix("dy", a.d_dy, a.m, a.n, a.ld_dy, a.dtype));
     LF_TRY(check_matrix("z", a.d_z, a.m, 2 * a.n, a.ld_z, a.dtype));
