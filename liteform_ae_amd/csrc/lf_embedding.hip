@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "lf_dense.h"
+#include "lf_rules.h"
 
 namespace {
 
@@ -154,10 +155,7 @@ template <typename C> __device__ __forceinline__ uint32_t rank_in_wave(C* count,
     return seen + before;
 }
 
-// With so few counts workgroups add up one another's themselves, which spares a launch (32 loads a thread take as long as one; 84 took 20 us, in two launches 14).
-constexpr int kFewCounts = 32 * kSortThreads;
-
-// FEW: `counts` is what sort_count_kernel left
+// FEW: `counts` is what sort_count_kernel left, and each workgroup adds up those of all (sort_adds_counts)
 template <bool FEW>
 __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(SortArgs a) {
     constexpr int WAVES = kSortThreads / 64, ROUNDS = kTile / kSortThreads, MINE = kMostDigits / kSortThreads;
@@ -714,7 +712,7 @@ int lf_embedding_grad(const lf_embedding_grad_args* h_args, void* d_work, size_t
                 s.last = pass == p.passes - 1;
                 sort_count_kernel<<<s.groups, kSortThreads, 0, st>>>(s);
                 LF_HIP(hipGetLastError());
-                const bool few = (s.groups << p.bits) <= kFewCounts;
+                const bool few = sort_adds_counts(s.groups, p.bits);
                 if (!few) {
                     sort_offsets_kernel<<<(unsigned)ceil_div(1 << p.bits, 16), 1024, 0, st>>>(s);
                     LF_HIP(hipGetLastError());

@@ -46,5 +46,13 @@ constexpr int bsr_lane_features(int feat, int block, long long block_rows, long 
     return blocks > 0 && blocks <= most_blocks && block_rows <= most_rows ? 4 : 8;
 }
 
+// ---- sort of an embedding's ids (lf_embedding.hip)
+// Whether the workgroups that move the entries of a digit of `bits` bits add up one another's counts themselves, which spares the launch that would do so.  Each of up to
+// 512 threads takes four digits and reads the counts of all groups for them, one after the other: few groups, and fewer where all threads do.  Spared -> launched, us a
+// gradient of 16 columns: 200 rows (8 bits), 8 groups 25.6 -> 28.2, 16 29.0 -> 30.5; 32,000 rows (twice 8 bits), 16 38.3 -> 41.6; beyond, 20 31.5 -> 31.0, 32 34.0 -> 32.6,
+// 64 47.6 -> 41.5 and 64 -> 52; 2M ids of 10 rows of 64 (977 groups) 391 -> 151.  2000 rows (11 bits), 8 29.4 -> 29.9; beyond, 10 31.0 -> 30.0, 16 33.2 -> 30.6, 64 66 -> 43; a million rows (twice 10 bits), 8 46.6 -> 50.8,
+// beyond, 12 52.9 -> 51.7, 14 55.5 -> 52.0, 64 77 -> 57.
+constexpr bool sort_adds_counts(long long groups, int bits) { return groups <= (bits <= 8 ? 16 : 8); }
+
 }  // namespace lf
 #endif
