@@ -613,9 +613,8 @@ template <typename DT, typename S, int G> int launch_sums(Sums<S> a, hipStream_t
     a.slices = (uint32_t)slices;
     a.groups = (uint32_t)(a.sum_groups + fill);
     // Neighbouring workgroups take the slices of a row, so that it is read and written whole by what is on the GPU at once (16,384 ids of 32,000 x 4096
-    // bf16 104 us, one slice after the other 128; 17 ids of 28,215 x 3824 f32 98 and 109).  Slices of float32 are 2 KB, and among many ids the
-    // wavefronts that add up are few: there filling one slice had better lie between adding up two (19,908 ids of 24,964 x 1792 106, else 121).
-    a.by_slice = sizeof(DT) == 4 && a.n >= a.rows / 4;
+    // bf16 104 us, one slice after the other 128), but for some sizes of float32.
+    a.by_slice = sizeof(DT) == 4 && sums_by_slice(a.n, a.rows, a.dim);
     LF_REQUIRE((a.sum_groups + fill) * slices < (1ll << 32) / kSumThreads, LF_ERR_UNSUPPORTED, "too many rows");
     embedding_sums_kernel<DT, S, G><<<(unsigned)((a.sum_groups + fill) * slices), kSumThreads, (kSumThreads / G * a.each + 2) * sizeof(Entry), st>>>(a);
     LF_HIP(hipGetLastError());

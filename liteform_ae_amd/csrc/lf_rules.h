@@ -47,12 +47,26 @@ constexpr int bsr_lane_features(int feat, int block, long long block_rows, long 
 }
 
 // ---- sort of an embedding's ids (lf_embedding.hip)
-// Whether the workgroups that move the entries of a digit of `bits` bits add up one another's counts themselves, which spares the launch that would do so.  Each of up to
-// 512 threads takes four digits and reads the counts of all groups for them, one after the other: few groups, and fewer where all threads do.  Spared -> launched, us a
-// gradient of 16 columns: 200 rows (8 bits), 8 groups 25.6 -> 28.2, 16 29.0 -> 30.5; 32,000 rows (twice 8 bits), 16 38.3 -> 41.6; beyond, 20 31.5 -> 31.0, 32 34.0 -> 32.6,
-// 64 47.6 -> 41.5 and 64 -> 52; 2M ids of 10 rows of 64 (977 groups) 391 -> 151.  2000 rows (11 bits), 8 29.4 -> 29.9; beyond, 10 31.0 -> 30.0, 16 33.2 -> 30.6, 64 66 -> 43; a million rows (twice 10 bits), 8 46.6 -> 50.8,
-// beyond, 12 52.9 -> 51.7, 14 55.5 -> 52.0, 64 77 -> 57.
+// Whether the workgroups that move the entries of a digit of `bits` bits add up one another's counts themselves, which spares the launch that would do so.  Each of
+// up to 512 threads takes four digits and reads the counts of all groups for them, one after the other: few groups, and fewer where all threads do.  Spared ->
+// launched, us a gradient of 16 columns: 200 rows (8 bits), 8 groups 25.6 -> 28.2, 16 29.0 -> 30.5; 32,000 rows (twice 8 bits), 16 38.3 -> 41.6; beyond, 20 31.5 -> 31.0,
+// 32 34.0 -> 32.6, 64 47.6 -> 41.5 and 64 -> 52; 2M ids of 10 rows of 64 (977 groups) 391 -> 151.  2000 rows (11 bits), 8 29.4 -> 29.9; beyond, 10 31.0 -> 30.0, 16
+// 33.2 -> 30.6, 64 66 -> 43; a million rows (twice 10 bits), 8 46.6 -> 50.8; beyond, 12 52.9 -> 51.7, 14 55.5 -> 52.0, 64 77 -> 57.
 constexpr bool sort_adds_counts(long long groups, int bits) { return groups <= (bits <= 8 ? 16 : 8); }
+
+// ---- sums of an embedding's gradient in float32
+// Whether one slice of 512 columns comes after the other, for all ids and all rows without, and not all slices of a row at once.  Rows of up to a slice and a half: what
+// fills the second slice, with most of its threads idle, then does not hold up the others.  Large gradients with about as many ids as rows: filling one slice lies between
+// adding up two.  Not where rows are multiples of 4 KB apart, of which a slice is the same part of the memory's channels each time.
+// All at once -> one after the other, us: 576 columns of 65,104 rows, ids a 32nd of them 57.8 -> 46.4, a quarter 73.8 -> 65.4, as many 115.7 -> 105.3; 640 of 60,000, twice
+// as many 150.8 -> 144.4; 768 of 48,828, as many 107.5 -> 94.1; beyond, 576, four times as many 219.7 -> 232.7.  1300 of 28,846, as many 108.9 -> 102.2; 1792 of 24,964,
+// 0.8 109.8 -> 100.1, a half 89.6 -> 92.7, a quarter 81.8 -> 83.5; 2300 of 16,304 99.8 -> 94.1, a quarter 49.1 -> 52.9; 3300 of 11,363 104.6 -> 97.1, a quarter 47.9 -> 51.7, four
+// times as many 223.0 -> 224.3; 2816 of 2663 (30 MB) four times as many 64.7 -> 73.3.  1024 of 30,000, as many 83.7 -> 90.1, twice 114.5 -> 137.1; 4096 of 8000 77.1 -> 87.5.
+constexpr bool sums_by_slice(long long ids, long long rows, long long dim) {
+    if (dim <= 512 || dim % 1024 == 0) return false;
+    if (dim <= 768) return ids <= 2 * rows;
+    return rows * dim * 4 >= (64ll << 20) && 4 * ids >= 3 * rows && 2 * ids <= 3 * rows;
+}
 
 }  // namespace lf
 #endif
