@@ -1,8 +1,8 @@
-"""Layer norm of rows whose elements are equal, or differ in their last places, at any distance from zero."""
+"""Layer norm of rows whose elements are equal, or differ in their last places, at any distance from zero; sums of its gradient over many rows."""
 import pytest
 
-from test_gpu_layer_ops import E, F32, gen, normal, within
-from test_gpu_training_ops import check_layer_grad, check_layer_norm
+from test_gpu_layer_ops import BF16, E, F32, TINY, U, gen, normal, within
+from test_gpu_training_ops import check_layer_grad, check_layer_norm, layer_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,28 @@ def test_rows_that_differ_in_their_last_places(lo, dim):
     for eps in (1e-5, 1e-12):
         check_layer_norm(lo, x, w, b, None, eps, F32, (dim, eps))
         check_layer_grad(lo, dy, x, w, eps, None, (dim, eps))
+
+
+def depth_of(rows, dim):
+    """Additions that a term of dw and db goes through: rows of a thread, row groups of a workgroup, workgroups of a slice, slices."""
+    threads = 8 if dim <= 64 else 16 if dim <= 128 else 32 if dim <= 256 else 64 if dim <= 1024 else 256 if dim <= 4096 else 512 if dim <= 8192 else 1024
+    size = max(threads, 256)
+    each = size // threads
+    groups = min(-(-rows // each), 4 * 256 * 256 // size, max(1, (1 << 25) // dim))
+    return -(-rows // (groups * each)) + each + -(-groups // 64) + 64
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 24), (1025, 3000), (70_001, 24), (40_003, 96), (20_003, 200), (9_001, 513), (3_001, 3000), (1_101, 12_000), (603, 17_000)])
+def test_sums_over_many_rows(lo, rows, dim):
+    """A row that is left out or counted twice is seen: the bound is that of the additions that there are, and sums of whole numbers are exact."""
+    g = gen(63)
+    h, w = normal((rows, dim), F32, g, 2.0), normal((1, dim), F32, g)[0]
+    for dtype in (F32, BF16):
+        dy = torch.randint(-8, 9, (rows, dim), device="cuda", generator=g).to(dtype)
+        _, dw, db = lo.layer_norm_grad(dy, h, w, bias_dtype=F32)
+        assert torch.equal(db.double(), dy.double().sum(dim=0))           # (below 2^24 in magnitude)
+        _, t, _, _, t_off = layer_reference(h, None, None, None, 1e-5)
+        terms = dy.double() * t
+        bound = terms.abs().sum(dim=0) * (depth_of(rows, dim) + 2) * E + (dy.double().abs() * t_off).sum(dim=0)
+        want = terms.sum(dim=0)
+        within(dw, want, want.abs() * U[F32] + bound * 1.01 + TINY[F32], "dw")
