@@ -11,7 +11,7 @@
 //
 // Measured with inputs that no cache holds: 57,001 rows of 2.45M x 128 f16 8 us; gradient of 16,384 ids of 32,000 x 4096 bf16, most of them a few ids, 104 us: sort
 // 25 in four launches, sums and rows of zeros 75 (396 MB: 5.3 TB/s), join 6.  Bound by memory where rows are long; else by launches and by
-// the latency of each pass (100,000 ids of 16 columns: 59 us).  Counts of the next digit made with atomic additions while the entries move, a launch less: 94 us
+// the latency of each pass (100,000 ids of 45,000 x 16 f32: 51 us).  Counts of the next digit made with atomic additions while the entries move, a launch less: 94 us
 // became 110, 72 (432k ids of 82) became 95.
 #include <algorithm>
 
@@ -584,7 +584,8 @@ template <typename F> void of_type(int32_t t, F f) {
 }
 
 inline size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
-// Entries that some threads take one after the other: enough of them for 8192 wavefronts, and few where there are few (1440 ids of 16 columns 17 us, in sixteens 22).
+// Entries that some threads take one after the other: eight up to 1024 wavefronts of eights (1440 ids of 16 columns 17 us, in sixteens 22), then as many as leave up to 8192
+// wavefronts, and 64 for more.
 int entries_each(int64_t n, int64_t dim) {
     const int64_t waves = n * ceil_div(dim, 8 * group_of(dim)) * group_of(dim) / 64;
     return waves <= 8 * 1024 ? 8 : waves <= 16 * 8192 ? 16 : waves <= 32 * 8192 ? 32 : kMostEach;

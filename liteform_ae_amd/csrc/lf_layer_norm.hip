@@ -600,7 +600,7 @@ template <typename F> auto of_types(int32_t a, int32_t b, F f) {
     return a == LF_DTYPE_F32 ? second(0.f) : a == LF_DTYPE_BF16 ? second((__bf16)0.f) : second((_Float16)0.f);
 }
 
-// Workgroups of 256 threads, as for the norms of lf_norm.hip.
+// Workgroups of 256 threads, as many as for the norms of lf_norm.hip; in the gradient each leaves two partial rows, where theirs leaves one.
 constexpr int kNormGroups = 12 * 256, kGradGroups = 4 * 256;
 unsigned grad_groups(int64_t rows, int64_t dim) {
     return std::min(workgroups(rows, shape_of(dim), kGradGroups), (unsigned)std::max<int64_t>(1, (1ll << 25) / dim));

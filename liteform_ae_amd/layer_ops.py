@@ -502,8 +502,9 @@ def embedding(ids, table, scale: float = 1.0, out_dtype=None):
 
 
 def embedding_grad(dy, ids, rows: int, scale: float = 1.0, out_dtype=None):
-    """The gradient (rows, features) of ``embedding``'s table from that of y, ``dy`` (n, features): ``scale`` times the sum of dy's rows of each id, in 32 bits and in their
-    order, zeros for ids that do not occur.  It is of ``out_dtype`` (default: dy's); ids outside 0 .. rows - 1 have none."""
+    """The gradient (rows, features) of ``embedding``'s table from that of y, ``dy`` (n, features): ``scale`` times the sum of dy's rows of each id, in their order, zeros for
+    ids that do not occur.  Sums of float32 are in 64 bits; of 16-bit types in 32 bits over up to 2048 rows, and in 64 from there on.  It is of
+    ``out_dtype`` (default: dy's); ids outside 0 .. rows - 1 have none."""
     torch, lib, device = _begin()
     gp, ldg, gt = _matrix("dy", dy, _FLOATS, device)
     n, dim = dy.shape

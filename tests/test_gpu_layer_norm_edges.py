@@ -53,18 +53,18 @@ def test_rows_of_equal_elements(lo, dim):
 def test_rows_that_differ_in_their_last_places(lo, dim):
     """Elements of 0 to 3 last places more than a value: nothing but these is left, and it has all its digits."""
     g = gen(62)
-    bits = magnitudes()[8:].view(torch.int32)                             # (squares of differences below 10^-17 vanish beside any eps)
+    bits = magnitudes()[8:].view(torch.int32)                             # (squares of differences below 10^-17 vanish beside either eps)
     x = (bits[:, None] + torch.randint(0, 4, (len(bits), dim), device="cuda", generator=g, dtype=torch.int32)).view(F32)
     x[:, 0] = bits.view(F32)
     x[:, -1] = (bits + 3).view(F32)                                       # (no two ends alike)
     w, b, dy = normal((1, dim), F32, g)[0], normal((1, dim), F32, g)[0], normal(x.shape, F32, g)
-    for eps in (1e-5, 1e-12):
+    for eps in (1e-5, 1e-12, 0.0):
         check_layer_norm(lo, x, w, b, None, eps, F32, (dim, eps))
         check_layer_grad(lo, dy, x, w, eps, None, (dim, eps))
     # one element of a row
     x = bits.view(F32)[:, None].repeat(1, dim)
     x[:, dim // 2] = (bits + 1).view(F32)
-    for eps in (1e-5, 1e-12):
+    for eps in (1e-5, 1e-12, 0.0):
         check_layer_norm(lo, x, w, b, None, eps, F32, (dim, eps))
         check_layer_grad(lo, dy, x, w, eps, None, (dim, eps))
 
