@@ -100,7 +100,7 @@ struct Centre {
                 } else if (f.by == 1.f && !(var >= kTiny && var < __builtin_inff())) {
                     moves = 0;
                     f = var < kTiny ? Change{mean, 1.f / kTiny} : Change{0.f, kTiny};
-                    more = var < kTiny ? eps * f.by * f.by : 0.f;        // (eps is nothing beside squares that overflow)
+                    more = eps * f.by * f.by;
                     mean = first(f) * inv_dim;
                 } else {
                     break;
@@ -109,7 +109,7 @@ struct Centre {
             }
             change(f);
             by = f.by;
-            if (by < 1.f && var == 0.f && eps > 0.f) {
+            if (by < 1.f && var == 0.f && eps > 0.f) {                   // (equal elements: eps alone, which the power of two has taken away)
                 by = 1.f;
                 var = eps;
             }

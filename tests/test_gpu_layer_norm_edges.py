@@ -92,3 +92,13 @@ def test_sums_over_many_rows(lo, rows, dim):
         bound = terms.abs().sum(dim=0) * (depth_of(rows, dim) + 2) * E + (dy.double().abs() * t_off).sum(dim=0)
         want = terms.sum(dim=0)
         within(dw, want, want.abs() * U[F32] + bound * 1.01 + TINY[F32], "dw")
+
+
+@pytest.mark.parametrize("dim", [5, 100, 3001, 20_001])
+def test_an_eps_beside_squares_that_overflow(lo, dim):
+    """Variance and eps, each in the range of float32 or not, whose sum is beyond it."""
+    g = gen(64)
+    x, w, b, dy = normal((9, dim), F32, g), normal((1, dim), F32, g)[0], normal((1, dim), F32, g)[0], normal((9, dim), F32, g)
+    for scale, eps in ((1e19, 3e38), (3e18, 3.4e38), (1e20, 3e38), (1e21, 1e38)):
+        check_layer_norm(lo, x * scale, w, b, None, eps, F32, (dim, scale, eps))
+        check_layer_grad(lo, dy, x * scale, w, eps, None, (dim, scale, eps))
