@@ -535,9 +535,9 @@ size_t lf_embedding_grad_work_bytes(int64_t n, int64_t rows, int64_t dim, int32_
 int lf_embedding_grad(const lf_embedding_grad_args* h_args, void* d_work, size_t work_bytes, lf_stream_t stream);
 
 /* lf_clip_gradients: *d_norm (device memory) = sqrt(sum over n tensors of their elements' squares), added in 64 bits; each d_dst = d_src * min(1, most / (norm + eps)),
- * which is 1 for a norm of 0 and for an infinite limit.  A norm that is NaN leaves NaN; an infinite one, under a finite limit, zeros and, of the infinities, NaN.  d_dst NULL in all tensors: the norm alone.  d_dst may be
- * d_src (with its ld), but may lie on no other tensor: LF_ERR_INVALID.  The tensors are read before the call returns; nothing is copied to
- * the GPU.  Work space as lf_clip_work_bytes says, 16-byte aligned. */
+ * which is 1 for a norm of 0 and for an infinite limit.  A norm that is NaN leaves NaN; an infinite one, under a finite limit, zeros and, of the infinities, NaN.  d_dst
+ * NULL in all tensors: the norm alone.  d_dst may be d_src (with its ld), but may lie on no other tensor: LF_ERR_INVALID.  The tensors are read before the call returns;
+ * nothing is copied to the GPU.  Work space as lf_clip_work_bytes says, 16-byte aligned. */
 typedef struct lf_tensor_desc {
     const void* d_src; void* d_dst;
     int64_t rows, cols, ld_src, ld_dst;
