@@ -440,7 +440,8 @@ def gated_linear_8bit(x, x_scale, weight, weight_scale, bias=None, activation="s
 def gated_linear_grad(dy, x, weight, z, activation="silu", bias_dtype=None, want_dx: bool = True, want_dweight: bool = True):
     """``(dx, dweight, dbias)`` of ``gated_linear`` from the gradient ``dy`` (rows, n) of y and the ``z`` that it returned: dz = [dy u act'(g) | dy act(g)], dx = dz
     weight, dweight (2 n, k) = dz^T x, dbias (2 n) = column sums of dz.  All of one type but dbias, which is of ``bias_dtype`` (None: not computed).
-    Gradients that are not wanted are None.  dz is rounded to the operands' type before the products."""
+    Gradients that are not wanted are None.  dz is rounded to the operands' type before the products (in float16 what exceeds 65504 becomes infinite, as in any
+    gradient of that type)."""
     torch, lib, device = _begin()
     act = _activation(activation)
     xp, ldx, xt = _matrix("x", x, _FLOATS, device)
