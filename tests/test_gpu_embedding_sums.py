@@ -61,3 +61,24 @@ def test_sums_of_many_rows(lo, dtype):
         for out in (F32, dtype):
             got = lo.embedding_grad(dy, ids, rows, scale=scale, out_dtype=out)
             within(got, want * scale, (want * scale).abs() * U[out] + bound * (1 + U[out]) + (count > 0) * TINY[out], (n, rows, dim))
+
+
+@pytest.mark.parametrize("n,rows,dim", [(30_000, 200, 24), (50_000, 200, 24), (50_000, 3000, 24), (40_000, 2_000_000, 8), (9000, 8000, 1300), (2000, 30_000, 600)])
+def test_both_ways_of_the_sort_and_the_sums_in_a_graph(lo, n, rows, dim):
+    """Recorded once and replayed with other ids and rows in the same buffers, between eager calls."""
+    g = gen(73)
+    dy, ids = normal((n, dim), F32, g), ids_of(n, rows, g)
+    lo.embedding_grad(dy, ids, rows)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = lo.embedding_grad(dy, ids, rows)
+    for _ in range(3):
+        dy.copy_(normal((n, dim), F32, g))
+        ids.copy_(ids_of(n, rows, g, "zipf"))
+        want = lo.embedding_grad(dy, ids, rows)
+        got.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
